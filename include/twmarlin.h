@@ -473,6 +473,61 @@ int twm_gemm_tw_marlin_m1_indirect(twm_ctx *ctx, const float *a_dev, const uint8
                                    const uint32_t *packed_offsets_dev, const uint16_t *scales_buf_dev,
                                    const uint32_t *scales_offsets_dev, int expert_idx, float *c_dev, uint32_t n, uint32_t k);
 
+/* ---- linear layers in 8-bit floating point, and the rows that feed them ------------- */
+
+/* No counterpart in the reference, whose quantized layers are TW-Marlin ones: for models whose checkpoints hold e4m3 weights
+ * (OCP 8-bit floating point: 448 the largest value, no infinities) with one scale per block of 128 x 128.
+ *
+ *   rows    : u8 [M][K] e4m3 codes,  f32 scales [M][ceil(K / 128)]: value = scale * code
+ *   weights : u8 [N][K] e4m3 codes, as a checkpoint holds a linear layer, f32 scales [ceil(N / 128)][ceil(K / 128)]
+ *
+ * A last block that K or N cuts short has a scale like any other.  Nothing is repacked and no handle is made.  Pointers are
+ * aligned to their elements, the codes of twm_gemm_fp8 to 16 bytes; dimensions go to 2^24.  The calls are asynchronous on the
+ * context's stream, allocate nothing and can be captured; twm_gemm_fp8 uses the context's scratch like twm_gemm. */
+
+/* C[m][n] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] * (sum over the block's features of A[m][k] * W[n][k]),
+ * products and sums in f32, C row-major f32 (c_dtype TWM_F32) or rounded to f16 at the end (TWM_F16).  K must be a multiple of
+ * 16 (TWM_SHAPE_ERROR); M and N are any size, from one row on.  K = 0 stores zeros.  Deterministic: the same call gives the
+ * same bits. */
+int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, const uint8_t *w_dev, const float *w_scales_dev,
+                 uint32_t m, uint32_t n, uint32_t k, void *c_dev, int c_dtype);
+/* Rows of f16 or f32 as e4m3 rows for twm_gemm_fp8: scale = max(max |x| of the row's 128 columns, 1e-30) / 448,
+ * code = e4m3_rne(x / scale).  A block with an infinity or a NaN gets a NaN scale.  cols is any size (twm_gemm_fp8 asks for a
+ * multiple of 16). */
+int twm_quantize_rows_fp8(twm_ctx *ctx, const void *x_dev, int x_dtype, uint32_t rows, uint32_t cols, uint8_t *q_dev, float *scales_dev);
+/* twm_swiglu_rows and twm_geglu_rows with f16 or f32 rows in and e4m3 rows out: the gate of fused gate/up rows ahead of a down
+ * projection in 8 bits.  gate_up [batch, 2 * dim], paired as in twm_swiglu_rows (dim a multiple of 32 then);
+ * q [batch, dim], scales [batch, ceil(dim / 128)] as in twm_quantize_rows_fp8.  The gate is computed in f32. */
+int twm_swiglu_rows_fp8(twm_ctx *ctx, const void *gate_up_dev, int dtype, uint32_t batch, uint32_t ffn_dim, int paired, uint8_t *q_dev,
+                        float *scales_dev);
+int twm_geglu_rows_fp8(twm_ctx *ctx, const void *gate_up_dev, int dtype, uint32_t batch, uint32_t dim, int paired, uint8_t *q_dev,
+                       float *scales_dev);
+/* The residual's addition and the root-mean-square norm ahead of a layer's projections, in one pass over the rows:
+ *   s = x + residual (residual_dev NULL: s = x),   y = s / sqrt(mean(s^2) + eps) * weight,   q, scales of y as above.
+ * x f16 or f32, residual, weight [cols] and sums f32.  sum_dev receives s (it may be residual_dev: the residual stream is
+ * updated in place; NULL: s is not stored); normed_dev_f16 receives y rounded to f16, for projections that take f16 rows
+ * (NULL: not stored).  No other two buffers may overlap.  eps < 0 or NaN returns TWM_SHAPE_ERROR. */
+int twm_add_rms_norm_fp8(twm_ctx *ctx, const void *x_dev, int x_dtype, const float *residual_dev, const float *weight_dev, float eps,
+                         uint32_t rows, uint32_t cols, float *sum_dev, uint8_t *q_dev, float *scales_dev, uint16_t *normed_dev_f16);
+
+/* ---- sampling ------------------------------------------------------------------------ */
+
+/* One token per row of logits [rows, cols], where twm_argmax_f32 takes the largest: the caller gives every row a uniform number
+ * u in [0, 1) and, as arrays of one entry per row or NULL for all rows alike, its temperature (NULL: 1), top_k (NULL, 0 or
+ * less: no limit), top_p (NULL or NaN: 1) and min_p (NULL or NaN: 0).
+ *   w[i] = exp((x[i] - max x) / temperature); a temperature that is not above 0 takes the first largest logit.
+ *   In descending order of x, equal logits by index, the first top_k tokens remain; of these the shortest run whose weights
+ *   reach top_p of their sum, at least one; of these the ones with w >= min_p (the largest always does).
+ *   The token is the first by index at which the running sum of what remains exceeds u times the whole (u below 0 or NaN: 0;
+ *   1 or more: the last token with any weight).
+ * Weights are computed in 64 bits and summed as whole numbers of at least 2^-38 of the largest, so that the result depends neither on the
+ * launch nor on other rows; a token below half that step of the largest weight is never chosen.
+ * -infinity masks a token and NaN counts as that; a row of nothing else yields 0, as do rows without columns.  +infinity shares
+ * the choice with its equals.  out [rows] i32. */
+int twm_sample_f32(twm_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t cols, const float *uniform_dev,
+                   const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev,
+                   int32_t *out_dev);
+
 /* The library's split-K choice for MI355X (256 CUs) with f16 activations; same role as quantize.rs:1317-1325.
  * 1 where the plan needs no split (among others wherever M <= 16 runs on column sub-tiles). */
 uint32_t twm_pick_splits(uint32_t k, uint32_t n, uint32_t m);

@@ -97,6 +97,12 @@ SIGNATURES = {
     "twm_batched_marlin_down_axpy": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32]),
     "twm_batched_marlin_split_geglu": (_int, [_vp, _vp, _vp, _u32, _u32]),
     "twm_gemm_tw_marlin_m1_indirect": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _u32, _u32]),
+    "twm_gemm_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _int]),
+    "twm_quantize_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _vp, _vp]),
+    "twm_swiglu_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp]),
+    "twm_geglu_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp]),
+    "twm_add_rms_norm_fp8": (_int, [_vp, _vp, _int, _vp, _vp, C.c_float, _u32, _u32, _vp, _vp, _vp, _vp]),
+    "twm_sample_f32": (_int, [_vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "twm_pick_splits": (_u32, [_u32, _u32, _u32]),
     "twm_graph_begin": (_int, [_vp]),
     "twm_graph_end": (_vp, [_vp]),

@@ -3,6 +3,7 @@
 //   twm_api.hip          contexts, device memory, events, format operations, the GEMV on the reference's arrays, graphs
 //   twm_api_weights.hip  repacked weight handles and their byte blob
 //   twm_api_gemm.hip     launch planners, the dispatcher of twm_gemm and its variants, measured plans
+//   twm_api_fp8.hip      8-bit floating point: products, the rows that feed them; token sampling
 //   twm_api_moe.hip      expert banks and the reference's MoE launches on raw slabs
 #pragma once
 #include "../../include/twmarlin.h"

@@ -224,4 +224,16 @@ hipError_t launch_raw_gemv(hipStream_t s, const RawView &v, const float *a, uint
 hipError_t launch_raw_down_axpy(hipStream_t s, const RawView &v, const float *a_all, const float *ids, const float *weights,
                                 uint32_t slots, float *accum, int force_sub = 0, int force_waves = 0);
 
+// rows in e4m3 with a scale per row and 128 columns (twm_fp8_rows.hip); gate: 0 = the rows as they are, 1 / 2 = gelu_tanh(gate) * up /
+// silu(gate) * up of rows of 2 * cols columns
+hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t rows, uint32_t cols, int gate, bool paired, uint8_t *q, float *scales);
+hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *residual, const float *weight, float eps, uint32_t rows,
+                           uint32_t cols, float *sum, uint8_t *q, float *scales, uint16_t *normed);
+// the product of such rows and a matrix in e4m3 with a scale per 128 x 128 block (twm_fp8_gemm.hip)
+hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scales, const uint8_t *w, const float *w_scales, uint32_t m,
+                           uint32_t n, uint32_t k, void *c, bool c_f16, float *ws, size_t ws_bytes);
+// a token per row of logits (twm_sample.hip)
+hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint32_t cols, const float *uniform, const float *temperature,
+                         const int *top_k, const float *top_p, const float *min_p, int *out);
+
 }  // namespace twm

@@ -1,0 +1,516 @@
+"""The 8-bit floating point path -- rows with scales, their product with block-scaled weights -- and the token sampler, through
+the C ABI, against plain numpy in 64 bits.
+
+Tolerances count roundings.  e4m3 has three mantissa bits: a code is off by at most 2^-4 of its value, or 2^-10 where it is
+subnormal.  Row functions compute y in f32 with no more than sixteen roundings of 2^-24: 2^-20 of y (and of gate * up, where
+1 + tanh cancels).  A product of two e4m3 values is exact in f32; a block of 128 of them is added with at most 128 roundings (of
+2^-23, should the matrix unit cut off instead of rounding), then comes one for the scales' product, one for the scaling and one
+per addition of a block, a wave's or a K-range's sum."""
+import numpy as np
+import pytest
+
+import tensorwarp_amd as T
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 128
+
+
+@pytest.fixture(scope="module")
+def dev():
+    with T.WarpDevice(0) as d:
+        yield d
+
+
+def blocks(n):
+    return -(-n // BLOCK)
+
+
+def e4m3_table():
+    t = np.zeros(256, np.float64)
+    for c in range(256):
+        e, m = (c >> 3) & 15, c & 7
+        v = np.nan if e == 15 and m == 7 else m * 2.0 ** -9 if e == 0 else (8 + m) * 2.0 ** (e - 10)
+        t[c] = -v if c & 128 else v
+    return t
+
+
+E4M3 = e4m3_table()
+
+
+class Out:
+    """An output buffer with sentinels on both sides, so that a store outside of it shows."""
+
+    def __init__(self, dev, shape, dtype):
+        self.n, self.shape, self.kind = int(np.prod(shape)), shape, dtype
+        np_type = {"f32": np.float32, "f16": np.uint16, "u8": np.uint8, "i32": np.int32}[dtype]
+        self.pad = 64
+        self.fill = np.full(self.n + 2 * self.pad, 0x5A, np.uint8) if dtype == "u8" else np.full(self.n + 2 * self.pad, 12345, np_type)
+        self.whole = T.GpuTensor.from_host(dev, self.fill, dtype)
+        self.dtype, self.numel = dtype, self.n
+        self.ptr = self.whole.ptr + self.pad * self.fill.itemsize
+
+    def get(self):
+        h = self.whole.to_host()
+        assert np.array_equal(h[:self.pad], self.fill[:self.pad]) and np.array_equal(h[self.pad + self.n:], self.fill[self.pad + self.n:])
+        v = h[self.pad:self.pad + self.n].reshape(self.shape)
+        return v.view(np.float16) if self.kind == "f16" else v
+
+
+class At:
+    """A device array that begins `skip` elements into its allocation."""
+
+    def __init__(self, dev, array, skip=0):
+        flat = np.ascontiguousarray(array).reshape(-1)
+        self.whole = T.GpuTensor.from_host(dev, np.concatenate([flat[:1].repeat(skip), flat]) if flat.size else np.zeros(16, flat.dtype))
+        self.dtype = self.whole.dtype
+        self.ptr = self.whole.ptr + skip * flat.itemsize
+
+
+def check_codes(q, scales, y, y_err):
+    """q, scales of rows y whose values are known within y_err (f64 arrays)."""
+    rows, cols = y.shape
+    kb = blocks(cols)
+    for b in range(kb):
+        at = slice(b * BLOCK, min((b + 1) * BLOCK, cols))
+        amax, err = np.abs(y[:, at]).max(axis=1), y_err[:, at].max(axis=1)
+        want = np.maximum(amax, 1e-30) / 448.0
+        assert (np.abs(scales[:, b] - want) <= err / 448.0 + 2.0 ** -22 * want).all()
+        s = scales[:, b].astype(np.float64)[:, None]
+        v, off = y[:, at] / s, y_err[:, at] / s
+        got = E4M3[q[:, at]]
+        # half a step, the roundings of y * (448 / amax), and what y itself may be off
+        assert (np.abs(got - v) <= np.maximum(2.0 ** -4 * np.abs(v), 2.0 ** -10) + 2.0 ** -21 * np.abs(v) + off).all()
+        big = np.abs(got).max(axis=1)   # the block's largest is the largest code
+        assert (big[amax > 1e-29] == 448.0).all()
+
+
+SHAPES = [(1, 1), (1, 128), (3, 7), (2, 129), (1, 896), (5, 1000), (4, 2048), (3, 2049), (2, 4096), (2, 4104), (3, 5001), (2, 16392), (1, 50001)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantize_rows(dev, rows, cols, dtype):
+    rng = np.random.default_rng(rows * 100003 + cols)
+    x = (rng.standard_normal((rows, cols)) * np.exp(rng.uniform(-6, 4, (rows, 1)))).astype(np.float16 if dtype == "f16" else np.float32)
+    x[:, :min(cols, 40)] *= (rng.random((rows, min(cols, 40))) > 0.5)   # some zeros
+    q, s = Out(dev, (rows, cols), "u8"), Out(dev, (rows, blocks(cols)), "f32")
+    T.quantize_rows_fp8(dev, At(dev, x), q, s, rows, cols)
+    y = x.astype(np.float64)
+    check_codes(q.get(), s.get(), y, np.zeros_like(y))
+
+
+@pytest.mark.parametrize("skip", [1, 2, 4])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_rows_at_odd_addresses_are_the_aligned_rows(dev, dtype, skip):
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((3, 512)).astype(np.float16 if dtype == "f16" else np.float32)
+    got = []
+    for off in (0, skip):
+        q, s = Out(dev, (3, 512), "u8"), Out(dev, (3, 4), "f32")
+        T.quantize_rows_fp8(dev, At(dev, x, off), q, s, 3, 512)
+        q2, s2 = Out(dev, (3, 256), "u8"), Out(dev, (3, 2), "f32")
+        T.swiglu_rows_fp8(dev, At(dev, x, off), q2, s2, 256, 3)
+        q3, s3, n3 = Out(dev, (3, 512), "u8"), Out(dev, (3, 4), "f32"), Out(dev, (3, 512), "f16")
+        T.add_rms_norm_fp8(dev, At(dev, x, off), None, At(dev, np.ones(512, np.float32), off), 1e-6, 3, 512, q3, s3, normed=n3)
+        got.append([t.get() for t in (q, s, q2, s2, q3, s3, n3)])
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)
+
+
+def test_blocks_of_zeros_tiny_values_infinities_and_nans(dev):
+    x = np.zeros((1, 6 * BLOCK), np.float32)
+    x[0, 128:256] = 1e-38
+    x[0, 256 + 5] = np.inf
+    x[0, 384 + 7] = np.nan
+    x[0, 512:640] = 3.0e38
+    x[0, 640:768] = -2.0
+    q, s = Out(dev, x.shape, "u8"), Out(dev, (1, 6), "f32")
+    T.quantize_rows_fp8(dev, At(dev, x), q, s, 1, x.shape[1])
+    q, s = q.get()[0], s.get()[0]
+    assert (q[:256] & 0x7F == 0).all() and (s[:2] > 0).all() and (s[:2] < 1e-30).all()
+    assert np.isnan(s[2]) and np.isnan(s[3])
+    assert (E4M3[q[512:640]] == 448.0).all() and abs(s[4] / (3.0e38 / 448) - 1) < 2.0 ** -22
+    assert (E4M3[q[640:]] == -448.0).all() and abs(s[5] * 448 - 2.0) < 2.0 ** -22
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,dim,paired", [(1, 1, 0), (3, 31, 0), (8, 704, 1), (2, 130, 0), (5, 1184, 1), (2, 4099, 0), (3, 2816, 0), (1, 32, 1), (33, 160, 1)])
+def test_gated_rows(dev, rows, dim, paired, dtype, act):
+    rng = np.random.default_rng(rows * 1009 + dim)
+    x = (2.5 * rng.standard_normal((rows, 2 * dim))).astype(np.float16 if dtype == "f16" else np.float32)
+    x[0, :2] = [-60.0, 60.0][:2]
+    q, s = Out(dev, (rows, dim), "u8"), Out(dev, (rows, blocks(dim)), "f32")
+    (T.swiglu_rows_fp8 if act == "silu" else T.geglu_rows_fp8)(dev, At(dev, x), q, s, dim, rows, paired=bool(paired))
+    v = x.astype(np.float64)
+    if paired:
+        v = v.reshape(rows, dim // 32, 2, 32)
+        g, u = v[:, :, 0].reshape(rows, dim), v[:, :, 1].reshape(rows, dim)
+    else:
+        g, u = v[:, :dim], v[:, dim:]
+    y = g / (1 + np.exp(-g)) * u if act == "silu" else 0.5 * g * (1 + np.tanh(np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3))) * u
+    check_codes(q.get(), s.get(), y, 2.0 ** -20 * (np.abs(y) + (np.abs(g * u) if act == "gelu" else 0)) + 1e-37)
+
+
+@pytest.mark.parametrize("with_residual,with_sum,with_normed", [(1, 1, 1), (1, 0, 0), (0, 0, 1), (0, 1, 0)])
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_add_rms_norm(dev, rows, cols, dtype, with_residual, with_sum, with_normed):
+    rng = np.random.default_rng(rows * 7919 + cols)
+    x = rng.standard_normal((rows, cols)).astype(np.float16 if dtype == "f16" else np.float32)
+    r = (3 * rng.standard_normal((rows, cols))).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(cols)).astype(np.float32)
+    eps = 1e-5
+    q, s = Out(dev, (rows, cols), "u8"), Out(dev, (rows, blocks(cols)), "f32")
+    total = Out(dev, (rows, cols), "f32") if with_sum else None
+    normed = Out(dev, (rows, cols), "f16") if with_normed else None
+    T.add_rms_norm_fp8(dev, At(dev, x), At(dev, r) if with_residual else None, At(dev, w), eps, rows, cols, q, s, sum=total, normed=normed)
+    v = x.astype(np.float32) + r if with_residual else x.astype(np.float32)
+    if with_sum:
+        assert np.array_equal(total.get(), v)
+    v = v.astype(np.float64)
+    y = v / np.sqrt((v * v).mean(axis=1, keepdims=True) + np.float64(np.float32(eps))) * w
+    if with_normed:
+        assert (np.abs(normed.get().astype(np.float64) - y) <= (2.0 ** -11 + 2.0 ** -20) * np.abs(y) + 2.0 ** -25).all()
+    check_codes(q.get(), s.get(), y, 2.0 ** -20 * np.abs(y))
+
+
+@pytest.mark.parametrize("cols", [512, 4096, 20000, 777])
+def test_the_residual_is_updated_in_place(dev, cols):
+    rng = np.random.default_rng(cols)
+    x, r, w = (rng.standard_normal(s).astype(np.float32) for s in ((3, cols), (3, cols), (cols,)))
+    q, s, apart = Out(dev, (3, cols), "u8"), Out(dev, (3, blocks(cols)), "f32"), Out(dev, (3, cols), "f32")
+    T.add_rms_norm_fp8(dev, At(dev, x), At(dev, r), At(dev, w), 1e-6, 3, cols, q, s, sum=apart)
+    q2, s2, same = Out(dev, (3, cols), "u8"), Out(dev, (3, blocks(cols)), "f32"), At(dev, r)
+    T.add_rms_norm_fp8(dev, At(dev, x), same, At(dev, w), 1e-6, 3, cols, q2, s2, sum=same)
+    assert np.array_equal(same.whole.to_host().reshape(3, cols), apart.get())
+    assert np.array_equal(q.get(), q2.get()) and np.array_equal(s.get(), s2.get())
+
+
+def test_a_norm_of_zeros_and_of_an_infinity(dev):
+    x = np.zeros((3, 300), np.float32)
+    x[1, 7] = np.inf
+    x[2] = 1.0
+    q, s, n = Out(dev, (3, 300), "u8"), Out(dev, (3, 3), "f32"), Out(dev, (3, 300), "f16")
+    T.add_rms_norm_fp8(dev, At(dev, x), None, At(dev, np.ones(300, np.float32)), 0.0, 3, 300, q, s, normed=n)
+    # 0 / sqrt(0 + 0) is no number; the rows beside are left alone
+    assert np.isnan(s.get()[0]).all() and np.isnan(s.get()[1]).any()
+    assert np.allclose(n.get()[2], 1.0) and (E4M3[q.get()[2]] == 448.0).all()
+    q, s = Out(dev, (3, 300), "u8"), Out(dev, (3, 3), "f32")
+    T.add_rms_norm_fp8(dev, At(dev, x), None, At(dev, np.ones(300, np.float32)), 1e-6, 3, 300, q, s)
+    assert (q.get()[0] & 0x7F == 0).all() and np.isfinite(s.get()[0]).all()
+
+
+# ---- products --------------------------------------------------------------------------------------------------------
+
+def codes(rng, rows, cols):
+    """Every code but the two NaNs, subnormal ones and zeros among them."""
+    c = rng.integers(0, 254, (rows, cols), dtype=np.uint8)
+    return c + (c >= 0x7F)
+
+
+def gemm_truth(a, a_s, w, w_s):
+    """(sum in 64 bits, sum of magnitudes)"""
+    m, k = a.shape
+    n = w.shape[0]
+    af = E4M3[a] * np.repeat(a_s.astype(np.float64), BLOCK, axis=1)[:, :k]
+    wf = E4M3[w] * np.repeat(np.repeat(w_s.astype(np.float64), BLOCK, axis=0)[:n], BLOCK, axis=1)[:, :k]
+    return af @ wf.T, np.abs(af) @ np.abs(wf).T
+
+
+def gemm_inputs(rng, m, n, k):
+    a, w = codes(rng, m, k), codes(rng, n, k)
+    a_s = np.exp(rng.uniform(-6, -3, (m, blocks(k)))).astype(np.float32)
+    w_s = np.exp(rng.uniform(-8, -5, (blocks(n), blocks(k)))).astype(np.float32)
+    return a, a_s, w, w_s
+
+
+def check_gemm(dev, inputs, m, n, k, dtype, skip=0):
+    a, a_s, w, w_s = inputs
+    c = Out(dev, (m, n), dtype)
+    T.gemm_fp8(dev, At(dev, a), At(dev, a_s, skip), At(dev, w), At(dev, w_s, skip), m, n, k, c)
+    got = c.get().astype(np.float64)
+    truth, size = gemm_truth(*inputs)
+    tol = (128 * 2.0 ** -23 + (blocks(k) + 32) * 2.0 ** -24) * size
+    if dtype == "f16":
+        tol += 2.0 ** -11 * np.abs(truth) + 2.0 ** -25
+    worst = (np.abs(got - truth) - tol).max() if got.size else 0
+    assert worst <= 0, worst
+    return c
+
+
+GEMMS = [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 130, 272), (3, 64, 112), (1, 896, 896), (5, 256, 1024), (15, 129, 704), (16, 100, 2816), (17, 260, 640),
+         (31, 384, 1040), (32, 128, 4096), (33, 1, 256), (40, 640, 704), (64, 300, 1152), (65, 96, 512), (77, 513, 384), (100, 255, 2064), (128, 512, 1024),
+         (129, 257, 1040), (200, 384, 256), (256, 256, 128), (257, 640, 1296), (300, 1000, 528), (513, 130, 896), (1, 4096, 18944), (13, 4096, 4096), (7, 8, 16),
+         (1030, 520, 272), (48, 3584, 2048)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("m,n,k", GEMMS)
+def test_gemm(dev, m, n, k, dtype):
+    check_gemm(dev, gemm_inputs(np.random.default_rng(m * 31 + n * 17 + k), m, n, k), m, n, k, dtype, skip=(m + n) % 4)
+
+
+def test_gemm_without_features_or_results(dev):
+    one = At(dev, np.zeros(16, np.uint8))
+    s = At(dev, np.ones(4, np.float32))
+    for dtype in ("f32", "f16"):
+        c = Out(dev, (3, 5), dtype)
+        T.gemm_fp8(dev, one, s, one, s, 3, 5, 0, c)
+        assert (c.get() == 0).all()
+        c = Out(dev, (1, 1), dtype)
+        T.gemm_fp8(dev, one, s, one, s, 0, 5, 16, c)
+        T.gemm_fp8(dev, one, s, one, s, 5, 0, 16, c)
+        assert c.whole.to_host()[c.pad] == 12345
+
+
+@pytest.mark.parametrize("m", [1, 20, 70, 300])
+def test_gemm_nan_rows_stay_in_their_row_and_column(dev, m):
+    # a NaN code or a NaN scale reaches its own row or column and nothing else, also where K ends inside a block
+    n, k = 200, 400
+    a, a_s, w, w_s = gemm_inputs(np.random.default_rng(m), m, n, k)
+    a[m - 1, 399] = 0x7F
+    w[150, 3] = 0xFF
+    c = Out(dev, (m, n), "f32")
+    T.gemm_fp8(dev, At(dev, a), At(dev, a_s), At(dev, w), At(dev, w_s), m, n, k, c)
+    got = np.isnan(c.get())
+    want = np.zeros((m, n), bool)
+    want[m - 1] = True
+    want[:, 150] = True
+    assert np.array_equal(got, want)
+
+
+def test_gemm_is_the_same_every_time(dev):
+    for m, n, k in ((1, 512, 8192), (24, 640, 4096), (200, 384, 4096)):
+        inputs = [At(dev, v) for v in gemm_inputs(np.random.default_rng(m), m, n, k)]
+        got = []
+        for _ in range(3):
+            c = Out(dev, (m, n), "f32")
+            T.gemm_fp8(dev, *inputs, m, n, k, c)
+            got.append(c.get())
+        assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+# ---- sampling --------------------------------------------------------------------------------------------------------
+
+def pick(x, u, temperature, top_k, top_p, min_p):
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if x.size == 0 or np.all(x == -np.inf):
+        return 0
+    if not temperature > 0:
+        return int(np.argmax(x))
+    order = np.lexsort((np.arange(x.size), -x))
+    order = order[x[order] > -np.inf]
+    if top_k > 0:
+        order = order[:top_k]
+    top = x[order[0]]
+    with np.errstate(invalid="ignore"):
+        w = np.where(x[order] == top, 1.0, np.exp((x[order] - top) / float(temperature)))
+    sums = np.cumsum(w)
+    if not np.isnan(top_p):
+        keep = max(1, int((sums - w < float(top_p) * sums[-1]).sum())) if top_p < 1 else w.size
+        order, w = order[:keep], w[:keep]
+    if not np.isnan(min_p):
+        keep = w >= min(1.0, float(min_p))
+        order, w = order[keep], w[keep]
+    at = np.argsort(order)
+    order, sums = order[at], np.cumsum(w[at])
+    goal = 0.0 if not u > 0 else float(u) * sums[-1]
+    found = np.nonzero(sums > goal)[0] if u < 1 or not u > 0 else []
+    return int(order[found[0]]) if len(found) else int(order[np.nonzero(w[at] > 2.0 ** -38)[0][-1]])
+
+
+def draw_tokens(dev, x, u, t=None, k=None, p=None, mp=None):
+    rows, cols = x.shape
+    as_f32 = lambda v: None if v is None else At(dev, np.asarray(v, np.float32))  # noqa: E731
+    out = Out(dev, (rows,), "i32")
+    T.sample(dev, At(dev, x), as_f32(u), out, rows, cols, temperature=as_f32(t), top_k=None if k is None else At(dev, np.asarray(k, np.int32)),
+             top_p=as_f32(p), min_p=as_f32(mp))
+    got = out.get()
+    want = [pick(x[r], np.float32(u[r]), np.float32(1 if t is None else t[r]), 0 if k is None else int(k[r]), np.float32(np.nan if p is None else p[r]),
+                 np.float32(np.nan if mp is None else mp[r])) for r in range(rows)]
+    return got, np.asarray(want, np.int32)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (5, 63), (4, 64), (9, 1000), (2, 1024), (3, 1025), (1, 4097), (17, 5000), (2, 16385), (6, 32000), (70, 8200),
+                                       (1, 152064), (5, 151936), (300, 257)])
+@pytest.mark.parametrize("spread", [0.3, 3.0])
+def test_sample(dev, rows, cols, spread):
+    rng = np.random.default_rng(rows * 13 + cols)
+    x = (spread * rng.standard_normal((rows, cols))).astype(np.float32)
+    u = rng.random(rows)
+    assert np.array_equal(*draw_tokens(dev, x, u))
+    t = rng.uniform(0.3, 1.5, rows)
+    assert np.array_equal(*draw_tokens(dev, x, u, t))
+    k = rng.integers(-1, 2 * cols if cols < 50 else 60, rows)
+    assert np.array_equal(*draw_tokens(dev, x, u, t, k=k))
+    assert np.array_equal(*draw_tokens(dev, x, u, t, p=rng.uniform(0.05, 1.0, rows)))
+    assert np.array_equal(*draw_tokens(dev, x, u, t, mp=rng.uniform(0, 0.5, rows)))
+    t[rng.random(rows) < 0.2] = 0
+    assert np.array_equal(*draw_tokens(dev, x, u, t, k=rng.integers(1, cols + 1, rows), p=rng.uniform(0.5, 1.0, rows), mp=rng.uniform(0, 0.05, rows)))
+
+
+@pytest.mark.parametrize("cols", [7, 1000, 40000])
+def test_sample_among_equal_logits(dev, cols):
+    # few distinct values, so that top-k and top-p end among equals, where the lower index stays
+    rng = np.random.default_rng(cols)
+    rows = 24
+    x = rng.integers(0, 3, (rows, cols)).astype(np.float32) * np.float32(0.7)
+    x[0] = 1.5
+    x[1] = -0.0
+    x[1, ::2] = 0.0
+    u = rng.random(rows)
+    k = rng.integers(1, cols + 1, rows)
+    assert np.array_equal(*draw_tokens(dev, x, u, k=k))
+    assert np.array_equal(*draw_tokens(dev, x, u, k=np.full(rows, 1)))
+    assert np.array_equal(*draw_tokens(dev, x, u, mp=np.ones(rows)))
+    # (sums of ones are exact: 3 of 8 of a row of equals)
+    assert np.array_equal(*draw_tokens(dev, np.full((rows, cols), 2.5, np.float32), u, p=np.full(rows, 0.375)))
+    assert np.array_equal(*draw_tokens(dev, x, u, t=np.zeros(rows)))
+
+
+@pytest.mark.parametrize("cols", [50, 3000, 70000])
+def test_sample_masks_and_numbers_that_are_none(dev, cols):
+    rng = np.random.default_rng(cols)
+    rows = 12
+    x = (2 * rng.standard_normal((rows, cols))).astype(np.float32)
+    x[0] = -np.inf                      # nothing allowed
+    x[1] = np.nan
+    x[2, :] = -np.inf
+    x[2, cols - 1] = -5.0               # one token
+    x[3, rng.random(cols) < 0.9] = -np.inf
+    x[4, rng.random(cols) < 0.5] = np.nan
+    x[5, [3, cols // 2]] = np.inf       # two that share the choice
+    x[6] = np.finfo(np.float32).min     # a mask of the type's lowest value, over everything
+    x[7, 5:] = np.finfo(np.float32).min
+    x[8, cols // 3] = 3e38
+    u = rng.random(rows)
+    t = rng.uniform(0.5, 1.2, rows)
+    for k, p, mp in ((None, None, None), (np.full(rows, 5), None, None), (None, np.full(rows, 0.9), None), (None, None, np.full(rows, 0.01)),
+                     (np.full(rows, 40), np.full(rows, 0.8), np.full(rows, 0.02))):
+        assert np.array_equal(*draw_tokens(dev, x, u, t, k=k, p=p, mp=mp))
+        assert np.array_equal(*draw_tokens(dev, x, u, np.zeros(rows), k=k, p=p, mp=mp))
+
+
+def test_sample_rules_at_their_ends(dev):
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((9, 300)).astype(np.float32)
+    u = np.array([0.0, -1.0, np.nan, 1.0, 2.0, np.float32(1) - np.float32(2.0 ** -24), 0.5, 0.5, 0.5])
+    assert np.array_equal(*draw_tokens(dev, x, u))
+    some = rng.random(9)
+    assert np.array_equal(*draw_tokens(dev, x, some, p=[0.0, -1.0, np.nan, 1.0, 2.0, 1e-30, 0.5, 0.999999, 0.1]))
+    assert np.array_equal(*draw_tokens(dev, x, some, mp=[0.0, -1.0, np.nan, 1.0, 2.0, 1e-30, 0.5, 0.999999, 0.1]))
+    assert np.array_equal(*draw_tokens(dev, x, some, t=[0.0, -1.0, np.nan, 1e-30, 1e30, np.inf, 1e-3, 50.0, -0.0]))
+    assert np.array_equal(*draw_tokens(dev, x, some, k=[0, -5, 1, 2, 299, 300, 301, 2 ** 31 - 1, -2 ** 31]))
+
+
+def test_sample_rows_without_columns(dev):
+    out = Out(dev, (3,), "i32")
+    T.sample(dev, At(dev, np.zeros(1, np.float32)), At(dev, np.zeros(3, np.float32)), out, 3, 0)
+    assert np.array_equal(out.get(), [0, 0, 0])
+
+
+def test_a_rows_token_does_not_depend_on_the_batch(dev):
+    rng = np.random.default_rng(4)
+    x = (2 * rng.standard_normal((80, 9000))).astype(np.float32)
+    u, p = rng.random(80), np.full(80, 0.95)
+    together, _ = draw_tokens(dev, x, u, p=p)
+    for r in (0, 41, 79):
+        alone, _ = draw_tokens(dev, x[r:r + 1], u[r:r + 1], p=p[:1])
+        assert alone[0] == together[r]
+
+
+# ---- the run of them, as a decode step makes it ------------------------------------------------------------------------
+
+class Step:
+    """A feed-forward block and the vocabulary's projection for m tokens: norm, gate and up, gate, down, norm, logits, token."""
+
+    def __init__(self, dev, m, hidden, ffn, vocab, seed):
+        rng = np.random.default_rng(seed)
+        self.dev, self.m, self.hidden, self.ffn, self.vocab = dev, m, hidden, ffn, vocab
+        self.h_w = {name: (codes(rng, n, k) & 0xBF, np.exp(rng.uniform(-4, -3, (blocks(n), blocks(k)))).astype(np.float32))
+                    for name, n, k in (("gate_up", 2 * ffn, hidden), ("down", hidden, ffn), ("head", vocab, hidden))}
+        self.w = {name: (At(dev, c), At(dev, s)) for name, (c, s) in self.h_w.items()}
+        self.h_norms = [(1 + 0.1 * rng.standard_normal(hidden)).astype(np.float32) for _ in range(2)]
+        self.norms = [At(dev, v) for v in self.h_norms]
+        self.x, self.residual, self.uniform = (T.GpuTensor(dev, s, "f32") for s in ((m, hidden), (m, hidden), (m,)))
+        self.stream_rows = T.GpuTensor(dev, (m, hidden), "f32")
+        self.out = {"sum": Out(dev, (m, hidden), "f32"), "q1": Out(dev, (m, hidden), "u8"), "s1": Out(dev, (m, blocks(hidden)), "f32"),
+                    "gate_up": Out(dev, (m, 2 * ffn), "f16"), "q2": Out(dev, (m, ffn), "u8"), "s2": Out(dev, (m, blocks(ffn)), "f32"),
+                    "down": Out(dev, (m, hidden), "f32"), "sum2": Out(dev, (m, hidden), "f32"), "q3": Out(dev, (m, hidden), "u8"),
+                    "s3": Out(dev, (m, blocks(hidden)), "f32"), "logits": Out(dev, (m, vocab), "f32"), "token": Out(dev, (m,), "i32")}
+        self.k, self.p = At(dev, np.full(m, 50, np.int32)), At(dev, np.full(m, 0.95, np.float32))
+
+    def give(self, seed):
+        rng = np.random.default_rng(seed)
+        self.h_x, self.h_residual = (rng.standard_normal((self.m, self.hidden)).astype(np.float32) for _ in range(2))
+        self.h_uniform = rng.random(self.m).astype(np.float32)
+        self.x.copy_from_host(self.h_x)
+        self.residual.copy_from_host(self.h_residual)
+        self.uniform.copy_from_host(self.h_uniform)
+
+    def run(self):
+        o, m, h, f, v, dev = self.out, self.m, self.hidden, self.ffn, self.vocab, self.dev
+        T.add_rms_norm_fp8(dev, self.x, self.residual, self.norms[0], 1e-6, m, h, o["q1"], o["s1"], sum=o["sum"])
+        T.gemm_fp8(dev, o["q1"], o["s1"], *self.w["gate_up"], m, 2 * f, h, o["gate_up"])
+        T.swiglu_rows_fp8(dev, o["gate_up"], o["q2"], o["s2"], f, m)
+        T.gemm_fp8(dev, o["q2"], o["s2"], *self.w["down"], m, h, f, o["down"])
+        T.add_rms_norm_fp8(dev, o["down"], o["sum"], self.norms[1], 1e-6, m, h, o["q3"], o["s3"], sum=o["sum2"])
+        T.gemm_fp8(dev, o["q3"], o["s3"], *self.w["head"], m, v, h, o["logits"])
+        T.sample(dev, o["logits"], self.uniform, o["token"], m, v, top_k=self.k, top_p=self.p)
+
+    def got(self):
+        return {name: t.get() for name, t in self.out.items()}
+
+    def check(self, g):
+        """Every stage against 64 bits, from what the stage before it left."""
+        def rows_of(x, w):
+            v = x.astype(np.float64)
+            return v / np.sqrt((v * v).mean(axis=1, keepdims=True) + 1e-6) * w
+        assert np.array_equal(g["sum"], self.h_x + self.h_residual) and np.array_equal(g["sum2"], g["down"] + g["sum"])
+        for q, s, total, w in (("q1", "s1", "sum", self.h_norms[0]), ("q3", "s3", "sum2", self.h_norms[1])):
+            y = rows_of(g[total], w)
+            check_codes(g[q], g[s], y, 2.0 ** -20 * np.abs(y))
+        for q, s, w, c, k in (("q1", "s1", "gate_up", "gate_up", self.hidden), ("q2", "s2", "down", "down", self.ffn), ("q3", "s3", "head", "logits", self.hidden)):
+            truth, size = gemm_truth(g[q], g[s], *self.h_w[w])
+            tol = (128 * 2.0 ** -23 + (blocks(k) + 32) * 2.0 ** -24) * size
+            if c == "gate_up":
+                tol += 2.0 ** -11 * np.abs(truth) + 2.0 ** -25
+            assert (np.abs(g[c].astype(np.float64) - truth) <= tol).all(), c
+        gu = g["gate_up"].astype(np.float64)
+        gate, up = gu[:, :self.ffn], gu[:, self.ffn:]
+        y = gate / (1 + np.exp(-gate)) * up
+        check_codes(g["q2"], g["s2"], y, 2.0 ** -20 * np.abs(y) + 1e-37)
+        want = [pick(g["logits"][r], self.h_uniform[r], np.float32(1), 50, np.float32(0.95), np.float32(np.nan)) for r in range(self.m)]
+        assert np.array_equal(g["token"], want)
+
+
+@pytest.mark.parametrize("m,hidden,ffn,vocab", [(1, 256, 704, 5000), (7, 384, 512, 2001), (140, 256, 640, 1000)])
+def test_a_step_eager_captured_and_on_another_stream(dev, m, hidden, ffn, vocab):
+    step = Step(dev, m, hidden, ffn, vocab, m)
+    step.give(1)
+    step.run()
+    first = step.got()
+    step.check(first)
+    graph = T.GraphCapture.record_with_device(dev, step.run)
+    for seed in (2, 1, 3):
+        step.give(seed)
+        graph.replay()
+        dev.synchronize()
+        replayed = step.got()
+        step.run()   # eager work between the replays
+        dev.synchronize()
+        eager = step.got()
+        assert all(np.array_equal(replayed[name], eager[name], equal_nan=True) for name in eager)
+        step.check(eager)
+    graph.destroy()
+    lib = T._lib.load()
+    stream = lib.twm_stream_create(dev.handle)
+    dev.with_stream(stream)
+    step.give(1)
+    step.run()
+    again = step.got()
+    dev.with_stream(None)
+    assert lib.twm_stream_destroy(dev.handle, stream) == T._lib.OK
+    assert all(np.array_equal(first[name], again[name]) for name in first)
