@@ -16,6 +16,7 @@ PRELOAD = ["-mllvm", "-amdgpu-kernarg-preload-count=16"]
 PER_FILE_FLAGS = {"twm_gemv4s.hip": PRELOAD, "twm_splitk.hip": PRELOAD, "twm_gemv4g.hip": PRELOAD, "twm_gemv4.hip": PRELOAD, "twm_moe.hip": PRELOAD, "twm_stream.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] + PRELOAD,
                   "twm_batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] + PRELOAD,
                   "twm_waves_exact.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] + PRELOAD,
+                  "twm_fp8_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
                   "twm_batch_range.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] + PRELOAD,
                   "twm_waves.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"] + PRELOAD}
 # -packed-fp32-ops off: v_pk_{add,mul,fma}_f32 are not to be generated on this hardware pool.

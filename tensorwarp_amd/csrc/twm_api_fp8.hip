@@ -26,7 +26,8 @@ struct DeviceGuard {
     }
 };
 
-constexpr uint32_t kFp8MostDim = 1u << 24;   // rows, columns and features of one call
+constexpr uint32_t kFp8MostDim = 1u << 24;   // rows and columns of one call
+constexpr uint32_t kFp8MostK = 1u << 20;     // features of a product (256 rows of codes are within a buffer's 32-bit offsets)
 
 bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 bool row_type(int dtype) { return dtype == TWM_F32 || dtype == TWM_F16; }
@@ -65,7 +66,8 @@ int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, 
     if (!ctx) return api_fail(TWM_INVALID_HANDLE, "%s: null context", who);
     if (!row_type(c_dtype)) return api_fail(TWM_UNSUPPORTED_OP, "%s: results must be f16 or f32", who);
     if (k % 16 != 0) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) must be divisible by 16", who, k);
-    if (m > kFp8MostDim || n > kFp8MostDim || k > kFp8MostDim) return api_fail(TWM_SHAPE_ERROR, "%s: %u x %u x %u is beyond 2^24 in a dimension", who, m, n, k);
+    if (m > kFp8MostDim || n > kFp8MostDim) return api_fail(TWM_SHAPE_ERROR, "%s: %u x %u is beyond 2^24 rows or columns", who, m, n);
+    if (k > kFp8MostK) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) is beyond 2^20", who, k);
     if (m == 0 || n == 0) return TWM_OK;
     if (!c_dev || (k != 0 && (!a_dev || !a_scales_dev || !w_dev || !w_scales_dev))) return api_fail(TWM_INVALID_HANDLE, "%s: null pointer", who);
     if (misaligned(a_dev, 16) || misaligned(w_dev, 16)) return api_fail(TWM_SHAPE_ERROR, "%s: A and W must be 16-byte aligned", who);

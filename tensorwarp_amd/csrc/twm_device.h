@@ -10,6 +10,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
 typedef unsigned int uint2v __attribute__((ext_vector_type(2)));
 
+#define TWM_CONSTANT __attribute__((address_space(4)))   // memory that the kernel does not write, for scalar loads
 #define TWM_GLOBAL __attribute__((address_space(1)))   // a pointer into device memory, for the builtins that ask for one
 
 // SwiGLU gate of the reference (warp_fused_silu_mul, crates/kernels/src/ops.rs:966-976):

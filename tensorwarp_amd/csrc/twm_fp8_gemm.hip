@@ -13,6 +13,8 @@
 // both operands agree.
 #include "twm_device.h"
 
+#include <type_traits>
+
 namespace twm {
 
 typedef int int8v __attribute__((ext_vector_type(8)));
@@ -137,12 +139,314 @@ __global__ __launch_bounds__(WAVES * 64) void k_fp8_gemm_simple(const Fp8Gemm g,
     }
 }
 
+// ---- many rows: tiles staged in LDS --------------------------------------------------------------------------------------
+//
+// A workgroup computes BM rows x BN columns in blocks of 128 features.  Both operands' blocks (128 bytes a row) go from memory
+// to LDS directly, two buffers; eight rows per load instruction, lane l = (row l / 8, 16-byte slot l % 8).  Slot s of row r
+// holds the row's piece s ^ (r / 2 % 8): two rows span the 64 banks, so that sixteen neighbouring rows' reads of one piece fall
+// on all of them (with s ^ (r % 8) half the cycles of the reads were conflicts).  Waves own S * TN columns x S * TM rows each
+// (columns within one 128-column block of W's scales).  The rows' scales come to LDS four blocks at a time, 16 bytes a row:
+// read from memory by the lanes that need them, each was a cache line of its own, half as many again as the operands' (254 us
+// at 2048 x 22016 x 4096 with them, 197 without).
+//
+// S = 16: v_mfma_f32_16x16x128_f8f6f4 takes a tile's whole block at once.  Results in f16 only: within each eight neighbouring
+// features the unit cuts products off at 2^-13 of the largest one's power of two.
+// S = 32: the codes become f16 between LDS and eight v_mfma_f32_32x32x16_f16; every product and sum in f32.
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+namespace {
+
+typedef __attribute__((address_space(3))) void *LdsPtr;
+// `bytes` from p on: reads behind them give zeros
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00020000);
+}
+
+template <int BM, int BN> struct Fp8Tile {
+    uint8_t w[2][BN * 128];
+    uint8_t a[2][BM * 128];
+    float scales[2][BM * 4];   // of four blocks of A
+};
+
+// a lane's part of one operand tile of S rows x 128 features, and of the tile's result
+template <int S> struct Fp8Mfma;
+template <> struct Fp8Mfma<16> {
+    typedef float4v Sum;
+    int8v part;
+    // bytes 32 (lane / 16) .. + 31 of row lane % 16; base: the tile in LDS
+    __device__ __forceinline__ void read(const uint8_t *base, const uint32_t (&at)[4])
+    {
+        const uint4v lo = *(const uint4v *)(base + at[0]), hi = *(const uint4v *)(base + at[1]);
+        part = int8v{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    }
+    static __device__ __forceinline__ void places(uint32_t lane, uint32_t (&at)[4])
+    {
+        for (uint32_t p = 0; p < 2; p++) at[p] = (lane & 15u) * 128u + (((2u * (lane >> 4) + p) ^ (lane >> 1 & 7u)) * 16u);
+        at[2] = at[3] = 0;
+    }
+    static __device__ __forceinline__ Sum product(const Fp8Mfma &w, const Fp8Mfma &a)
+    {
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.part, a.part, Sum{}, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <> struct Fp8Mfma<32> {
+    typedef float16v Sum;
+    uint4v part[4];
+    // bytes 64 h + 32 (lane / 32) .. + 31 of row lane % 32, h = 0, 1
+    __device__ __forceinline__ void read(const uint8_t *base, const uint32_t (&at)[4])
+    {
+#pragma unroll
+        for (int p = 0; p < 4; p++) part[p] = *(const uint4v *)(base + at[p]);
+    }
+    static __device__ __forceinline__ void places(uint32_t lane, uint32_t (&at)[4])
+    {
+        for (uint32_t p = 0; p < 4; p++) at[p] = (lane & 31u) * 128u + (((4u * (p >> 1) + 2u * (lane >> 5) + (p & 1u)) ^ (lane >> 1 & 7u)) * 16u);
+    }
+    static __device__ __forceinline__ Sum product(const Fp8Mfma &w, const Fp8Mfma &a)
+    {
+        Sum d = {};
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+                d = __builtin_amdgcn_mfma_f32_32x32x16_f16(to_f16((int)w.part[p][e], (int)w.part[p][e + 1]), to_f16((int)a.part[p][e], (int)a.part[p][e + 1]), d, 0, 0, 0);
+        return d;
+    }
+};
+
+}  // namespace
+
+template <int S, int TN, int TM, int WN, int WM>
+__global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint32_t vec, uint32_t blocks_n, uint32_t blocks_m, uint32_t kb_per_split,
+                                                           float *__restrict__ partials, uint32_t n_ld)
+{
+    typedef Fp8Mfma<S> Mfma;
+    constexpr int BN = S * TN * WN, BM = S * TM * WM, WAVES = WN * WM;
+    constexpr int LW = BN / 8 / WAVES, LA = BM / 8 / WAVES;   // load instructions of eight rows per wave
+    constexpr int DEPTH = S == 16 ? 3 : 2;                    // results of the matrix unit in flight
+    // A block's loads, from the last row of products of the block two before on.  Eight waves issue theirs one by one, with every
+    // second product (issued together they held every wave of the CU up until the last had been taken: 2048 x 22016 x 4096 204 us,
+    // now 196); of four waves' workgroups two share a CU and take turns.
+    constexpr int PARTS = LW + LA, EVERY = WAVES == 8 && TN * TM >= 32 ? 2 : 1, PER = WAVES == 8 && S == 16 ? 1 : WAVES == 8 ? (PARTS + TM - 1) / TM : PARTS;
+    constexpr int EARLY = TM / EVERY * PER < PARTS ? TM / EVERY * PER : PARTS;   // those of the last row
+    static_assert(LW % 2 == 0 && LA % 2 == 0 && (PARTS - EARLY + PER - 1) / PER * EVERY <= (TN - 1) * TM);
+    static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && 128 % (S * TN) == 0 && TN % 2 == 0);
+    extern __shared__ uint8_t lds[];
+    Fp8Tile<BM, BN> &tile = *(Fp8Tile<BM, BN> *)lds;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    const uint32_t wn = wave % WN, wm = wave / WN;
+
+    // Which tile: workgroups go to the eight XCDs in turn; XCD x takes the x-th eighth of a list of the tiles that runs in
+    // bands of eight row blocks, so that what an XCD works on at a time shares its operands in that XCD's L2.
+    constexpr uint32_t kBand = 8;
+    const uint32_t tiles = blocks_n * blocks_m, share = tiles >> 3, rest = tiles & 7u, x8 = blockIdx.x & 7u;
+    const uint32_t t = x8 * share + (x8 < rest ? x8 : rest) + (blockIdx.x >> 3);
+    const uint32_t band = t / (kBand * blocks_n), u = t - band * kBand * blocks_n;
+    const uint32_t high = blocks_m - band * kBand < kBand ? blocks_m - band * kBand : kBand;
+    const uint32_t n0 = (u / high) * BN, m0 = (band * kBand + u % high) * BM;
+    const uint32_t kb0 = blockIdx.y * kb_per_split, kb1 = min(kb0 + kb_per_split, g.kb);
+
+    // Loads: instruction j of a wave fills eight rows; this lane's row and piece of instructions 0 and 1, the others 16 rows further
+    // each.  The buffers' limits are checked on the lane's offset: a row behind the end, or a piece behind the end of K, reads as
+    // zeros.  (The block's offset k0 stands outside of the check: a lane in a row and in K stays in that row.)
+    const uint32_t l_row = lane >> 3, piece[2] = {((lane & 7u) ^ (l_row >> 1)) * 16u, ((lane & 7u) ^ (l_row >> 1) ^ 4u) * 16u};
+    const __amdgpu_buffer_rsrc_t w_buf = buffer_of(g.w + (size_t)n0 * g.k, min((uint32_t)BN, g.n - n0) * g.k);
+    const __amdgpu_buffer_rsrc_t a_buf = buffer_of(g.a + (size_t)m0 * g.k, min((uint32_t)BM, g.m - m0) * g.k);
+    const uint32_t w_row = (wave * LW * 8u + l_row) * g.k, a_row = (wave * LA * 8u + l_row) * g.k;
+    auto load = [&](uint32_t buf, uint32_t b, int part) {
+        const int j = part < LW ? part : part - LW;
+        const uint32_t k0 = b * 128u, in_k = piece[j & 1] < g.k - k0, from = (part < LW ? w_row : a_row) + piece[j & 1] + j * 8u * g.k;
+        uint8_t *to = part < LW ? &tile.w[buf][(wave * LW + j) * 1024u] : &tile.a[buf][(wave * LA + j) * 1024u];
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(part < LW ? w_buf : a_buf, (LdsPtr)to, 16, in_k ? from : 0xFFFFFFFFu, k0, 0, 0);
+    };
+    // Scales of blocks kb0 + 4 c .. + 3 of a row per lane, 64 rows a wave; where a row has no four blocks left, one by one
+    const float *as = g.a_scales + (size_t)m0 * g.kb;
+    const __amdgpu_buffer_rsrc_t as_buf = buffer_of(as, min((uint32_t)BM, g.m - m0) * g.kb * 4u);
+    auto load_scales = [&](uint32_t c) {
+        if (wave >= BM / 64) return;
+        const uint32_t r = wave * 64u + lane, b = kb0 + 4u * c;
+        float *to = &tile.scales[c & 1u][wave * 256u];
+        if (b + 4u <= g.kb) {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(as_buf, (LdsPtr)to, 16, r * g.kb * 4u, b * 4u, 0, 0);
+        } else {
+            const float *from = as + (size_t)min(r, g.m - 1u - m0) * g.kb;
+            *(float4v *)(to + lane * 4u) = float4v{from[min(b, g.kb - 1u)], from[min(b + 1u, g.kb - 1u)], from[min(b + 2u, g.kb - 1u)], from[g.kb - 1u]};
+        }
+    };
+
+    uint32_t at[4];   // this lane's pieces of an operand tile
+    Mfma::places(lane, at);
+    const uint32_t row = lane % S;   // the lane's row of A in a tile
+    // (columns behind the end have no scale: any block's will do)
+    const TWM_CONSTANT float *ws_row = (const TWM_CONSTANT float *)(g.w_scales + (size_t)min((n0 + wn * TN * S) >> 7, (g.n - 1u) >> 7) * g.kb);
+    // the factor of row tile j in the block `done` blocks from kb0
+    auto scale = [&](int j, uint32_t done) { return tile.scales[done >> 2 & 1u][((wm * TM + j) * S + row) * 4u + (done & 3u)]; };
+
+    typename Mfma::Sum acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+        for (int j = 0; j < TM; j++) acc[i][j] = typename Mfma::Sum{};
+
+    if (kb0 < kb1) {
+        load_scales(0);
+#pragma unroll
+        for (int part = 0; part < PARTS; part++) load(0, kb0, part);
+#pragma unroll
+        for (int part = 0; part < EARLY; part++)
+            if (kb0 + 1 < kb1) load(1, kb0 + 1, part);
+        Mfma w[2], a[TM];
+        float s_next[TM], ws_next = ws_row[kb0];
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TM; j++) s_next[j] = scale(j, 0);
+        w[0].read(&tile.w[0][wn * TN * S * 128u], at);
+#pragma unroll
+        for (int j = 0; j < TM; j++) a[j].read(&tile.a[0][(wm * TM + j) * S * 128u], at);
+        // (the buffer is a constant of each of two copies of the step, so that LDS addresses are a register and an offset)
+        auto step = [&](auto which, uint32_t b) {
+            constexpr uint32_t buf = decltype(which)::value;
+            float s[TM];
+#pragma unroll
+            for (int j = 0; j < TM; j++) s[j] = s_next[j] * ws_next;
+            const uint32_t done_b = b - kb0;
+            ws_next = ws_row[b + 1 < kb1 ? b + 1 : b];
+            typename Mfma::Sum d[DEPTH];
+#pragma unroll
+            for (int t = 0; t < TN * TM + DEPTH - 1; t++) {
+                const int i = t / TM, j = t % TM;
+                if (t < TN * TM) {
+                    if (j == 0) {
+                        if (i + 1 < TN) {
+                            w[(i + 1) & 1].read(&tile.w[buf][(wn * TN + i + 1) * S * 128u], at);
+                        } else {
+                            // every operand of this block is in registers: once all waves are here the buffer can be filled again,
+                            // and the next block is complete
+                            __builtin_amdgcn_s_waitcnt(0);
+                            __builtin_amdgcn_s_barrier();
+                            // (four blocks' scales ahead of their first use, when the half that they replace has been read)
+                            if ((done_b & 3u) == 1u && b + 3 < kb1) load_scales((done_b >> 2) + 1u);
+#pragma unroll
+                            for (int jj = 0; jj < TM; jj++) s_next[jj] = scale(jj, done_b + 1u);
+                            w[(i + 1) & 1].read(&tile.w[buf ^ 1u][wn * TN * S * 128u], at);
+                        }
+                    }
+                    d[t % DEPTH] = Mfma::product(w[i & 1], a[j]);
+                    const int last_row = t - (TN - 1) * TM;
+#pragma unroll
+                    for (int part = 0; part < PER && t % EVERY == 0; part++) {
+                        const int early = last_row / EVERY * PER + part, late = EARLY + t / EVERY * PER + part;
+                        if (last_row >= 0 && early < EARLY && b + 2 < kb1) load(buf, b + 2, early);
+                        if (late < PARTS && b + 1 < kb1) load(buf ^ 1u, b + 1, late);
+                    }
+                    if (i == TN - 1) a[j].read(&tile.a[buf ^ 1u][(wm * TM + j) * S * 128u], at);
+                }
+                const int done = t - (DEPTH - 1);
+                if (done >= 0) {
+                    typename Mfma::Sum &sum = acc[done / TM][done % TM];
+                    sum += d[done % DEPTH] * s[done % TM];
+                    asm volatile("" : "+v"(sum));   // (here: the compiler moved these down past all products, whose results then held a register each)
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        for (uint32_t b = kb0; b < kb1; b += 2) {
+            step(std::integral_constant<uint32_t, 0>{}, b);
+            if (b + 1 < kb1) step(std::integral_constant<uint32_t, 1>{}, b + 1);
+        }
+    }
+    // register e of a lane: column (512 / S) (e / 4) % S + 4 (lane / S) + e % 4 of the tile, row lane % S
+#pragma unroll
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+        for (int j = 0; j < TM; j++)
+#pragma unroll
+            for (int e = 0; e < S * S / 64; e += 4) {
+                const uint32_t n = n0 + (wn * TN + i) * S + 2u * e + 4u * (lane / S), m = m0 + (wm * TM + j) * S + row;
+                const float4v v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                if (partials) {
+                    if (m < g.m && n < n_ld) *(float4v *)(partials + ((size_t)blockIdx.y * g.m + m) * n_ld + n) = v;
+                } else {
+                    store_quad(g, vec, m, n, v);
+                }
+            }
+}
+
+// The sum of the K-ranges' results, in their order; a thread per four columns.
+__global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, uint32_t vec, const float *__restrict__ partials, uint32_t n_ld, uint32_t splits)
+{
+    const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    const uint32_t quads = n_ld / 4u;
+    const uint64_t m = i / quads;
+    if (m >= g.m) return;
+    const uint32_t n = (uint32_t)(i - m * quads) * 4u;
+    const float *at = partials + m * n_ld + n;
+    const size_t step = (size_t)g.m * n_ld;
+    float4v s = *(const float4v *)at;
+    for (uint32_t z = 1; z < splits; z++) s += *(const float4v *)(at + z * step);
+    store_quad(g, vec, (uint32_t)m, n, s);
+}
+
+namespace {
+
+struct Fp8Plan {
+    uint32_t form, splits;
+};
+// columns x rows of a form, and its kernel
+struct Fp8Form {
+    uint32_t bn, bm, threads, lds;
+    void (*kernel)(const Fp8Gemm, uint32_t, uint32_t, uint32_t, uint32_t, float *, uint32_t);
+};
+#define TWM_FP8_FORM(S, TN, TM, WN, WM) \
+    Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>}
+const Fp8Form kFp8Forms[] = {
+    TWM_FP8_FORM(16, 8, 4, 2, 4),   // 0: 256 columns x 256 rows, eight waves
+    TWM_FP8_FORM(16, 8, 2, 2, 4),   // 1: 256 x 128, eight waves
+    TWM_FP8_FORM(16, 4, 4, 2, 2),   // 2: 128 x 128
+    TWM_FP8_FORM(16, 4, 2, 2, 2),   // 3: 128 columns x 64 rows
+    TWM_FP8_FORM(32, 2, 2, 2, 2),   // 4: 128 x 128, sums of exact products
+    TWM_FP8_FORM(32, 2, 1, 2, 2),   // 5: 128 columns x 64 rows, sums of exact products
+};
+[[maybe_unused]] constexpr uint32_t kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];
+
+hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, Fp8Plan plan, float *ws, size_t ws_bytes)
+{
+    const Fp8Form &f = kFp8Forms[plan.form];
+    const uint32_t bn = (g.n + f.bn - 1) / f.bn, bm = (g.m + f.bm - 1) / f.bm, n_ld = (g.n + 3u) & ~3u;
+    uint32_t splits = plan.splits;
+    while (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) splits--;
+    const uint32_t per = (g.kb + splits - 1) / splits;
+    splits = (g.kb + per - 1) / per;
+    float *partials = splits > 1 ? ws : nullptr;
+    hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, fp8_vec_store(g), bn, bm, per, partials, n_ld);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_vec_store(g), partials, n_ld, splits);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// Once per device, outside any stream capture: the forms with more LDS than a launch gets unasked.
+hipError_t init_fp8_gemm()
+{
+    for (const Fp8Form &f : kFp8Forms) {
+        const hipError_t e = hipFuncSetAttribute((const void *)f.kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)f.lds);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scales, const uint8_t *w, const float *w_scales, uint32_t m,
                            uint32_t n, uint32_t k, void *c, bool c_f16, float *ws, size_t ws_bytes)
 {
     if (m == 0 || n == 0) return hipSuccess;
     const Fp8Gemm g = {a, w, a_scales, w_scales, m, n, k, (k + 127u) / 128u, c, c_f16 ? 1u : 0u};
     const uint32_t tiles_m = (m + 15u) / 16u, tiles_n = (n + 15u) / 16u;
+    if (m > 32) return launch_fp8_tile(s, g, Fp8Plan{c_f16 ? (m > 128 ? 2u : 3u) : (m > 128 ? 4u : 5u), 1}, ws, ws_bytes);
     if (tiles_m == 1) hipLaunchKernelGGL((k_fp8_gemm_simple<1, 8>), dim3(tiles_n, 1), dim3(512), 0, s, g, fp8_vec_store(g));
     else hipLaunchKernelGGL((k_fp8_gemm_simple<4, 4>), dim3(tiles_n, (tiles_m + 3u) / 4u), dim3(256), 0, s, g, fp8_vec_store(g));
     return hipGetLastError();

@@ -232,6 +232,7 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
 // the product of such rows and a matrix in e4m3 with a scale per 128 x 128 block (twm_fp8_gemm.hip)
 hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scales, const uint8_t *w, const float *w_scales, uint32_t m,
                            uint32_t n, uint32_t k, void *c, bool c_f16, float *ws, size_t ws_bytes);
+hipError_t init_fp8_gemm();
 // a token per row of logits (twm_sample.hip)
 hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint32_t cols, const float *uniform, const float *temperature,
                          const int *top_k, const float *top_p, const float *min_p, int *out);
