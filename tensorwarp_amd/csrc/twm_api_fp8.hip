@@ -129,7 +129,9 @@ int twm_sample_f32(twm_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_
         return api_fail(TWM_SHAPE_ERROR, "%s: a pointer is not aligned to its elements", who);
     DeviceGuard on(ctx);
     HIP_TRY(on.status, TWM_DEVICE_ERROR, who);
-    HIP_TRY(launch_sample(ctx->stream, logits_dev, rows, cols, uniform_dev, temperature_dev, top_k_dev, top_p_dev, min_p_dev, out_dev), TWM_DEVICE_ERROR, who);
+    HIP_TRY(launch_sample(ctx->stream, logits_dev, rows, cols, uniform_dev, temperature_dev, top_k_dev, top_p_dev, min_p_dev, out_dev, ctx->ws, ctx->ws_bytes,
+                          ctx->counters, ctx->n_counters),
+            TWM_DEVICE_ERROR, who);
     return TWM_OK;
 }
 

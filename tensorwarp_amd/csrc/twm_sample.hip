@@ -9,13 +9,26 @@
 //   prefix of the order, so what remains is the tokens whose key -- the bits of x that order as x does, then the inverted
 //   index -- is at least one 64-bit number, and with w >= min_p.
 //   The token is the first by index at which the running sum of what remains exceeds u times the whole.
+//
+// How a row is worked through: its largest logit; then, where top-k or top-p ask for it, a histogram of the tokens' numbers and
+// weights over 2048 bins of (max - x) / temperature, 1/64 wide, in LDS; from its running sums the one or two bins in which top-k
+// and top-p end; then one more pass that adds the weights of the tokens in the bins before those and lists the tokens in them
+// (some hundred), whose exact order is settled by comparing each with each; and at last the running sum through the one part of
+// the row that u falls into.  A row whose list would be too long (thousands of nearly equal logits) is settled eight bits of the
+// key at a time instead.  Many rows: a workgroup each, one launch.  Few rows: parts of a row each have a workgroup, in up to
+// three launches, the last workgroup of a row to arrive doing what concerns the whole row.
+// Bound: latency, of the launches and of the passes over a row (and the exponentials in 64 bits on many rows).
 #include "twm_device.h"
 
 namespace twm {
 
 namespace {
 
-constexpr uint32_t kSampleThreads = 1024;
+constexpr uint32_t kSampleBins = 2048, kSampleList = 2048, kSampleSpans = 64;
+constexpr uint32_t kSampleBatch = 8;          // loads of a thread in flight
+constexpr uint32_t kSampleCounterStep = 32;   // a row's arrival counter has a cache line of its own
+constexpr uint32_t kNoBin = 0xFFFFFFFFu;
+constexpr uint32_t kSampleFewRows = 64;
 
 // a number that orders as the float does (-0 as 0); NaN below everything
 __device__ __forceinline__ uint32_t sample_order(float v)
@@ -27,27 +40,101 @@ __device__ __forceinline__ float sample_value(uint32_t order)
 {
     return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
+// a token's place in the order: larger for a larger logit and, among equal ones, for a smaller index
+__device__ __forceinline__ uint64_t sample_key(float v, uint32_t i) { return (uint64_t)sample_order(v) << 32 | (0xFFFFFFFFu - i); }
 
-struct RowRules {
-    double largest, temperature, top_p, min_p, scale;
-    uint64_t top_k;
-    bool greedy;
+// One row's inputs
+struct SampleArgs {
+    const float *logits, *uniform, *temperature, *top_p, *min_p;
+    const int *top_k;
+    int *out;
+    uint32_t cols, spans, span;   // a row's parts: `spans` of `span` columns, the last one shorter
+    double scale;                 // 2^S
 };
 
-// 2^S w of one logit
-__device__ __forceinline__ uint64_t sample_weight(const RowRules &r, float x, double &w)
+struct SampleRules {
+    float largest, per_bin, per_one;   // per_bin = 64 / temperature, per_one = 1 / temperature, in 32 bits
+    double temperature, top_p, min_p, scale;
+    uint64_t top_k;   // 0: no limit
+    bool greedy;
+
+    // 2^S w of one logit
+    __device__ __forceinline__ uint64_t weight(float v, double &w) const
+    {
+        w = 0.0;
+        if (v == largest) {
+            w = 1.0;
+        } else if (v < largest && v > -INFINITY && !((largest - v) * per_one > 40.0f)) {   // (e^-40 < 2^-53)
+            w = exp(((double)v - (double)largest) / temperature);
+        }
+        return (uint64_t)rint(w * scale);
+    }
+    // falls as v grows, like its weight's logarithm; every rounding in it keeps the order
+    __device__ __forceinline__ uint32_t bin(float v) const
+    {
+        const float f = (largest - v) * per_bin;
+        return v == largest ? 0u : f < (float)(kSampleBins - 1) ? (uint32_t)f : kSampleBins - 1;
+    }
+    __device__ __forceinline__ bool limited() const { return top_k != 0 || top_p < 1.0; }
+};
+
+__device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, uint32_t row, float largest)
 {
-    const double v = x;
-    w = v == r.largest ? 1.0 : v < r.largest && x > -INFINITY ? exp((v - r.largest) / r.temperature) : 0.0;
-    return (uint64_t)rint(w * r.scale);
+    SampleRules r;
+    r.largest = largest;
+    const float t = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f;
+    const int k = a.top_k ? a.top_k[row] : 0;
+    r.greedy = !(t > 0.0f);
+    r.temperature = t;
+    r.per_one = 1.0f / t;
+    r.per_bin = 64.0f / t;
+    r.top_p = p < 1.0f ? (double)p : 1.0;   // (NaN: no limit)
+    r.min_p = m < 1.0f ? (double)m : m != m ? 0.0 : 1.0;
+    r.top_k = k > 0 && (uint32_t)k < a.cols ? (uint64_t)k : 0u;
+    r.scale = a.scale;
+    return r;
 }
 
+// Where the limits end, from the histogram: the tokens of bin k_bin are the last of the first top_k; p_first .. p_last are the
+// bins in which top_p can end (which one depends on the tokens of k_bin that are in).  kNoBin: no such limit.
+struct SampleCut {
+    uint32_t k_bin, p_first, p_last;
+    uint32_t above_k;          // tokens in the bins before k_bin
+    uint64_t mass_k, mass_p;   // weights in the bins before k_bin and before p_first; mass_k: of all bins where there is no k_bin
+
+    __device__ __forceinline__ uint32_t last() const { return p_last != kNoBin ? p_last : k_bin; }                  // (bins behind it are out)
+    __device__ __forceinline__ uint32_t sure() const { return p_first != kNoBin ? p_first : k_bin; }                // (bins before it are in)
+    __device__ __forceinline__ bool listed(uint32_t b) const { return b == k_bin || (b >= p_first && b <= p_last && p_first != kNoBin); }
+};
+
+// What a row's workgroups leave for each other between and within launches
+struct SampleRow {
+    uint64_t key[kSampleSpans], mass[kSampleSpans];
+    uint64_t bin_mass[kSampleBins];
+    uint32_t bin_count[kSampleBins];
+    uint64_t list_key[kSampleList], list_mass[kSampleList];
+    SampleCut cut;
+    uint32_t listed;
+};
+
 struct SampleShared {
-    uint64_t mass[256];
-    uint32_t count[256];
-    uint64_t wave64[kSampleThreads / 64];
-    uint64_t prefix, taken_count, taken_mass;
-    uint32_t largest, stop;
+    union {
+        struct {
+            uint64_t mass[kSampleBins];
+            uint32_t count[kSampleBins];
+        } bins;
+        struct {
+            uint64_t key[kSampleList];
+            uint64_t mass[kSampleList];   // bit 63: the token is above min_p
+            uint8_t state[kSampleList];   // bit 0: among the first top_k; bit 1: remains
+        } list;
+    };
+    uint64_t spans[kSampleSpans];
+    uint64_t wave64[16];
+    uint32_t wave32[16];
+    SampleCut cut;
+    uint64_t largest, prefix, taken_mass, least;
+    uint32_t listed, taken_count, stop, base;
 };
 
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v)
@@ -56,98 +143,300 @@ __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v)
     for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
     return v;
 }
-
-// the sum over the workgroup, in every thread
-__device__ uint64_t block_sum_u64(SampleShared &sh, uint64_t v)
+__device__ __forceinline__ uint64_t wave_most_u64(uint64_t v)
 {
-    v = wave_sum_u64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63u) == 0) sh.wave64[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-    for (uint32_t w = 0; w < kSampleThreads / 64; w++) v += sh.wave64[w];
+#pragma unroll
+    for (int step = 32; step; step >>= 1) {
+        const uint64_t other = __shfl_xor(v, step);
+        v = other > v ? other : v;
+    }
     return v;
 }
 
-}  // namespace
+template <uint32_t THREADS> struct Sampler {
+    static constexpr uint32_t kWaves = THREADS / 64;
+    const SampleArgs &a;
+    SampleShared &sh;
+    const float *x;
+    uint32_t row, tid, lane, wave;
 
-__global__ __launch_bounds__(1024) void k_sample(const float *__restrict__ logits, uint32_t cols, const float *__restrict__ uniform,
-                                                 const float *__restrict__ temperature, const int *__restrict__ top_k,
-                                                 const float *__restrict__ top_p, const float *__restrict__ min_p, double scale, int *__restrict__ out)
-{
-    __shared__ SampleShared sh;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x;
-    const float *x = logits + (size_t)row * cols;
-    if (tid == 0) sh.largest = 0;
-    __syncthreads();
-    uint32_t most = 0;
-    for (uint64_t i = tid; i < cols; i += kSampleThreads) most = max(most, sample_order(x[i]));
-    atomicMax(&sh.largest, most);
-    __syncthreads();
-    most = sh.largest;
-    if (most <= sample_order(-INFINITY)) {   // nothing but -infinity and NaN
-        if (tid == 0) out[row] = 0;
-        return;
+    __device__ __forceinline__ Sampler(const SampleArgs &args, SampleShared &shared, uint32_t r)
+        : a(args), sh(shared), x(args.logits + (size_t)r * args.cols), row(r), tid(threadIdx.x), lane(threadIdx.x & 63u), wave(threadIdx.x >> 6)
+    {
     }
-    RowRules r;
-    r.largest = sample_value(most);
-    const float t = temperature ? temperature[row] : 1.0f;
-    r.greedy = !(t > 0.0f);
-    r.temperature = t;
-    r.scale = scale;
-    const int k = top_k ? top_k[row] : 0;
-    r.top_k = r.greedy ? 1u : k > 0 ? (uint64_t)k : ~0ull;
-    const float p = top_p ? top_p[row] : 1.0f;
-    r.top_p = p != p ? 1.0 : p;
-    const float mp = min_p ? min_p[row] : 0.0f;
-    r.min_p = mp != mp ? 0.0 : mp > 1.0f ? 1.0 : mp;
-    if (r.greedy) r.temperature = 1.0;
 
-    auto key_of = [&](uint64_t i, float v) { return (uint64_t)sample_order(v) << 32 | (0xFFFFFFFFu - (uint32_t)i); };
+    // f(v, i) for the columns of one part of the row
+    template <typename F> __device__ __forceinline__ void each(uint32_t span, F &&f) const
+    {
+        const uint64_t end = (uint64_t)(span + 1) * a.span < a.cols ? (uint64_t)(span + 1) * a.span : a.cols;
+        for (uint64_t i0 = (uint64_t)span * a.span + tid; i0 < end; i0 += kSampleBatch * THREADS) {
+            float v[kSampleBatch];
+#pragma unroll
+            for (uint32_t j = 0; j < kSampleBatch; j++) {
+                const uint64_t i = i0 + j * THREADS;
+                v[j] = x[i < end ? i : i0];
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kSampleBatch; j++)
+                if (i0 + j * THREADS < end) f(v[j], (uint32_t)i0 + j * THREADS);
+        }
+    }
 
-    // the smallest key among the first `want` of the order (by_mass false) or among those before which less than `goal` lies;
-    // keys below `least` do not take part
-    auto select = [&](bool by_mass, uint64_t want, double goal, uint64_t least) -> uint64_t {
+    __device__ __forceinline__ uint64_t block_sum(uint64_t v)
+    {
+        v = wave_sum_u64(v);
+        __syncthreads();
+        if (lane == 0) sh.wave64[wave] = v;
+        __syncthreads();
+        v = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) v += sh.wave64[w];
+        return v;
+    }
+
+    // the largest key of a part, in thread 0
+    __device__ __forceinline__ uint64_t largest(uint32_t span)
+    {
+        uint64_t most = 0;
+        each(span, [&](float v, uint32_t i) {
+            const uint64_t key = sample_key(v, i);
+            most = key > most ? key : most;
+        });
+        most = wave_most_u64(most);
+        __syncthreads();
+        if (lane == 0) sh.wave64[wave] = most;
+        __syncthreads();
+        if (tid == 0)
+            for (uint32_t w = 1; w < kWaves; w++) most = sh.wave64[w] > most ? sh.wave64[w] : most;
+        return most;
+    }
+
+    __device__ __forceinline__ void clear_bins()
+    {
+        for (uint32_t b = tid; b < kSampleBins; b += THREADS) {
+            sh.bins.mass[b] = 0;
+            sh.bins.count[b] = 0;
+        }
+        __syncthreads();
+    }
+
+    __device__ __forceinline__ void histogram(const SampleRules &r, uint32_t span)
+    {
+        each(span, [&](float v, uint32_t) {
+            double w;
+            const uint64_t whole = r.weight(v, w);
+            if (whole) {
+                const uint32_t b = r.bin(v);
+                atomicAdd(&sh.bins.count[b], 1u);
+                atomicAdd((unsigned long long *)&sh.bins.mass[b], (unsigned long long)whole);
+            }
+        });
+    }
+
+    // sh.cut from the whole row's histogram in sh.bins
+    __device__ __forceinline__ void find_cut(const SampleRules &r)
+    {
+        constexpr uint32_t kEach = kSampleBins / THREADS;
+        uint32_t count = 0;
+        uint64_t mass = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; j++) {
+            count += sh.bins.count[tid * kEach + j];
+            mass += sh.bins.mass[tid * kEach + j];
+        }
+        uint32_t run_count = count;
+        uint64_t run_mass = mass;
+#pragma unroll
+        for (int step = 1; step < 64; step <<= 1) {
+            const uint32_t c = __shfl_up(run_count, step);
+            const uint64_t m = __shfl_up(run_mass, step);
+            if (lane >= (uint32_t)step) {
+                run_count += c;
+                run_mass += m;
+            }
+        }
+        if (lane == 63u) {
+            sh.wave32[wave] = run_count;
+            sh.wave64[wave] = run_mass;
+        }
+        if (tid == 0) sh.cut = SampleCut{kNoBin, kNoBin, kNoBin, 0, 0, 0};
+        __syncthreads();
+        uint32_t all_count = 0;
+        uint64_t all_mass = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; w++) {
+            if (w == wave) {
+                run_count += all_count;
+                run_mass += all_mass;
+            }
+            all_count += sh.wave32[w];
+            all_mass += sh.wave64[w];
+        }
+        // f(bin, tokens before it, in it, weights before it, in it)
+        auto each_bin = [&](auto &&f) {
+            uint32_t c0 = run_count - count;
+            uint64_t m0 = run_mass - mass;
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; j++) {
+                const uint32_t b = tid * kEach + j, c = sh.bins.count[b];
+                const uint64_t m = sh.bins.mass[b];
+                if (c) f(b, c0, c, m0, m);
+                c0 += c;
+                m0 += m;
+            }
+        };
+        const bool by_k = r.top_k != 0 && r.top_k < all_count;
+        if (!by_k && tid == 0) sh.cut.mass_k = all_mass;
+        if (by_k)
+            each_bin([&](uint32_t b, uint32_t c0, uint32_t c, uint64_t m0, uint64_t m) {
+                if (c0 < r.top_k && c0 + c >= r.top_k) {
+                    sh.cut.k_bin = b;
+                    sh.cut.above_k = c0;
+                    sh.cut.mass_k = m0;
+                    sh.taken_mass = m0 + m;
+                }
+            });
+        __syncthreads();
+        if (r.top_p < 1.0) {
+            const double low = goal(r.top_p, sh.cut.mass_k), high = goal(r.top_p, by_k ? sh.taken_mass : all_mass);
+            each_bin([&](uint32_t b, uint32_t, uint32_t, uint64_t m0, uint64_t m) {
+                if ((double)m0 < low && (double)(m0 + m) >= low) {
+                    sh.cut.p_first = b;
+                    sh.cut.mass_p = m0;
+                }
+                if ((double)m0 < high && (double)(m0 + m) >= high) sh.cut.p_last = b;
+            });
+        }
+        __syncthreads();
+    }
+
+    // the sum before which a token has to begin to remain (the first one always does)
+    static __device__ __forceinline__ double goal(double top_p, uint64_t mass)
+    {
+        const double g = top_p * (double)mass;
+        return g > 0.5 ? g : 0.5;
+    }
+
+    // Adds the weights of a part that are in for certain, and lists the tokens of the bins that are not settled; sh.listed counts
+    // on past the end of a full list.
+    __device__ __forceinline__ uint64_t gather(const SampleRules &r, const SampleCut &cut, uint32_t span)
+    {
+        uint64_t sum = 0;
+        const uint32_t sure = cut.sure();
+        each(span, [&](float v, uint32_t i) {
+            const uint32_t b = r.bin(v);
+            if (b >= sure && !cut.listed(b)) return;
+            double w;
+            const uint64_t whole = r.weight(v, w);
+            if (whole == 0) return;
+            const bool above = w >= r.min_p;
+            if (b < sure) {
+                if (above) sum += whole;
+                return;
+            }
+            const uint32_t at = atomicAdd(&sh.listed, 1u);
+            if (at < kSampleList) {
+                sh.list.key[at] = sample_key(v, i);
+                sh.list.mass[at] = whole | (above ? 1ull << 63 : 0ull);
+            }
+        });
+        return sum;
+    }
+
+    // Settles the listed tokens: adds the weights of those that remain to sh.spans, their lowest key is sh.least (none: all ones).
+    // Each token is compared with each by 2^k neighbouring lanes, as many as there are threads for.
+    __device__ __forceinline__ void settle(const SampleRules &r, const SampleCut &cut, uint32_t n)
+    {
+        uint32_t lanes = 1;
+        while (lanes < 64u && n * lanes * 2u <= THREADS) lanes *= 2u;
+        const uint32_t part = tid & (lanes - 1u), step = THREADS / lanes;
+        auto bin_of = [&](uint64_t key) { return r.bin(sample_value((uint32_t)(key >> 32))); };
+        if (tid == 0) sh.least = ~0ull;
+        uint64_t in_k = 0;
+        for (uint32_t i0 = 0; i0 < n; i0 += step) {
+            const uint32_t i = i0 + tid / lanes;
+            const uint64_t key = sh.list.key[i < n ? i : 0u];
+            const uint32_t b = bin_of(key);
+            uint32_t before = 0;
+            if (b == cut.k_bin && i < n)
+                for (uint32_t j = part; j < n; j += lanes) before += sh.list.key[j] > key && bin_of(sh.list.key[j]) == b;
+            for (uint32_t k = 1; k < lanes; k *= 2u) before += __shfl_xor(before, (int)k);
+            if (i < n && part == 0) {
+                const bool in = b != cut.k_bin || before + cut.above_k < r.top_k;
+                if (in && b == cut.k_bin) in_k += sh.list.mass[i] & ~(1ull << 63);
+                sh.list.state[i] = in ? 3 : 0;
+            }
+        }
+        in_k = block_sum(in_k);   // (and the states are there)
+        if (cut.p_first != kNoBin) {
+            const double end = goal(r.top_p, cut.mass_k + in_k);
+            for (uint32_t i0 = 0; i0 < n; i0 += step) {
+                const uint32_t i = i0 + tid / lanes;
+                const uint64_t key = sh.list.key[i < n ? i : 0u];
+                const uint32_t b = bin_of(key);
+                uint64_t before = 0;
+                if (b <= cut.p_last && i < n)
+                    for (uint32_t j = part; j < n; j += lanes)
+                        before += sh.list.key[j] > key && (sh.list.state[j] & 1u) ? sh.list.mass[j] & ~(1ull << 63) : 0ull;
+                for (uint32_t k = 1; k < lanes; k *= 2u) before += __shfl_xor(before, (int)k);
+                // (bit 1: remains; bit 0 is still read)
+                if (i < n && part == 0 && (b > cut.p_last || !(sh.list.state[i] & 1u) || (double)(before + cut.mass_p) >= end)) sh.list.state[i] &= 1u;
+            }
+            __syncthreads();
+        }
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            if ((sh.list.state[i] & 2u) == 0) continue;
+            const uint64_t key = sh.list.key[i], mass = sh.list.mass[i];
+            atomicMin((unsigned long long *)&sh.least, (unsigned long long)key);
+            if (mass >> 63) atomicAdd((unsigned long long *)&sh.spans[(0xFFFFFFFFu - (uint32_t)key) / a.span], (unsigned long long)(mass & ~(1ull << 63)));
+        }
+        __syncthreads();
+    }
+
+    // The lowest key that remains, eight bits at a time over the whole row: of the first `want` keys (by_mass false) or of those
+    // before which less than `end` lies; keys below `least` do not take part.
+    __device__ uint64_t select(const SampleRules &r, bool by_mass, uint64_t want, double end, uint64_t least)
+    {
+        __syncthreads();
         if (tid == 0) {
             sh.prefix = 0;
             sh.taken_count = 0;
             sh.taken_mass = 0;
         }
         for (int shift = 56; shift >= 0; shift -= 8) {
-            if (tid < 256) {
-                sh.mass[tid] = 0;
-                sh.count[tid] = 0;
+            for (uint32_t b = tid; b < 256; b += THREADS) {
+                sh.bins.mass[b] = 0;
+                sh.bins.count[b] = 0;
             }
             __syncthreads();
             const uint64_t prefix = sh.prefix;
-            for (uint64_t i = tid; i < cols; i += kSampleThreads) {
-                const float v = x[i];
-                const uint64_t key = key_of(i, v);
-                if (key < least || (shift < 56 && (key >> (shift + 8)) != prefix)) continue;
-                double w;
-                const uint64_t whole = sample_weight(r, v, w);
-                if (whole == 0) continue;
-                atomicAdd(&sh.count[(key >> shift) & 255u], 1u);
-                atomicAdd((unsigned long long *)&sh.mass[(key >> shift) & 255u], (unsigned long long)whole);
-            }
+            for (uint32_t span = 0; span < a.spans; span++)
+                each(span, [&](float v, uint32_t i) {
+                    const uint64_t key = sample_key(v, i);
+                    if (key < least || (shift < 56 && (key >> (shift + 8)) != prefix)) return;
+                    double w;
+                    const uint64_t whole = r.weight(v, w);
+                    if (whole == 0) return;
+                    atomicAdd(&sh.bins.count[(key >> shift) & 255u], 1u);
+                    atomicAdd((unsigned long long *)&sh.bins.mass[(key >> shift) & 255u], (unsigned long long)whole);
+                });
             __syncthreads();
             if (tid == 0) {
                 uint32_t last = 256;
                 for (int b = 255; b >= 0; b--) {
-                    if (sh.count[b] == 0) continue;
+                    if (sh.bins.count[b] == 0) continue;
                     if (last < 256) {
                         // whether the order goes on into this bin
-                        const bool on = by_mass ? (double)(sh.taken_mass + sh.mass[last]) < goal : sh.taken_count + sh.count[last] < want;
+                        const bool on = by_mass ? (double)(sh.taken_mass + sh.bins.mass[last]) < end : sh.taken_count + sh.bins.count[last] < want;
                         if (!on) break;
-                        sh.taken_count += sh.count[last];
-                        sh.taken_mass += sh.mass[last];
+                        sh.taken_count += sh.bins.count[last];
+                        sh.taken_mass += sh.bins.mass[last];
                     }
                     last = (uint32_t)b;
                 }
                 sh.prefix = prefix << 8 | last;
                 // all of a bin's tokens are in, or it holds one: any key down to the bin's lowest will do
-                const bool whole_bin = by_mass ? sh.count[last] == 1 : sh.taken_count + sh.count[last] <= want;
-                sh.stop = whole_bin;
+                sh.stop = by_mass ? sh.bins.count[last] == 1 : sh.taken_count + sh.bins.count[last] <= want;
             }
             __syncthreads();
             if (sh.stop) {
@@ -159,62 +448,265 @@ __global__ __launch_bounds__(1024) void k_sample(const float *__restrict__ logit
         const uint64_t found = sh.prefix;
         __syncthreads();
         return found;
-    };
-
-    uint64_t least = 0;
-    if (r.top_k < cols) least = select(false, r.top_k, 0.0, 0);
-    if (r.top_p < 1.0 && !r.greedy) {
-        uint64_t sum = 0;
-        for (uint64_t i = tid; i < cols; i += kSampleThreads) {
-            const float v = x[i];
-            double w;
-            if (key_of(i, v) >= least) sum += sample_weight(r, v, w);
-        }
-        sum = block_sum_u64(sh, sum);
-        const uint64_t by_p = select(true, 0, r.top_p * (double)sum, least);
-        least = by_p > least ? by_p : least;
     }
 
-    // what remains of one logit
-    auto left = [&](uint64_t i) -> uint64_t {
-        if (i >= cols) return 0;
-        const float v = x[i];
-        if (key_of(i, v) < least) return 0;
-        double w;
-        const uint64_t whole = sample_weight(r, v, w);
-        return w >= r.min_p ? whole : 0;
-    };
-    uint64_t total = 0;
-    for (uint64_t i = tid; i < cols; i += kSampleThreads) total += left(i);
-    total = block_sum_u64(sh, total);
-    const double u = uniform[row];
-    // the first index at which the running sum is above `goal`: u times the whole, below the whole for any u
-    double goal_f = u > 0.0 ? u * (double)total : 0.0;
-    const uint64_t goal = goal_f >= (double)total ? total - 1u : (uint64_t)goal_f;
-    uint64_t before = 0;
-    for (uint64_t at = 0; at < cols; at += kSampleThreads) {
-        const uint64_t mine = left(at + tid);
-        uint64_t run = mine;   // sum up to and with this lane
+    // the weights that remain of the whole row, with the lowest key by select
+    __device__ void settle_long(const SampleRules &r)
+    {
+        uint64_t least = 0;
+        if (r.top_k) least = select(r, false, r.top_k, 0.0, 0);
+        if (r.top_p < 1.0) {
+            uint64_t sum = 0;
+            for (uint32_t span = 0; span < a.spans; span++)
+                each(span, [&](float v, uint32_t i) {
+                    double w;
+                    if (sample_key(v, i) >= least) sum += r.weight(v, w);
+                });
+            sum = block_sum(sum);
+            const uint64_t by_p = select(r, true, 0, goal(r.top_p, sum), least);
+            least = by_p > least ? by_p : least;
+        }
+        for (uint32_t span = 0; span < a.spans; span++) {
+            uint64_t sum = 0;
+            each(span, [&](float v, uint32_t i) {
+                double w;
+                if (sample_key(v, i) < least) return;
+                const uint64_t whole = r.weight(v, w);
+                if (w >= r.min_p) sum += whole;
+            });
+            sum = block_sum(sum);
+            if (tid == 0) sh.spans[span] = sum;
+        }
+        if (tid == 0) sh.least = least;
+        __syncthreads();
+    }
+
+    // The token, from the parts' sums in sh.spans; in(v, i): whether the limits leave a token
+    template <typename F> __device__ __forceinline__ void choose(const SampleRules &r, F &&in)
+    {
+        uint64_t total = 0;
+        for (uint32_t s = 0; s < a.spans; s++) total += sh.spans[s];
+        const double u = a.uniform[row];
+        // the first index at which the running sum is above u times the whole, below the whole for any u
+        const double g = u > 0.0 ? u * (double)total : 0.0;
+        const uint64_t end = g >= (double)total ? total - 1u : (uint64_t)g;
+        uint64_t before = 0;
+        uint32_t span = 0;
+        for (; span + 1 < a.spans && before + sh.spans[span] <= end; span++) before += sh.spans[span];
+        const uint64_t last = (uint64_t)(span + 1) * a.span < a.cols ? (uint64_t)(span + 1) * a.span : a.cols;
+        // four neighbouring columns a thread
+        for (uint64_t at = (uint64_t)span * a.span; at < last; at += 4u * THREADS) {
+            uint64_t mine[4], sum = 0;
 #pragma unroll
-        for (int step = 1; step < 64; step <<= 1) {
-            const uint64_t other = __shfl_up(run, step);
-            if ((tid & 63u) >= (uint32_t)step) run += other;
+            for (uint32_t j = 0; j < 4; j++) {
+                const uint64_t i = at + tid * 4u + j;
+                mine[j] = 0;
+                if (i < last) {
+                    const float v = x[i];
+                    if (in(v, (uint32_t)i)) {
+                        double w;
+                        const uint64_t whole = r.weight(v, w);
+                        mine[j] = w >= r.min_p ? whole : 0;
+                    }
+                }
+                sum += mine[j];
+            }
+            uint64_t run = sum;
+#pragma unroll
+            for (int step = 1; step < 64; step <<= 1) {
+                const uint64_t other = __shfl_up(run, step);
+                if (lane >= (uint32_t)step) run += other;
+            }
+            __syncthreads();
+            if (lane == 63u) sh.wave64[wave] = run;
+            __syncthreads();
+            uint64_t tile = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < kWaves; w++) {
+                if (w == wave) run += before + tile;
+                tile += sh.wave64[w];
+            }
+            run -= sum;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++) {
+                if (mine[j] && run <= end && run + mine[j] > end) a.out[row] = (int)(at + tid * 4u + j);
+                run += mine[j];
+            }
+            before += tile;
+            if (before > end) break;
         }
-        __syncthreads();
-        if ((tid & 63u) == 63u) sh.wave64[tid >> 6] = run;
-        __syncthreads();
-        uint64_t tile = 0;
-        for (uint32_t w = 0; w < kSampleThreads / 64; w++) {
-            if (w == (tid >> 6)) run += before + tile;
-            tile += sh.wave64[w];
+    }
+
+    // from sh.list (n tokens found) and sh.spans to the token
+    __device__ __forceinline__ void finish(const SampleRules &r, const SampleCut &cut, uint32_t n)
+    {
+        if (n > kSampleList) {
+            settle_long(r);
+            const uint64_t least = sh.least;
+            choose(r, [=](float v, uint32_t i) { return sample_key(v, i) >= least; });
+            return;
         }
-        if (mine && run > goal && run - mine <= goal) out[row] = (int)(at + tid);
-        before += tile;
-        if (before > goal) break;
+        settle(r, cut, n);
+        const uint64_t least = sh.least;
+        const uint32_t sure = cut.sure();
+        choose(r, [=](float v, uint32_t i) { return r.bin(v) < sure || sample_key(v, i) >= least; });
+    }
+};
+
+// whether a row's largest key is of a token that can be chosen
+__device__ __forceinline__ bool sample_any(uint64_t key) { return (uint32_t)(key >> 32) > sample_order(-INFINITY); }
+__device__ __forceinline__ int sample_index(uint64_t key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
+
+}  // namespace
+
+// A workgroup per row
+__global__ __launch_bounds__(1024) void k_sample(const SampleArgs a)
+{
+    __shared__ SampleShared sh;
+    Sampler<1024> s(a, sh, blockIdx.x);
+    if (s.tid == 0) sh.largest = 0;
+    for (uint32_t span = 0; span < a.spans; span++) {
+        const uint64_t key = s.largest(span);
+        if (s.tid == 0 && key > sh.largest) sh.largest = key;
+    }
+    __syncthreads();
+    const uint64_t key = sh.largest;
+    const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
+    if (!sample_any(key) || r.greedy) {
+        if (s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
+        return;
+    }
+    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
+    if (r.limited()) {
+        s.clear_bins();
+        for (uint32_t span = 0; span < a.spans; span++) s.histogram(r, span);
+        __syncthreads();
+        s.find_cut(r);
+        cut = sh.cut;
+    }
+    if (s.tid == 0) sh.listed = 0;
+    __syncthreads();
+    for (uint32_t span = 0; span < a.spans; span++) {
+        const uint64_t sum = s.block_sum(s.gather(r, cut, span));
+        if (s.tid == 0) sh.spans[span] = sum;
+    }
+    __syncthreads();
+    s.finish(r, cut, sh.listed);
+}
+
+// ---- few rows: a workgroup per part of a row ------------------------------------------------------------------------------
+
+namespace {
+
+template <typename V> __device__ __forceinline__ void leave(V *to, V v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ V left(const V *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Whether this workgroup is the row's last to arrive, what all of them left being in memory then; the counter is zero again after
+__device__ __forceinline__ bool last_to_arrive(SampleShared &sh, unsigned *counter, uint32_t spans)
+{
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == spans - 1u;
+        if (last) leave(counter, 0u);
+        sh.stop = last;
+    }
+    __syncthreads();
+    return sh.stop != 0;
+}
+
+// the row's largest key, from its parts' (of the launch before)
+__device__ __forceinline__ uint64_t row_key(const SampleRow &state, uint32_t spans)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    return wave_most_u64(lane < spans ? state.key[lane] : 0);
+}
+
+}  // namespace
+
+__global__ __launch_bounds__(1024) void k_sample_largest(const SampleArgs a, SampleRow *__restrict__ rows)
+{
+    __shared__ SampleShared sh;
+    Sampler<1024> s(a, sh, blockIdx.y);
+    SampleRow &state = rows[blockIdx.y];
+    for (uint32_t b = blockIdx.x * 1024u + s.tid; b < kSampleBins; b += a.spans * 1024u) {
+        state.bin_mass[b] = 0;
+        state.bin_count[b] = 0;
+    }
+    const uint64_t key = s.largest(blockIdx.x);
+    if (s.tid == 0) {
+        state.key[blockIdx.x] = key;
+        if (blockIdx.x == 0) state.listed = 0;
     }
 }
 
-// 2^S: the largest power of two whose product with `cols` stays below 2^63 (and is a double's 52 bits at most)
+__global__ __launch_bounds__(1024) void k_sample_limits(const SampleArgs a, SampleRow *__restrict__ rows, unsigned *__restrict__ counters)
+{
+    __shared__ SampleShared sh;
+    Sampler<1024> s(a, sh, blockIdx.y);
+    SampleRow &state = rows[blockIdx.y];
+    const uint64_t key = row_key(state, a.spans);
+    const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
+    if (!sample_any(key) || r.greedy || !r.limited()) return;
+    s.clear_bins();
+    s.histogram(r, blockIdx.x);
+    __syncthreads();
+    for (uint32_t b = s.tid; b < kSampleBins; b += 1024u) {
+        if (sh.bins.count[b] == 0) continue;
+        __hip_atomic_fetch_add(&state.bin_count[b], sh.bins.count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_fetch_add(&state.bin_mass[b], sh.bins.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep], a.spans)) return;
+    for (uint32_t b = s.tid; b < kSampleBins; b += 1024u) {
+        sh.bins.count[b] = left(&state.bin_count[b]);
+        sh.bins.mass[b] = left(&state.bin_mass[b]);
+    }
+    __syncthreads();
+    s.find_cut(r);
+    if (s.tid == 0) state.cut = sh.cut;
+}
+
+__global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, SampleRow *__restrict__ rows, unsigned *__restrict__ counters)
+{
+    __shared__ SampleShared sh;
+    Sampler<1024> s(a, sh, blockIdx.y);
+    SampleRow &state = rows[blockIdx.y];
+    const uint64_t key = row_key(state, a.spans);
+    const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
+    if (!sample_any(key) || r.greedy) {
+        if (blockIdx.x == 0 && s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
+        return;
+    }
+    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
+    if (r.limited()) cut = state.cut;
+    if (s.tid == 0) sh.listed = 0;
+    __syncthreads();
+    const uint64_t sum = s.block_sum(s.gather(r, cut, blockIdx.x));
+    const uint32_t mine = sh.listed, there = mine < kSampleList ? mine : kSampleList;
+    if (s.tid == 0) {
+        leave(&state.mass[blockIdx.x], sum);
+        sh.base = mine ? __hip_atomic_fetch_add(&state.listed, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
+    }
+    __syncthreads();
+    for (uint32_t i = s.tid; i < there; i += 1024u) {
+        const uint32_t at = sh.base + i;
+        if (at < kSampleList) {
+            leave(&state.list_key[at], sh.list.key[i]);
+            leave(&state.list_mass[at], sh.list.mass[i]);
+        }
+    }
+    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep], a.spans)) return;
+    const uint32_t n = left(&state.listed);
+    for (uint32_t i = s.tid; i < n && i < kSampleList; i += 1024u) {
+        sh.list.key[i] = left(&state.list_key[i]);
+        sh.list.mass[i] = left(&state.list_mass[i]);
+    }
+    if (s.tid < a.spans) sh.spans[s.tid] = left(&state.mass[s.tid]);
+    __syncthreads();
+    s.finish(r, cut, n);
+}
+
+// 2^S: the largest power of two whose product with `cols` stays below 2^63 (and within a double's 53 bits)
 static double sample_scale(uint32_t cols)
 {
     int bits = 0;
@@ -224,10 +716,29 @@ static double sample_scale(uint32_t cols)
 }
 
 hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint32_t cols, const float *uniform, const float *temperature,
-                         const int *top_k, const float *top_p, const float *min_p, int *out)
+                         const int *top_k, const float *top_p, const float *min_p, int *out, void *scratch, size_t scratch_bytes,
+                         unsigned *counters, uint32_t n_counters)
 {
     if (rows == 0) return hipSuccess;
-    hipLaunchKernelGGL(k_sample, dim3(rows), dim3(kSampleThreads), 0, s, logits, cols, uniform, temperature, top_k, top_p, min_p, sample_scale(cols), out);
+    SampleArgs a = {logits, uniform, temperature, top_p, min_p, top_k, out, cols, 1, 4096, sample_scale(cols)};
+    // parts of 4096 columns, longer ones where there would be too many
+    auto spans_of_at_least = [&](uint32_t least) {
+        const uint32_t each = (uint32_t)(((uint64_t)cols + kSampleSpans - 1) / kSampleSpans);
+        a.span = each < least ? least : (each + 4095u) / 4096u * 4096u;
+        a.spans = cols ? (cols + a.span - 1) / a.span : 1u;
+    };
+    spans_of_at_least(4096u);
+    if (rows <= kSampleFewRows && a.spans > 1 && scratch && counters && (uint64_t)rows * kSampleCounterStep <= n_counters &&
+        (uint64_t)rows * sizeof(SampleRow) <= scratch_bytes) {
+        // about a thousand workgroups of all rows' parts
+        while (rows * a.spans > 1024u && a.spans > 1) spans_of_at_least(a.span * 2u);
+        SampleRow *state = (SampleRow *)scratch;
+        hipLaunchKernelGGL(k_sample_largest, dim3(a.spans, rows), dim3(1024), 0, s, a, state);
+        if (top_k || top_p) hipLaunchKernelGGL(k_sample_limits, dim3(a.spans, rows), dim3(1024), 0, s, a, state, counters);
+        hipLaunchKernelGGL(k_sample_token, dim3(a.spans, rows), dim3(1024), 0, s, a, state, counters);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(k_sample, dim3(rows), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 
