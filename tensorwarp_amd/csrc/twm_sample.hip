@@ -54,7 +54,7 @@ struct SampleArgs {
 
 struct SampleRules {
     float largest, per_bin, per_one;   // per_bin = 64 / temperature, per_one = 1 / temperature, in 32 bits
-    double temperature, top_p, min_p, scale;
+    double temperature, top_p, min_p, scale, uniform;
     uint64_t top_k;   // 0: no limit
     bool greedy;
 
@@ -92,6 +92,7 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, uint32_
     r.min_p = m < 1.0f ? (double)m : m != m ? 0.0 : 1.0;
     r.top_k = k > 0 && (uint32_t)k < a.cols ? (uint64_t)k : 0u;
     r.scale = a.scale;
+    r.uniform = a.uniform[row];
     return r;
 }
 
@@ -118,39 +119,71 @@ struct SampleRow {
 };
 
 struct SampleShared {
-    union {
-        struct {
-            uint64_t mass[kSampleBins];
-            uint32_t count[kSampleBins];
-        } bins;
-        struct {
-            uint64_t key[kSampleList];
-            uint64_t mass[kSampleList];   // bit 63: the token is above min_p
-            uint8_t state[kSampleList];   // bit 0: among the first top_k; bit 1: remains
-        } list;
-    };
+    struct {
+        uint64_t mass[kSampleBins];
+        uint32_t count[kSampleBins];
+    } bins;
+    struct {
+        uint64_t key[kSampleList];
+        uint64_t mass[kSampleList];   // bit 63: the token is above min_p
+    } list;
+    uint64_t few_key[64], few_mass[64];
     uint64_t spans[kSampleSpans];
     uint64_t wave64[16];
     uint32_t wave32[16];
     SampleCut cut;
-    uint64_t largest, prefix, taken_mass, least;
+    uint64_t largest, prefix, taken_mass, least, low, high;
     uint32_t listed, taken_count, stop, base;
 };
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v)
+// the sums up to and with each lane (DPP: shifts within sixteen lanes, then their last lane to the lanes behind)
+__device__ __forceinline__ uint64_t wave_running(uint64_t v)
 {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) v += __shfl_xor(v, step);
+#define TWM_SCAN_STEP(CTRL, ROWS) \
+    v += (uint64_t)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false) << 32 | \
+         (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)
+    TWM_SCAN_STEP(0x111, 0xf);   // row_shr:1
+    TWM_SCAN_STEP(0x112, 0xf);
+    TWM_SCAN_STEP(0x114, 0xf);
+    TWM_SCAN_STEP(0x118, 0xf);
+    TWM_SCAN_STEP(0x142, 0xa);   // row_bcast:15 into the second and fourth sixteen
+    TWM_SCAN_STEP(0x143, 0xc);   // row_bcast:31 into the upper half
+#undef TWM_SCAN_STEP
     return v;
+}
+__device__ __forceinline__ uint32_t wave_running(uint32_t v)
+{
+#define TWM_SCAN_STEP(CTRL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)
+    TWM_SCAN_STEP(0x111, 0xf);
+    TWM_SCAN_STEP(0x112, 0xf);
+    TWM_SCAN_STEP(0x114, 0xf);
+    TWM_SCAN_STEP(0x118, 0xf);
+    TWM_SCAN_STEP(0x142, 0xa);
+    TWM_SCAN_STEP(0x143, 0xc);
+#undef TWM_SCAN_STEP
+    return v;
+}
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane)
+{
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane_value(wave_running(v), 63); }
+__device__ __forceinline__ uint32_t wave_most_u32(uint32_t v)
+{
+#define TWM_MAX_STEP(N) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + N, 0xf, 0xf, true))   // row_ror:N
+    TWM_MAX_STEP(8);
+    TWM_MAX_STEP(4);
+    TWM_MAX_STEP(2);
+    TWM_MAX_STEP(1);
+#undef TWM_MAX_STEP
+    const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+    const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+    return max(max(a, b), max(c, d));
 }
 __device__ __forceinline__ uint64_t wave_most_u64(uint64_t v)
 {
-#pragma unroll
-    for (int step = 32; step; step >>= 1) {
-        const uint64_t other = __shfl_xor(v, step);
-        v = other > v ? other : v;
-    }
-    return v;
+    const uint32_t high = wave_most_u32((uint32_t)(v >> 32));
+    return (uint64_t)high << 32 | wave_most_u32((uint32_t)(v >> 32) == high ? (uint32_t)v : 0u);
 }
 
 template <uint32_t THREADS> struct Sampler {
@@ -165,11 +198,11 @@ template <uint32_t THREADS> struct Sampler {
     {
     }
 
-    // f(v, i) for the columns of one part of the row
-    template <typename F> __device__ __forceinline__ void each(uint32_t span, F &&f) const
+    // f(v, i) for the columns of parts first .. last of the row
+    template <typename F> __device__ __forceinline__ void each(uint32_t first, uint32_t last, F &&f) const
     {
-        const uint64_t end = (uint64_t)(span + 1) * a.span < a.cols ? (uint64_t)(span + 1) * a.span : a.cols;
-        for (uint64_t i0 = (uint64_t)span * a.span + tid; i0 < end; i0 += kSampleBatch * THREADS) {
+        const uint64_t end = (uint64_t)(last + 1) * a.span < a.cols ? (uint64_t)(last + 1) * a.span : a.cols;
+        for (uint64_t i0 = (uint64_t)first * a.span + tid; i0 < end; i0 += kSampleBatch * THREADS) {
             float v[kSampleBatch];
 #pragma unroll
             for (uint32_t j = 0; j < kSampleBatch; j++) {
@@ -194,19 +227,19 @@ template <uint32_t THREADS> struct Sampler {
         return v;
     }
 
-    // the largest key of a part, in thread 0
-    __device__ __forceinline__ uint64_t largest(uint32_t span)
+    // the largest key of parts first .. last, in thread 0
+    __device__ __forceinline__ uint64_t largest(uint32_t first, uint32_t last)
     {
         uint64_t most = 0;
-        each(span, [&](float v, uint32_t i) {
+        each(first, last, [&](float v, uint32_t i) {
             const uint64_t key = sample_key(v, i);
             most = key > most ? key : most;
         });
         most = wave_most_u64(most);
-        __syncthreads();
         if (lane == 0) sh.wave64[wave] = most;
         __syncthreads();
         if (tid == 0)
+#pragma unroll
             for (uint32_t w = 1; w < kWaves; w++) most = sh.wave64[w] > most ? sh.wave64[w] : most;
         return most;
     }
@@ -220,9 +253,9 @@ template <uint32_t THREADS> struct Sampler {
         __syncthreads();
     }
 
-    __device__ __forceinline__ void histogram(const SampleRules &r, uint32_t span)
+    __device__ __forceinline__ void histogram(const SampleRules &r, uint32_t first, uint32_t last)
     {
-        each(span, [&](float v, uint32_t) {
+        each(first, last, [&](float v, uint32_t) {
             double w;
             const uint64_t whole = r.weight(v, w);
             if (whole) {
@@ -233,10 +266,14 @@ template <uint32_t THREADS> struct Sampler {
         });
     }
 
-    // sh.cut from the whole row's histogram in sh.bins
-    __device__ __forceinline__ void find_cut(const SampleRules &r)
+    // f(bin, tokens before it, in it, weights before it, in it) for the bins with tokens, and the sums over all
+    struct Running {
+        uint32_t count, all_count;
+        uint64_t mass, all_mass;   // count, mass: before this thread's bins
+    };
+    static constexpr uint32_t kEach = kSampleBins / THREADS;
+    __device__ __forceinline__ Running running()
     {
-        constexpr uint32_t kEach = kSampleBins / THREADS;
         uint32_t count = 0;
         uint64_t mass = 0;
 #pragma unroll
@@ -244,51 +281,48 @@ template <uint32_t THREADS> struct Sampler {
             count += sh.bins.count[tid * kEach + j];
             mass += sh.bins.mass[tid * kEach + j];
         }
-        uint32_t run_count = count;
-        uint64_t run_mass = mass;
-#pragma unroll
-        for (int step = 1; step < 64; step <<= 1) {
-            const uint32_t c = __shfl_up(run_count, step);
-            const uint64_t m = __shfl_up(run_mass, step);
-            if (lane >= (uint32_t)step) {
-                run_count += c;
-                run_mass += m;
-            }
-        }
+        const uint32_t run_count = wave_running(count);
+        const uint64_t run_mass = wave_running(mass);
         if (lane == 63u) {
             sh.wave32[wave] = run_count;
             sh.wave64[wave] = run_mass;
         }
-        if (tid == 0) sh.cut = SampleCut{kNoBin, kNoBin, kNoBin, 0, 0, 0};
         __syncthreads();
-        uint32_t all_count = 0;
-        uint64_t all_mass = 0;
+        Running all = {run_count - count, 0, run_mass - mass, 0};
 #pragma unroll
         for (uint32_t w = 0; w < kWaves; w++) {
             if (w == wave) {
-                run_count += all_count;
-                run_mass += all_mass;
+                all.count += all.all_count;
+                all.mass += all.all_mass;
             }
-            all_count += sh.wave32[w];
-            all_mass += sh.wave64[w];
+            all.all_count += sh.wave32[w];
+            all.all_mass += sh.wave64[w];
         }
-        // f(bin, tokens before it, in it, weights before it, in it)
-        auto each_bin = [&](auto &&f) {
-            uint32_t c0 = run_count - count;
-            uint64_t m0 = run_mass - mass;
+        return all;
+    }
+    template <typename F> __device__ __forceinline__ void each_bin(const Running &all, F &&f)
+    {
+        uint32_t c0 = all.count;
+        uint64_t m0 = all.mass;
 #pragma unroll
-            for (uint32_t j = 0; j < kEach; j++) {
-                const uint32_t b = tid * kEach + j, c = sh.bins.count[b];
-                const uint64_t m = sh.bins.mass[b];
-                if (c) f(b, c0, c, m0, m);
-                c0 += c;
-                m0 += m;
-            }
-        };
-        const bool by_k = r.top_k != 0 && r.top_k < all_count;
-        if (!by_k && tid == 0) sh.cut.mass_k = all_mass;
+        for (uint32_t j = 0; j < kEach; j++) {
+            const uint32_t b = tid * kEach + j, c = sh.bins.count[b];
+            const uint64_t m = sh.bins.mass[b];
+            if (c) f(b, c0, c, m0, m);
+            c0 += c;
+            m0 += m;
+        }
+    }
+
+    // sh.cut from the whole row's histogram in sh.bins
+    __device__ __forceinline__ void find_cut(const SampleRules &r)
+    {
+        if (tid == 0) sh.cut = SampleCut{kNoBin, kNoBin, kNoBin, 0, 0, 0};
+        const Running all = running();
+        const bool by_k = r.top_k != 0 && r.top_k < all.all_count;
+        if (!by_k && tid == 0) sh.cut.mass_k = all.all_mass;
         if (by_k)
-            each_bin([&](uint32_t b, uint32_t c0, uint32_t c, uint64_t m0, uint64_t m) {
+            each_bin(all, [&](uint32_t b, uint32_t c0, uint32_t c, uint64_t m0, uint64_t m) {
                 if (c0 < r.top_k && c0 + c >= r.top_k) {
                     sh.cut.k_bin = b;
                     sh.cut.above_k = c0;
@@ -298,8 +332,8 @@ template <uint32_t THREADS> struct Sampler {
             });
         __syncthreads();
         if (r.top_p < 1.0) {
-            const double low = goal(r.top_p, sh.cut.mass_k), high = goal(r.top_p, by_k ? sh.taken_mass : all_mass);
-            each_bin([&](uint32_t b, uint32_t, uint32_t, uint64_t m0, uint64_t m) {
+            const double low = goal(r.top_p, sh.cut.mass_k), high = goal(r.top_p, by_k ? sh.taken_mass : all.all_mass);
+            each_bin(all, [&](uint32_t b, uint32_t, uint32_t, uint64_t m0, uint64_t m) {
                 if ((double)m0 < low && (double)(m0 + m) >= low) {
                     sh.cut.p_first = b;
                     sh.cut.mass_p = m0;
@@ -317,80 +351,143 @@ template <uint32_t THREADS> struct Sampler {
         return g > 0.5 ? g : 0.5;
     }
 
-    // Adds the weights of a part that are in for certain, and lists the tokens of the bins that are not settled; sh.listed counts
-    // on past the end of a full list.
-    __device__ __forceinline__ uint64_t gather(const SampleRules &r, const SampleCut &cut, uint32_t span)
+    // Adds the weights of parts first .. last that are in for certain to sh.spans, and lists the tokens of the bins that are not
+    // settled; sh.listed counts on past the end of a full list.  (Both are clear and the workgroup has seen that.)
+    __device__ __forceinline__ void gather(const SampleRules &r, const SampleCut &cut, uint32_t first, uint32_t last)
     {
-        uint64_t sum = 0;
         const uint32_t sure = cut.sure();
-        each(span, [&](float v, uint32_t i) {
-            const uint32_t b = r.bin(v);
-            if (b >= sure && !cut.listed(b)) return;
-            double w;
-            const uint64_t whole = r.weight(v, w);
-            if (whole == 0) return;
-            const bool above = w >= r.min_p;
-            if (b < sure) {
-                if (above) sum += whole;
-                return;
-            }
-            const uint32_t at = atomicAdd(&sh.listed, 1u);
-            if (at < kSampleList) {
-                sh.list.key[at] = sample_key(v, i);
-                sh.list.mass[at] = whole | (above ? 1ull << 63 : 0ull);
-            }
-        });
-        return sum;
+        for (uint32_t span = first; span <= last; span++) {
+            uint64_t sum = 0;
+            each(span, span, [&](float v, uint32_t i) {
+                const uint32_t b = r.bin(v);
+                if (b >= sure && !cut.listed(b)) return;
+                double w;
+                const uint64_t whole = r.weight(v, w);
+                if (whole == 0) return;
+                const bool above = w >= r.min_p;
+                if (b < sure) {
+                    if (above) sum += whole;
+                    return;
+                }
+                const uint32_t at = atomicAdd(&sh.listed, 1u);
+                if (at < kSampleList) {
+                    sh.list.key[at] = sample_key(v, i);
+                    sh.list.mass[at] = whole | (above ? 1ull << 63 : 0ull);
+                }
+            });
+            sum = wave_sum_u64(sum);
+            if (lane == 0 && sum) atomicAdd((unsigned long long *)&sh.spans[span], (unsigned long long)sum);
+        }
     }
 
-    // Settles the listed tokens: adds the weights of those that remain to sh.spans, their lowest key is sh.least (none: all ones).
-    // Each token is compared with each by 2^k neighbouring lanes, as many as there are threads for.
-    __device__ __forceinline__ void settle(const SampleRules &r, const SampleCut &cut, uint32_t n)
+    // Of the listed tokens with keys of at least `least` in bins first .. last, the lowest key that remains: of the first `want` in the
+    // row (by_mass false) or of those before which less than `end` lies, `count` tokens and `mass` weights being before them all.
+    // The range of their keys is cut into 2048 parts, and the part in which the end falls again, until it holds no more tokens than a
+    // wave has lanes (once, but for equal logits); those are compared with each other.
+    __device__ __forceinline__ uint64_t narrow(const SampleRules &r, uint32_t n, uint32_t first, uint32_t last, uint64_t least, bool by_mass, uint64_t want,
+                                               double end, uint64_t count, uint64_t mass)
     {
-        uint32_t lanes = 1;
-        while (lanes < 64u && n * lanes * 2u <= THREADS) lanes *= 2u;
-        const uint32_t part = tid & (lanes - 1u), step = THREADS / lanes;
         auto bin_of = [&](uint64_t key) { return r.bin(sample_value((uint32_t)(key >> 32))); };
-        if (tid == 0) sh.least = ~0ull;
-        uint64_t in_k = 0;
-        for (uint32_t i0 = 0; i0 < n; i0 += step) {
-            const uint32_t i = i0 + tid / lanes;
-            const uint64_t key = sh.list.key[i < n ? i : 0u];
-            const uint32_t b = bin_of(key);
-            uint32_t before = 0;
-            if (b == cut.k_bin && i < n)
-                for (uint32_t j = part; j < n; j += lanes) before += sh.list.key[j] > key && bin_of(sh.list.key[j]) == b;
-            for (uint32_t k = 1; k < lanes; k *= 2u) before += __shfl_xor(before, (int)k);
-            if (i < n && part == 0) {
-                const bool in = b != cut.k_bin || before + cut.above_k < r.top_k;
-                if (in && b == cut.k_bin) in_k += sh.list.mass[i] & ~(1ull << 63);
-                sh.list.state[i] = in ? 3 : 0;
-            }
+        if (tid == 0) {
+            sh.low = ~0ull;
+            sh.high = 0;
         }
-        in_k = block_sum(in_k);   // (and the states are there)
-        if (cut.p_first != kNoBin) {
-            const double end = goal(r.top_p, cut.mass_k + in_k);
-            for (uint32_t i0 = 0; i0 < n; i0 += step) {
-                const uint32_t i = i0 + tid / lanes;
-                const uint64_t key = sh.list.key[i < n ? i : 0u];
-                const uint32_t b = bin_of(key);
-                uint64_t before = 0;
-                if (b <= cut.p_last && i < n)
-                    for (uint32_t j = part; j < n; j += lanes)
-                        before += sh.list.key[j] > key && (sh.list.state[j] & 1u) ? sh.list.mass[j] & ~(1ull << 63) : 0ull;
-                for (uint32_t k = 1; k < lanes; k *= 2u) before += __shfl_xor(before, (int)k);
-                // (bit 1: remains; bit 0 is still read)
-                if (i < n && part == 0 && (b > cut.p_last || !(sh.list.state[i] & 1u) || (double)(before + cut.mass_p) >= end)) sh.list.state[i] &= 1u;
+        __syncthreads();
+        uint64_t low = ~0ull, high = 0;
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const uint64_t key = sh.list.key[i];
+            const uint32_t b = bin_of(key);
+            if (key < least || b < first || b > last) continue;
+            low = key < low ? key : low;
+            high = key > high ? key : high;
+        }
+        low = ~wave_most_u64(~low);
+        high = wave_most_u64(high);
+        if (lane == 0 && high) {
+            atomicMin((unsigned long long *)&sh.low, (unsigned long long)low);
+            atomicMax((unsigned long long *)&sh.high, (unsigned long long)high);
+        }
+        __syncthreads();
+        low = sh.low;
+        high = sh.high;
+        uint32_t held = n;
+        while (low < high && held > 64u) {
+            const int bits = 64 - __clzll((long long)(high - low)), shift = bits > 11 ? bits - 11 : 0;
+            clear_bins();
+            for (uint32_t i = tid; i < n; i += THREADS) {
+                const uint64_t key = sh.list.key[i];
+                if (key < low || key > high) continue;   // (between them every listed key is one of the bins first .. last)
+                const uint32_t b = (uint32_t)((high - key) >> shift);
+                atomicAdd(&sh.bins.count[b], 1u);
+                atomicAdd((unsigned long long *)&sh.bins.mass[b], (unsigned long long)(sh.list.mass[i] & ~(1ull << 63)));
+            }
+            if (tid == 0) sh.stop = 0;   // (nothing ends here: every one of them remains)
+            __syncthreads();
+            each_bin(running(), [&](uint32_t b, uint32_t c0, uint32_t c, uint64_t m0, uint64_t m) {
+                const bool here = by_mass ? (double)(mass + m0) < end && (double)(mass + m0 + m) >= end : count + c0 < want && count + c0 + c >= want;
+                if (!here) return;
+                const uint64_t top = high - ((uint64_t)b << shift), part = (1ull << shift) - 1u;
+                sh.high = top;
+                sh.low = top - low > part ? top - part : low;
+                sh.taken_count = (uint32_t)(count + c0);
+                sh.taken_mass = mass + m0;
+                sh.stop = c;
+            });
+            __syncthreads();
+            held = sh.stop;
+            if (held) {
+                low = sh.low;
+                high = sh.high;
+                count = sh.taken_count;
+                mass = sh.taken_mass;
             }
             __syncthreads();
         }
+        if (low >= high || held == 0) return low;
+        if (tid == 0) sh.taken_count = 0;
+        __syncthreads();
         for (uint32_t i = tid; i < n; i += THREADS) {
-            if ((sh.list.state[i] & 2u) == 0) continue;
-            const uint64_t key = sh.list.key[i], mass = sh.list.mass[i];
-            atomicMin((unsigned long long *)&sh.least, (unsigned long long)key);
-            if (mass >> 63) atomicAdd((unsigned long long *)&sh.spans[(0xFFFFFFFFu - (uint32_t)key) / a.span], (unsigned long long)(mass & ~(1ull << 63)));
+            const uint64_t key = sh.list.key[i];
+            if (key < low || key > high) continue;
+            const uint32_t at = atomicAdd(&sh.taken_count, 1u);
+            sh.few_key[at] = key;
+            sh.few_mass[at] = sh.list.mass[i] & ~(1ull << 63);
         }
         __syncthreads();
+        const uint64_t key = lane < held ? sh.few_key[lane] : 0ull;
+        held = sh.taken_count;   // (at most the 64 there is room for)
+        for (uint32_t j = 0; j < held; j++) {
+            const bool before = sh.few_key[j] > key;
+            count += before;
+            mass += before ? sh.few_mass[j] : 0ull;
+        }
+        const bool in = lane < held && (by_mass ? (double)mass < end : count < want);
+        return ~wave_most_u64(in ? ~key : 0ull);
+    }
+
+    // Settles the listed tokens: adds the weights of those that remain to sh.spans, returns their lowest key (none: all ones)
+    __device__ __forceinline__ uint64_t settle(const SampleRules &r, const SampleCut &cut, uint32_t n)
+    {
+        uint64_t least = 0;
+        if (n == 0) return ~0ull;
+        if (cut.k_bin != kNoBin) least = narrow(r, n, cut.k_bin, cut.k_bin, 0, false, r.top_k, 0.0, cut.above_k, cut.mass_k);
+        if (cut.p_first != kNoBin) {
+            uint64_t in_k = 0;
+            if (cut.k_bin != kNoBin)
+                for (uint32_t i = tid; i < n; i += THREADS) {
+                    const uint64_t key = sh.list.key[i];
+                    if (key >= least && r.bin(sample_value((uint32_t)(key >> 32))) == cut.k_bin) in_k += sh.list.mass[i] & ~(1ull << 63);
+                }
+            in_k = block_sum(in_k);
+            const uint64_t by_p = narrow(r, n, cut.p_first, cut.p_last, least, true, 0, goal(r.top_p, cut.mass_k + in_k), 0, cut.mass_p);
+            least = by_p > least ? by_p : least;
+        }
+        for (uint32_t i = tid; i < n; i += THREADS) {
+            const uint64_t key = sh.list.key[i], mass = sh.list.mass[i];
+            if (key >= least && mass >> 63) atomicAdd((unsigned long long *)&sh.spans[(0xFFFFFFFFu - (uint32_t)key) / a.span], (unsigned long long)(mass & ~(1ull << 63)));
+        }
+        __syncthreads();
+        return least;
     }
 
     // The lowest key that remains, eight bits at a time over the whole row: of the first `want` keys (by_mass false) or of those
@@ -410,8 +507,7 @@ template <uint32_t THREADS> struct Sampler {
             }
             __syncthreads();
             const uint64_t prefix = sh.prefix;
-            for (uint32_t span = 0; span < a.spans; span++)
-                each(span, [&](float v, uint32_t i) {
+            each(0, a.spans - 1u, [&](float v, uint32_t i) {
                     const uint64_t key = sample_key(v, i);
                     if (key < least || (shift < 56 && (key >> (shift + 8)) != prefix)) return;
                     double w;
@@ -457,8 +553,7 @@ template <uint32_t THREADS> struct Sampler {
         if (r.top_k) least = select(r, false, r.top_k, 0.0, 0);
         if (r.top_p < 1.0) {
             uint64_t sum = 0;
-            for (uint32_t span = 0; span < a.spans; span++)
-                each(span, [&](float v, uint32_t i) {
+            each(0, a.spans - 1u, [&](float v, uint32_t i) {
                     double w;
                     if (sample_key(v, i) >= least) sum += r.weight(v, w);
                 });
@@ -468,7 +563,7 @@ template <uint32_t THREADS> struct Sampler {
         }
         for (uint32_t span = 0; span < a.spans; span++) {
             uint64_t sum = 0;
-            each(span, [&](float v, uint32_t i) {
+            each(span, span, [&](float v, uint32_t i) {
                 double w;
                 if (sample_key(v, i) < least) return;
                 const uint64_t whole = r.weight(v, w);
@@ -484,15 +579,14 @@ template <uint32_t THREADS> struct Sampler {
     // The token, from the parts' sums in sh.spans; in(v, i): whether the limits leave a token
     template <typename F> __device__ __forceinline__ void choose(const SampleRules &r, F &&in)
     {
-        uint64_t total = 0;
-        for (uint32_t s = 0; s < a.spans; s++) total += sh.spans[s];
-        const double u = a.uniform[row];
+        // (a lane per part)
+        const uint64_t part = lane < a.spans ? sh.spans[lane] : 0, parts = wave_running(part), total = lane_value(parts, 63);
+        const double u = r.uniform;
         // the first index at which the running sum is above u times the whole, below the whole for any u
         const double g = u > 0.0 ? u * (double)total : 0.0;
         const uint64_t end = g >= (double)total ? total - 1u : (uint64_t)g;
-        uint64_t before = 0;
-        uint32_t span = 0;
-        for (; span + 1 < a.spans && before + sh.spans[span] <= end; span++) before += sh.spans[span];
+        const uint32_t span = (uint32_t)__builtin_ctzll(__ballot(parts > end));
+        uint64_t before = lane_value(parts - part, (int)span);
         const uint64_t last = (uint64_t)(span + 1) * a.span < a.cols ? (uint64_t)(span + 1) * a.span : a.cols;
         // four neighbouring columns a thread
         for (uint64_t at = (uint64_t)span * a.span; at < last; at += 4u * THREADS) {
@@ -511,12 +605,7 @@ template <uint32_t THREADS> struct Sampler {
                 }
                 sum += mine[j];
             }
-            uint64_t run = sum;
-#pragma unroll
-            for (int step = 1; step < 64; step <<= 1) {
-                const uint64_t other = __shfl_up(run, step);
-                if (lane >= (uint32_t)step) run += other;
-            }
+            uint64_t run = wave_running(sum);
             __syncthreads();
             if (lane == 63u) sh.wave64[wave] = run;
             __syncthreads();
@@ -546,8 +635,7 @@ template <uint32_t THREADS> struct Sampler {
             choose(r, [=](float v, uint32_t i) { return sample_key(v, i) >= least; });
             return;
         }
-        settle(r, cut, n);
-        const uint64_t least = sh.least;
+        const uint64_t least = settle(r, cut, n);
         const uint32_t sure = cut.sure();
         choose(r, [=](float v, uint32_t i) { return r.bin(v) < sure || sample_key(v, i) >= least; });
     }
@@ -564,10 +652,11 @@ __global__ __launch_bounds__(1024) void k_sample(const SampleArgs a)
 {
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.x);
-    if (s.tid == 0) sh.largest = 0;
-    for (uint32_t span = 0; span < a.spans; span++) {
-        const uint64_t key = s.largest(span);
-        if (s.tid == 0 && key > sh.largest) sh.largest = key;
+    if (s.tid < kSampleSpans) sh.spans[s.tid] = 0;
+    const uint64_t most = s.largest(0, a.spans - 1u);
+    if (s.tid == 0) {
+        sh.largest = most;
+        sh.listed = 0;
     }
     __syncthreads();
     const uint64_t key = sh.largest;
@@ -579,17 +668,12 @@ __global__ __launch_bounds__(1024) void k_sample(const SampleArgs a)
     SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
     if (r.limited()) {
         s.clear_bins();
-        for (uint32_t span = 0; span < a.spans; span++) s.histogram(r, span);
+        s.histogram(r, 0, a.spans - 1u);
         __syncthreads();
         s.find_cut(r);
         cut = sh.cut;
     }
-    if (s.tid == 0) sh.listed = 0;
-    __syncthreads();
-    for (uint32_t span = 0; span < a.spans; span++) {
-        const uint64_t sum = s.block_sum(s.gather(r, cut, span));
-        if (s.tid == 0) sh.spans[span] = sum;
-    }
+    s.gather(r, cut, 0, a.spans - 1u);
     __syncthreads();
     s.finish(r, cut, sh.listed);
 }
@@ -633,7 +717,7 @@ __global__ __launch_bounds__(1024) void k_sample_largest(const SampleArgs a, Sam
         state.bin_mass[b] = 0;
         state.bin_count[b] = 0;
     }
-    const uint64_t key = s.largest(blockIdx.x);
+    const uint64_t key = s.largest(blockIdx.x, blockIdx.x);
     if (s.tid == 0) {
         state.key[blockIdx.x] = key;
         if (blockIdx.x == 0) state.listed = 0;
@@ -649,7 +733,7 @@ __global__ __launch_bounds__(1024) void k_sample_limits(const SampleArgs a, Samp
     const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
     if (!sample_any(key) || r.greedy || !r.limited()) return;
     s.clear_bins();
-    s.histogram(r, blockIdx.x);
+    s.histogram(r, blockIdx.x, blockIdx.x);
     __syncthreads();
     for (uint32_t b = s.tid; b < kSampleBins; b += 1024u) {
         if (sh.bins.count[b] == 0) continue;
@@ -679,12 +763,14 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
     }
     SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
     if (r.limited()) cut = state.cut;
+    if (s.tid < kSampleSpans) sh.spans[s.tid] = 0;
     if (s.tid == 0) sh.listed = 0;
     __syncthreads();
-    const uint64_t sum = s.block_sum(s.gather(r, cut, blockIdx.x));
+    s.gather(r, cut, blockIdx.x, blockIdx.x);
+    __syncthreads();
     const uint32_t mine = sh.listed, there = mine < kSampleList ? mine : kSampleList;
     if (s.tid == 0) {
-        leave(&state.mass[blockIdx.x], sum);
+        leave(&state.mass[blockIdx.x], sh.spans[blockIdx.x]);
         sh.base = mine ? __hip_atomic_fetch_add(&state.listed, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
     }
     __syncthreads();
