@@ -26,9 +26,10 @@ namespace {
 
 constexpr uint32_t kSampleBins = 2048, kSampleList = 2048, kSampleSpans = 64;
 constexpr uint32_t kSampleBatch = 8;          // loads of a thread in flight
+constexpr uint32_t kSamplePart = 4096;        // columns of a part, or a multiple: half a batch of 1024 threads
 constexpr uint32_t kSampleCounterStep = 32;   // a row's arrival counter has a cache line of its own
 constexpr uint32_t kNoBin = 0xFFFFFFFFu;
-constexpr uint32_t kSampleFewRows = 64;
+constexpr uint32_t kSampleFewRows = 64, kSampleGroups = 256;   // rows whose parts have workgroups of their own, and how many of these
 
 // a number that orders as the float does (-0 as 0); NaN below everything
 __device__ __forceinline__ uint32_t sample_order(float v)
@@ -49,25 +50,44 @@ struct SampleArgs {
     const int *top_k;
     int *out;
     uint32_t cols, spans, span;   // a row's parts: `spans` of `span` columns, the last one shorter
-    double scale;                 // 2^S
+    uint32_t each;                // parts per workgroup
+    int s;                        // S
 };
 
 struct SampleRules {
     float largest, per_bin, per_one;   // per_bin = 64 / temperature, per_one = 1 / temperature, in 32 bits
-    double temperature, top_p, min_p, scale, uniform;
+    double log2_one, top_p, least, uniform;   // log2_one = log2(e) / temperature; least = 2^S min_p
     uint64_t top_k;   // 0: no limit
+    int s;
     bool greedy;
 
-    // 2^S w of one logit
-    __device__ __forceinline__ uint64_t weight(float v, double &w) const
+    // round(2^S w) of one logit, and whether w is at least min_p.  2^z = 2^n e^(ln2 f), n whole and |f| <= 1/2: the exponential's
+    // series up to the twelfth power, whose rest is below 2^-52; a fifth of the instructions of exp and a division (a decode batch's
+    // rows spent most of their time on those).  Nothing below e^-40 < 2^-57.
+    __device__ __forceinline__ uint64_t weight(float v, bool &above) const
     {
-        w = 0.0;
-        if (v == largest) {
-            w = 1.0;
-        } else if (v < largest && v > -INFINITY && !((largest - v) * per_one > 40.0f)) {   // (e^-40 < 2^-53)
-            w = exp(((double)v - (double)largest) / temperature);
-        }
-        return (uint64_t)rint(w * scale);
+        const bool top = v == largest;
+        above = false;
+        if (!top && !((largest - v) * per_one <= 40.0f)) return 0;   // (NaN: -infinity or a NaN, or less than an infinity)
+        const double z = top ? 0.0 : ((double)v - (double)largest) * log2_one;
+        const double n = rint(z), x = (z - n) * 0.6931471805599453;
+        double e = 1.0 / 479001600.0;
+        e = fma(e, x, 1.0 / 39916800.0);
+        e = fma(e, x, 1.0 / 3628800.0);
+        e = fma(e, x, 1.0 / 362880.0);
+        e = fma(e, x, 1.0 / 40320.0);
+        e = fma(e, x, 1.0 / 5040.0);
+        e = fma(e, x, 1.0 / 720.0);
+        e = fma(e, x, 1.0 / 120.0);
+        e = fma(e, x, 1.0 / 24.0);
+        e = fma(e, x, 1.0 / 6.0);
+        e = fma(e, x, 0.5);
+        e = fma(e, x, 1.0);
+        e = fma(e, x, 1.0);
+        e = ldexp(e, (int)n + s);
+        above = e >= least;
+        // (2^52 added leaves the nearest whole number in the low bits)
+        return (uint64_t)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
     // falls as v grows, like its weight's logarithm; every rounding in it keeps the order
     __device__ __forceinline__ uint32_t bin(float v) const
@@ -85,13 +105,13 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, uint32_
     const float t = a.temperature ? a.temperature[row] : 1.0f, p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f;
     const int k = a.top_k ? a.top_k[row] : 0;
     r.greedy = !(t > 0.0f);
-    r.temperature = t;
+    r.log2_one = 1.4426950408889634 / (double)t;
     r.per_one = 1.0f / t;
     r.per_bin = 64.0f / t;
     r.top_p = p < 1.0f ? (double)p : 1.0;   // (NaN: no limit)
-    r.min_p = m < 1.0f ? (double)m : m != m ? 0.0 : 1.0;
+    r.s = a.s;
+    r.least = ldexp(m < 1.0f ? (double)m : m != m ? 0.0 : 1.0, a.s);   // (NaN: no limit; the largest always remains)
     r.top_k = k > 0 && (uint32_t)k < a.cols ? (uint64_t)k : 0u;
-    r.scale = a.scale;
     r.uniform = a.uniform[row];
     return r;
 }
@@ -187,6 +207,7 @@ __device__ __forceinline__ uint64_t wave_most_u64(uint64_t v)
 }
 
 template <uint32_t THREADS> struct Sampler {
+    static_assert(kSampleBatch * THREADS == 2 * kSamplePart);
     static constexpr uint32_t kWaves = THREADS / 64;
     const SampleArgs &a;
     SampleShared &sh;
@@ -198,21 +219,26 @@ template <uint32_t THREADS> struct Sampler {
     {
     }
 
-    // f(v, i) for the columns of parts first .. last of the row
-    template <typename F> __device__ __forceinline__ void each(uint32_t first, uint32_t last, F &&f) const
+    // f(v, i, j) for the columns of parts first .. last of the row, the j-th of a batch of eight loads; then(base) after each batch of
+    // 8 * THREADS columns
+    template <typename F, typename G> __device__ __forceinline__ void each(uint32_t first, uint32_t last, F &&f, G &&then) const
     {
-        const uint64_t end = (uint64_t)(last + 1) * a.span < a.cols ? (uint64_t)(last + 1) * a.span : a.cols;
-        for (uint64_t i0 = (uint64_t)first * a.span + tid; i0 < end; i0 += kSampleBatch * THREADS) {
+        const uint64_t begin = (uint64_t)first * a.span, end = (uint64_t)(last + 1) * a.span < a.cols ? (uint64_t)(last + 1) * a.span : a.cols;
+        for (uint64_t base = begin; base < end; base += kSampleBatch * THREADS) {
+            const float *from = x + base;
+            const uint32_t most = (uint32_t)(end - base < kSampleBatch * THREADS ? end - base : kSampleBatch * THREADS);
             float v[kSampleBatch];
 #pragma unroll
-            for (uint32_t j = 0; j < kSampleBatch; j++) {
-                const uint64_t i = i0 + j * THREADS;
-                v[j] = x[i < end ? i : i0];
-            }
+            for (uint32_t j = 0; j < kSampleBatch; j++) v[j] = from[min(j * THREADS + tid, most - 1u)];
 #pragma unroll
             for (uint32_t j = 0; j < kSampleBatch; j++)
-                if (i0 + j * THREADS < end) f(v[j], (uint32_t)i0 + j * THREADS);
+                if (j * THREADS + tid < most) f(v[j], (uint32_t)base + j * THREADS + tid, j);
+            then(base);
         }
+    }
+    template <typename F> __device__ __forceinline__ void each(uint32_t first, uint32_t last, F &&f) const
+    {
+        each(first, last, [&](float v, uint32_t i, uint32_t) { f(v, i); }, [](uint64_t) {});
     }
 
     __device__ __forceinline__ uint64_t block_sum(uint64_t v)
@@ -253,15 +279,16 @@ template <uint32_t THREADS> struct Sampler {
         __syncthreads();
     }
 
+    // Tokens per bin for top-k, weights per bin for top-p
     __device__ __forceinline__ void histogram(const SampleRules &r, uint32_t first, uint32_t last)
     {
         each(first, last, [&](float v, uint32_t) {
-            double w;
-            const uint64_t whole = r.weight(v, w);
+            bool above;
+            const uint64_t whole = r.weight(v, above);
             if (whole) {
                 const uint32_t b = r.bin(v);
-                atomicAdd(&sh.bins.count[b], 1u);
-                atomicAdd((unsigned long long *)&sh.bins.mass[b], (unsigned long long)whole);
+                if (r.top_k) atomicAdd(&sh.bins.count[b], 1u);
+                if (r.top_p < 1.0) atomicAdd((unsigned long long *)&sh.bins.mass[b], (unsigned long long)whole);
             }
         });
     }
@@ -308,7 +335,7 @@ template <uint32_t THREADS> struct Sampler {
         for (uint32_t j = 0; j < kEach; j++) {
             const uint32_t b = tid * kEach + j, c = sh.bins.count[b];
             const uint64_t m = sh.bins.mass[b];
-            if (c) f(b, c0, c, m0, m);
+            if (c || m) f(b, c0, c, m0, m);
             c0 += c;
             m0 += m;
         }
@@ -356,28 +383,42 @@ template <uint32_t THREADS> struct Sampler {
     __device__ __forceinline__ void gather(const SampleRules &r, const SampleCut &cut, uint32_t first, uint32_t last)
     {
         const uint32_t sure = cut.sure();
-        for (uint32_t span = first; span <= last; span++) {
-            uint64_t sum = 0;
-            each(span, span, [&](float v, uint32_t i) {
+        // (a part is half a batch long or whole batches)
+        uint64_t sum[2] = {0, 0};
+        uint32_t pending = 0;   // those of a thread's batch that are to be listed: seldom more than one, and not worth eight tries a wave
+        each(
+            first, last,
+            [&](float v, uint32_t i, uint32_t j) {
                 const uint32_t b = r.bin(v);
-                if (b >= sure && !cut.listed(b)) return;
-                double w;
-                const uint64_t whole = r.weight(v, w);
-                if (whole == 0) return;
-                const bool above = w >= r.min_p;
-                if (b < sure) {
-                    if (above) sum += whole;
+                if (b >= sure) {
+                    if (cut.listed(b)) pending |= 1u << j;
                     return;
                 }
-                const uint32_t at = atomicAdd(&sh.listed, 1u);
-                if (at < kSampleList) {
-                    sh.list.key[at] = sample_key(v, i);
-                    sh.list.mass[at] = whole | (above ? 1ull << 63 : 0ull);
+                bool above;
+                const uint64_t whole = r.weight(v, above);
+                if (above) sum[j * 2 / kSampleBatch] += whole;
+            },
+            [&](uint64_t base) {
+                while (pending) {
+                    const uint32_t i = (uint32_t)base + (uint32_t)__builtin_ctz(pending) * THREADS + tid;
+                    pending &= pending - 1u;
+                    const float v = x[i];
+                    bool above;
+                    const uint64_t whole = r.weight(v, above);
+                    if (whole == 0) continue;
+                    const uint32_t at = atomicAdd(&sh.listed, 1u);
+                    if (at < kSampleList) {
+                        sh.list.key[at] = sample_key(v, i);
+                        sh.list.mass[at] = whole | (above ? 1ull << 63 : 0ull);
+                    }
+                }
+#pragma unroll
+                for (uint32_t h = 0; h < 2; h++) {
+                    const uint64_t half = wave_sum_u64(sum[h]);
+                    if (lane == 0 && half) atomicAdd((unsigned long long *)&sh.spans[(uint32_t)(base + h * (kSampleBatch / 2 * THREADS)) / a.span], (unsigned long long)half);
+                    sum[h] = 0;
                 }
             });
-            sum = wave_sum_u64(sum);
-            if (lane == 0 && sum) atomicAdd((unsigned long long *)&sh.spans[span], (unsigned long long)sum);
-        }
     }
 
     // Of the listed tokens with keys of at least `least` in bins first .. last, the lowest key that remains: of the first `want` in the
@@ -510,8 +551,8 @@ template <uint32_t THREADS> struct Sampler {
             each(0, a.spans - 1u, [&](float v, uint32_t i) {
                     const uint64_t key = sample_key(v, i);
                     if (key < least || (shift < 56 && (key >> (shift + 8)) != prefix)) return;
-                    double w;
-                    const uint64_t whole = r.weight(v, w);
+                    bool above;
+                    const uint64_t whole = r.weight(v, above);
                     if (whole == 0) return;
                     atomicAdd(&sh.bins.count[(key >> shift) & 255u], 1u);
                     atomicAdd((unsigned long long *)&sh.bins.mass[(key >> shift) & 255u], (unsigned long long)whole);
@@ -554,8 +595,8 @@ template <uint32_t THREADS> struct Sampler {
         if (r.top_p < 1.0) {
             uint64_t sum = 0;
             each(0, a.spans - 1u, [&](float v, uint32_t i) {
-                    double w;
-                    if (sample_key(v, i) >= least) sum += r.weight(v, w);
+                    bool above;
+                    if (sample_key(v, i) >= least) sum += r.weight(v, above);
                 });
             sum = block_sum(sum);
             const uint64_t by_p = select(r, true, 0, goal(r.top_p, sum), least);
@@ -564,10 +605,10 @@ template <uint32_t THREADS> struct Sampler {
         for (uint32_t span = 0; span < a.spans; span++) {
             uint64_t sum = 0;
             each(span, span, [&](float v, uint32_t i) {
-                double w;
+                bool above;
                 if (sample_key(v, i) < least) return;
-                const uint64_t whole = r.weight(v, w);
-                if (w >= r.min_p) sum += whole;
+                const uint64_t whole = r.weight(v, above);
+                if (above) sum += whole;
             });
             sum = block_sum(sum);
             if (tid == 0) sh.spans[span] = sum;
@@ -598,9 +639,9 @@ template <uint32_t THREADS> struct Sampler {
                 if (i < last) {
                     const float v = x[i];
                     if (in(v, (uint32_t)i)) {
-                        double w;
-                        const uint64_t whole = r.weight(v, w);
-                        mine[j] = w >= r.min_p ? whole : 0;
+                        bool above;
+                        const uint64_t whole = r.weight(v, above);
+                        mine[j] = above ? whole : 0;
                     }
                 }
                 sum += mine[j];
@@ -685,13 +726,17 @@ namespace {
 template <typename V> __device__ __forceinline__ void leave(V *to, V v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename V> __device__ __forceinline__ V left(const V *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// The parts that workgroup x of a row takes
+__device__ __forceinline__ uint32_t first_part(const SampleArgs &a) { return blockIdx.x * a.each; }
+__device__ __forceinline__ uint32_t last_part(const SampleArgs &a) { return min(blockIdx.x * a.each + a.each, a.spans) - 1u; }
+
 // Whether this workgroup is the row's last to arrive, what all of them left being in memory then; the counter is zero again after
-__device__ __forceinline__ bool last_to_arrive(SampleShared &sh, unsigned *counter, uint32_t spans)
+__device__ __forceinline__ bool last_to_arrive(SampleShared &sh, unsigned *counter)
 {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (threadIdx.x == 0) {
-        const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == spans - 1u;
+        const bool last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1u;
         if (last) leave(counter, 0u);
         sh.stop = last;
     }
@@ -699,11 +744,11 @@ __device__ __forceinline__ bool last_to_arrive(SampleShared &sh, unsigned *count
     return sh.stop != 0;
 }
 
-// the row's largest key, from its parts' (of the launch before)
-__device__ __forceinline__ uint64_t row_key(const SampleRow &state, uint32_t spans)
+// the row's largest key, from its workgroups' (of the launch before)
+__device__ __forceinline__ uint64_t row_key(const SampleRow &state, uint32_t groups)
 {
     const uint32_t lane = threadIdx.x & 63u;
-    return wave_most_u64(lane < spans ? state.key[lane] : 0);
+    return wave_most_u64(lane < groups ? state.key[lane] : 0);
 }
 
 }  // namespace
@@ -713,11 +758,11 @@ __global__ __launch_bounds__(1024) void k_sample_largest(const SampleArgs a, Sam
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.y);
     SampleRow &state = rows[blockIdx.y];
-    for (uint32_t b = blockIdx.x * 1024u + s.tid; b < kSampleBins; b += a.spans * 1024u) {
+    for (uint32_t b = blockIdx.x * 1024u + s.tid; b < kSampleBins; b += gridDim.x * 1024u) {
         state.bin_mass[b] = 0;
         state.bin_count[b] = 0;
     }
-    const uint64_t key = s.largest(blockIdx.x, blockIdx.x);
+    const uint64_t key = s.largest(first_part(a), last_part(a));
     if (s.tid == 0) {
         state.key[blockIdx.x] = key;
         if (blockIdx.x == 0) state.listed = 0;
@@ -729,18 +774,17 @@ __global__ __launch_bounds__(1024) void k_sample_limits(const SampleArgs a, Samp
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.y);
     SampleRow &state = rows[blockIdx.y];
-    const uint64_t key = row_key(state, a.spans);
+    const uint64_t key = row_key(state, gridDim.x);
     const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
     if (!sample_any(key) || r.greedy || !r.limited()) return;
     s.clear_bins();
-    s.histogram(r, blockIdx.x, blockIdx.x);
+    s.histogram(r, first_part(a), last_part(a));
     __syncthreads();
     for (uint32_t b = s.tid; b < kSampleBins; b += 1024u) {
-        if (sh.bins.count[b] == 0) continue;
-        __hip_atomic_fetch_add(&state.bin_count[b], sh.bins.count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_fetch_add(&state.bin_mass[b], sh.bins.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (sh.bins.count[b]) __hip_atomic_fetch_add(&state.bin_count[b], sh.bins.count[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (sh.bins.mass[b]) __hip_atomic_fetch_add(&state.bin_mass[b], sh.bins.mass[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
-    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep], a.spans)) return;
+    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep])) return;
     for (uint32_t b = s.tid; b < kSampleBins; b += 1024u) {
         sh.bins.count[b] = left(&state.bin_count[b]);
         sh.bins.mass[b] = left(&state.bin_mass[b]);
@@ -755,7 +799,7 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.y);
     SampleRow &state = rows[blockIdx.y];
-    const uint64_t key = row_key(state, a.spans);
+    const uint64_t key = row_key(state, gridDim.x);
     const SampleRules r = sample_rules(a, s.row, sample_value((uint32_t)(key >> 32)));
     if (!sample_any(key) || r.greedy) {
         if (blockIdx.x == 0 && s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
@@ -766,11 +810,11 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
     if (s.tid < kSampleSpans) sh.spans[s.tid] = 0;
     if (s.tid == 0) sh.listed = 0;
     __syncthreads();
-    s.gather(r, cut, blockIdx.x, blockIdx.x);
+    s.gather(r, cut, first_part(a), last_part(a));
     __syncthreads();
     const uint32_t mine = sh.listed, there = mine < kSampleList ? mine : kSampleList;
+    if (s.tid >= first_part(a) && s.tid <= last_part(a)) leave(&state.mass[s.tid], sh.spans[s.tid]);
     if (s.tid == 0) {
-        leave(&state.mass[blockIdx.x], sh.spans[blockIdx.x]);
         sh.base = mine ? __hip_atomic_fetch_add(&state.listed, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0u;
     }
     __syncthreads();
@@ -781,7 +825,7 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
             leave(&state.list_mass[at], sh.list.mass[i]);
         }
     }
-    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep], a.spans)) return;
+    if (!last_to_arrive(sh, &counters[s.row * kSampleCounterStep])) return;
     const uint32_t n = left(&state.listed);
     for (uint32_t i = s.tid; i < n && i < kSampleList; i += 1024u) {
         sh.list.key[i] = left(&state.list_key[i]);
@@ -792,13 +836,12 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
     s.finish(r, cut, n);
 }
 
-// 2^S: the largest power of two whose product with `cols` stays below 2^63 (and within a double's 53 bits)
-static double sample_scale(uint32_t cols)
+// S: the largest for which 2^S times `cols` stays below 2^63 (51 at most: see weight)
+static int sample_bits(uint32_t cols)
 {
     int bits = 0;
     while (bits < 32 && (1ull << bits) < cols) bits++;
-    const int s = 62 - bits < 52 ? 62 - bits : 52;
-    return (double)(1ull << s);
+    return 62 - bits < 51 ? 62 - bits : 51;
 }
 
 hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint32_t cols, const float *uniform, const float *temperature,
@@ -806,22 +849,19 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
                          unsigned *counters, uint32_t n_counters)
 {
     if (rows == 0) return hipSuccess;
-    SampleArgs a = {logits, uniform, temperature, top_p, min_p, top_k, out, cols, 1, 4096, sample_scale(cols)};
     // parts of 4096 columns, longer ones where there would be too many
-    auto spans_of_at_least = [&](uint32_t least) {
-        const uint32_t each = (uint32_t)(((uint64_t)cols + kSampleSpans - 1) / kSampleSpans);
-        a.span = each < least ? least : (each + 4095u) / 4096u * 4096u;
-        a.spans = cols ? (cols + a.span - 1) / a.span : 1u;
-    };
-    spans_of_at_least(4096u);
-    if (rows <= kSampleFewRows && a.spans > 1 && scratch && counters && (uint64_t)rows * kSampleCounterStep <= n_counters &&
+    uint32_t span = (uint32_t)(((uint64_t)cols + kSampleSpans - 1) / kSampleSpans);
+    span = span <= kSamplePart ? kSamplePart : (span + 2 * kSamplePart - 1) / (2 * kSamplePart) * (2 * kSamplePart);
+    const uint32_t spans = cols ? (cols + span - 1) / span : 1u;
+    SampleArgs a = {logits, uniform, temperature, top_p, min_p, top_k, out, cols, spans, span, spans, sample_bits(cols)};
+    if (rows <= kSampleFewRows && spans > 1 && scratch && counters && (uint64_t)rows * kSampleCounterStep <= n_counters &&
         (uint64_t)rows * sizeof(SampleRow) <= scratch_bytes) {
-        // about a thousand workgroups of all rows' parts
-        while (rows * a.spans > 1024u && a.spans > 1) spans_of_at_least(a.span * 2u);
+        a.each = (rows * spans + kSampleGroups - 1) / kSampleGroups;
+        const uint32_t groups = (spans + a.each - 1) / a.each;
         SampleRow *state = (SampleRow *)scratch;
-        hipLaunchKernelGGL(k_sample_largest, dim3(a.spans, rows), dim3(1024), 0, s, a, state);
-        if (top_k || top_p) hipLaunchKernelGGL(k_sample_limits, dim3(a.spans, rows), dim3(1024), 0, s, a, state, counters);
-        hipLaunchKernelGGL(k_sample_token, dim3(a.spans, rows), dim3(1024), 0, s, a, state, counters);
+        hipLaunchKernelGGL(k_sample_largest, dim3(groups, rows), dim3(1024), 0, s, a, state);
+        if (top_k || top_p) hipLaunchKernelGGL(k_sample_limits, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
+        hipLaunchKernelGGL(k_sample_token, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(k_sample, dim3(rows), dim3(1024), 0, s, a);
