@@ -482,18 +482,21 @@ int twm_gemm_tw_marlin_m1_indirect(twm_ctx *ctx, const float *a_dev, const uint8
  *   weights : u8 [N][K] e4m3 codes, as a checkpoint holds a linear layer, f32 scales [ceil(N / 128)][ceil(K / 128)]
  *
  * A last block that K or N cuts short has a scale like any other.  Nothing is repacked and no handle is made.  Pointers are
- * aligned to their elements, the codes of twm_gemm_fp8 to 16 bytes; rows and columns go to 2^24, K to 2^20.  The calls are asynchronous on the
+ * aligned to their elements, the codes of twm_gemm_fp8 to 16 bytes; rows and columns go to 2^24, K to 2^20, M x N to 2^36.  The calls are asynchronous on the
  * context's stream, allocate nothing and can be captured; twm_gemm_fp8 uses the context's scratch like twm_gemm. */
 
 /* C[m][n] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] * (sum over the block's features of A[m][k] * W[n][k]),
  * C row-major f32 (c_dtype TWM_F32) or f16, rounded at the end (TWM_F16).  K must be a multiple of 16 (TWM_SHAPE_ERROR); M and N
  * are any size, from one row on.  K = 0 stores zeros.  Deterministic: the same call gives the same bits.
- * f32 results: every product and every sum in f32.  f16 results of more than 32 rows use the matrix unit's 8-bit instructions,
+ * f32 results: every product and every sum in f32.  f16 results of more than 16 rows may use the matrix unit's 8-bit instructions,
  * which add eight neighbouring products (features 8 i .. 8 i + 7) after cutting each off below 2^-13 of the largest one's power
  * of two, and everything else in f32: on bell-shaped values 1.5e-5 of the result's norm, where rounding to f16 costs 2e-4.  A
  * caller to whom that matters asks for f32 results. */
 int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, const uint8_t *w_dev, const float *w_scales_dev,
                  uint32_t m, uint32_t n, uint32_t k, void *c_dev, int c_dtype);
+/* What twm_gemm_fp8 launches for these sizes, as one line of text (see twm_plan_describe): the kernel, its workgroup's shape, the
+ * matrix instructions and the K-split.  Touches no device. */
+int twm_plan_describe_fp8(uint32_t m, uint32_t n, uint32_t k, int c_dtype, char *text, size_t bytes);
 /* Rows of f16 or f32 as e4m3 rows for twm_gemm_fp8: scale = max(max |x| of the row's 128 columns, 1e-30) / 448,
  * code = e4m3_rne(x / scale).  A block with an infinity or a NaN gets a NaN scale.  cols is any size (twm_gemm_fp8 asks for a
  * multiple of 16). */

@@ -98,6 +98,7 @@ SIGNATURES = {
     "twm_batched_marlin_split_geglu": (_int, [_vp, _vp, _vp, _u32, _u32]),
     "twm_gemm_tw_marlin_m1_indirect": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _u32, _u32]),
     "twm_gemm_fp8": (_int, [_vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _int]),
+    "twm_plan_describe_fp8": (_int, [_u32, _u32, _u32, _int, _vp, _sz]),
     "twm_quantize_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _vp, _vp]),
     "twm_swiglu_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp]),
     "twm_geglu_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp]),

@@ -59,15 +59,22 @@ int gated_rows(const char *who, twm_ctx *ctx, const void *gate_up_dev, int dtype
 
 extern "C" {
 
+static int check_gemm_fp8(const char *who, uint32_t m, uint32_t n, uint32_t k, int c_dtype)
+{
+    if (!row_type(c_dtype)) return api_fail(TWM_UNSUPPORTED_OP, "%s: results must be f16 or f32", who);
+    if (k % 16 != 0) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) must be divisible by 16", who, k);
+    if (m > kFp8MostDim || n > kFp8MostDim) return api_fail(TWM_SHAPE_ERROR, "%s: %u x %u is beyond 2^24 rows or columns", who, m, n);
+    if ((uint64_t)m * n > 1ull << 36) return api_fail(TWM_SHAPE_ERROR, "%s: %u x %u results are more than 2^36", who, m, n);
+    if (k > kFp8MostK) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) is beyond 2^20", who, k);
+    return TWM_OK;
+}
+
 int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, const uint8_t *w_dev, const float *w_scales_dev, uint32_t m, uint32_t n,
                  uint32_t k, void *c_dev, int c_dtype)
 {
     const char *who = "twm_gemm_fp8";
     if (!ctx) return api_fail(TWM_INVALID_HANDLE, "%s: null context", who);
-    if (!row_type(c_dtype)) return api_fail(TWM_UNSUPPORTED_OP, "%s: results must be f16 or f32", who);
-    if (k % 16 != 0) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) must be divisible by 16", who, k);
-    if (m > kFp8MostDim || n > kFp8MostDim) return api_fail(TWM_SHAPE_ERROR, "%s: %u x %u is beyond 2^24 rows or columns", who, m, n);
-    if (k > kFp8MostK) return api_fail(TWM_SHAPE_ERROR, "%s: K (%u) is beyond 2^20", who, k);
+    if (int rc = check_gemm_fp8(who, m, n, k, c_dtype)) return rc;
     if (m == 0 || n == 0) return TWM_OK;
     if (!c_dev || (k != 0 && (!a_dev || !a_scales_dev || !w_dev || !w_scales_dev))) return api_fail(TWM_INVALID_HANDLE, "%s: null pointer", who);
     if (misaligned(a_dev, 16) || misaligned(w_dev, 16)) return api_fail(TWM_SHAPE_ERROR, "%s: A and W must be 16-byte aligned", who);
@@ -77,6 +84,15 @@ int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, 
     HIP_TRY(on.status, TWM_DEVICE_ERROR, who);
     HIP_TRY(launch_fp8_gemm(ctx->stream, a_dev, a_scales_dev, w_dev, w_scales_dev, m, n, k, c_dev, c_dtype == TWM_F16, ctx->ws, ctx->ws_bytes),
             TWM_DEVICE_ERROR, who);
+    return TWM_OK;
+}
+
+int twm_plan_describe_fp8(uint32_t m, uint32_t n, uint32_t k, int c_dtype, char *text, size_t bytes)
+{
+    const char *who = "twm_plan_describe_fp8";
+    if (!text || bytes == 0) return api_fail(TWM_INVALID_HANDLE, "%s: null buffer", who);
+    if (int rc = check_gemm_fp8(who, m, n, k, c_dtype)) return rc;
+    describe_fp8_gemm(m, n, k, c_dtype == TWM_F16, kWsBytes, text, bytes);
     return TWM_OK;
 }
 

@@ -13,6 +13,7 @@
 // both operands agree.
 #include "twm_device.h"
 
+#include <cstdio>
 #include <type_traits>
 
 namespace twm {
@@ -94,48 +95,75 @@ bool fp8_vec_store(const Fp8Gemm &g) { return g.n % 4 == 0 && ((uintptr_t)g.c & 
 
 }  // namespace
 
-// 16 columns x 16 * MT rows per workgroup, K shared out among its waves block by block; the waves' sums are added in LDS in wave
-// order.
-template <int MT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void k_fp8_gemm_simple(const Fp8Gemm g, uint32_t vec)
+// ---- few rows: every wave its own blocks ---------------------------------------------------------------------------------
+//
+// 16 * NT columns x 16 * MT rows per workgroup; wave w takes the blocks w, w + WAVES, ... of the workgroup's range of K, U of them
+// in flight, and the waves' sums are added in LDS in wave order.  Operands go from memory to registers.  TAIL: K ends inside a
+// block.  Bound: the weights' way through memory.
+template <int MT, int NT, int U, int WAVES, bool TAIL>
+__global__ __launch_bounds__(WAVES * 64) void k_fp8_rows_few(const Fp8Gemm g, uint32_t vec, uint32_t kb_per_split, float *__restrict__ partials, uint32_t n_ld)
 {
-    __shared__ float4v sums[WAVES][MT][64];
+    __shared__ float4v sums[WAVES][NT * MT][64];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    const uint32_t n0 = blockIdx.x * 16u, m0 = blockIdx.y * (16u * MT), part = (lane >> 4) * 32u;
+    const uint32_t n0 = blockIdx.x * (16u * NT), m0 = blockIdx.y * (16u * MT), part = (lane >> 4) * 32u;
+    const uint32_t b0 = blockIdx.z * kb_per_split, b1 = min(b0 + kb_per_split, g.kb);
     // rows behind the end replay the last one and are not stored
-    const uint32_t n_row = min(n0 + (lane & 15u), g.n - 1u);
-    const uint8_t *w_row = g.w + (size_t)n_row * g.k;
-    const uint8_t *a_row[MT];
+    const uint8_t *w_row[NT], *a_row[MT];
     const float *as_row[MT];
+    const TWM_CONSTANT float *ws_row[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        w_row[t] = g.w + (size_t)min(n0 + 16u * t + (lane & 15u), g.n - 1u) * g.k;
+        ws_row[t] = (const TWM_CONSTANT float *)(g.w_scales + (size_t)(min(n0 + 16u * t, g.n - 1u) >> 7) * g.kb);
+    }
 #pragma unroll
     for (int t = 0; t < MT; t++) {
         const uint32_t m_row = min(m0 + 16u * t + (lane & 15u), g.m - 1u);
         a_row[t] = g.a + (size_t)m_row * g.k;
         as_row[t] = g.a_scales + (size_t)m_row * g.kb;
     }
-    const float *ws_row = g.w_scales + (size_t)(n0 >> 7) * g.kb;
-    float4v acc[MT] = {};
-    for (uint32_t b = wave; b < g.kb; b += WAVES) {
-        const uint32_t k0 = b * 128u + part;
-        const bool tail = b * 128u + 128u > g.k;
-        const int8v w = tail ? load_32<true>(w_row, k0, g.k) : load_32<false>(w_row, k0, g.k);
-        const float ws = ws_row[b];
+    float4v acc[NT][MT] = {};
+    for (uint32_t b = b0 + wave; b < b1; b += WAVES * U) {
+        int8v w[U][NT], a[U][MT];
+        float as[U][MT], ws[U][NT];
 #pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const int8v a = tail ? load_32<true>(a_row[t], k0, g.k) : load_32<false>(a_row[t], k0, g.k);
-            const float4v d = block_sum(w, a);
-            acc[t] += d * (as_row[t][b] * ws);
+        for (uint32_t u = 0; u < U; u++) {
+            const uint32_t at = min(b + u * WAVES, b1 - 1u), k0 = at * 128u + part;   // (past the end the last block, which is not added)
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                w[u][t] = load_32<TAIL>(w_row[t], k0, g.k);
+                ws[u][t] = ws_row[t][at];
+            }
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                a[u][t] = load_32<TAIL>(a_row[t], k0, g.k);
+                as[u][t] = as_row[t][at];
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < U; u++) {
+            if (u && b + u * WAVES >= b1) break;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int j = 0; j < MT; j++) acc[t][j] += block_sum(w[u][t], a[u][j]) * (as[u][j] * ws[u][t]);
         }
     }
 #pragma unroll
-    for (int t = 0; t < MT; t++) sums[wave][t][lane] = acc[t];
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) sums[wave][t * MT + j][lane] = acc[t][j];
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < MT * 64u; i += WAVES * 64u) {
-        const uint32_t t = i >> 6, l = i & 63u;
+    for (uint32_t i = threadIdx.x; i < NT * MT * 64u; i += WAVES * 64u) {
+        const uint32_t t = i >> 6, l = i & 63u, m = m0 + 16u * (t % MT) + (l & 15u), n = n0 + 16u * (t / MT) + (l >> 4) * 4u;
         float4v s = sums[0][t][l];
 #pragma unroll
         for (int w = 1; w < WAVES; w++) s += sums[w][t][l];
-        store_quad(g, vec, m0 + 16u * t + (l & 15u), n0 + (l >> 4) * 4u, s);
+        if (partials) {
+            if (m < g.m && n < n_ld) *(float4v *)(partials + ((size_t)blockIdx.z * g.m + m) * n_ld + n) = s;
+        } else {
+            store_quad(g, vec, m, n, s);
+        }
     }
 }
 
@@ -392,40 +420,114 @@ __global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, uint32_t ve
 
 namespace {
 
-struct Fp8Plan {
-    uint32_t form, splits;
-};
-// columns x rows of a form, and its kernel
+// columns x rows of a form, its kernel, and what it was measured to take: us per block of 128 features of a workgroup alone on a
+// CU, of one among as many as the CU holds, and per workgroup besides
 struct Fp8Form {
     uint32_t bn, bm, threads, lds;
     void (*kernel)(const Fp8Gemm, uint32_t, uint32_t, uint32_t, uint32_t, float *, uint32_t);
+    uint32_t per_cu;
+    float block_alone, block_among, besides;
 };
-#define TWM_FP8_FORM(S, TN, TM, WN, WM) \
-    Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>}
+#define TWM_FP8_FORM(S, TN, TM, WN, WM, ...) \
+    Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>, __VA_ARGS__}
 const Fp8Form kFp8Forms[] = {
-    TWM_FP8_FORM(16, 8, 4, 2, 4),   // 0: 256 columns x 256 rows, eight waves
-    TWM_FP8_FORM(16, 8, 2, 2, 4),   // 1: 256 x 128, eight waves
-    TWM_FP8_FORM(16, 4, 4, 2, 2),   // 2: 128 x 128
-    TWM_FP8_FORM(16, 4, 2, 2, 2),   // 3: 128 columns x 64 rows
-    TWM_FP8_FORM(32, 2, 2, 2, 2),   // 4: 128 x 128, sums of exact products
-    TWM_FP8_FORM(32, 2, 1, 2, 2),   // 5: 128 columns x 64 rows, sums of exact products
+    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.56f, 1.30f, 6.4f),   // 256 columns x 256 rows, eight waves
+    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.76f, 0.59f, 2.6f),   // 128 x 128
+    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.40f, 1.5f),   // 128 columns x 64 rows
+    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.99f, 0.79f, 3.4f),   // 128 x 128, sums of exact products
+    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.73f, 0.53f, 1.7f),   // 128 columns x 64 rows, sums of exact products
 };
-[[maybe_unused]] constexpr uint32_t kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];
+constexpr uint32_t kFp8Fast = 3, kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];   // the first ones: 8-bit instructions
 
-hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, Fp8Plan plan, float *ws, size_t ws_bytes)
+hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, uint32_t form, uint32_t splits, float *ws)
 {
-    const Fp8Form &f = kFp8Forms[plan.form];
+    const Fp8Form &f = kFp8Forms[form];
     const uint32_t bn = (g.n + f.bn - 1) / f.bn, bm = (g.m + f.bm - 1) / f.bm, n_ld = (g.n + 3u) & ~3u;
-    uint32_t splits = plan.splits;
-    while (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) splits--;
-    const uint32_t per = (g.kb + splits - 1) / splits;
-    splits = (g.kb + per - 1) / per;
+    const uint32_t per = splits > 1 ? (g.kb + splits - 1) / splits : g.kb;
     float *partials = splits > 1 ? ws : nullptr;
     hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, fp8_vec_store(g), bn, bm, per, partials, n_ld);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
     hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_vec_store(g), partials, n_ld, splits);
     return hipGetLastError();
+}
+
+// columns per workgroup (in 16s), blocks in flight and waves of the kernel for few rows; 16 * MT rows
+template <int MT, int NT, int U, int WAVES>
+hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, float *ws)
+{
+    const uint32_t n_ld = (g.n + 3u) & ~3u, per = splits > 1 ? (g.kb + splits - 1) / splits : g.kb;
+    float *partials = splits > 1 ? ws : nullptr;
+    auto kernel = g.k % 128 ? k_fp8_rows_few<MT, NT, U, WAVES, true> : k_fp8_rows_few<MT, NT, U, WAVES, false>;
+    hipLaunchKernelGGL(kernel, dim3((g.n + 16u * NT - 1) / (16u * NT), (g.m + 16u * MT - 1) / (16u * MT), splits), dim3(WAVES * 64), 0, s, g, fp8_vec_store(g), per,
+                       partials, n_ld);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_vec_store(g), partials, n_ld, splits);
+    return hipGetLastError();
+}
+
+// Which kernel: few = 1, 2, 4: k_fp8_rows_few with that many times 16 rows; 0: k_fp8_tile in `form`.  splits: ranges of K.
+struct Fp8Plan {
+    uint32_t few, form, splits;
+};
+
+constexpr double kFp8Bandwidth = 5.2e6, kFp8SplitBandwidth = 6.2e6;   // bytes per us: operands from memory; ranges' sums out and in
+constexpr double kFp8Launch = 2.9, kFp8SecondLaunch = 2.2;            // us
+
+// Up to 16 rows the kernel for few rows (8 x 3584 x 3584 5.4 us, in tiles 8.5; 16 x 3739 x 15200 19.6 and 20.5; only above a hundred MB of
+// weights are tiles a tenth ahead).  Above, whichever is expected to take the least time, by the figures above: fitted to the
+// times of 150 shapes in every form and split, 17 .. 2048 rows, of which the choice is 1.5 % behind the best in the mean.
+Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
+{
+    if (m <= 16) return Fp8Plan{1, 0, 1};
+    const uint32_t kb = (k + 127u) / 128u;
+    const uint64_t n_ld = (n + 3u) & ~3u;
+    Fp8Plan best = {0, f16 ? kFp8Fast - 1 : kFp8FormCount - 1, 1};
+    double least = 1e30;
+    static const uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
+    for (uint32_t want : kSplits) {
+        if (want > 1 && kb / want < 2) break;
+        const uint32_t per = want > 1 ? (kb + want - 1) / want : kb, splits = per ? (kb + per - 1) / per : 1;
+        if (splits > 1 && splits * m * n_ld * 4 > ws_bytes) break;
+        const double joined = splits > 1 ? kFp8SecondLaunch + (double)splits * m * n * 8 / kFp8SplitBandwidth : 0.0;
+        for (uint32_t i = f16 ? 0 : kFp8Fast; i < (f16 ? kFp8Fast : kFp8FormCount); i++) {
+            const Fp8Form &f = kFp8Forms[i];
+            const uint64_t groups = (uint64_t)((n + f.bn - 1) / f.bn) * ((m + f.bm - 1) / f.bm) * splits, full = groups / (256u * f.per_cu),
+                           rest = (groups % (256u * f.per_cu) + 255u) / 256u;
+            if (splits > 1 && groups > 1100) continue;
+            auto turn = [&](uint64_t among) { return per * (f.block_alone > among * f.block_among ? f.block_alone : among * f.block_among) + f.besides; };
+            double us = full * turn(f.per_cu) + (rest ? turn(rest) : 0.0);
+            const double memory = ((double)n * k + (double)m * k) / kFp8Bandwidth;
+            us = (us > memory ? us : memory) + kFp8Launch + joined;
+            if (us < least) {
+                least = us;
+                best = Fp8Plan{0, i, splits};
+            }
+        }
+        if (m <= 128 && splits <= 4) {
+            const uint32_t mt = m <= 32 ? 2u : 4u;
+            const uint64_t groups = (uint64_t)((n + 15) / 16) * ((m + 16 * mt - 1) / (16 * mt)) * splits;
+            const double us = (mt == 2 ? 2.36 + (per + 7) / 8 * 0.51 + groups * per * 0.182 / 256 : 1.51 + (per + 7) / 8 * 1.78 + groups * per * 0.291 / 256) + joined;
+            if (us < least && (splits == 1 || groups <= 512)) {
+                least = us;
+                best = Fp8Plan{mt, 0, splits};
+            }
+        }
+    }
+    return best;
+}
+
+// one to sixteen rows: one round of workgroups where there is one, of 32 columns where 16 would take two, and sixteen waves each as
+// there are few (m = 1: 3584 x 3584 4.8 us, eight waves 5.1; 3584 x 4608 with 32 columns 6.3, 16 columns 6.5, at 8 rows 7.0 and 8.1;
+// 4096 x 11008 with four waves 10.8, sixteen 11.3; 3584 x 37888 with 32 columns 24.7, 16 columns 25.5, at 16 rows 31 and 39)
+enum Fp8Few { kFewNarrow, kFewTwo, kFewTwoShallow, kFewMany };
+Fp8Few fp8_few_form(uint32_t n, uint32_t k)
+{
+    const uint32_t tiles = (n + 15u) / 16u;
+    if (tiles <= 256u) return kFewNarrow;
+    if (tiles > 512u && tiles <= 1024u) return kFewMany;
+    return k < 16u * 128u ? kFewTwoShallow : kFewTwo;
 }
 
 }  // namespace
@@ -445,11 +547,33 @@ hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scale
 {
     if (m == 0 || n == 0) return hipSuccess;
     const Fp8Gemm g = {a, w, a_scales, w_scales, m, n, k, (k + 127u) / 128u, c, c_f16 ? 1u : 0u};
-    const uint32_t tiles_m = (m + 15u) / 16u, tiles_n = (n + 15u) / 16u;
-    if (m > 32) return launch_fp8_tile(s, g, Fp8Plan{c_f16 ? (m > 128 ? 2u : 3u) : (m > 128 ? 4u : 5u), 1}, ws, ws_bytes);
-    if (tiles_m == 1) hipLaunchKernelGGL((k_fp8_gemm_simple<1, 8>), dim3(tiles_n, 1), dim3(512), 0, s, g, fp8_vec_store(g));
-    else hipLaunchKernelGGL((k_fp8_gemm_simple<4, 4>), dim3(tiles_n, (tiles_m + 3u) / 4u), dim3(256), 0, s, g, fp8_vec_store(g));
-    return hipGetLastError();
+    const Fp8Plan plan = plan_fp8(m, n, k, c_f16, ws_bytes);
+    if (plan.few == 0) return launch_fp8_tile(s, g, plan.form, plan.splits, ws);
+    if (plan.few == 2) return launch_fp8_few<2, 1, 1, 8>(s, g, plan.splits, ws);
+    if (plan.few == 4) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws);
+    switch (fp8_few_form(n, k)) {
+    case kFewNarrow: return launch_fp8_few<1, 1, 1, 16>(s, g, 1, ws);
+    case kFewTwo: return launch_fp8_few<1, 2, 1, 16>(s, g, 1, ws);
+    case kFewTwoShallow: return launch_fp8_few<1, 2, 1, 8>(s, g, 1, ws);
+    default: return launch_fp8_few<1, 1, 2, 4>(s, g, 1, ws);
+    }
+}
+
+void describe_fp8_gemm(uint32_t m, uint32_t n, uint32_t k, bool c_f16, size_t ws_bytes, char *text, size_t bytes)
+{
+    const Fp8Plan plan = plan_fp8(m, n, k, c_f16, ws_bytes);
+    if (m == 0 || n == 0) {
+        snprintf(text, bytes, "nothing to launch");
+    } else if (plan.few == 0) {
+        const Fp8Form &f = kFp8Forms[plan.form];
+        snprintf(text, bytes, "k_fp8_tile: %u columns x %u rows, %u waves, %s instructions, %u K-split%s", f.bn, f.bm, f.threads / 64, plan.form < kFp8Fast ? "8-bit" : "f16",
+                 plan.splits, plan.splits == 1 ? "" : "s");
+    } else {
+        const Fp8Few form = plan.few == 1 ? fp8_few_form(n, k) : kFewTwoShallow;
+        snprintf(text, bytes, "k_fp8_rows_few: %u columns x %u rows, %u waves, f16 instructions, %u K-split%s",
+                 plan.few == 1 && (form == kFewTwo || form == kFewTwoShallow) ? 32u : 16u, 16u * plan.few, form == kFewMany ? 4u : form == kFewTwoShallow ? 8u : 16u, plan.splits,
+                 plan.splits == 1 ? "" : "s");
+    }
 }
 
 }  // namespace twm

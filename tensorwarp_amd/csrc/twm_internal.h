@@ -233,6 +233,8 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
 hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scales, const uint8_t *w, const float *w_scales, uint32_t m,
                            uint32_t n, uint32_t k, void *c, bool c_f16, float *ws, size_t ws_bytes);
 hipError_t init_fp8_gemm();
+// what launch_fp8_gemm would launch, as text
+void describe_fp8_gemm(uint32_t m, uint32_t n, uint32_t k, bool c_f16, size_t ws_bytes, char *text, size_t bytes);
 // a token per row of logits (twm_sample.hip); counters are zero between launches
 hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint32_t cols, const float *uniform, const float *temperature,
                          const int *top_k, const float *top_p, const float *min_p, int *out, void *scratch, size_t scratch_bytes,

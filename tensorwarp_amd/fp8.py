@@ -2,6 +2,8 @@
 sampling: thin calls into libtwmarlin_hip.so like those of quantize.py.  The reference has no counterpart; the kinds of arrays
 are described in include/twmarlin.h.
 """
+import ctypes as C
+
 from . import _lib
 from .quantize import _check
 
@@ -19,6 +21,13 @@ def _ptr(t):
 def gemm_fp8(device, a, a_scales, w, w_scales, m, n, k, c):
     """C [m, n] (f32 or f16) = A [m, k] x W [n, k]^T, both e4m3; a_scales [m, ceil(k / 128)], w_scales [ceil(n / 128), ceil(k / 128)]."""
     _check(device._l.twm_gemm_fp8(device.handle, a.ptr, a_scales.ptr, w.ptr, w_scales.ptr, m, n, k, c.ptr, _dtype(c)))
+
+
+def plan_fp8(m, n, k, dtype="f32"):
+    """What gemm_fp8() launches for these sizes, as a line of text."""
+    buf = C.create_string_buffer(256)
+    _check(_lib.load().twm_plan_describe_fp8(m, n, k, {"f32": _lib.F32, "f16": _lib.F16}.get(dtype, -1), buf, 256))
+    return buf.value.decode()
 
 
 def quantize_rows_fp8(device, x, q, scales, rows, cols):

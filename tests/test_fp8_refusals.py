@@ -58,6 +58,7 @@ def test_gemm_refusals(ctx):
     for name in ("m", "n"):
         refused(gemm(ctx, **{name: (1 << 24) + 16}), _lib.SHAPE_ERROR, b"beyond 2^24")
     refused(gemm(ctx, k=(1 << 20) + 16), _lib.SHAPE_ERROR, b"beyond 2^20")
+    refused(gemm(ctx, m=1 << 20, n=(1 << 16) + 1), _lib.SHAPE_ERROR, b"more than 2^36")
     assert gemm(ctx, m=0) == _lib.OK and gemm(ctx, n=0, c=None) == _lib.OK
 
 
