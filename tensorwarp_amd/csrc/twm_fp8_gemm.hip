@@ -91,7 +91,13 @@ __device__ __forceinline__ void store_quad(const Fp8Gemm &g, bool vec, uint32_t 
     }
 }
 
-bool fp8_vec_store(const Fp8Gemm &g) { return g.n % 4 == 0 && ((uintptr_t)g.c & (g.c_f16 ? 7 : 15)) == 0; }
+// How results are stored: element by element, four columns at once, or (f16) rows of whole 16-byte pieces
+constexpr uint32_t kFp8Single = 0, kFp8Quads = 1, kFp8Rows16 = 2;
+uint32_t fp8_store_of(const Fp8Gemm &g)
+{
+    if (g.c_f16 && g.n % 8 == 0 && ((uintptr_t)g.c & 15) == 0) return kFp8Rows16;
+    return g.n % 4 == 0 && ((uintptr_t)g.c & (g.c_f16 ? 7 : 15)) == 0 ? kFp8Quads : kFp8Single;
+}
 
 }  // namespace
 
@@ -192,6 +198,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *p, uint3
     return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00020000);
 }
 
+// (a wave's results, 64 columns in f32 or twice as many in f16, take the operands' place at the end)
 template <int BM, int BN> struct Fp8Tile {
     uint8_t w[2][BN * 128];
     uint8_t a[2][BM * 128];
@@ -244,6 +251,83 @@ template <> struct Fp8Mfma<32> {
     }
 };
 
+// Which tile: workgroups go to the eight XCDs in turn; XCD x takes the x-th eighth of a list of the tiles that runs in bands of
+// eight row blocks, so that what an XCD works on at a time shares its operands in that XCD's L2.
+__device__ __forceinline__ void tile_of(uint32_t blocks_n, uint32_t blocks_m, uint32_t &bn, uint32_t &bm)
+{
+    constexpr uint32_t kBand = 8;
+    const uint32_t tiles = blocks_n * blocks_m, share = tiles >> 3, rest = tiles & 7u, x8 = blockIdx.x & 7u;
+    const uint32_t t = x8 * share + (x8 < rest ? x8 : rest) + (blockIdx.x >> 3);
+    const uint32_t band = t / (kBand * blocks_n), u = t - band * kBand * blocks_n;
+    const uint32_t high = blocks_m - band * kBand < kBand ? blocks_m - band * kBand : kBand;
+    bn = u / high;
+    bm = band * kBand + u % high;
+}
+
+// The results of a wave, TM x TN tiles from row m0 and column n0 on.  Every wave of the workgroup comes here, its reads of LDS done.
+template <int S, int TN, int TM>
+__device__ __forceinline__ void store_tile(const Fp8Gemm &g, uint32_t vec, const typename Fp8Mfma<S>::Sum (&acc)[TN][TM], uint8_t *lds, uint32_t wave, uint32_t lane,
+                                           uint32_t m0, uint32_t n0, float *partials, uint32_t n_ld)
+{
+    const uint32_t row = lane % S;
+    // Registers 4 e .. 4 e + 3 of a lane: columns (256 / S) e + 4 (lane / S) .. + 3 of the tile, row lane % S.
+    if ((S == 16 && vec == kFp8Rows16) || partials || (!g.c_f16 && vec == kFp8Quads)) {
+        // Rows of whole 16-byte pieces, by way of LDS, so that a row leaves in whole lines: up to 128 columns at a time in f16, 64 in
+        // f32, 256 bytes a row; piece p of row r stands at p ^ (r % PIECES).  (Stored from the registers, 32 or 64 bytes a row: 2048 x
+        // 22016 x 4096 198 us, now 184; 2048 x 8192 x 1024 33.8 and 24.1.)
+        __builtin_amdgcn_s_waitcnt(0);
+        __builtin_amdgcn_s_barrier();
+        const bool f16 = g.c_f16 && !partials;
+        const uint32_t ld = partials ? n_ld : g.n;
+        auto rows = [&](auto which) {
+            constexpr bool F16 = decltype(which)::value;
+            constexpr uint32_t COLS = F16 ? S * TN : 64, ROW = COLS * (F16 ? 2 : 4), PIECES = ROW / 16, TILES = COLS / S;
+            uint8_t *mine = lds + wave * (S * TM * ROW);
+#pragma unroll
+            for (uint32_t i0 = 0; i0 < TN; i0 += TILES) {
+#pragma unroll
+                for (uint32_t i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int j = 0; j < TM; j++)
+#pragma unroll
+                        for (uint32_t e = 0; e < S * S / 256; e++) {
+                            const uint32_t r = j * S + row, quad = i * (S / 4) + e * (64 / S) + lane / S;   // columns 4 quad .. + 3
+                            const auto &v = acc[i0 + i][j];
+                            if constexpr (F16) {
+                                typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+                                *(half4 *)(mine + r * ROW + ((quad >> 1) ^ (r % PIECES)) * 16u + (quad & 1u) * 8u) =
+                                    half4{(_Float16)v[4 * e], (_Float16)v[4 * e + 1], (_Float16)v[4 * e + 2], (_Float16)v[4 * e + 3]};
+                            } else {
+                                *(float4v *)(mine + r * ROW + (quad ^ (r % PIECES)) * 16u) = float4v{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
+                            }
+                        }
+                // (a wave reads what it has written itself)
+#pragma unroll
+                for (uint32_t at = 0; at < S * TM * PIECES; at += 64u) {
+                    const uint32_t r = (at + lane) / PIECES, p = (at + lane) % PIECES, m = m0 + r;
+                    const uint32_t n = n0 + i0 * S + p * (F16 ? 8u : 4u);
+                    const uint4v v = *(const uint4v *)(mine + r * ROW + (p ^ (r % PIECES)) * 16u);
+                    if (m >= g.m || n >= ld) continue;
+                    if constexpr (F16) *(uint4v *)((_Float16 *)g.c + (size_t)m * ld + n) = v;
+                    else *(uint4v *)((partials ? partials + (size_t)blockIdx.y * g.m * ld : (float *)g.c) + (size_t)m * ld + n) = v;
+                }
+            }
+        };
+        if (S == 16 && f16) rows(std::integral_constant<bool, true>{});
+        else rows(std::integral_constant<bool, false>{});
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < TN; i++)
+#pragma unroll
+        for (int j = 0; j < TM; j++)
+#pragma unroll
+            for (int e = 0; e < S * S / 256; e++) {
+                const uint32_t n = n0 + i * S + (256 / S) * e + 4u * (lane / S), m = m0 + j * S + row;
+                store_quad(g, vec != kFp8Single, m, n, float4v{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]});
+            }
+}
+
 }  // namespace
 
 template <int S, int TN, int TM, int WN, int WM>
@@ -261,19 +345,16 @@ __global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint
     constexpr int EARLY = TM / EVERY * PER < PARTS ? TM / EVERY * PER : PARTS;   // those of the last row
     static_assert(LW % 2 == 0 && LA % 2 == 0 && (PARTS - EARLY + PER - 1) / PER * EVERY <= (TN - 1) * TM);
     static_assert(BN % (8 * WAVES) == 0 && BM % (8 * WAVES) == 0 && 128 % (S * TN) == 0 && TN % 2 == 0);
+    static_assert(S * TN % 64 == 0 && WAVES * S * TM * 256u <= sizeof(Fp8Tile<BM, BN>));
     extern __shared__ uint8_t lds[];
     Fp8Tile<BM, BN> &tile = *(Fp8Tile<BM, BN> *)lds;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t wn = wave % WN, wm = wave / WN;
 
-    // Which tile: workgroups go to the eight XCDs in turn; XCD x takes the x-th eighth of a list of the tiles that runs in
-    // bands of eight row blocks, so that what an XCD works on at a time shares its operands in that XCD's L2.
-    constexpr uint32_t kBand = 8;
-    const uint32_t tiles = blocks_n * blocks_m, share = tiles >> 3, rest = tiles & 7u, x8 = blockIdx.x & 7u;
-    const uint32_t t = x8 * share + (x8 < rest ? x8 : rest) + (blockIdx.x >> 3);
-    const uint32_t band = t / (kBand * blocks_n), u = t - band * kBand * blocks_n;
-    const uint32_t high = blocks_m - band * kBand < kBand ? blocks_m - band * kBand : kBand;
-    const uint32_t n0 = (u / high) * BN, m0 = (band * kBand + u % high) * BM;
+    uint32_t n0, m0;
+    tile_of(blocks_n, blocks_m, n0, m0);
+    n0 *= BN;
+    m0 *= BM;
     const uint32_t kb0 = blockIdx.y * kb_per_split, kb1 = min(kb0 + kb_per_split, g.kb);
 
     // Loads: instruction j of a wave fills eight rows; this lane's row and piece of instructions 0 and 1, the others 16 rows further
@@ -386,21 +467,7 @@ __global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint
             if (b + 1 < kb1) step(std::integral_constant<uint32_t, 1>{}, b + 1);
         }
     }
-    // register e of a lane: column (512 / S) (e / 4) % S + 4 (lane / S) + e % 4 of the tile, row lane % S
-#pragma unroll
-    for (int i = 0; i < TN; i++)
-#pragma unroll
-        for (int j = 0; j < TM; j++)
-#pragma unroll
-            for (int e = 0; e < S * S / 64; e += 4) {
-                const uint32_t n = n0 + (wn * TN + i) * S + 2u * e + 4u * (lane / S), m = m0 + (wm * TM + j) * S + row;
-                const float4v v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                if (partials) {
-                    if (m < g.m && n < n_ld) *(float4v *)(partials + ((size_t)blockIdx.y * g.m + m) * n_ld + n) = v;
-                } else {
-                    store_quad(g, vec, m, n, v);
-                }
-            }
+    store_tile<S, TN, TM>(g, vec, acc, lds, wave, lane, m0 + wm * TM * S, n0 + wn * TN * S, partials, n_ld);
 }
 
 // The sum of the K-ranges' results, in their order; a thread per four columns.
@@ -421,49 +488,51 @@ __global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, uint32_t ve
 namespace {
 
 // columns x rows of a form, its kernel, and what it was measured to take: us per block of 128 features of a workgroup alone on a
-// CU, of one among as many as the CU holds, and per workgroup besides
+// CU, of one among as many as the CU holds, per workgroup besides, and per block for a part of W that no other row block reads
 struct Fp8Form {
     uint32_t bn, bm, threads, lds;
     void (*kernel)(const Fp8Gemm, uint32_t, uint32_t, uint32_t, uint32_t, float *, uint32_t);
     uint32_t per_cu;
-    float block_alone, block_among, besides;
+    float block_alone, block_among, besides, block_cold;
 };
 #define TWM_FP8_FORM(S, TN, TM, WN, WM, ...) \
     Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>, __VA_ARGS__}
 const Fp8Form kFp8Forms[] = {
-    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.56f, 1.30f, 6.4f),   // 256 columns x 256 rows, eight waves
-    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.76f, 0.59f, 2.6f),   // 128 x 128
-    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.40f, 1.5f),   // 128 columns x 64 rows
-    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.99f, 0.79f, 3.4f),   // 128 x 128, sums of exact products
-    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.73f, 0.53f, 1.7f),   // 128 columns x 64 rows, sums of exact products
+    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.46f, 0.91f, 7.6f, 0.00f),   // 256 columns x 256 rows, eight waves
+    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.77f, 0.57f, 2.8f, 0.00f),   // 128 x 128
+    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.39f, 1.7f, 0.22f),   // 128 columns x 64 rows
+    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.91f, 0.77f, 4.2f, 0.06f),   // 128 x 128, sums of exact products
+    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.64f, 0.48f, 2.3f, 0.11f),   // 128 columns x 64 rows, sums of exact products
 };
 constexpr uint32_t kFp8Fast = 3, kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];   // the first ones: 8-bit instructions
 
-hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, uint32_t form, uint32_t splits, float *ws)
+hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, uint32_t form, uint32_t splits, float *ws, size_t ws_bytes)
 {
     const Fp8Form &f = kFp8Forms[form];
     const uint32_t bn = (g.n + f.bn - 1) / f.bn, bm = (g.m + f.bm - 1) / f.bm, n_ld = (g.n + 3u) & ~3u;
     const uint32_t per = splits > 1 ? (g.kb + splits - 1) / splits : g.kb;
+    if (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) return hipErrorInvalidValue;   // (the planner's splits fit)
     float *partials = splits > 1 ? ws : nullptr;
-    hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, fp8_vec_store(g), bn, bm, per, partials, n_ld);
+    hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, fp8_store_of(g), bn, bm, per, partials, n_ld);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_vec_store(g), partials, n_ld, splits);
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_store_of(g), partials, n_ld, splits);
     return hipGetLastError();
 }
 
 // columns per workgroup (in 16s), blocks in flight and waves of the kernel for few rows; 16 * MT rows
 template <int MT, int NT, int U, int WAVES>
-hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, float *ws)
+hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, float *ws, size_t ws_bytes)
 {
     const uint32_t n_ld = (g.n + 3u) & ~3u, per = splits > 1 ? (g.kb + splits - 1) / splits : g.kb;
+    if (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) return hipErrorInvalidValue;
     float *partials = splits > 1 ? ws : nullptr;
     auto kernel = g.k % 128 ? k_fp8_rows_few<MT, NT, U, WAVES, true> : k_fp8_rows_few<MT, NT, U, WAVES, false>;
-    hipLaunchKernelGGL(kernel, dim3((g.n + 16u * NT - 1) / (16u * NT), (g.m + 16u * MT - 1) / (16u * MT), splits), dim3(WAVES * 64), 0, s, g, fp8_vec_store(g), per,
+    hipLaunchKernelGGL(kernel, dim3((g.n + 16u * NT - 1) / (16u * NT), (g.m + 16u * MT - 1) / (16u * MT), splits), dim3(WAVES * 64), 0, s, g, fp8_store_of(g), per,
                        partials, n_ld);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_vec_store(g), partials, n_ld, splits);
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_store_of(g), partials, n_ld, splits);
     return hipGetLastError();
 }
 
@@ -472,12 +541,12 @@ struct Fp8Plan {
     uint32_t few, form, splits;
 };
 
-constexpr double kFp8Bandwidth = 5.2e6, kFp8SplitBandwidth = 6.2e6;   // bytes per us: operands from memory; ranges' sums out and in
-constexpr double kFp8Launch = 2.9, kFp8SecondLaunch = 2.2;            // us
+constexpr double kFp8Bandwidth = 6.4e6, kFp8SplitBandwidth = 6.1e6;             // bytes per us: operands from memory; ranges' sums out and in
+constexpr double kFp8Launch = 2.4, kFp8SecondLaunch = 1.5, kFp8PerSplit = 0.15;   // us
 
 // Up to 16 rows the kernel for few rows (8 x 3584 x 3584 5.4 us, in tiles 8.5; 16 x 3739 x 15200 19.6 and 20.5; only above a hundred MB of
 // weights are tiles a tenth ahead).  Above, whichever is expected to take the least time, by the figures above: fitted to the
-// times of 150 shapes in every form and split, 17 .. 2048 rows, of which the choice is 1.5 % behind the best in the mean.
+// times of 170 shapes of 17 .. 2048 rows in every form and split, of which the choice is 0.9 % behind the best in the mean.
 Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
 {
     if (m <= 16) return Fp8Plan{1, 0, 1};
@@ -490,13 +559,15 @@ Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
         if (want > 1 && kb / want < 2) break;
         const uint32_t per = want > 1 ? (kb + want - 1) / want : kb, splits = per ? (kb + per - 1) / per : 1;
         if (splits > 1 && splits * m * n_ld * 4 > ws_bytes) break;
-        const double joined = splits > 1 ? kFp8SecondLaunch + (double)splits * m * n * 8 / kFp8SplitBandwidth : 0.0;
+        const double joined = splits > 1 ? kFp8SecondLaunch + kFp8PerSplit * splits + (double)splits * m * n * 8 / kFp8SplitBandwidth : 0.0;
         for (uint32_t i = f16 ? 0 : kFp8Fast; i < (f16 ? kFp8Fast : kFp8FormCount); i++) {
             const Fp8Form &f = kFp8Forms[i];
-            const uint64_t groups = (uint64_t)((n + f.bn - 1) / f.bn) * ((m + f.bm - 1) / f.bm) * splits, full = groups / (256u * f.per_cu),
+            const uint32_t blocks_m = (m + f.bm - 1) / f.bm;
+            const uint64_t groups = (uint64_t)((n + f.bn - 1) / f.bn) * blocks_m * splits, full = groups / (256u * f.per_cu),
                            rest = (groups % (256u * f.per_cu) + 255u) / 256u;
             if (splits > 1 && groups > 1100) continue;
-            auto turn = [&](uint64_t among) { return per * (f.block_alone > among * f.block_among ? f.block_alone : among * f.block_among) + f.besides; };
+            const double alone = f.block_alone + f.block_cold / blocks_m;
+            auto turn = [&](uint64_t among) { return per * (alone > among * f.block_among ? alone : among * f.block_among) + f.besides; };
             double us = full * turn(f.per_cu) + (rest ? turn(rest) : 0.0);
             const double memory = ((double)n * k + (double)m * k) / kFp8Bandwidth;
             us = (us > memory ? us : memory) + kFp8Launch + joined;
@@ -508,7 +579,7 @@ Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
         if (m <= 128 && splits <= 4) {
             const uint32_t mt = m <= 32 ? 2u : 4u;
             const uint64_t groups = (uint64_t)((n + 15) / 16) * ((m + 16 * mt - 1) / (16 * mt)) * splits;
-            const double us = (mt == 2 ? 2.36 + (per + 7) / 8 * 0.51 + groups * per * 0.182 / 256 : 1.51 + (per + 7) / 8 * 1.78 + groups * per * 0.291 / 256) + joined;
+            const double us = (mt == 2 ? 2.55 + (per + 7) / 8 * 0.54 + groups * per * 0.162 / 256 : 1.93 + (per + 7) / 8 * 0.96 + groups * per * 0.276 / 256) + joined;
             if (us < least && (splits == 1 || groups <= 512)) {
                 least = us;
                 best = Fp8Plan{mt, 0, splits};
@@ -548,14 +619,14 @@ hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scale
     if (m == 0 || n == 0) return hipSuccess;
     const Fp8Gemm g = {a, w, a_scales, w_scales, m, n, k, (k + 127u) / 128u, c, c_f16 ? 1u : 0u};
     const Fp8Plan plan = plan_fp8(m, n, k, c_f16, ws_bytes);
-    if (plan.few == 0) return launch_fp8_tile(s, g, plan.form, plan.splits, ws);
-    if (plan.few == 2) return launch_fp8_few<2, 1, 1, 8>(s, g, plan.splits, ws);
-    if (plan.few == 4) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws);
+    if (plan.few == 0) return launch_fp8_tile(s, g, plan.form, plan.splits, ws, ws_bytes);
+    if (plan.few == 2) return launch_fp8_few<2, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
+    if (plan.few == 4) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
     switch (fp8_few_form(n, k)) {
-    case kFewNarrow: return launch_fp8_few<1, 1, 1, 16>(s, g, 1, ws);
-    case kFewTwo: return launch_fp8_few<1, 2, 1, 16>(s, g, 1, ws);
-    case kFewTwoShallow: return launch_fp8_few<1, 2, 1, 8>(s, g, 1, ws);
-    default: return launch_fp8_few<1, 1, 2, 4>(s, g, 1, ws);
+    case kFewNarrow: return launch_fp8_few<1, 1, 1, 16>(s, g, 1, ws, ws_bytes);
+    case kFewTwo: return launch_fp8_few<1, 2, 1, 16>(s, g, 1, ws, ws_bytes);
+    case kFewTwoShallow: return launch_fp8_few<1, 2, 1, 8>(s, g, 1, ws, ws_bytes);
+    default: return launch_fp8_few<1, 1, 2, 4>(s, g, 1, ws, ws_bytes);
     }
 }
 
