@@ -10,6 +10,8 @@
 // bit patterns (which order as the magnitudes do and put NaN above infinity above all numbers).
 #include "twm_device.h"
 
+#include <type_traits>
+
 namespace twm {
 
 namespace {
@@ -28,6 +30,18 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t v)
     TWM_MAX_STEP(1);
 #undef TWM_MAX_STEP
     return v;
+}
+
+// act(g) * u with silu(g) = g / (1 + e^-g), or gelu's tanh form, g / (1 + e^-2z) with z = sqrt(2 / pi) (g + 0.044715 g^3) (which is
+// 0.5 g (1 + tanh z) without the difference of nearly equal numbers).  e^-x = 2^t with t = -x log2(e) in two f32 terms and the
+// hardware's exponential and reciprocal, each within a unit in the last place: the result is within 2^-21.  Below x = -88 the
+// result is g u times less than 2^-126.  (GATE: 1 gelu, 2 silu.)
+template <int GATE> __device__ __forceinline__ float gate_rows(float g, float u)
+{
+    const float all = GATE == 1 ? 1.5957691216f * fmaf(0.044715f * g * g, g, g) : g;   // 2 sqrt(2 / pi)
+    const float x = __builtin_amdgcn_fmed3f(all, -88.0f, 1e4f), t = x * -1.44269502f;
+    const float low = fmaf(x, -1.92596303e-8f, fmaf(x, -1.44269502f, -t)), e = __builtin_amdgcn_exp2f(t);
+    return g * u * __builtin_amdgcn_rcpf(fmaf(e, low * 0.693147182f, e) + 1.0f);
 }
 
 // Columns col .. col + 7 of a row that ends at `cols`; zeros behind the end.  VEC: eight columns are 16 (f16) or 32 (f32)
@@ -118,20 +132,18 @@ template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t *q, floa
 
 }  // namespace
 
-// Sixteen lanes per (row, block).  GATE: y = act(gate) * up of a row of 2 * cols columns, gate columns then up columns or in the
-// paired order; otherwise y = x.
-template <bool F16, bool VEC, bool GATE>
-__global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, uint32_t cols, uint32_t blocks, uint64_t items, uint32_t act,
-                                                  uint32_t paired, uint8_t *__restrict__ q, float *__restrict__ scales)
+// Sixteen lanes per (row, block).  GATE 1, 2: y = gelu(gate) * up, silu(gate) * up of a row of 2 * cols columns, gate columns then up
+// columns or in the paired order; 0: y = x.  Bound: the rows' way through memory.
+template <bool F16, bool VEC, int GATE>
+__global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, uint32_t cols, uint32_t blocks, uint32_t items, uint32_t paired, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
-    const uint64_t item = ((uint64_t)blockIdx.x * 256u + threadIdx.x) >> 4;
+    const uint32_t item = blockIdx.x * 16u + (threadIdx.x >> 4);
     if (item >= items) return;   // (all sixteen lanes of an item)
-    const uint64_t row = item / blocks;
-    const uint32_t block = (uint32_t)(item - row * blocks), col = block * 128u + (threadIdx.x & 15u) * kFp8Each;
+    const uint32_t row = item / blocks, block = item - row * blocks, col = block * 128u + (threadIdx.x & 15u) * kFp8Each;
     constexpr size_t kEach = F16 ? 2 : 4;
     const char *src = (const char *)in + (size_t)row * cols * (GATE ? 2 * kEach : kEach);
     float v[8];
-    if constexpr (GATE) {
+    if constexpr (GATE != 0) {
         // (a run of 32 paired columns is whole: eight columns never cross into the up half)
         const uint32_t g_col = paired ? paired_col(col) : col, u_col = paired ? g_col + kPairWidth : col + cols;
         const bool in_row = col < cols;
@@ -139,14 +151,15 @@ __global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, u
         load_8<F16, VEC>(g, src, in_row ? g_col : 2u * cols, paired ? 2u * cols : cols);
         load_8<F16, VEC>(u, src, in_row ? u_col : 2u * cols, 2u * cols);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = gated_mul(act, g[j], u[j]);
+        for (int j = 0; j < 8; j++) v[j] = gate_rows<GATE>(g[j], u[j]);
     } else {
         load_8<F16, VEC>(v, src, col, cols);
     }
     store_codes<VEC>(q + (size_t)row * cols, scales + item, col, cols, v);
 }
 
-// A workgroup per row.  s = x (+ residual) stays in registers up to 8 * THREADS * HELD columns; a longer row is read again for its
+// A workgroup per row.  Bound: the rows' way through memory (2048 x 4096 f16 rows with every output 22.4 us, 4.9 TB/s; a copy reaches
+// 4.7).  s = x (+ residual) stays in registers up to 8 * THREADS * HELD columns; a longer row is read again for its
 // second pass.  sum: where s goes, or null; it may be the residual itself, whose elements are read by the lane that writes them.
 template <bool F16, bool VEC, uint32_t THREADS, uint32_t HELD>
 __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float *residual, const float *__restrict__ weight, float eps,
@@ -225,15 +238,27 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     }
 }
 
+constexpr uint64_t kFp8MostItems = 1ull << 27, kFp8MostRows = 1u << 22;   // of one launch (its threads stay below 2^32)
+
 hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t rows, uint32_t cols, int gate, bool paired, uint8_t *q, float *scales)
 {
     if (rows == 0 || cols == 0) return hipSuccess;
     const uint32_t blocks = (cols + 127u) / 128u;
-    const uint64_t items = (uint64_t)rows * blocks;
     const bool vec = cols % 8 == 0 && ((uintptr_t)in & 15) == 0 && ((uintptr_t)q & 7) == 0;
-    auto kernel = gate ? (f16 ? (vec ? k_fp8_rows<true, true, true> : k_fp8_rows<true, false, true>) : (vec ? k_fp8_rows<false, true, true> : k_fp8_rows<false, false, true>))
-                       : (f16 ? (vec ? k_fp8_rows<true, true, false> : k_fp8_rows<true, false, false>) : (vec ? k_fp8_rows<false, true, false> : k_fp8_rows<false, false, false>));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((items + 15) / 16)), dim3(256), 0, s, in, cols, blocks, items, gate == 1 ? 1u : 0u, paired ? 1u : 0u, q, scales);
+    auto kernel_of = [&](auto which) {
+        constexpr int GATE = decltype(which)::value;
+        return f16 ? (vec ? k_fp8_rows<true, true, GATE> : k_fp8_rows<true, false, GATE>) : (vec ? k_fp8_rows<false, true, GATE> : k_fp8_rows<false, false, GATE>);
+    };
+    auto kernel = gate == 0   ? kernel_of(std::integral_constant<int, 0>{})
+                  : gate == 1 ? kernel_of(std::integral_constant<int, 1>{})
+                              : kernel_of(std::integral_constant<int, 2>{});
+    const size_t row_bytes = (size_t)cols * (gate ? 2 : 1) * (f16 ? 2 : 4);
+    const uint32_t most = (uint32_t)(kFp8MostItems / blocks);
+    for (uint32_t row = 0; row < rows; row += most) {
+        const uint32_t items = (rows - row < most ? rows - row : most) * blocks;
+        hipLaunchKernelGGL(kernel, dim3((items + 15) / 16), dim3(256), 0, s, (const char *)in + row * row_bytes, cols, blocks, items, paired ? 1u : 0u,
+                           q + (size_t)row * cols, scales + (size_t)row * blocks);
+    }
     return hipGetLastError();
 }
 
@@ -244,8 +269,24 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
     const uint32_t blocks = (cols + 127u) / 128u;
     const uintptr_t quads = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)sum | (uintptr_t)normed;
     const bool vec = cols % 8 == 0 && (quads & 15) == 0 && ((uintptr_t)q & 7) == 0;
-    auto kernel = f16 ? (vec ? k_fp8_norm<true, true, 256, 2> : k_fp8_norm<true, false, 256, 2>) : (vec ? k_fp8_norm<false, true, 256, 2> : k_fp8_norm<false, false, 256, 2>);
-    hipLaunchKernelGGL(kernel, dim3(rows), dim3(256), 0, s, x, residual, weight, eps, cols, blocks, sum, q, scales, (_Float16 *)normed);
+    // Sixteen waves for a row where four would hold less than all of it, or there are fewer rows than CUs (1024 x 8192 f16 rows with every
+    // output 24.5 us on four, 22.1 on sixteen; 1 x 8192 5.1 and 3.8; but 2048 x 4096 f32 rows 9.2 and 12.1)
+    // and two for short rows (9362 x 896 11.9 us on four, 9.3 on two)
+    const bool wide = cols > 4096 || (rows <= 256 && cols > 2048), brief = cols <= 1024;
+    auto kernel_of = [&](auto threads, auto held) {
+        constexpr uint32_t THREADS = decltype(threads)::value, HELD = decltype(held)::value;
+        return f16 ? (vec ? k_fp8_norm<true, true, THREADS, HELD> : k_fp8_norm<true, false, THREADS, HELD>)
+                   : (vec ? k_fp8_norm<false, true, THREADS, HELD> : k_fp8_norm<false, false, THREADS, HELD>);
+    };
+    auto kernel = wide    ? kernel_of(std::integral_constant<uint32_t, 1024>{}, std::integral_constant<uint32_t, 1>{})
+                  : brief ? kernel_of(std::integral_constant<uint32_t, 128>{}, std::integral_constant<uint32_t, 1>{})
+                          : kernel_of(std::integral_constant<uint32_t, 256>{}, std::integral_constant<uint32_t, 2>{});
+    for (uint32_t row = 0; row < rows; row += kFp8MostRows) {
+        const uint32_t here = rows - row < kFp8MostRows ? rows - row : (uint32_t)kFp8MostRows;
+        const size_t at = (size_t)row * cols;
+        hipLaunchKernelGGL(kernel, dim3(here), dim3(wide ? 1024 : brief ? 128 : 256), 0, s, (const char *)x + at * (f16 ? 2 : 4), residual ? residual + at : nullptr, weight, eps, cols, blocks,
+                           sum ? sum + at : nullptr, q + at, scales + (size_t)row * blocks, normed ? (_Float16 *)normed + at : nullptr);
+    }
     return hipGetLastError();
 }
 

@@ -864,7 +864,18 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
         hipLaunchKernelGGL(k_sample_token, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(k_sample, dim3(rows), dim3(1024), 0, s, a);
+    constexpr uint32_t kMost = 1u << 21;   // rows of one launch (its threads stay below 2^32)
+    for (uint32_t row = 0; row < rows; row += kMost) {
+        SampleArgs part = a;
+        part.logits = logits + (size_t)row * cols;
+        part.uniform = uniform + row;
+        part.temperature = temperature ? temperature + row : nullptr;
+        part.top_k = top_k ? top_k + row : nullptr;
+        part.top_p = top_p ? top_p + row : nullptr;
+        part.min_p = min_p ? min_p + row : nullptr;
+        part.out = out + row;
+        hipLaunchKernelGGL(k_sample, dim3(rows - row < kMost ? rows - row : kMost), dim3(1024), 0, s, part);
+    }
     return hipGetLastError();
 }
 

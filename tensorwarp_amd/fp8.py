@@ -10,8 +10,11 @@ from .quantize import _check
 FP8_BLOCK = 128   # features (and weight columns) that share a scale
 
 
+_DTYPES = {"f32": _lib.F32, "f16": _lib.F16}
+
+
 def _dtype(t):
-    return {"f32": _lib.F32, "f16": _lib.F16}.get(t.dtype, -1)
+    return _DTYPES.get(t.dtype, -1)
 
 
 def _ptr(t):
@@ -26,7 +29,7 @@ def gemm_fp8(device, a, a_scales, w, w_scales, m, n, k, c):
 def plan_fp8(m, n, k, dtype="f32"):
     """What gemm_fp8() launches for these sizes, as a line of text."""
     buf = C.create_string_buffer(256)
-    _check(_lib.load().twm_plan_describe_fp8(m, n, k, {"f32": _lib.F32, "f16": _lib.F16}.get(dtype, -1), buf, 256))
+    _check(_lib.load().twm_plan_describe_fp8(m, n, k, _DTYPES.get(dtype, -1), buf, 256))
     return buf.value.decode()
 
 
