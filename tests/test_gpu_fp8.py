@@ -191,6 +191,20 @@ def test_the_residual_is_updated_in_place(dev, cols):
     assert np.array_equal(q.get(), q2.get()) and np.array_equal(s.get(), s2.get())
 
 
+def test_more_rows_than_one_launch_takes(dev):
+    rows = (1 << 22) + 77
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((rows, 1)).astype(np.float32)
+    q, s, total = Out(dev, (rows, 1), "u8"), Out(dev, (rows, 1), "f32"), Out(dev, (rows, 1), "f32")
+    T.add_rms_norm_fp8(dev, At(dev, x), At(dev, x), At(dev, np.array([0.5], np.float32)), 0.0, rows, 1, q, s, sum=total)
+    assert np.array_equal(total.get(), x + x)
+    # a row of one column is its own norm: 0.5 times its sign
+    assert np.array_equal(E4M3[q.get()], np.sign(x) * 448.0) and (np.abs(s.get() * 448 - 0.5) < 2.0 ** -22).all()
+    q, s = Out(dev, (rows, 1), "u8"), Out(dev, (rows, 1), "f32")
+    T.quantize_rows_fp8(dev, At(dev, x), q, s, rows, 1)
+    assert np.array_equal(E4M3[q.get()], np.sign(x) * 448.0) and (np.abs(s.get() * 448 - np.abs(x)) <= 2.0 ** -22 * np.abs(x)).all()
+
+
 def test_a_norm_of_zeros_and_of_an_infinity(dev):
     x = np.zeros((3, 300), np.float32)
     x[1, 7] = np.inf
@@ -269,7 +283,7 @@ def check_gemm(dev, inputs, m, n, k, dtype, skip=0):
 GEMMS = [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 130, 272), (3, 64, 112), (1, 896, 896), (5, 256, 1024), (15, 129, 704), (16, 100, 2816), (17, 260, 640),
          (31, 384, 1040), (32, 128, 4096), (33, 1, 256), (40, 640, 704), (64, 300, 1152), (65, 96, 512), (77, 513, 384), (100, 255, 2064), (128, 512, 1024),
          (129, 257, 1040), (200, 384, 256), (256, 256, 128), (257, 640, 1296), (300, 1000, 528), (513, 130, 896), (1, 4096, 18944), (13, 4096, 4096), (7, 8, 16),
-         (1030, 520, 272), (48, 3584, 2048), (17, 17, 6464), (30, 400, 8208), (50, 40, 3216), (70, 264, 4112)]
+         (1030, 520, 272), (48, 3584, 2048), (17, 17, 6464), (30, 400, 8208), (50, 40, 3216), (70, 264, 4112), (70001, 5, 32), (1, 300001, 16), (3, 70000, 48)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -471,6 +485,56 @@ def test_sample_rows_without_columns(dev):
     assert np.array_equal(out.get(), [0, 0, 0])
 
 
+def test_sample_more_rows_than_one_launch_takes(dev):
+    rows = (1 << 21) + 5
+    rng = np.random.default_rng(10)
+    x = rng.standard_normal((rows, 2)).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    out = Out(dev, (rows,), "i32")
+    T.sample(dev, At(dev, x), At(dev, u), out, rows, 2)
+    p0 = 1.0 / (1.0 + np.exp(x[:, 1].astype(np.float64) - x[:, 0]))
+    clear = np.abs(p0 - u) > 1e-9   # (nearer than that, two roundings of 2^-50 could decide)
+    assert clear.sum() > rows - 10 and np.array_equal(out.get()[clear], (u >= p0)[clear].astype(np.int32))
+
+
+def test_sampling_leaves_the_counters_that_others_share_at_zero(dev):
+    # arrival counters belong to the context: argmax over several spans and the few-row sampler in turn, twice
+    rng = np.random.default_rng(6)
+    x = (2 * rng.standard_normal((5, 60000))).astype(np.float32)
+    xd, top = At(dev, x), Out(dev, (5,), "i32")
+    for _ in range(2):
+        assert np.array_equal(*draw_tokens(dev, x, rng.random(5), p=np.full(5, 0.9)))
+        T.argmax(dev, xd, top, 5, 60000)
+        assert np.array_equal(top.get(), np.argmax(x, axis=1))
+        assert np.array_equal(*draw_tokens(dev, x, rng.random(5), k=np.full(5, 30)))
+
+
+def test_two_captured_graphs_that_share_the_scratch(dev):
+    # a product with K-splits and a sampler of few rows each park sums in the context's scratch; replayed in turn, with other work
+    # between, both give what the eager calls give
+    rng = np.random.default_rng(12)
+    m, n, k = 20, 500, 9088
+    assert "splits" in T.plan_fp8(m, n, k)
+    inputs = [At(dev, v) for v in gemm_inputs(rng, m, n, k)]
+    logits, u = At(dev, (2 * rng.standard_normal((3, 50000))).astype(np.float32)), At(dev, rng.random(3).astype(np.float32))
+    p = At(dev, np.full(3, 0.9, np.float32))
+    c, token = Out(dev, (m, n), "f32"), Out(dev, (3,), "i32")
+    calls = [lambda: T.gemm_fp8(dev, *inputs, m, n, k, c), lambda: T.sample(dev, logits, u, token, 3, 50000, top_p=p)]
+    for call in calls:
+        call()
+    want = c.get(), token.get()
+    graphs = [T.GraphCapture.record_with_device(dev, call) for call in calls]
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1), (1, 0, 1)):
+        c.whole.copy_from_host(c.fill)
+        token.whole.copy_from_host(token.fill)
+        for i in order:
+            graphs[i].replay()
+        assert np.array_equal(c.get(), want[0]) and np.array_equal(token.get(), want[1])
+        calls[order[0]]()
+    for g in graphs:
+        g.destroy()
+
+
 def test_a_rows_token_does_not_depend_on_the_batch(dev):
     rng = np.random.default_rng(4)
     x = (2 * rng.standard_normal((80, 9000))).astype(np.float32)
@@ -479,6 +543,102 @@ def test_a_rows_token_does_not_depend_on_the_batch(dev):
     for r in (0, 41, 79):
         alone, _ = draw_tokens(dev, x[r:r + 1], u[r:r + 1], p=p[:1])
         assert alone[0] == together[r]
+
+
+# ---- arrays beyond 4 GB ------------------------------------------------------------------------------------------------
+
+class Big:
+    """Zeros in device memory that are written and read in places."""
+
+    def __init__(self, dev, nbytes):
+        self.dev, self.lib, nbytes = dev, T._lib.load(), (nbytes + 3) // 4 * 4
+        self.ptr = self.lib.twm_malloc(dev.handle, nbytes)
+        assert self.ptr, self.lib.twm_last_error()
+        self.nbytes = nbytes
+        T.quantize._check(self.lib.twm_memset_zero(dev.handle, self.ptr, nbytes))
+
+    def put(self, at, array):
+        array = np.ascontiguousarray(array)
+        assert at + array.nbytes <= self.nbytes
+        T.quantize._check(self.lib.twm_memcpy_h2d(self.dev.handle, self.ptr + at, array.ctypes.data, array.nbytes))
+
+    def take(self, at, count, dtype):
+        out = np.empty(count, dtype)
+        assert at + out.nbytes <= self.nbytes
+        T.quantize._check(self.lib.twm_memcpy_d2h(self.dev.handle, out.ctypes.data, self.ptr + at, out.nbytes))
+        return out
+
+    def free(self):
+        self.lib.twm_free(self.dev.handle, self.ptr)
+
+
+@pytest.mark.parametrize("m,dtype", [(1, "f32"), (20, "f32"), (150, "f16"), (150, "f32")])
+def test_gemm_with_weights_beyond_4_gb(dev, m, dtype):
+    n, k, some = 270001, 16400, 300
+    a, a_s, w, w_s = gemm_inputs(np.random.default_rng(m), m, some + BLOCK, k)
+    first = (n - some) // BLOCK * BLOCK   # the last columns are not zeros: their rows' blocks begin here
+    w, w_s = w[:n - first], np.exp(np.random.default_rng(1).uniform(-8, -5, (blocks(n), blocks(k)))).astype(np.float32)
+    weights, c = Big(dev, n * k + 16), Big(dev, m * n * 4 + 16)
+    weights.put(first * k, w)
+    out = At(dev, np.zeros(1, np.float32))
+    out.ptr, out.dtype = c.ptr, dtype
+    rows = At(dev, w)
+    rows.ptr = weights.ptr
+    T.gemm_fp8(dev, At(dev, a), At(dev, a_s), rows, At(dev, w_s), m, n, k, out)
+    got = c.take(0, m * n, np.float32 if dtype == "f32" else np.float16).reshape(m, n).astype(np.float64)
+    assert (got[:, :first] == 0).all()
+    inputs = a, a_s, w, w_s[first // BLOCK:]
+    truth, size = gemm_truth(*inputs)
+    tol = (128 * 2.0 ** -23 + (blocks(k) + 32) * 2.0 ** -24) * size
+    if dtype == "f16":
+        tol += cut_off(*inputs)
+        tol += 2.0 ** -11 * (np.abs(truth) + tol) + 2.0 ** -25
+    assert (np.abs(got[:, first:] - truth) <= tol).all()
+    weights.free()
+    c.free()
+
+
+def test_rows_beyond_4_gb(dev):
+    rows, cols = 1050001, 4104
+    x, q, s = Big(dev, rows * cols * 2), Big(dev, rows * cols + 3), Big(dev, rows * blocks(cols) * 4)
+    last = np.random.default_rng(2).standard_normal((2, cols)).astype(np.float16)
+    x.put((rows - 2) * cols * 2, last)
+    as_array = lambda big, dtype: type("Rows", (), {"ptr": big.ptr, "dtype": dtype})  # noqa: E731
+    one = At(dev, np.ones(cols, np.float32))
+    for norm in (False, True):
+        if norm:
+            T.add_rms_norm_fp8(dev, as_array(x, "f16"), None, one, 1e-6, rows, cols, as_array(q, "u8"), as_array(s, "f32"))
+        else:
+            T.quantize_rows_fp8(dev, as_array(x, "f16"), as_array(q, "u8"), as_array(s, "f32"), rows, cols)
+        y = last.astype(np.float64)
+        y = y / np.sqrt((y * y).mean(axis=1, keepdims=True) + 1e-6) if norm else y
+        codes_, scales = q.take((rows - 2) * cols, 2 * cols, np.uint8), s.take((rows - 2) * blocks(cols) * 4, 2 * blocks(cols), np.float32)
+        check_codes(codes_.reshape(2, cols), scales.reshape(2, -1), y, 2.0 ** -20 * np.abs(y))
+        assert (q.take((rows - 3) * cols, cols, np.uint8) == 0).all()
+    # (as a gate's rows: two of 2 * 2052 columns)
+    T.swiglu_rows_fp8(dev, as_array(x, "f16"), as_array(q, "u8"), as_array(s, "f32"), cols // 2, rows)
+    g, u = last.astype(np.float64)[:, :cols // 2], last.astype(np.float64)[:, cols // 2:]
+    y = g / (1 + np.exp(-g)) * u
+    kb = blocks(cols // 2)
+    codes_, scales = q.take((rows - 2) * (cols // 2), cols, np.uint8), s.take((rows - 2) * kb * 4, 2 * kb, np.float32)
+    check_codes(codes_.reshape(2, -1), scales.reshape(2, -1), y, 2.0 ** -20 * np.abs(y) + 1e-37)
+    for big in (x, q, s):
+        big.free()
+
+
+def test_sample_logits_beyond_4_gb(dev):
+    rows, cols = 20000, 65540
+    x = Big(dev, rows * cols * 4)
+    last = (3 * np.random.default_rng(3).standard_normal((1, cols))).astype(np.float32)
+    x.put((rows - 1) * cols * 4, last)
+    t = np.zeros(rows, np.float32)
+    t[-1] = 0.8
+    u = np.full(rows, 0.6, np.float32)
+    out = Out(dev, (rows,), "i32")
+    T.sample(dev, type("Rows", (), {"ptr": x.ptr, "dtype": "f32"}), At(dev, u), out, rows, cols, temperature=At(dev, t))
+    got = out.get()
+    assert (got[:-1] == 0).all() and got[-1] == pick(last[0], u[-1], t[-1], 0, np.float32(np.nan), np.float32(np.nan))
+    x.free()
 
 
 # ---- the run of them, as a decode step makes it ------------------------------------------------------------------------
