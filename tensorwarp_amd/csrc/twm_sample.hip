@@ -15,8 +15,9 @@
 // and top-p end; then one more pass that adds the weights of the tokens in the bins before those and lists the tokens in them
 // (some hundred), whose exact order is settled by ranges of their keys until a wave's lanes hold them; and at last the running sum
 // through the one part of the row that u falls into.  A row whose list would be too long (thousands of nearly equal logits) is
-// settled eight bits of the key at a time instead.  Many rows: a workgroup each, one launch.  Few rows: parts of a row each have a
-// workgroup, in up to three launches, the last workgroup of a row to arrive doing what concerns the whole row.
+// settled eight bits of the key at a time instead.  Many rows, or short ones: a workgroup each, one launch.  A few long
+// rows: parts of a row each have a workgroup, in up to three launches, the last workgroup of a row to arrive doing what concerns the
+// whole row.
 //
 // Measured: 1 row of 152064 logits 14 us without limits, 22 with top-k, 26 with top-p; 32 such rows 42; 256 rows of 32000 23 without
 // limits and 40 with top-p.  Bound: for one row latency (three launches, 2.5 us from the end of one to the first load of the next; the
@@ -34,7 +35,7 @@ constexpr uint32_t kSampleBatch = 8;          // loads of a thread in flight
 constexpr uint32_t kSamplePart = 4096;        // columns of a part, or a multiple: half a batch of 1024 threads
 constexpr uint32_t kSampleCounterStep = 32;   // a row's arrival counter has a cache line of its own
 constexpr uint32_t kNoBin = 0xFFFFFFFFu;
-constexpr uint32_t kSampleFewRows = 64, kSampleGroups = 256;   // rows whose parts have workgroups of their own, and how many of these
+constexpr uint32_t kSampleGroups = 256;       // workgroups that run at once, one a compute unit
 
 // a number that orders as the float does (-0 as 0); NaN below everything
 __device__ __forceinline__ uint32_t sample_order(float v)
@@ -894,9 +895,13 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
     span = span <= kSamplePart ? kSamplePart : (span + 2 * kSamplePart - 1) / (2 * kSamplePart) * (2 * kSamplePart);
     const uint32_t spans = cols ? (cols + span - 1) / span : 1u;
     SampleArgs a = {logits, uniform, temperature, top_p, min_p, top_k, out, cols, spans, span, spans, sample_bits(cols)};
-    if (rows <= kSampleFewRows && spans > 1 && scratch && counters && (uint64_t)rows * kSampleCounterStep <= n_counters &&
+    // A workgroup per row takes 15 us and 0.72 for each 1000 columns, several of them 22 us and 0.85 for each 1000 columns that one of
+    // them works through (measured at 1 to 250 rows of 8000 to 152064 columns, top-p: 128 rows of 60000 59 us and 50, 66 of 20000 28
+    // either way, 20 of 10000 20 and 24).
+    const uint32_t most_groups = rows < kSampleGroups ? kSampleGroups / rows : 1u, each = (spans + most_groups - 1) / most_groups;
+    if (5ull * cols > 50000ull + 6ull * each * span && scratch && counters && (uint64_t)rows * kSampleCounterStep <= n_counters &&
         (uint64_t)rows * sizeof(SampleRow) <= scratch_bytes) {
-        a.each = (rows * spans + kSampleGroups - 1) / kSampleGroups;
+        a.each = each;
         const uint32_t groups = (spans + a.each - 1) / a.each;
         SampleRow *state = (SampleRow *)scratch;
         hipLaunchKernelGGL(k_sample_largest, dim3(groups, rows), dim3(1024), 0, s, a, state);

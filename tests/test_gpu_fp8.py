@@ -408,7 +408,7 @@ def draw_tokens(dev, x, u, t=None, k=None, p=None, mp=None):
 
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 2), (5, 63), (4, 64), (9, 1000), (2, 1024), (3, 1025), (1, 4097), (17, 5000), (2, 16385), (6, 32000), (70, 8200),
-                                       (1, 152064), (5, 151936), (300, 257)])
+                                       (1, 152064), (5, 151936), (300, 257), (90, 60000), (520, 2100)])
 @pytest.mark.parametrize("spread", [0.3, 3.0])
 def test_sample(dev, rows, cols, spread):
     rng = np.random.default_rng(rows * 13 + cols)
