@@ -526,8 +526,9 @@ int twm_add_rms_norm_fp8(twm_ctx *ctx, const void *x_dev, int x_dtype, const flo
  *   reach top_p of their sum, at least one; of these the ones with w >= min_p (the largest always does).
  *   The token is the first by index at which the running sum of what remains exceeds u times the whole (u below 0 or NaN: 0;
  *   1 or more: the last token with any weight).
- * Weights are computed in 64 bits and summed as whole numbers of at least 2^-38 of the largest, so that the result depends neither on the
- * launch nor on other rows; a token below half that step of the largest weight is never chosen.
+ * Weights are computed in 64 bits, rounded to whole steps of 2^-38 of the largest or finer (2^-44 for 152064 columns) and summed as whole
+ * numbers, so that the result depends neither on the launch nor on other rows; a token of less than half a step is never chosen, nor is
+ * one whose distance to the largest logit no f32 holds.
  * -infinity masks a token and NaN counts as that; a row of nothing else yields 0, as do rows without columns.  +infinity shares
  * the choice with its equals.  out [rows] i32. */
 int twm_sample_f32(twm_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t cols, const float *uniform_dev,

@@ -3,14 +3,21 @@
 //
 //   C[m][n] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] * (sum over the block's k of A[m][k] * W[n][k])
 //
-// The matrix unit's 8-bit instructions are not used where sums are to hold 32 bits: they cut every product of eight
-// neighbouring features off below 2^-13 of the largest one's power of two before they add (measured: 2^14 + 2^0 is 2^14 within a
-// group of eight and exact across two, against the exact sum results were off by 1.2e-5 of their norm on bell-shaped values and
-// 5e-5 on evenly drawn codes).  The codes become f16 instead, which holds each exactly, as do the f32 products of
-// v_mfma_f32_16x16x32_f16.  A block's sum is scaled by one f32 factor per lane (the rows of A are the lanes' columns of the
+// Two ways to a block's sum.  The matrix unit's 8-bit instructions cut every product of eight neighbouring features off below 2^-13 of
+// the largest one's power of two before they add (measured: 2^14 + 2^0 is 2^14 within a group of eight and exact across two; against the
+// exact sum results were off by 1.2e-5 of their norm on bell-shaped values and 5e-5 on evenly drawn codes).  That is below the rounding
+// of an f16 result (2^-11), so f16 results of more than 16 rows use them.  f32 results, which are to hold 32-bit sums, do not, and
+// those of up to 16 rows, which wait for the weights, have no need to: the codes become f16 there, which holds each exactly, as do the
+// f32 products of the f16 instructions.  A block's sum is scaled by one f32 factor per lane (the rows of A are the lanes' columns of the
 // result, those of W lie in its registers) and added to the f32 sum.  Both arrays are read as the caller holds them, row by
 // row: a lane's operand is 32 consecutive bytes of a row, and which of the 128 features a lane holds does not matter as long as
 // both operands agree.
+//
+// Measured, and what bounds it: one row of 3584 -> 37888 24.8 us, 5.5 TB/s: the weights' way from memory; 13 rows of 11008 -> 4096 12.1,
+// 3.7 TB/s: the ramp and the tail of a launch of 256 workgroups; 333 rows of 18944 -> 3584 40: tiles 33 (the operands' way to LDS) and the six
+// ranges' sums 6; 2048 rows of 4096 -> 22016 179, 2.06 PFLOP/s in f16: products with the factors' multiplications take 104 to 116 by
+// themselves, the operands' way to LDS 149 (9.4 TB/s over the chip), and the two do not overlap wholly.  A ring of five buffers with two
+// blocks' loads in flight took 187 to 190 where this took 172, tiles of 256 x 192 were behind but for a few row counts.
 #include "twm_device.h"
 
 #include <cstdio>
@@ -178,10 +185,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_fp8_rows_few(const Fp8Gemm g, ui
 // A workgroup computes BM rows x BN columns in blocks of 128 features.  Both operands' blocks (128 bytes a row) go from memory
 // to LDS directly, two buffers; eight rows per load instruction, lane l = (row l / 8, 16-byte slot l % 8).  Slot s of row r
 // holds the row's piece s ^ (r / 2 % 8): two rows span the 64 banks, so that sixteen neighbouring rows' reads of one piece fall
-// on all of them (with s ^ (r % 8) half the cycles of the reads were conflicts).  Waves own S * TN columns x S * TM rows each
-// (columns within one 128-column block of W's scales).  The rows' scales come to LDS four blocks at a time, 16 bytes a row:
-// read from memory by the lanes that need them, each was a cache line of its own, half as many again as the operands' (254 us
-// at 2048 x 22016 x 4096 with them, 197 without).
+// on all of them (the 16-byte reads of a wave take eight cycles each so; with s ^ (r % 8) they took as many).  Waves own S * TN
+// columns x S * TM rows each (columns within one 128-column block of W's scales).  The rows' scales come to LDS four blocks at a time,
+// 16 bytes a row: read from memory by the lanes that need them, each was a cache line of its own, half as many again as the operands'
+// (2048 x 22016 x 4096 254 us, with none of them read 197).
 //
 // S = 16: v_mfma_f32_16x16x128_f8f6f4 takes a tile's whole block at once.  Results in f16 only: within each eight neighbouring
 // features the unit cuts products off at 2^-13 of the largest one's power of two.
@@ -274,7 +281,7 @@ __device__ __forceinline__ void store_tile(const Fp8Gemm &g, uint32_t vec, const
     if ((S == 16 && vec == kFp8Rows16) || partials || (!g.c_f16 && vec == kFp8Quads)) {
         // Rows of whole 16-byte pieces, by way of LDS, so that a row leaves in whole lines: up to 128 columns at a time in f16, 64 in
         // f32, 256 bytes a row; piece p of row r stands at p ^ (r % PIECES).  (Stored from the registers, 32 or 64 bytes a row: 2048 x
-        // 22016 x 4096 198 us, now 184; 2048 x 8192 x 1024 33.8 and 24.1.)
+        // 22016 x 4096 198 us, by way of LDS 184; 2048 x 8192 x 1024 33.8 and 24.1.)
         __builtin_amdgcn_s_waitcnt(0);
         __builtin_amdgcn_s_barrier();
         const bool f16 = g.c_f16 && !partials;
@@ -340,7 +347,7 @@ __global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint
     constexpr int DEPTH = S == 16 ? 3 : 2;                    // results of the matrix unit in flight
     // A block's loads, from the last row of products of the block two before on.  Eight waves issue theirs one by one, with every
     // second product (issued together they held every wave of the CU up until the last had been taken: 2048 x 22016 x 4096 204 us,
-    // now 196); of four waves' workgroups two share a CU and take turns.
+    // one by one 196); of four waves' workgroups two share a CU and take turns.
     constexpr int PARTS = LW + LA, EVERY = WAVES == 8 && TN * TM >= 32 ? 2 : 1, PER = WAVES == 8 && S == 16 ? 1 : WAVES == 8 ? (PARTS + TM - 1) / TM : PARTS;
     constexpr int EARLY = TM / EVERY * PER < PARTS ? TM / EVERY * PER : PARTS;   // those of the last row
     static_assert(LW % 2 == 0 && LA % 2 == 0 && (PARTS - EARLY + PER - 1) / PER * EVERY <= (TN - 1) * TM);
