@@ -35,13 +35,14 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t v)
 // act(g) * u with silu(g) = g / (1 + e^-g), or gelu's tanh form, g / (1 + e^-2z) with z = sqrt(2 / pi) (g + 0.044715 g^3) (which is
 // 0.5 g (1 + tanh z) without the difference of nearly equal numbers).  e^-x = 2^t with t = -x log2(e) in two f32 terms and the
 // hardware's exponential and reciprocal, each within a unit in the last place: the result is within 2^-21.  Below x = -88 the
-// result is g u times less than 2^-126.  (GATE: 1 gelu, 2 silu.)
+// gate is g times less than 2^-126.  (GATE: 1 gelu, 2 silu.)
 template <int GATE> __device__ __forceinline__ float gate_rows(float g, float u)
 {
     const float all = GATE == 1 ? 1.5957691216f * fmaf(0.044715f * g * g, g, g) : g;   // 2 sqrt(2 / pi)
     const float x = __builtin_amdgcn_fmed3f(all, -88.0f, 1e4f), t = x * -1.44269502f;
     const float low = fmaf(x, -1.92596303e-8f, fmaf(x, -1.44269502f, -t)), e = __builtin_amdgcn_exp2f(t);
-    return g * u * __builtin_amdgcn_rcpf(fmaf(e, low * 0.693147182f, e) + 1.0f);
+    // (act(g) first: it is small where g u may be beyond f32)
+    return g * __builtin_amdgcn_rcpf(fmaf(e, low * 0.693147182f, e) + 1.0f) * u;
 }
 
 // Columns col .. col + 7 of a row that ends at `cols`; zeros behind the end.  VEC: eight columns are 16 (f16) or 32 (f32)
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     const uint32_t col0 = threadIdx.x * kFp8Each;
 
     float v[HELD][8];
-    double squares = 0.0;   // (a lane's eight in 32 bits, their sum over a row of any length in 64)
+    double squares = 0.0;   // (in 64 bits, which hold the square of any f32 and the sum over a row of any length)
     auto take = [&](float (&s)[8], uint32_t col) {
         load_8<F16, VEC>(s, x_row, col, cols);
         if (r_row) {
@@ -186,10 +187,8 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
         }
     };
     auto add = [&](const float (&s)[8]) {
-        float part = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) part += s[j] * s[j];
-        squares += (double)part;
+        for (int j = 0; j < 8; j++) squares = fma((double)s[j], (double)s[j], squares);
     };
 #pragma unroll
     for (uint32_t h = 0; h < HELD; h++) take(v[h], col0 + h * kSpan);
@@ -213,7 +212,11 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     squares = 0.0;
 #pragma unroll
     for (uint32_t w = 0; w < kWaves; w++) squares += parts[w];
-    const float scale = 1.0f / sqrtf((float)(squares / cols) + eps);
+    // 1 / sqrt(mean + eps) as a power of two, which takes a row of any magnitude half way to one, and the rest: neither need be beyond f32
+    // where the result is not
+    const double whole = 1.0 / sqrt(squares / cols + (double)eps);
+    const int half_way = __builtin_amdgcn_frexp_exp(whole) / 2;
+    const float power = ldexpf(1.0f, half_way), scale = (float)ldexp(whole, -half_way);
 
     // (whole groups of sixteen lanes: the columns of a block behind the row's end count as zeros)
     auto finish = [&](float (&s)[8], uint64_t col) {
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
         float w[8];
         load_8<false, VEC>(w, weight, (uint32_t)col, cols);
 #pragma unroll
-        for (int j = 0; j < 8; j++) s[j] = s[j] * scale * w[j];
+        for (int j = 0; j < 8; j++) s[j] = s[j] * power * scale * w[j];
         if (normed) store_f16_8<VEC>(normed + row * cols, (uint32_t)col, cols, s);
         store_codes<VEC>(q + row * cols, scales + row * blocks + (uint32_t)(col >> 7), (uint32_t)col, cols, s);
     };

@@ -156,6 +156,35 @@ def test_gated_rows(dev, rows, dim, paired, dtype, act):
     check_codes(q.get(), s.get(), y, 2.0 ** -20 * (np.abs(y) + (np.abs(g * u) if act == "gelu" else 0)) + 1e-37)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_whose_plain_product_no_f32_holds(dev, act):
+    # act(g) is small enough for u, g u is not (e^-g is off by |g| roundings of 2^-24, act(g) by some more, for gelu |2 z| of them: 32 in all
+    # at g = -5, where 2 z = 17)
+    g = np.array([-20.0, -12.0, -3.0, 0.25] if act == "silu" else [-5.0, -3.0, -1.0, 0.25], np.float32)
+    x = np.zeros((4, 64), np.float32)
+    x[:, :32] = g[:, None]
+    x[:, 32:] = np.float32(2.5e38) * np.linspace(-1, 1, 32).astype(np.float32)
+    q, s = Out(dev, (4, 32), "u8"), Out(dev, (4, 1), "f32")
+    (T.swiglu_rows_fp8 if act == "silu" else T.geglu_rows_fp8)(dev, At(dev, x), q, s, 32, 4)
+    v, u = x[:, :32].astype(np.float64), x[:, 32:].astype(np.float64)
+    y = v / (1 + np.exp(-v)) * u if act == "silu" else 0.5 * v * (1 + np.tanh(np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3))) * u
+    check_codes(q.get(), s.get(), y, 2.0 ** -19 * np.abs(y))
+
+
+@pytest.mark.parametrize("cols", [130, 1000, 4096, 9001])
+def test_norm_of_rows_whose_squares_no_f32_holds(dev, cols):
+    # without eps the norm of a row does not depend on its magnitude
+    rng = np.random.default_rng(cols)
+    x = (rng.standard_normal((6, cols)) * np.array([1e-36, 1e-30, 1e-21, 1e20, 1e30, 3e37])[:, None]).astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(cols)).astype(np.float32)
+    q, s, n = Out(dev, (6, cols), "u8"), Out(dev, (6, blocks(cols)), "f32"), Out(dev, (6, cols), "f16")
+    T.add_rms_norm_fp8(dev, At(dev, x), None, At(dev, w), 0.0, 6, cols, q, s, normed=n)
+    v = x.astype(np.float64)
+    y = v / np.sqrt((v * v).mean(axis=1, keepdims=True)) * w
+    assert (np.abs(n.get().astype(np.float64) - y) <= (2.0 ** -11 + 2.0 ** -20) * np.abs(y) + 2.0 ** -25).all()
+    check_codes(q.get(), s.get(), y, 2.0 ** -20 * np.abs(y))
+
+
 @pytest.mark.parametrize("with_residual,with_sum,with_normed", [(1, 1, 1), (1, 0, 0), (0, 0, 1), (0, 1, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("rows,cols", SHAPES)
