@@ -71,39 +71,37 @@ template <bool TAIL> __device__ __forceinline__ int8v load_32(const uint8_t *row
     return int8v{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
-// columns n .. n + 3 of row m; VEC: N is a multiple of four and C aligned to four columns
-__device__ __forceinline__ void store_quad(const Fp8Gemm &g, bool vec, uint32_t m, uint32_t n, const float4v &v)
+// Rows of results begin where the ones before them end, on any element's boundary; the memory takes vectors there too
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef half4 half4_any __attribute__((aligned(2)));
+typedef float4v float4v_any __attribute__((aligned(4)));
+typedef uint4v uint4v_any __attribute__((aligned(2)));
+
+// columns n .. n + 3 of row m
+__device__ __forceinline__ void store_quad(const Fp8Gemm &g, uint32_t m, uint32_t n, const float4v &v)
 {
     if (m >= g.m || n >= g.n) return;
     const size_t at = (size_t)m * g.n + n;
+    const bool whole = n + 4u <= g.n;
     if (g.c_f16) {
         _Float16 *c = (_Float16 *)g.c + at;
-        if (vec) {
-            typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-            *(half4 *)c = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+        if (whole) {
+            *(half4_any *)c = half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
+            for (uint32_t j = 0; j < 3; j++)
                 if (n + j < g.n) c[j] = (_Float16)v[j];
         }
     } else {
         float *c = (float *)g.c + at;
-        if (vec) {
-            *(float4v *)c = v;
+        if (whole) {
+            *(float4v_any *)c = v;
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
+            for (uint32_t j = 0; j < 3; j++)
                 if (n + j < g.n) c[j] = v[j];
         }
     }
-}
-
-// How results are stored: element by element, four columns at once, or (f16) rows of whole 16-byte pieces
-constexpr uint32_t kFp8Single = 0, kFp8Quads = 1, kFp8Rows16 = 2;
-uint32_t fp8_store_of(const Fp8Gemm &g)
-{
-    if (g.c_f16 && g.n % 8 == 0 && ((uintptr_t)g.c & 15) == 0) return kFp8Rows16;
-    return g.n % 4 == 0 && ((uintptr_t)g.c & (g.c_f16 ? 7 : 15)) == 0 ? kFp8Quads : kFp8Single;
 }
 
 }  // namespace
@@ -114,7 +112,7 @@ uint32_t fp8_store_of(const Fp8Gemm &g)
 // in flight, and the waves' sums are added in LDS in wave order.  Operands go from memory to registers.  TAIL: K ends inside a
 // block.  Bound: the weights' way through memory.
 template <int MT, int NT, int U, int WAVES, bool TAIL>
-__global__ __launch_bounds__(WAVES * 64) void k_fp8_rows_few(const Fp8Gemm g, uint32_t vec, uint32_t kb_per_split, float *__restrict__ partials, uint32_t n_ld)
+__global__ __launch_bounds__(WAVES * 64) void k_fp8_rows_few(const Fp8Gemm g, uint32_t kb_per_split, float *__restrict__ partials, uint32_t n_ld)
 {
     __shared__ float4v sums[WAVES][NT * MT][64];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
@@ -175,7 +173,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_fp8_rows_few(const Fp8Gemm g, ui
         if (partials) {
             if (m < g.m && n < n_ld) *(float4v *)(partials + ((size_t)blockIdx.z * g.m + m) * n_ld + n) = s;
         } else {
-            store_quad(g, vec, m, n, s);
+            store_quad(g, m, n, s);
         }
     }
 }
@@ -273,72 +271,68 @@ __device__ __forceinline__ void tile_of(uint32_t blocks_n, uint32_t blocks_m, ui
 
 // The results of a wave, TM x TN tiles from row m0 and column n0 on.  Every wave of the workgroup comes here, its reads of LDS done.
 template <int S, int TN, int TM>
-__device__ __forceinline__ void store_tile(const Fp8Gemm &g, uint32_t vec, const typename Fp8Mfma<S>::Sum (&acc)[TN][TM], uint8_t *lds, uint32_t wave, uint32_t lane,
+__device__ __forceinline__ void store_tile(const Fp8Gemm &g, const typename Fp8Mfma<S>::Sum (&acc)[TN][TM], uint8_t *lds, uint32_t wave, uint32_t lane,
                                            uint32_t m0, uint32_t n0, float *partials, uint32_t n_ld)
 {
     const uint32_t row = lane % S;
-    // Registers 4 e .. 4 e + 3 of a lane: columns (256 / S) e + 4 (lane / S) .. + 3 of the tile, row lane % S.
-    if ((S == 16 && vec == kFp8Rows16) || partials || (!g.c_f16 && vec == kFp8Quads)) {
-        // Rows of whole 16-byte pieces, by way of LDS, so that a row leaves in whole lines: up to 128 columns at a time in f16, 64 in
-        // f32, 256 bytes a row; piece p of row r stands at p ^ (r % PIECES).  (Stored from the registers, 32 or 64 bytes a row: 2048 x
-        // 22016 x 4096 198 us, by way of LDS 184; 2048 x 8192 x 1024 33.8 and 24.1.)
-        __builtin_amdgcn_s_waitcnt(0);
-        __builtin_amdgcn_s_barrier();
-        const bool f16 = g.c_f16 && !partials;
-        const uint32_t ld = partials ? n_ld : g.n;
-        auto rows = [&](auto which) {
-            constexpr bool F16 = decltype(which)::value;
-            constexpr uint32_t COLS = F16 ? S * TN : 64, ROW = COLS * (F16 ? 2 : 4), PIECES = ROW / 16, TILES = COLS / S;
-            uint8_t *mine = lds + wave * (S * TM * ROW);
+    // Registers 4 e .. 4 e + 3 of a lane: columns (256 / S) e + 4 (lane / S) .. + 3 of the tile, row lane % S.  They leave by way of LDS,
+    // so that a row leaves in whole lines: up to 128 columns at a time in f16, 64 in f32, 256 bytes a row; piece p of row r stands at
+    // p ^ (r % PIECES).  (Stored from the registers, 32 or 64 bytes a row: 2048 x 22016 x 4096 198 us, by way of LDS 184; 2048 x 8192 x
+    // 1024 33.8 and 24.1; where rows begin on any element's boundary, 711 x 34978 x 384, 53.1 element by element and 22.8 so.)
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    const bool f16 = g.c_f16 && !partials;
+    const uint32_t ld = partials ? n_ld : g.n;
+    auto rows = [&](auto which) {
+        constexpr bool F16 = decltype(which)::value;
+        constexpr uint32_t COLS = F16 ? S * TN : 64, ROW = COLS * (F16 ? 2 : 4), PIECES = ROW / 16, TILES = COLS / S;
+        uint8_t *mine = lds + wave * (S * TM * ROW);
 #pragma unroll
-            for (uint32_t i0 = 0; i0 < TN; i0 += TILES) {
+        for (uint32_t i0 = 0; i0 < TN; i0 += TILES) {
 #pragma unroll
-                for (uint32_t i = 0; i < TILES; i++)
+            for (uint32_t i = 0; i < TILES; i++)
 #pragma unroll
-                    for (int j = 0; j < TM; j++)
+                for (int j = 0; j < TM; j++)
 #pragma unroll
-                        for (uint32_t e = 0; e < S * S / 256; e++) {
-                            const uint32_t r = j * S + row, quad = i * (S / 4) + e * (64 / S) + lane / S;   // columns 4 quad .. + 3
-                            const auto &v = acc[i0 + i][j];
-                            if constexpr (F16) {
-                                typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-                                *(half4 *)(mine + r * ROW + ((quad >> 1) ^ (r % PIECES)) * 16u + (quad & 1u) * 8u) =
-                                    half4{(_Float16)v[4 * e], (_Float16)v[4 * e + 1], (_Float16)v[4 * e + 2], (_Float16)v[4 * e + 3]};
-                            } else {
-                                *(float4v *)(mine + r * ROW + (quad ^ (r % PIECES)) * 16u) = float4v{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
-                            }
+                    for (uint32_t e = 0; e < S * S / 256; e++) {
+                        const uint32_t r = j * S + row, quad = i * (S / 4) + e * (64 / S) + lane / S;   // columns 4 quad .. + 3
+                        const auto &v = acc[i0 + i][j];
+                        if constexpr (F16) {
+                            *(half4 *)(mine + r * ROW + ((quad >> 1) ^ (r % PIECES)) * 16u + (quad & 1u) * 8u) =
+                                half4{(_Float16)v[4 * e], (_Float16)v[4 * e + 1], (_Float16)v[4 * e + 2], (_Float16)v[4 * e + 3]};
+                        } else {
+                            *(float4v *)(mine + r * ROW + (quad ^ (r % PIECES)) * 16u) = float4v{v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]};
                         }
-                // (a wave reads what it has written itself)
+                    }
+            // (a wave reads what it has written itself)
 #pragma unroll
-                for (uint32_t at = 0; at < S * TM * PIECES; at += 64u) {
-                    const uint32_t r = (at + lane) / PIECES, p = (at + lane) % PIECES, m = m0 + r;
-                    const uint32_t n = n0 + i0 * S + p * (F16 ? 8u : 4u);
-                    const uint4v v = *(const uint4v *)(mine + r * ROW + (p ^ (r % PIECES)) * 16u);
-                    if (m >= g.m || n >= ld) continue;
-                    if constexpr (F16) *(uint4v *)((_Float16 *)g.c + (size_t)m * ld + n) = v;
-                    else *(uint4v *)((partials ? partials + (size_t)blockIdx.y * g.m * ld : (float *)g.c) + (size_t)m * ld + n) = v;
+            for (uint32_t at = 0; at < S * TM * PIECES; at += 64u) {
+                const uint32_t r = (at + lane) / PIECES, p = (at + lane) % PIECES, m = m0 + r;
+                const uint32_t n = n0 + i0 * S + p * (F16 ? 8u : 4u);
+                typedef std::conditional_t<F16, _Float16, float> Result;
+                constexpr uint32_t EACH = 16u / sizeof(Result);
+                const Result *from = (const Result *)(mine + r * ROW + (p ^ (r % PIECES)) * 16u);
+                const uint4v v = *(const uint4v *)from;
+                if (m >= g.m || n >= ld) continue;
+                Result *to = (!F16 && partials ? (Result *)partials + (size_t)blockIdx.y * g.m * ld : (Result *)g.c) + (size_t)m * ld + n;
+                if (n + EACH <= ld) {
+                    *(uint4v_any *)to = v;
+                } else {
+#pragma unroll
+                    for (uint32_t e = 0; e < EACH - 1u; e++)
+                        if (n + e < ld) to[e] = from[e];
                 }
             }
-        };
-        if (S == 16 && f16) rows(std::integral_constant<bool, true>{});
-        else rows(std::integral_constant<bool, false>{});
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < TN; i++)
-#pragma unroll
-        for (int j = 0; j < TM; j++)
-#pragma unroll
-            for (int e = 0; e < S * S / 256; e++) {
-                const uint32_t n = n0 + i * S + (256 / S) * e + 4u * (lane / S), m = m0 + j * S + row;
-                store_quad(g, vec != kFp8Single, m, n, float4v{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]});
-            }
+        }
+    };
+    if (S == 16 && f16) rows(std::integral_constant<bool, true>{});
+    else rows(std::integral_constant<bool, false>{});
 }
 
 }  // namespace
 
 template <int S, int TN, int TM, int WN, int WM>
-__global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint32_t vec, uint32_t blocks_n, uint32_t blocks_m, uint32_t kb_per_split,
+__global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint32_t blocks_n, uint32_t blocks_m, uint32_t kb_per_split,
                                                            float *__restrict__ partials, uint32_t n_ld)
 {
     typedef Fp8Mfma<S> Mfma;
@@ -474,11 +468,11 @@ __global__ __launch_bounds__(WN * WM * 64) void k_fp8_tile(const Fp8Gemm g, uint
             if (b + 1 < kb1) step(std::integral_constant<uint32_t, 1>{}, b + 1);
         }
     }
-    store_tile<S, TN, TM>(g, vec, acc, lds, wave, lane, m0 + wm * TM * S, n0 + wn * TN * S, partials, n_ld);
+    store_tile<S, TN, TM>(g, acc, lds, wave, lane, m0 + wm * TM * S, n0 + wn * TN * S, partials, n_ld);
 }
 
 // The sum of the K-ranges' results, in their order; a thread per four columns.
-__global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, uint32_t vec, const float *__restrict__ partials, uint32_t n_ld, uint32_t splits)
+__global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, const float *__restrict__ partials, uint32_t n_ld, uint32_t splits)
 {
     const uint64_t i = (uint64_t)blockIdx.x * 256u + threadIdx.x;
     const uint32_t quads = n_ld / 4u;
@@ -489,7 +483,7 @@ __global__ __launch_bounds__(256) void k_fp8_splits(const Fp8Gemm g, uint32_t ve
     const size_t step = (size_t)g.m * n_ld;
     float4v s = *(const float4v *)at;
     for (uint32_t z = 1; z < splits; z++) s += *(const float4v *)(at + z * step);
-    store_quad(g, vec, (uint32_t)m, n, s);
+    store_quad(g, (uint32_t)m, n, s);
 }
 
 namespace {
@@ -498,7 +492,7 @@ namespace {
 // CU, of one among as many as the CU holds, per workgroup besides, and per block for a part of W that no other row block reads
 struct Fp8Form {
     uint32_t bn, bm, threads, lds;
-    void (*kernel)(const Fp8Gemm, uint32_t, uint32_t, uint32_t, uint32_t, float *, uint32_t);
+    void (*kernel)(const Fp8Gemm, uint32_t, uint32_t, uint32_t, float *, uint32_t);
     uint32_t per_cu;
     float block_alone, block_among, besides, block_cold;
 };
@@ -518,12 +512,13 @@ hipError_t launch_fp8_tile(hipStream_t s, const Fp8Gemm &g, uint32_t form, uint3
     const Fp8Form &f = kFp8Forms[form];
     const uint32_t bn = (g.n + f.bn - 1) / f.bn, bm = (g.m + f.bm - 1) / f.bm, n_ld = (g.n + 3u) & ~3u;
     const uint32_t per = splits > 1 ? (g.kb + splits - 1) / splits : g.kb;
-    if (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) return hipErrorInvalidValue;   // (the planner's splits fit)
+    // (the planner's splits fit, and its forms with 8-bit instructions are for f16 results, the others for f32)
+    if ((splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) || (form < kFp8Fast) != (g.c_f16 != 0)) return hipErrorInvalidValue;
     float *partials = splits > 1 ? ws : nullptr;
-    hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, fp8_store_of(g), bn, bm, per, partials, n_ld);
+    hipLaunchKernelGGL(f.kernel, dim3(bn * bm, splits), dim3(f.threads), f.lds, s, g, bn, bm, per, partials, n_ld);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_store_of(g), partials, n_ld, splits);
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, partials, n_ld, splits);
     return hipGetLastError();
 }
 
@@ -535,11 +530,11 @@ hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, floa
     if (splits > 1 && (uint64_t)splits * g.m * n_ld * 4 > ws_bytes) return hipErrorInvalidValue;
     float *partials = splits > 1 ? ws : nullptr;
     auto kernel = g.k % 128 ? k_fp8_rows_few<MT, NT, U, WAVES, true> : k_fp8_rows_few<MT, NT, U, WAVES, false>;
-    hipLaunchKernelGGL(kernel, dim3((g.n + 16u * NT - 1) / (16u * NT), (g.m + 16u * MT - 1) / (16u * MT), splits), dim3(WAVES * 64), 0, s, g, fp8_store_of(g), per,
+    hipLaunchKernelGGL(kernel, dim3((g.n + 16u * NT - 1) / (16u * NT), (g.m + 16u * MT - 1) / (16u * MT), splits), dim3(WAVES * 64), 0, s, g, per,
                        partials, n_ld);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, fp8_store_of(g), partials, n_ld, splits);
+    hipLaunchKernelGGL(k_fp8_splits, dim3((unsigned)(((uint64_t)g.m * (n_ld / 4) + 255) / 256)), dim3(256), 0, s, g, partials, n_ld, splits);
     return hipGetLastError();
 }
 

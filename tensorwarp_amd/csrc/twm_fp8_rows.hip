@@ -45,59 +45,58 @@ template <int GATE> __device__ __forceinline__ float gate_rows(float g, float u)
     return g * __builtin_amdgcn_rcpf(fmaf(e, low * 0.693147182f, e) + 1.0f) * u;
 }
 
-// Columns col .. col + 7 of a row that ends at `cols`; zeros behind the end.  VEC: eight columns are 16 (f16) or 32 (f32)
-// aligned bytes, wholly inside the row or outside.
-template <bool F16, bool VEC> __device__ __forceinline__ void load_8(float (&v)[8], const void *row, uint32_t col, uint32_t cols)
+// Rows begin where the ones before them end, on any element's boundary; the memory takes vectors there too (2048 x 11007 f16 gate
+// 64.6 us element by element, 28.6 so; 2048 x 4095 f16 norm with every output 68.4 and 29.4)
+typedef half8 half8_any __attribute__((aligned(2)));
+typedef float4v float4v_any __attribute__((aligned(4)));
+typedef uint2v uint2v_any __attribute__((aligned(1)));
+
+// Columns col .. col + 7 of a row that ends at `cols`; zeros behind the end.  WHOLE: the eight are wholly inside the row or outside
+// (cols is a multiple of eight).
+template <bool F16, bool WHOLE> __device__ __forceinline__ void load_8(float (&v)[8], const void *row, uint32_t col, uint32_t cols)
 {
-    if constexpr (VEC) {
-        if (col < cols) {
-            if constexpr (F16) {
-                const half8 h = *(const half8 *)((const _Float16 *)row + col);
+    if (WHOLE ? col < cols : (uint64_t)col + 8u <= cols) {
+        if constexpr (F16) {
+            const half8 h = *(const half8_any *)((const _Float16 *)row + col);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = (float)h[j];
-            } else {
-                const float4v a = *(const float4v *)((const float *)row + col), b = *(const float4v *)((const float *)row + col + 4);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    v[j] = a[j];
-                    v[4 + j] = b[j];
-                }
-            }
+            for (int j = 0; j < 8; j++) v[j] = (float)h[j];
         } else {
+            const float4v a = *(const float4v_any *)((const float *)row + col), b = *(const float4v_any *)((const float *)row + col + 4);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = 0.f;
+            for (int j = 0; j < 4; j++) {
+                v[j] = a[j];
+                v[4 + j] = b[j];
+            }
         }
-    } else {
+        return;
+    }
 #pragma unroll
-        for (uint32_t j = 0; j < 8; j++) {
-            v[j] = 0.f;
-            if (col + j < cols) v[j] = F16 ? (float)((const _Float16 *)row)[col + j] : ((const float *)row)[col + j];
-        }
+    for (uint32_t j = 0; j < 8; j++) {
+        v[j] = 0.f;
+        if (!WHOLE && col + j < cols) v[j] = F16 ? (float)((const _Float16 *)row)[col + j] : ((const float *)row)[col + j];
     }
 }
 
-template <bool VEC> __device__ __forceinline__ void store_f32_8(float *row, uint32_t col, uint32_t cols, const float (&v)[8])
+template <bool WHOLE> __device__ __forceinline__ void store_f32_8(float *row, uint32_t col, uint32_t cols, const float (&v)[8])
 {
-    if constexpr (VEC) {
-        if (col < cols) {
-            *(float4v *)(row + col) = float4v{v[0], v[1], v[2], v[3]};
-            *(float4v *)(row + col + 4) = float4v{v[4], v[5], v[6], v[7]};
-        }
-    } else {
+    if (WHOLE ? col < cols : (uint64_t)col + 8u <= cols) {
+        *(float4v_any *)(row + col) = float4v{v[0], v[1], v[2], v[3]};
+        *(float4v_any *)(row + col + 4) = float4v{v[4], v[5], v[6], v[7]};
+    } else if (!WHOLE) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++)
             if (col + j < cols) row[col + j] = v[j];
     }
 }
 
-template <bool VEC> __device__ __forceinline__ void store_f16_8(_Float16 *row, uint32_t col, uint32_t cols, const float (&v)[8])
+template <bool WHOLE> __device__ __forceinline__ void store_f16_8(_Float16 *row, uint32_t col, uint32_t cols, const float (&v)[8])
 {
-    if constexpr (VEC) {
+    if (WHOLE ? col < cols : (uint64_t)col + 8u <= cols) {
         half8 h;
 #pragma unroll
         for (int j = 0; j < 8; j++) h[j] = (_Float16)v[j];
-        if (col < cols) *(half8 *)(row + col) = h;
-    } else {
+        *(half8_any *)(row + col) = h;
+    } else if (!WHOLE) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++)
             if (col + j < cols) row[col + j] = (_Float16)v[j];
@@ -106,7 +105,7 @@ template <bool VEC> __device__ __forceinline__ void store_f16_8(_Float16 *row, u
 
 // The codes of eight values whose block spans this lane's sixteen, and from its first lane the block's scale (null where the
 // block lies behind the row's end).  q: column 0 of the row.
-template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t *q, float *scale, uint32_t col, uint32_t cols, const float (&v)[8])
+template <bool WHOLE> __device__ __forceinline__ void store_codes(uint8_t *q, float *scale, uint32_t col, uint32_t cols, const float (&v)[8])
 {
     uint32_t bits = 0;
 #pragma unroll
@@ -122,9 +121,9 @@ template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t *q, floa
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * to_code, v[3] * to_code, lo, true);
     int hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * to_code, v[5] * to_code, 0, false);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * to_code, v[7] * to_code, hi, true);
-    if constexpr (VEC) {
-        if (col < cols) *(uint2v *)(q + col) = uint2v{(uint32_t)lo, (uint32_t)hi};
-    } else {
+    if (WHOLE ? col < cols : (uint64_t)col + 8u <= cols) {
+        *(uint2v_any *)(q + col) = uint2v{(uint32_t)lo, (uint32_t)hi};
+    } else if (!WHOLE) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; j++)
             if (col + j < cols) q[col + j] = (uint8_t)((uint32_t)(j < 4 ? lo : hi) >> (8 * (j & 3u)));
@@ -135,7 +134,7 @@ template <bool VEC> __device__ __forceinline__ void store_codes(uint8_t *q, floa
 
 // Sixteen lanes per (row, block).  GATE 1, 2: y = gelu(gate) * up, silu(gate) * up of a row of 2 * cols columns, gate columns then up
 // columns or in the paired order; 0: y = x.  Bound: the rows' way through memory.
-template <bool F16, bool VEC, int GATE>
+template <bool F16, bool WHOLE, int GATE>
 __global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, uint32_t cols, uint32_t blocks, uint32_t items, uint32_t paired, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
     const uint32_t item = blockIdx.x * 16u + (threadIdx.x >> 4);
@@ -149,20 +148,20 @@ __global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, u
         const uint32_t g_col = paired ? paired_col(col) : col, u_col = paired ? g_col + kPairWidth : col + cols;
         const bool in_row = col < cols;
         float g[8], u[8];
-        load_8<F16, VEC>(g, src, in_row ? g_col : 2u * cols, paired ? 2u * cols : cols);
-        load_8<F16, VEC>(u, src, in_row ? u_col : 2u * cols, 2u * cols);
+        load_8<F16, WHOLE>(g, src, in_row ? g_col : 2u * cols, paired ? 2u * cols : cols);
+        load_8<F16, WHOLE>(u, src, in_row ? u_col : 2u * cols, 2u * cols);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = gate_rows<GATE>(g[j], u[j]);
     } else {
-        load_8<F16, VEC>(v, src, col, cols);
+        load_8<F16, WHOLE>(v, src, col, cols);
     }
-    store_codes<VEC>(q + (size_t)row * cols, scales + item, col, cols, v);
+    store_codes<WHOLE>(q + (size_t)row * cols, scales + item, col, cols, v);
 }
 
 // A workgroup per row.  Bound: the rows' way through memory (2048 x 4096 f16 rows with every output 22.4 us, 4.9 TB/s; a copy reaches
 // 4.7).  s = x (+ residual) stays in registers up to 8 * THREADS * HELD columns; a longer row is read again for its
 // second pass.  sum: where s goes, or null; it may be the residual itself, whose elements are read by the lane that writes them.
-template <bool F16, bool VEC, uint32_t THREADS, uint32_t HELD>
+template <bool F16, bool WHOLE, uint32_t THREADS, uint32_t HELD>
 __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float *residual, const float *__restrict__ weight, float eps,
                                                       uint32_t cols, uint32_t blocks, float *sum, uint8_t *__restrict__ q,
                                                       float *__restrict__ scales, _Float16 *__restrict__ normed)
@@ -178,10 +177,10 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     float v[HELD][8];
     double squares = 0.0;   // (in 64 bits, which hold the square of any f32 and the sum over a row of any length)
     auto take = [&](float (&s)[8], uint32_t col) {
-        load_8<F16, VEC>(s, x_row, col, cols);
+        load_8<F16, WHOLE>(s, x_row, col, cols);
         if (r_row) {
             float r[8];
-            load_8<false, VEC>(r, r_row, col, cols);
+            load_8<false, WHOLE>(r, r_row, col, cols);
 #pragma unroll
             for (int j = 0; j < 8; j++) s[j] += r[j];
         }
@@ -195,7 +194,7 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
 #pragma unroll
     for (uint32_t h = 0; h < HELD; h++) {
         add(v[h]);
-        if (s_row) store_f32_8<VEC>(s_row, col0 + h * kSpan, cols, v[h]);
+        if (s_row) store_f32_8<WHOLE>(s_row, col0 + h * kSpan, cols, v[h]);
     }
     for (uint64_t at = (uint64_t)kSpan * HELD; at < cols; at += kSpan) {
         const uint64_t col = at + col0;
@@ -203,7 +202,7 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
         float s[8];
         take(s, (uint32_t)col);
         add(s);
-        if (s_row) store_f32_8<VEC>(s_row, (uint32_t)col, cols, s);
+        if (s_row) store_f32_8<WHOLE>(s_row, (uint32_t)col, cols, s);
     }
 #pragma unroll
     for (int step = 32; step; step >>= 1) squares += __shfl_xor(squares, step);
@@ -222,11 +221,11 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     auto finish = [&](float (&s)[8], uint64_t col) {
         if (col >= (uint64_t)blocks * 128u) return;
         float w[8];
-        load_8<false, VEC>(w, weight, (uint32_t)col, cols);
+        load_8<false, WHOLE>(w, weight, (uint32_t)col, cols);
 #pragma unroll
         for (int j = 0; j < 8; j++) s[j] = s[j] * power * scale * w[j];
-        if (normed) store_f16_8<VEC>(normed + row * cols, (uint32_t)col, cols, s);
-        store_codes<VEC>(q + row * cols, scales + row * blocks + (uint32_t)(col >> 7), (uint32_t)col, cols, s);
+        if (normed) store_f16_8<WHOLE>(normed + row * cols, (uint32_t)col, cols, s);
+        store_codes<WHOLE>(q + row * cols, scales + row * blocks + (uint32_t)(col >> 7), (uint32_t)col, cols, s);
     };
 #pragma unroll
     for (uint32_t h = 0; h < HELD; h++) finish(v[h], col0 + h * kSpan);
@@ -235,7 +234,7 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
         if (col >= (uint64_t)blocks * 128u) break;
         float s[8];
         // (what this lane wrote, where the residual may have been written over)
-        if (s_row) load_8<false, VEC>(s, s_row, (uint32_t)col, cols);
+        if (s_row) load_8<false, WHOLE>(s, s_row, (uint32_t)col, cols);
         else take(s, (uint32_t)col);
         finish(s, col);
     }
@@ -247,10 +246,10 @@ hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t row
 {
     if (rows == 0 || cols == 0) return hipSuccess;
     const uint32_t blocks = (cols + 127u) / 128u;
-    const bool vec = cols % 8 == 0 && ((uintptr_t)in & 15) == 0 && ((uintptr_t)q & 7) == 0;
+    const bool whole = cols % 8 == 0;
     auto kernel_of = [&](auto which) {
         constexpr int GATE = decltype(which)::value;
-        return f16 ? (vec ? k_fp8_rows<true, true, GATE> : k_fp8_rows<true, false, GATE>) : (vec ? k_fp8_rows<false, true, GATE> : k_fp8_rows<false, false, GATE>);
+        return f16 ? (whole ? k_fp8_rows<true, true, GATE> : k_fp8_rows<true, false, GATE>) : (whole ? k_fp8_rows<false, true, GATE> : k_fp8_rows<false, false, GATE>);
     };
     auto kernel = gate == 0   ? kernel_of(std::integral_constant<int, 0>{})
                   : gate == 1 ? kernel_of(std::integral_constant<int, 1>{})
@@ -270,16 +269,15 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
 {
     if (rows == 0 || cols == 0) return hipSuccess;
     const uint32_t blocks = (cols + 127u) / 128u;
-    const uintptr_t quads = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)sum | (uintptr_t)normed;
-    const bool vec = cols % 8 == 0 && (quads & 15) == 0 && ((uintptr_t)q & 7) == 0;
+    const bool whole = cols % 8 == 0;
     // Sixteen waves for a row where four would hold less than all of it, or there are fewer rows than CUs (1024 x 8192 f16 rows with every
     // output 24.5 us on four, 22.1 on sixteen; 1 x 8192 5.1 and 3.8; but 2048 x 4096 f32 rows 9.2 and 12.1)
     // and two for short rows (9362 x 896 11.9 us on four, 9.3 on two)
     const bool wide = cols > 4096 || (rows <= 256 && cols > 2048), brief = cols <= 1024;
     auto kernel_of = [&](auto threads, auto held) {
         constexpr uint32_t THREADS = decltype(threads)::value, HELD = decltype(held)::value;
-        return f16 ? (vec ? k_fp8_norm<true, true, THREADS, HELD> : k_fp8_norm<true, false, THREADS, HELD>)
-                   : (vec ? k_fp8_norm<false, true, THREADS, HELD> : k_fp8_norm<false, false, THREADS, HELD>);
+        return f16 ? (whole ? k_fp8_norm<true, true, THREADS, HELD> : k_fp8_norm<true, false, THREADS, HELD>)
+                   : (whole ? k_fp8_norm<false, true, THREADS, HELD> : k_fp8_norm<false, false, THREADS, HELD>);
     };
     auto kernel = wide    ? kernel_of(std::integral_constant<uint32_t, 1024>{}, std::integral_constant<uint32_t, 1>{})
                   : brief ? kernel_of(std::integral_constant<uint32_t, 128>{}, std::integral_constant<uint32_t, 1>{})
