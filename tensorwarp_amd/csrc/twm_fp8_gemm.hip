@@ -499,11 +499,11 @@ struct Fp8Form {
 #define TWM_FP8_FORM(S, TN, TM, WN, WM, ...) \
     Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>, __VA_ARGS__}
 const Fp8Form kFp8Forms[] = {
-    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.46f, 0.91f, 7.6f, 0.00f),   // 256 columns x 256 rows, eight waves
-    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.77f, 0.57f, 2.8f, 0.00f),   // 128 x 128
-    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.39f, 1.7f, 0.22f),   // 128 columns x 64 rows
-    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.91f, 0.77f, 4.2f, 0.06f),   // 128 x 128, sums of exact products
-    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.64f, 0.48f, 2.3f, 0.11f),   // 128 columns x 64 rows, sums of exact products
+    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.56f, 1.15f, 5.6f, 0.00f),   // 256 columns x 256 rows, eight waves
+    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.76f, 0.57f, 2.6f, 0.00f),   // 128 x 128
+    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.39f, 1.7f, 0.07f),   // 128 columns x 64 rows
+    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.91f, 0.76f, 3.8f, 0.00f),   // 128 x 128, sums of exact products
+    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.64f, 0.48f, 1.9f, 0.12f),   // 128 columns x 64 rows, sums of exact products
 };
 constexpr uint32_t kFp8Fast = 3, kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];   // the first ones: 8-bit instructions
 
@@ -543,12 +543,12 @@ struct Fp8Plan {
     uint32_t few, form, splits;
 };
 
-constexpr double kFp8Bandwidth = 6.4e6, kFp8SplitBandwidth = 6.1e6;             // bytes per us: operands from memory; ranges' sums out and in
-constexpr double kFp8Launch = 2.4, kFp8SecondLaunch = 1.5, kFp8PerSplit = 0.15;   // us
+constexpr double kFp8Bandwidth = 6.5e6, kFp8SplitBandwidth = 6.2e6;             // bytes per us: operands from memory; ranges' sums out and in
+constexpr double kFp8Launch = 2.34, kFp8SecondLaunch = 1.61, kFp8PerSplit = 0.17;   // us
 
 // Up to 16 rows the kernel for few rows (8 x 3584 x 3584 5.4 us, in tiles 8.5; 16 x 3739 x 15200 19.6 and 20.5; only above a hundred MB of
 // weights are tiles a tenth ahead).  Above, whichever is expected to take the least time, by the figures above: fitted to the
-// times of 170 shapes of 17 .. 2048 rows in every form and split, of which the choice is 0.9 % behind the best in the mean.
+// times of 170 shapes of 17 .. 2048 rows in every form and split, of which the choice is 0.8 % behind the best in the mean.
 Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
 {
     if (m <= 16) return Fp8Plan{1, 0, 1};
@@ -581,7 +581,7 @@ Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
         if (m <= 128 && splits <= 4) {
             const uint32_t mt = m <= 32 ? 2u : 4u;
             const uint64_t groups = (uint64_t)((n + 15) / 16) * ((m + 16 * mt - 1) / (16 * mt)) * splits;
-            const double us = (mt == 2 ? 2.55 + (per + 7) / 8 * 0.54 + groups * per * 0.162 / 256 : 1.93 + (per + 7) / 8 * 0.96 + groups * per * 0.276 / 256) + joined;
+            const double us = (mt == 2 ? 2.18 + (per + 7) / 8 * 0.57 + groups * per * 0.162 / 256 : 2.0 + (per + 7) / 8 * 0.97 + groups * per * 0.254 / 256) + joined;
             if (us < least && (splits == 1 || groups <= 512)) {
                 least = us;
                 best = Fp8Plan{mt, 0, splits};
