@@ -19,11 +19,12 @@
 // rows: parts of a row each have a workgroup, in up to three launches, the last workgroup of a row to arrive doing what concerns the
 // whole row.
 //
-// Measured: 1 row of 152064 logits 14 us without limits, 22 with top-k, 26 with top-p; 32 such rows 42; 256 rows of 32000 23 without
-// limits and 40 with top-p.  Bound: for one row latency (three launches, 2.5 us from the end of one to the first load of the next; the
-// passes themselves 2 to 3 us; histogram to cut and list to token 4 and 7); for many rows the vector instructions of the weights, 33 a
-// token in each of two passes, eighteen of them in 64 bits: of 40 us for 256 rows of 32000 the largest logit takes 6, the histogram 11,
-// the cut 1.5, adding and listing 12, settling the list 3, the token 3.  Rows kept in registers over the passes changed nothing.
+// Measured: 1 row of 152064 logits 14 us without limits, 20 with top-k, 23 with top-k and top-p, 25 with top-p; 32 such rows 42 with
+// top-p and 31 with both; 256 rows of 32000 23 without limits, 24, 27 and 40.  Bound: for one row latency (three launches, 2.5 us from
+// the end of one to the first load of the next; the passes themselves 1 to 3 us; histogram to cut and list to token 4 and 7); for many
+// rows the vector instructions of the weights, 33 a token in each of two passes, eighteen of them in 64 bits: of 40 us for 256 rows of
+// 32000 the largest logit takes 6, the histogram 11, the cut 1.5, adding and listing 12, settling the list 3, the token 3.  Rows kept in
+// registers over the passes changed nothing.
 #include "twm_device.h"
 
 namespace twm {
@@ -31,6 +32,9 @@ namespace twm {
 namespace {
 
 constexpr uint32_t kSampleBins = 2048, kSampleList = 2048, kSampleSpans = 64;
+// A top_k up to which its tokens are listed one and all: a quarter of the list, the rest for those next to the last; on rows of up to
+// kSampleShort columns fewer than a wave's lanes
+constexpr uint32_t kSampleListAll = 512, kSampleListAllShort = 56, kSampleShort = 12288;
 constexpr uint32_t kSampleBatch = 8;          // loads of a thread in flight
 constexpr uint32_t kSamplePart = 4096;        // columns of a part, or a multiple: half a batch of 1024 threads
 constexpr uint32_t kSampleCounterStep = 32;   // a row's arrival counter has a cache line of its own
@@ -70,10 +74,12 @@ struct SampleArgs {
 };
 
 struct SampleRules {
+    static constexpr float kDeepest = 64.0f * 40.0f;   // depth (see there) from which on weights are nothing
     float largest, finite;             // finite: the largest, or 0 for an infinity
     float per_bin;                     // 64 / temperature, in 32 bits
     double log2_one, top_p, least, uniform;   // log2_one = 64 log2(e) / temperature; least = 2^S min_p
     uint64_t top_k;        // 0: no limit
+    uint32_t list_all;
     const double *power;   // 2^(S + j / 64), j = 0 .. 63, in LDS
     bool greedy;
 
@@ -85,7 +91,7 @@ struct SampleRules {
     __device__ __forceinline__ uint64_t weight(float v, bool &above) const
     {
         const bool top = v == largest;
-        const bool any = depth(v) <= 64.0f * 40.0f;   // (NaN: a NaN)
+        const bool any = depth(v) <= kDeepest;   // (NaN: a NaN)
         const double d = (double)(top ? finite : v) - (double)finite, at = fma(d, log2_one, 6755399441055744.0);
         const uint32_t n = (uint32_t)__double2loint(at);
         const double f = fma(d, log2_one, 6755399441055744.0 - at), p = power[n % 64u];
@@ -119,6 +125,12 @@ struct SampleRules {
     // is nothing)
     static __device__ __forceinline__ float begin(uint32_t b) { return b < kSampleBins ? (float)b : INFINITY; }
     __device__ __forceinline__ bool limited() const { return top_k != 0 || top_p < 1.0; }
+    // Whether the tokens of the bins are counted only: top_p does not matter, or it is settled among the listed tokens, which are then
+    // all of the first top_k (the weights of the others are not needed: 256 rows of 32000 with both limits 27.2 us instead of 33.3, with
+    // top-k alone 24.1 instead of 30.2).  On short rows only if the list then is short enough to be compared at once, since narrowing it
+    // takes more than the weights do (100 rows of 1000 with top_k 50 13.4 us
+    // instead of 15.0, but with top_k up to 99 16.2 instead of 14.7; 256 of 16000 24.8 and 25.0).
+    __device__ __forceinline__ bool counted() const { return top_k != 0 && (top_p >= 1.0 || top_k <= list_all); }
 };
 
 __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const double *power, uint32_t row, float largest)
@@ -135,6 +147,7 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const d
     r.power = power;
     r.least = ldexp(m < 1.0f ? (double)m : m != m ? 0.0 : 1.0, a.s);   // (NaN: no limit; the largest always remains)
     r.top_k = k > 0 && (uint32_t)k < a.cols ? (uint64_t)k : 0u;
+    r.list_all = a.cols > kSampleShort ? kSampleListAll : kSampleListAllShort;
     r.uniform = a.uniform[row];
     return r;
 }
@@ -144,6 +157,7 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const d
 struct SampleCut {
     uint32_t k_bin, p_first, p_last;
     uint32_t above_k;          // tokens in the bins before k_bin
+    uint32_t all;              // every token that may remain is listed (p_first 0, masses 0)
     uint64_t mass_k, mass_p;   // weights in the bins before k_bin and before p_first; mass_k: of all bins where there is no k_bin
 
     // bins before sure() are in, those from behind() on are out (p_last is k_bin at most where both are there)
@@ -327,6 +341,13 @@ template <uint32_t THREADS> struct Sampler {
     // Tokens per bin for top-k, weights per bin for top-p
     __device__ __forceinline__ void histogram(const SampleRules &r, uint32_t first, uint32_t last)
     {
+        if (r.counted()) {
+            // (of those that may have no weight, at the end of the order, too: that they take no place among top_k makes no difference)
+            each(first, last, [&](float v, uint32_t) {
+                if (r.depth(v) <= SampleRules::kDeepest) atomicAdd(&sh.bins.count[r.bin(v)], 1u);
+            });
+            return;
+        }
         each(first, last, [&](float v, uint32_t) {
             bool above;
             const uint64_t whole = r.weight(v, above);
@@ -382,7 +403,7 @@ template <uint32_t THREADS> struct Sampler {
     // sh.cut from the whole row's histogram in sh.bins
     __device__ __forceinline__ void find_cut(const SampleRules &r)
     {
-        if (tid == 0) sh.cut = SampleCut{kNoBin, kNoBin, kNoBin, 0, 0, 0};
+        if (tid == 0) sh.cut = SampleCut{kNoBin, kNoBin, kNoBin, 0, 0, 0, 0};
         const Running all = running();
         const bool by_k = r.top_k != 0 && r.top_k < all.all_count;
         if (!by_k && tid == 0) sh.cut.mass_k = all.all_mass;
@@ -396,7 +417,13 @@ template <uint32_t THREADS> struct Sampler {
                 }
             });
         __syncthreads();
-        if (r.top_p < 1.0) {
+        if (r.top_p < 1.0 && r.counted()) {
+            if (tid == 0) {
+                sh.cut.all = 1;
+                sh.cut.p_first = 0;
+                sh.cut.p_last = by_k ? sh.cut.k_bin : kSampleBins - 1u;
+            }
+        } else if (r.top_p < 1.0) {
             const double low = goal(r.top_p, sh.cut.mass_k), high = goal(r.top_p, by_k ? sh.taken_mass : all.all_mass);
             each_bin(all, [&](uint32_t b, uint32_t, uint32_t, uint64_t m0, uint64_t m) {
                 if ((double)m0 < low && (double)(m0 + m) >= low) {
@@ -421,7 +448,7 @@ template <uint32_t THREADS> struct Sampler {
     __device__ __forceinline__ void gather(const SampleRules &r, const SampleCut &cut, uint32_t first, uint32_t last)
     {
         // (a token that is neither in for certain nor out is looked at again below, where its bin is settled)
-        const float sure = SampleRules::begin(cut.sure()), end = SampleRules::begin(cut.behind());
+        const float sure = SampleRules::begin(cut.sure()), end = fminf(SampleRules::begin(cut.behind()), SampleRules::kDeepest + 1.0f);
         // (a part is half a batch long or whole batches)
         uint64_t sum[2] = {0, 0};
         uint32_t pending = 0;   // those of a thread's batch that are to be listed: seldom more than one, and not worth eight tries a wave
@@ -562,10 +589,10 @@ template <uint32_t THREADS> struct Sampler {
         if (cut.k_bin != kNoBin) least = narrow(r, n, cut.k_bin, cut.k_bin, 0, false, r.top_k, 0.0, cut.above_k, cut.mass_k);
         if (cut.p_first != kNoBin) {
             uint64_t in_k = 0;
-            if (cut.k_bin != kNoBin)
+            if (cut.k_bin != kNoBin || cut.all)
                 for (uint32_t i = tid; i < n; i += THREADS) {
                     const uint64_t key = sh.list.key[i];
-                    if (key >= least && r.bin(sample_value((uint32_t)(key >> 32))) == cut.k_bin) in_k += sh.list.mass[i] & ~(1ull << 63);
+                    if (key >= least && (cut.all || r.bin(sample_value((uint32_t)(key >> 32))) == cut.k_bin)) in_k += sh.list.mass[i] & ~(1ull << 63);
                 }
             in_k = block_sum(in_k);
             const uint64_t by_p = narrow(r, n, cut.p_first, cut.p_last, least, true, 0, goal(r.top_p, cut.mass_k + in_k), 0, cut.mass_p);
@@ -745,7 +772,7 @@ template <int WAVES> __global__ __launch_bounds__(1024, WAVES) void k_sample(con
         if (s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
         return;
     }
-    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
+    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0, 0};
     if (r.limited()) {
         s.clear_bins();
         s.histogram(r, 0, a.spans - 1u);
@@ -845,7 +872,7 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
         if (blockIdx.x == 0 && s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
         return;
     }
-    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0};
+    SampleCut cut = {kNoBin, kNoBin, kNoBin, 0, 0, 0, 0};
     if (r.limited()) cut = state.cut;
     s.fill_power();
     if (s.tid < kSampleSpans) sh.spans[s.tid] = 0;

@@ -454,6 +454,22 @@ def test_sample(dev, rows, cols, spread):
     assert np.array_equal(*draw_tokens(dev, x, u, t, k=rng.integers(1, cols + 1, rows), p=rng.uniform(0.5, 1.0, rows), mp=rng.uniform(0, 0.05, rows)))
 
 
+@pytest.mark.parametrize("rows,cols", [(6, 1000), (5, 12288), (5, 12289), (3, 60000), (70, 40000)])
+@pytest.mark.parametrize("most", [40, 100, 900])
+def test_sample_by_both_limits(dev, rows, cols, most):
+    # a small top_k's tokens are listed one and all, a large one's only where it ends; with few tokens that have any weight, and with many
+    rng = np.random.default_rng(rows * 31 + cols + most)
+    x = (2 * rng.standard_normal((rows, cols))).astype(np.float32)
+    x[0, rng.permutation(cols)[:cols - 30]] = -1e9
+    x[1, rng.permutation(cols)[:cols - 700]] = -np.inf
+    x[2, rng.permutation(cols)[:300]] = 9.0
+    u, t = rng.random(rows), rng.uniform(0.2, 1.5, rows)
+    k, p = rng.integers(1, most + 1, rows), rng.uniform(0.3, 1.0, rows)
+    for limits in (dict(k=k, p=p), dict(k=k), dict(k=np.full(rows, most), p=p), dict(k=k, p=np.ones(rows)), dict(k=k, p=np.full(rows, 1e-6)),
+                   dict(k=k, p=p, mp=rng.uniform(0, 0.2, rows))):
+        assert np.array_equal(*draw_tokens(dev, x, u, t, **limits))
+
+
 @pytest.mark.parametrize("cols", [7, 1000, 40000])
 def test_sample_among_equal_logits(dev, cols):
     # few distinct values, so that top-k and top-p end among equals, where the lower index stays
