@@ -499,11 +499,11 @@ struct Fp8Form {
 #define TWM_FP8_FORM(S, TN, TM, WN, WM, ...) \
     Fp8Form{S * TN * WN, S * TM * WM, WN * WM * 64, (uint32_t)sizeof(Fp8Tile<S * TM * WM, S * TN * WN>), k_fp8_tile<S, TN, TM, WN, WM>, __VA_ARGS__}
 const Fp8Form kFp8Forms[] = {
-    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.56f, 1.15f, 5.6f, 0.00f),   // 256 columns x 256 rows, eight waves
-    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.76f, 0.57f, 2.6f, 0.00f),   // 128 x 128
-    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.39f, 1.7f, 0.07f),   // 128 columns x 64 rows
-    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.91f, 0.76f, 3.8f, 0.00f),   // 128 x 128, sums of exact products
-    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.64f, 0.48f, 1.9f, 0.12f),   // 128 columns x 64 rows, sums of exact products
+    TWM_FP8_FORM(16, 8, 4, 2, 4, 1, 1.55f, 0.52f, 4.6f, 0.00f),   // 256 columns x 256 rows, eight waves
+    TWM_FP8_FORM(16, 4, 4, 2, 2, 2, 0.68f, 0.49f, 2.6f, 0.05f),   // 128 x 128
+    TWM_FP8_FORM(16, 4, 2, 2, 2, 3, 0.57f, 0.37f, 0.9f, 0.04f),   // 128 columns x 64 rows
+    TWM_FP8_FORM(32, 2, 2, 2, 2, 2, 0.91f, 0.72f, 3.9f, 0.00f),   // 128 x 128, sums of exact products
+    TWM_FP8_FORM(32, 2, 1, 2, 2, 3, 0.64f, 0.48f, 1.7f, 0.13f),   // 128 columns x 64 rows, sums of exact products
 };
 constexpr uint32_t kFp8Fast = 3, kFp8FormCount = sizeof kFp8Forms / sizeof kFp8Forms[0];   // the first ones: 8-bit instructions
 
@@ -538,17 +538,27 @@ hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, floa
     return hipGetLastError();
 }
 
-// Which kernel: few = 1, 2, 4: k_fp8_rows_few with that many times 16 rows; 0: k_fp8_tile in `form`.  splits: ranges of K.
+// Which kernel: few = 1, 2, 4: k_fp8_rows_few with that many times 16 rows and (few > 1) `form` times 16 columns; 0: k_fp8_tile in
+// `form`.  splits: ranges of K.
 struct Fp8Plan {
     uint32_t few, form, splits;
 };
 
-constexpr double kFp8Bandwidth = 6.5e6, kFp8SplitBandwidth = 6.2e6;             // bytes per us: operands from memory; ranges' sums out and in
-constexpr double kFp8Launch = 2.34, kFp8SecondLaunch = 1.61, kFp8PerSplit = 0.17;   // us
+constexpr double kFp8Bandwidth = 8.9e6, kFp8SplitBandwidth = 6.7e6;             // bytes per us: operands from memory; ranges' sums out and in
+constexpr double kFp8Launch = 1.93, kFp8SecondLaunch = 1.65, kFp8PerSplit = 0.33;   // us
+
+// The kernel for few rows above 16 of them, us: a launch, eight blocks of 128 features, a block of a workgroup alone on a CU, one of many,
+// and a workgroup besides
+struct Fp8FewForm {
+    uint32_t mt, nt;
+    double launch, eight, block_alone, block_among, besides;
+};
+const Fp8FewForm kFp8FewForms[] = {{2, 1, 2.32, 0.08, 0.148, 0.193, 0.114}, {4, 1, 2.13, 0.26, 0.316, 0.387, 0.099}, {4, 2, 2.0, 0.50, 0.375, 0.474, 0.213}};
 
 // Up to 16 rows the kernel for few rows (8 x 3584 x 3584 5.4 us, in tiles 8.5; 16 x 3739 x 15200 19.6 and 20.5; only above a hundred MB of
 // weights are tiles a tenth ahead).  Above, whichever is expected to take the least time, by the figures above: fitted to the
-// times of 170 shapes of 17 .. 2048 rows in every form and split, of which the choice is 0.8 % behind the best in the mean.
+// times of 370 shapes of 17 .. 2048 rows in every form and split, of which the choice is 0.8 % behind the best in the mean.  (The kernel
+// for few rows is ahead where tiles are far fewer than CUs: 200 x 851 x 1024 5.8 us, in tiles 6.9 for f16 results and 8.5 for f32.)
 Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
 {
     if (m <= 16) return Fp8Plan{1, 0, 1};
@@ -578,13 +588,15 @@ Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
                 best = Fp8Plan{0, i, splits};
             }
         }
-        if (m <= 128 && splits <= 4) {
-            const uint32_t mt = m <= 32 ? 2u : 4u;
-            const uint64_t groups = (uint64_t)((n + 15) / 16) * ((m + 16 * mt - 1) / (16 * mt)) * splits;
-            const double us = (mt == 2 ? 2.18 + (per + 7) / 8 * 0.57 + groups * per * 0.162 / 256 : 2.0 + (per + 7) / 8 * 0.97 + groups * per * 0.254 / 256) + joined;
-            if (us < least && (splits == 1 || groups <= 512)) {
+        for (const Fp8FewForm &f : kFp8FewForms) {
+            const uint64_t tiles = (uint64_t)((n + 16 * f.nt - 1) / (16 * f.nt)) * ((m + 16 * f.mt - 1) / (16 * f.mt)), groups = tiles * splits;
+            // (32 columns, with less than four blocks: most of the eight waves have none; 38 x 9269 x 256 5.8 us, in tiles 4.2)
+            if (m > 400 || (m <= 32) != (f.mt == 2) || (f.nt == 2 && kb < 4) || (splits > 1 && (splits > 4 || tiles > 192 || kb / splits < 4))) continue;
+            const double alone = per * f.block_alone, among = groups * (per * f.block_among + f.besides) / 256;
+            const double us = f.launch + (per + 7) / 8 * f.eight + (alone > among ? alone : among) + joined;
+            if (us < least) {
                 least = us;
-                best = Fp8Plan{mt, 0, splits};
+                best = Fp8Plan{f.mt, f.nt, splits};
             }
         }
     }
@@ -623,7 +635,8 @@ hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scale
     const Fp8Plan plan = plan_fp8(m, n, k, c_f16, ws_bytes);
     if (plan.few == 0) return launch_fp8_tile(s, g, plan.form, plan.splits, ws, ws_bytes);
     if (plan.few == 2) return launch_fp8_few<2, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
-    if (plan.few == 4) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
+    if (plan.few == 4 && plan.form == 1) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
+    if (plan.few == 4) return launch_fp8_few<4, 2, 1, 8>(s, g, plan.splits, ws, ws_bytes);
     switch (fp8_few_form(n, k)) {
     case kFewNarrow: return launch_fp8_few<1, 1, 1, 16>(s, g, 1, ws, ws_bytes);
     case kFewTwo: return launch_fp8_few<1, 2, 1, 16>(s, g, 1, ws, ws_bytes);
@@ -644,7 +657,7 @@ void describe_fp8_gemm(uint32_t m, uint32_t n, uint32_t k, bool c_f16, size_t ws
     } else {
         const Fp8Few form = plan.few == 1 ? fp8_few_form(n, k) : kFewTwoShallow;
         snprintf(text, bytes, "k_fp8_rows_few: %u columns x %u rows, %u waves, f16 instructions, %u K-split%s",
-                 plan.few == 1 && (form == kFewTwo || form == kFewTwoShallow) ? 32u : 16u, 16u * plan.few, form == kFewMany ? 4u : form == kFewTwoShallow ? 8u : 16u, plan.splits,
+                 (plan.few == 1 ? form == kFewTwo || form == kFewTwoShallow : plan.form == 2) ? 32u : 16u, 16u * plan.few, form == kFewMany ? 4u : form == kFewTwoShallow ? 8u : 16u, plan.splits,
                  plan.splits == 1 ? "" : "s");
     }
 }

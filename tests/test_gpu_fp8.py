@@ -312,7 +312,8 @@ def check_gemm(dev, inputs, m, n, k, dtype, skip=0):
 GEMMS = [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 130, 272), (3, 64, 112), (1, 896, 896), (5, 256, 1024), (15, 129, 704), (16, 100, 2816), (17, 260, 640),
          (31, 384, 1040), (32, 128, 4096), (33, 1, 256), (40, 640, 704), (64, 300, 1152), (65, 96, 512), (77, 513, 384), (100, 255, 2064), (128, 512, 1024),
          (129, 257, 1040), (200, 384, 256), (256, 256, 128), (257, 640, 1296), (300, 1000, 528), (513, 130, 896), (1, 4096, 18944), (13, 4096, 4096), (7, 8, 16),
-         (1030, 520, 272), (48, 3584, 2048), (17, 17, 6464), (30, 400, 8208), (50, 40, 3216), (70, 264, 4112), (70001, 5, 32), (1, 300001, 16), (3, 70000, 48)]
+         (1030, 520, 272), (48, 3584, 2048), (17, 17, 6464), (30, 400, 8208), (50, 40, 3216), (70, 264, 4112), (70001, 5, 32), (1, 300001, 16), (3, 70000, 48),
+         (33, 1401, 2064), (80, 2047, 256), (200, 850, 1040), (390, 333, 400), (450, 130, 1024), (450, 97, 400), (420, 260, 3216)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -325,7 +326,7 @@ def test_gemm(dev, m, n, k, dtype):
 LARGE_GEMMS = [(1500, 9000, 144, "f16"), (2049, 8200, 400, "f16"), (1500, 4100, 272, "f16"), (1500, 4100, 272, "f32"), (200, 9000, 4112, "f16"), (200, 9000, 4112, "f32"),
                (333, 3584, 18944, "f16"), (333, 3584, 18944, "f32"), (90, 5003, 2064, "f16"), (24, 3001, 9040, "f32"), (12, 20001, 1040, "f32"), (12, 20001, 4112, "f16"),
                (5, 9001, 1040, "f32"), (142, 11098, 5488, "f16"), (500, 24700, 272, "f16"), (1000, 24712, 400, "f16"),
-               (520, 24697, 272, "f16"), (140, 12001, 6800, "f16"), (140, 12000, 6800, "f16"), (266, 19760, 400, "f32")]
+               (520, 24697, 272, "f16"), (140, 12001, 6800, "f16"), (140, 12000, 6800, "f16"), (266, 19760, 400, "f32"), (137, 12001, 9040, "f16")]
 
 
 @pytest.mark.parametrize("m,n,k,dtype", LARGE_GEMMS)
