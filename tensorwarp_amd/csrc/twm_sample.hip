@@ -11,7 +11,7 @@
 //   The token is the first by index at which the running sum of what remains exceeds u times the whole.
 //
 // How a row is worked through: its largest logit; then, where top-k or top-p ask for it, a histogram of the tokens' numbers and
-// weights over 2048 bins of (max - x) / temperature, 1/64 wide, in LDS; from its running sums the one or two bins in which top-k
+// weights over 2048 bins of (max - x) / temperature, 1/64 wide or narrower, in LDS; from its running sums the one or two bins in which top-k
 // and top-p end; then one more pass that adds the weights of the tokens in the bins before those and lists the tokens in them
 // (some hundred), whose exact order is settled by ranges of their keys until a wave's lanes hold them; and at last the running sum
 // through the one part of the row that u falls into.  A row whose list would be too long (thousands of nearly equal logits) is
@@ -19,12 +19,13 @@
 // rows: parts of a row each have a workgroup, in up to three launches, the last workgroup of a row to arrive doing what concerns the
 // whole row.
 //
-// Measured: 1 row of 152064 logits 14 us without limits, 20 with top-k, 23 with top-k and top-p, 25 with top-p; 32 such rows 42 with
-// top-p and 31 with both; 256 rows of 32000 23 without limits, 24, 27 and 40.  Bound: for one row latency (three launches, 2.5 us from
+// Measured: 1 row of 152064 logits 14 us without limits, 20 with top-k, 24 with top-k and top-p, 25 with top-p; 32 such rows 43 with
+// top-p and 33 with both; 256 rows of 32000 23 without limits, 25, 28 and 40.  Bound: for one row latency (three launches, 2.5 us from
 // the end of one to the first load of the next; the passes themselves 1 to 3 us; histogram to cut and list to token 4 and 7); for many
 // rows the vector instructions of the weights, 33 a token in each of two passes, eighteen of them in 64 bits: of 40 us for 256 rows of
 // 32000 the largest logit takes 6, the histogram 11, the cut 1.5, adding and listing 12, settling the list 3, the token 3.  Rows kept in
-// registers over the passes changed nothing.
+// registers over the passes (25.5 us instead of 27.2 with both limits, 24.4 instead of 22.7 without any) and the tokens that are in
+// gathered ahead of their weights (40.1 and 40.3) were not worth their code.
 #include "twm_device.h"
 
 namespace twm {
@@ -74,9 +75,8 @@ struct SampleArgs {
 };
 
 struct SampleRules {
-    static constexpr float kDeepest = 64.0f * 40.0f;   // depth (see there) from which on weights are nothing
     float largest, finite;             // finite: the largest, or 0 for an infinity
-    float per_bin;                     // 64 / temperature, in 32 bits
+    float per_bin, deepest;            // bins / temperature, in 32 bits; depth (see there) from which on weights are nothing
     double log2_one, top_p, least, uniform;   // log2_one = 64 log2(e) / temperature; least = 2^S min_p
     uint64_t top_k;        // 0: no limit
     uint32_t list_all;
@@ -91,7 +91,7 @@ struct SampleRules {
     __device__ __forceinline__ uint64_t weight(float v, bool &above) const
     {
         const bool top = v == largest;
-        const bool any = depth(v) <= kDeepest;   // (NaN: a NaN)
+        const bool any = depth(v) <= deepest;   // (NaN: a NaN)
         const double d = (double)(top ? finite : v) - (double)finite, at = fma(d, log2_one, 6755399441055744.0);
         const uint32_t n = (uint32_t)__double2loint(at);
         const double f = fma(d, log2_one, 6755399441055744.0 - at), p = power[n % 64u];
@@ -114,7 +114,7 @@ struct SampleRules {
         const uint64_t whole = weight(v, above);
         return above ? whole : 0;
     }
-    // 64 (largest - v) / temperature: falls as v grows, like its weight's logarithm; every rounding in it keeps the order
+    // bins (largest - v) / temperature: falls as v grows, like its weight's logarithm; every rounding in it keeps the order
     __device__ __forceinline__ float depth(float v) const { return v == largest ? 0.0f : (largest - v) * per_bin; }
     __device__ __forceinline__ uint32_t bin(float v) const
     {
@@ -133,8 +133,16 @@ struct SampleRules {
     __device__ __forceinline__ bool counted() const { return top_k != 0 && (top_p >= 1.0 || top_k <= list_all); }
 };
 
-__device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const double *power, uint32_t row, float largest)
+// What a pass over the row leaves: the largest key, and the smallest logit above -infinity, as the inverted number that orders as it
+// does (0: none)
+struct SampleEnds {
+    uint64_t key;
+    uint32_t low;
+};
+
+__device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const double *power, uint32_t row, const SampleEnds &ends)
 {
+    const float largest = sample_value((uint32_t)(ends.key >> 32));
     SampleRules r;
     r.largest = largest;
     r.finite = fabsf(largest) < INFINITY ? largest : 0.0f;
@@ -142,7 +150,13 @@ __device__ __forceinline__ SampleRules sample_rules(const SampleArgs &a, const d
     const int k = a.top_k ? a.top_k[row] : 0;
     r.greedy = !(t > 0.0f);
     r.log2_one = 64.0 * 1.4426950408889634 / (double)t;
-    r.per_bin = 64.0f / t;
+    // 64 bins for a factor of e; more where the row's logits are so close that it needs less than all 2048 bins (thousands of tokens would
+    // share one, too many for the list: 152064 logits of a deviation of 0.1, top-p, 363 us with 64, 27 so).  2040: those of a last
+    // rounding stay below 2047.
+    const float per_one = 1.0f / t, range = (largest - sample_value(~ends.low)) * per_one, more = 2040.0f * __builtin_amdgcn_rcpf(fmaxf(range, 1e-3f));
+    const float bins = range < 31.0f && more * per_one < 1e37f ? more : 64.0f;   // (NaN: 64)
+    r.per_bin = bins * per_one;
+    r.deepest = 40.0f * bins;
     r.top_p = p < 1.0f ? (double)p : 1.0;   // (NaN: no limit)
     r.power = power;
     r.least = ldexp(m < 1.0f ? (double)m : m != m ? 0.0 : 1.0, a.s);   // (NaN: no limit; the largest always remains)
@@ -169,6 +183,7 @@ struct SampleCut {
 // What a row's workgroups leave for each other between and within launches
 struct SampleRow {
     uint64_t key[kSampleSpans], mass[kSampleSpans];
+    uint32_t low[kSampleSpans];
     uint64_t bin_mass[kSampleBins];
     uint32_t bin_count[kSampleBins];
     uint64_t list_key[kSampleList], list_mass[kSampleList];
@@ -192,7 +207,8 @@ struct SampleShared {
     uint64_t wave64[16];
     uint32_t wave32[16];
     SampleCut cut;
-    uint64_t largest, prefix, taken_mass, least, low, high;
+    SampleEnds ends;
+    uint64_t prefix, taken_mass, least, low, high;
     uint32_t listed, taken_count, stop, base;
 };
 
@@ -300,21 +316,24 @@ template <uint32_t THREADS> struct Sampler {
         return lane_value(wave_running<16>(sh.wave64[lane % 16u]), 15);
     }
 
-    // the largest key of parts first .. last, in thread 0
-    __device__ __forceinline__ uint64_t largest(uint32_t first, uint32_t last)
+    // of parts first .. last, in thread 0
+    __device__ __forceinline__ SampleEnds ends(uint32_t first, uint32_t last)
     {
-        uint64_t most = 0;
+        SampleEnds e = {0, 0};
         each(first, last, [&](float v, uint32_t i) {
             const uint64_t key = sample_key(v, i);
-            most = key > most ? key : most;
+            e.key = key > e.key ? key : e.key;
+            e.low = v > -INFINITY ? max(e.low, ~(uint32_t)(key >> 32)) : e.low;
         });
-        most = wave_most_u64(most);
-        if (lane == 0) sh.wave64[wave] = most;
+        e.key = wave_most_u64(e.key);
+        e.low = wave_most_u32(e.low);
+        if (lane == 0) {
+            sh.wave64[wave] = e.key;
+            sh.wave32[wave] = e.low;
+        }
         __syncthreads();
-        if (tid == 0)
-#pragma unroll
-            for (uint32_t w = 1; w < kWaves; w++) most = sh.wave64[w] > most ? sh.wave64[w] : most;
-        return most;
+        if (wave == 0) e = SampleEnds{wave_most_u64(sh.wave64[lane % 16u]), wave_most_u32(sh.wave32[lane % 16u])};
+        return e;
     }
 
     // SampleRules::power: the exponential's series up to the twelfth power, |x| <= ln 2 / 2 (seen after the workgroup's next barrier)
@@ -344,7 +363,7 @@ template <uint32_t THREADS> struct Sampler {
         if (r.counted()) {
             // (of those that may have no weight, at the end of the order, too: that they take no place among top_k makes no difference)
             each(first, last, [&](float v, uint32_t) {
-                if (r.depth(v) <= SampleRules::kDeepest) atomicAdd(&sh.bins.count[r.bin(v)], 1u);
+                if (r.depth(v) <= r.deepest) atomicAdd(&sh.bins.count[r.bin(v)], 1u);
             });
             return;
         }
@@ -448,7 +467,7 @@ template <uint32_t THREADS> struct Sampler {
     __device__ __forceinline__ void gather(const SampleRules &r, const SampleCut &cut, uint32_t first, uint32_t last)
     {
         // (a token that is neither in for certain nor out is looked at again below, where its bin is settled)
-        const float sure = SampleRules::begin(cut.sure()), end = fminf(SampleRules::begin(cut.behind()), SampleRules::kDeepest + 1.0f);
+        const float sure = SampleRules::begin(cut.sure()), end = fminf(SampleRules::begin(cut.behind()), r.deepest + 1.0f);
         // (a part is half a batch long or whole batches)
         uint64_t sum[2] = {0, 0};
         uint32_t pending = 0;   // those of a thread's batch that are to be listed: seldom more than one, and not worth eight tries a wave
@@ -587,6 +606,8 @@ template <uint32_t THREADS> struct Sampler {
         uint64_t least = 0;
         if (n == 0) return ~0ull;
         if (cut.k_bin != kNoBin) least = narrow(r, n, cut.k_bin, cut.k_bin, 0, false, r.top_k, 0.0, cut.above_k, cut.mass_k);
+        // (where the first top_k end among tokens that were counted but have no weight, the listed ones are all within them)
+        if (cut.all && least == ~0ull) least = 0;
         if (cut.p_first != kNoBin) {
             uint64_t in_k = 0;
             if (cut.k_bin != kNoBin || cut.all)
@@ -760,14 +781,14 @@ template <int WAVES> __global__ __launch_bounds__(1024, WAVES) void k_sample(con
     Sampler<1024> s(a, sh, blockIdx.x);
     s.fill_power();
     if (s.tid < kSampleSpans) sh.spans[s.tid] = 0;
-    const uint64_t most = s.largest(0, a.spans - 1u);
+    const SampleEnds ends = s.ends(0, a.spans - 1u);
     if (s.tid == 0) {
-        sh.largest = most;
+        sh.ends = ends;
         sh.listed = 0;
     }
     __syncthreads();
-    const uint64_t key = sh.largest;
-    const SampleRules r = sample_rules(a, sh.power, s.row, sample_value((uint32_t)(key >> 32)));
+    const uint64_t key = sh.ends.key;
+    const SampleRules r = sample_rules(a, sh.power, s.row, sh.ends);
     if (!sample_any(key) || r.greedy) {
         if (s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
         return;
@@ -810,11 +831,11 @@ __device__ __forceinline__ bool last_to_arrive(SampleShared &sh, unsigned *count
     return sh.stop != 0;
 }
 
-// the row's largest key, from its workgroups' (of the launch before)
-__device__ __forceinline__ uint64_t row_key(const SampleRow &state, uint32_t groups)
+// the row's ends, from its workgroups' (of the launch before)
+__device__ __forceinline__ SampleEnds row_ends(const SampleRow &state, uint32_t groups)
 {
     const uint32_t lane = threadIdx.x & 63u;
-    return wave_most_u64(lane < groups ? state.key[lane] : 0);
+    return SampleEnds{wave_most_u64(lane < groups ? state.key[lane] : 0), wave_most_u32(lane < groups ? state.low[lane] : 0u)};
 }
 
 }  // namespace
@@ -828,9 +849,10 @@ __global__ __launch_bounds__(1024) void k_sample_largest(const SampleArgs a, Sam
         state.bin_mass[b] = 0;
         state.bin_count[b] = 0;
     }
-    const uint64_t key = s.largest(first_part(a), last_part(a));
+    const SampleEnds ends = s.ends(first_part(a), last_part(a));
     if (s.tid == 0) {
-        state.key[blockIdx.x] = key;
+        state.key[blockIdx.x] = ends.key;
+        state.low[blockIdx.x] = ends.low;
         if (blockIdx.x == 0) state.listed = 0;
     }
 }
@@ -840,8 +862,9 @@ __global__ __launch_bounds__(1024) void k_sample_limits(const SampleArgs a, Samp
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.y);
     SampleRow &state = rows[blockIdx.y];
-    const uint64_t key = row_key(state, gridDim.x);
-    const SampleRules r = sample_rules(a, sh.power, s.row, sample_value((uint32_t)(key >> 32)));
+    const SampleEnds ends = row_ends(state, gridDim.x);
+    const uint64_t key = ends.key;
+    const SampleRules r = sample_rules(a, sh.power, s.row, ends);
     if (!sample_any(key) || r.greedy || !r.limited()) return;
     s.fill_power();
     s.clear_bins();
@@ -866,8 +889,9 @@ __global__ __launch_bounds__(1024) void k_sample_token(const SampleArgs a, Sampl
     __shared__ SampleShared sh;
     Sampler<1024> s(a, sh, blockIdx.y);
     SampleRow &state = rows[blockIdx.y];
-    const uint64_t key = row_key(state, gridDim.x);
-    const SampleRules r = sample_rules(a, sh.power, s.row, sample_value((uint32_t)(key >> 32)));
+    const SampleEnds ends = row_ends(state, gridDim.x);
+    const uint64_t key = ends.key;
+    const SampleRules r = sample_rules(a, sh.power, s.row, ends);
     if (!sample_any(key) || r.greedy) {
         if (blockIdx.x == 0 && s.tid == 0) a.out[s.row] = sample_any(key) ? sample_index(key) : 0;
         return;

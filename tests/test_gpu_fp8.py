@@ -455,6 +455,23 @@ def test_sample(dev, rows, cols, spread):
     assert np.array_equal(*draw_tokens(dev, x, u, t, k=rng.integers(1, cols + 1, rows), p=rng.uniform(0.5, 1.0, rows), mp=rng.uniform(0, 0.05, rows)))
 
 
+@pytest.mark.parametrize("rows,cols", [(4, 900), (3, 40000), (2, 152064), (70, 32000)])
+@pytest.mark.parametrize("spread", [1e-30, 1e-6, 0.003, 0.1])
+def test_sample_among_close_logits(dev, rows, cols, spread):
+    # thousands of tokens within a factor of e^(1/64); a row of equals, one that nothing but its first token sets apart, masks of the type's
+    # lowest value, and temperatures that spread the row out again
+    rng = np.random.default_rng(rows + cols)
+    x = (spread * rng.standard_normal((rows, cols)) + (0.0 if spread < 1e-7 else 3.0)).astype(np.float32)
+    x[0] = 0.7
+    x[1, 1:] = x[1, 2]
+    x[-1, ::3] = -np.inf
+    x[-1, 1] = np.finfo(np.float32).min if rows > 3 else x[-1, 1]
+    u = rng.random(rows)
+    for t in (None, np.full(rows, 2.0), np.full(rows, spread), np.full(rows, spread / 30)):
+        assert np.array_equal(*draw_tokens(dev, x, u, t, p=np.full(rows, 0.9)))
+        assert np.array_equal(*draw_tokens(dev, x, u, t, k=rng.integers(1, cols + 1, rows), p=rng.uniform(0.1, 1.0, rows)))
+
+
 @pytest.mark.parametrize("rows,cols", [(6, 1000), (5, 12288), (5, 12289), (3, 60000), (70, 40000)])
 @pytest.mark.parametrize("most", [40, 100, 900])
 def test_sample_by_both_limits(dev, rows, cols, most):
