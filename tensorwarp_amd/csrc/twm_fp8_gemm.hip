@@ -6,7 +6,7 @@
 // Two ways to a block's sum.  The matrix unit's 8-bit instructions cut every product of eight neighbouring features off below 2^-13 of
 // the largest one's power of two before they add (measured: 2^14 + 2^0 is 2^14 within a group of eight and exact across two; against the
 // exact sum results were off by 1.2e-5 of their norm on bell-shaped values and 5e-5 on evenly drawn codes).  That is below the rounding
-// of an f16 result (2^-11), so f16 results of more than 16 rows use them.  f32 results, which are to hold 32-bit sums, do not, and
+// of an f16 result (2^-11), so f16 results of more than 16 rows use them in tiles.  f32 results, which are to hold 32-bit sums, do not, and
 // those of up to 16 rows, which wait for the weights, have no need to: the codes become f16 there, which holds each exactly, as do the
 // f32 products of the f16 instructions.  A block's sum is scaled by one f32 factor per lane (the rows of A are the lanes' columns of the
 // result, those of W lie in its registers) and added to the f32 sum.  Both arrays are read as the caller holds them, row by
