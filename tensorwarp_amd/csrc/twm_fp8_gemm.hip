@@ -13,8 +13,8 @@
 // row: a lane's operand is 32 consecutive bytes of a row, and which of the 128 features a lane holds does not matter as long as
 // both operands agree.
 //
-// Measured, and what bounds it: one row of 3584 -> 37888 24.8 us, 5.5 TB/s: the weights' way from memory; 13 rows of 11008 -> 4096 12.1,
-// 3.7 TB/s: the ramp and the tail of a launch of 256 workgroups; 333 rows of 18944 -> 3584 40: tiles 33 (the operands' way to LDS) and the six
+// Measured, and what bounds it: one row of 3584 -> 37888 24.8 us, 5.5 TB/s: the weights' way from memory; 13 rows of 11008 -> 4096 11.7,
+// 3.9 TB/s: the ramp and the tail of a launch of 256 workgroups and the two ranges' sums; 333 rows of 18944 -> 3584 40: tiles 33 (the operands' way to LDS) and the six
 // ranges' sums 6; 2048 rows of 4096 -> 22016 179, 2.06 PFLOP/s in f16: products with the factors' multiplications take 104 to 116 by
 // themselves, the operands' way to LDS 149 (9.4 TB/s over the chip), and the two do not overlap wholly.  A ring of five buffers with two
 // blocks' loads in flight took 187 to 190 where this took 172, tiles of 256 x 192 were behind but for a few row counts.
@@ -538,14 +538,45 @@ hipError_t launch_fp8_few(hipStream_t s, const Fp8Gemm &g, uint32_t splits, floa
     return hipGetLastError();
 }
 
-// Which kernel: few = 1, 2, 4: k_fp8_rows_few with that many times 16 rows and (few > 1) `form` times 16 columns; 0: k_fp8_tile in
-// `form`.  splits: ranges of K.
+// Which kernel: few = 1: k_fp8_rows_few in that of kFp8OneForms, 2, 4: with that many times 16 rows and `form` times 16 columns; 0:
+// k_fp8_tile in `form`.  splits: ranges of K.
 struct Fp8Plan {
     uint32_t few, form, splits;
 };
 
 constexpr double kFp8Bandwidth = 8.9e6, kFp8SplitBandwidth = 6.7e6;             // bytes per us: operands from memory; ranges' sums out and in
 constexpr double kFp8Launch = 1.93, kFp8SecondLaunch = 1.65, kFp8PerSplit = 0.33;   // us
+
+// Up to 16 rows: columns (in 16s) and waves of the kernel for few rows
+struct Fp8OneForm {
+    uint32_t nt, waves;
+    hipError_t (*launch)(hipStream_t, const Fp8Gemm &, uint32_t, float *, size_t);
+};
+enum : uint32_t { kOneNarrow, kOneNarrowDeep, kOneTwo, kOneTwoShallow, kOneMany };
+const Fp8OneForm kFp8OneForms[] = {{1, 8, launch_fp8_few<1, 1, 2, 8>}, {1, 16, launch_fp8_few<1, 1, 2, 16>}, {2, 16, launch_fp8_few<1, 2, 1, 16>},
+                                   {2, 8, launch_fp8_few<1, 2, 1, 8>}, {1, 4, launch_fp8_few<1, 1, 2, 4>}};
+
+// One round of workgroups where there is one (of 32 columns where 16 would take two; 1 x 3584 x 4608 6.3 us, of 16 6.5, at 8 rows 7.0
+// and 8.1; 1 x 37888 x 3584 24.7 and 25.5, at 16 rows 31 and 39).  On narrow matrices two blocks a wave in flight in eight waves
+// (1 x 1100 x 4864 4.9 us, one in sixteen 5.1; 16 x 4096 x 2816 5.1 and 5.3), in sixteen where a few rows wait for much from memory
+// (1 x 4096 x 18944 15.4, in eight 18.4).  A long K is shared out: among four ranges where the columns fill less than half the CUs
+// (1 x 1100 x 18944 9.7 us, in one 13.3; 16 rows 12.0 and 20.3; 16 x 1100 x 8960 8.3 and 10.3), two where the rows are many enough for their
+// products to count (16 x 4096 x 18944 20.7 and 23.9, 8 x 3584 x 18944 16.7 and 20.4).
+void fp8_one_form(uint32_t m, uint32_t n, uint32_t k, uint32_t &form, uint32_t &splits)
+{
+    const uint32_t tiles = (n + 15u) / 16u, kb = (k + 127u) / 128u;
+    splits = 1;
+    if (tiles > 512u) {
+        form = tiles <= 1024u ? kOneMany : k < 16u * 128u ? kOneTwoShallow : kOneTwo;
+    } else if (tiles > 256u) {
+        form = k < 16u * 128u ? kOneTwoShallow : kOneTwo;
+    } else if ((tiles <= 128u && kb >= 64u) || (m >= 8u && kb >= 80u)) {
+        form = kOneTwoShallow;
+        splits = tiles <= 128u ? 4u : 2u;
+    } else {
+        form = m <= 4u && (uint64_t)n * k > 22000000u ? kOneNarrowDeep : kOneNarrow;
+    }
+}
 
 // The kernel for few rows above 16 of them, us: a launch, eight blocks of 128 features, a block of a workgroup alone on a CU, one of many,
 // and a workgroup besides
@@ -561,9 +592,16 @@ const Fp8FewForm kFp8FewForms[] = {{2, 1, 2.32, 0.08, 0.148, 0.193, 0.114}, {4, 
 // for few rows is ahead where tiles are far fewer than CUs: 200 x 851 x 1024 5.8 us, in tiles 6.9 for f16 results and 8.5 for f32.)
 Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
 {
-    if (m <= 16) return Fp8Plan{1, 0, 1};
     const uint32_t kb = (k + 127u) / 128u;
     const uint64_t n_ld = (n + 3u) & ~3u;
+    if (m <= 16) {
+        Fp8Plan one = {1, 0, 1};
+        fp8_one_form(m, n, k, one.form, one.splits);
+        const uint32_t per = (kb + one.splits - 1) / one.splits;
+        one.splits = per ? (kb + per - 1) / per : 1;
+        if (one.splits * m * n_ld * 4 > ws_bytes) one.splits = 1;
+        return one;
+    }
     Fp8Plan best = {0, f16 ? kFp8Fast - 1 : kFp8FormCount - 1, 1};
     double least = 1e30;
     static const uint32_t kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16};
@@ -603,18 +641,6 @@ Fp8Plan plan_fp8(uint32_t m, uint32_t n, uint32_t k, bool f16, size_t ws_bytes)
     return best;
 }
 
-// one to sixteen rows: one round of workgroups where there is one, of 32 columns where 16 would take two, and sixteen waves each as
-// there are few (m = 1: 3584 x 3584 4.8 us, eight waves 5.1; 3584 x 4608 with 32 columns 6.3, 16 columns 6.5, at 8 rows 7.0 and 8.1;
-// 4096 x 11008 with four waves 10.8, sixteen 11.3; 3584 x 37888 with 32 columns 24.7, 16 columns 25.5, at 16 rows 31 and 39)
-enum Fp8Few { kFewNarrow, kFewTwo, kFewTwoShallow, kFewMany };
-Fp8Few fp8_few_form(uint32_t n, uint32_t k)
-{
-    const uint32_t tiles = (n + 15u) / 16u;
-    if (tiles <= 256u) return kFewNarrow;
-    if (tiles > 512u && tiles <= 1024u) return kFewMany;
-    return k < 16u * 128u ? kFewTwoShallow : kFewTwo;
-}
-
 }  // namespace
 
 // Once per device, outside any stream capture: the forms with more LDS than a launch gets unasked.
@@ -637,12 +663,7 @@ hipError_t launch_fp8_gemm(hipStream_t s, const uint8_t *a, const float *a_scale
     if (plan.few == 2) return launch_fp8_few<2, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
     if (plan.few == 4 && plan.form == 1) return launch_fp8_few<4, 1, 1, 8>(s, g, plan.splits, ws, ws_bytes);
     if (plan.few == 4) return launch_fp8_few<4, 2, 1, 8>(s, g, plan.splits, ws, ws_bytes);
-    switch (fp8_few_form(n, k)) {
-    case kFewNarrow: return launch_fp8_few<1, 1, 1, 16>(s, g, 1, ws, ws_bytes);
-    case kFewTwo: return launch_fp8_few<1, 2, 1, 16>(s, g, 1, ws, ws_bytes);
-    case kFewTwoShallow: return launch_fp8_few<1, 2, 1, 8>(s, g, 1, ws, ws_bytes);
-    default: return launch_fp8_few<1, 1, 2, 4>(s, g, 1, ws, ws_bytes);
-    }
+    return kFp8OneForms[plan.form].launch(s, g, plan.splits, ws, ws_bytes);
 }
 
 void describe_fp8_gemm(uint32_t m, uint32_t n, uint32_t k, bool c_f16, size_t ws_bytes, char *text, size_t bytes)
@@ -655,9 +676,8 @@ void describe_fp8_gemm(uint32_t m, uint32_t n, uint32_t k, bool c_f16, size_t ws
         snprintf(text, bytes, "k_fp8_tile: %u columns x %u rows, %u waves, %s instructions, %u K-split%s", f.bn, f.bm, f.threads / 64, plan.form < kFp8Fast ? "8-bit" : "f16",
                  plan.splits, plan.splits == 1 ? "" : "s");
     } else {
-        const Fp8Few form = plan.few == 1 ? fp8_few_form(n, k) : kFewTwoShallow;
-        snprintf(text, bytes, "k_fp8_rows_few: %u columns x %u rows, %u waves, f16 instructions, %u K-split%s",
-                 (plan.few == 1 ? form == kFewTwo || form == kFewTwoShallow : plan.form == 2) ? 32u : 16u, 16u * plan.few, form == kFewMany ? 4u : form == kFewTwoShallow ? 8u : 16u, plan.splits,
+        const uint32_t nt = plan.few == 1 ? kFp8OneForms[plan.form].nt : plan.form, waves = plan.few == 1 ? kFp8OneForms[plan.form].waves : 8u;
+        snprintf(text, bytes, "k_fp8_rows_few: %u columns x %u rows, %u waves, f16 instructions, %u K-split%s", 16u * nt, 16u * plan.few, waves, plan.splits,
                  plan.splits == 1 ? "" : "s");
     }
 }

@@ -16,8 +16,9 @@ def form_of(m, n, k, dtype):
 
 def test_every_form_is_tested_on_the_gpu():
     tested = {form_of(m, n, k, dtype) for m, n, k in GEMMS for dtype in ("f32", "f16")} | {form_of(*shape) for shape in LARGE_GEMMS}
-    few = ["k_fp8_rows_few: %d columns x 16 rows, %d waves, f16 instructions" % v for v in ((16, 16), (32, 16), (32, 8), (16, 4))]
-    few += ["k_fp8_rows_few: 16 columns x %d rows, 8 waves, f16 instructions%s" % (rows, split) for rows in (32, 64) for split in ("", ", split")]
+    few = ["k_fp8_rows_few: %d columns x 16 rows, %d waves, f16 instructions" % v for v in ((16, 8), (16, 16), (32, 16), (32, 8), (16, 4))]
+    few += ["k_fp8_rows_few: 32 columns x 16 rows, 8 waves, f16 instructions, split"]
+    few += ["k_fp8_rows_few: %d columns x %d rows, 8 waves, f16 instructions%s" % (*form, split) for form in ((16, 32), (16, 64), (32, 64)) for split in ("", ", split")]
     tiles = ["k_fp8_tile: 128 columns x %d rows, 4 waves, %s instructions%s" % (rows, kind, split) for rows in (64, 128) for kind in ("8-bit", "f16")
              for split in ("", ", split")]
     tiles += ["k_fp8_tile: 256 columns x 256 rows, 8 waves, 8-bit instructions%s" % split for split in ("", ", split")]

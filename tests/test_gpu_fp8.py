@@ -313,7 +313,7 @@ GEMMS = [(1, 1, 16), (1, 16, 128), (1, 17, 144), (2, 130, 272), (3, 64, 112), (1
          (31, 384, 1040), (32, 128, 4096), (33, 1, 256), (40, 640, 704), (64, 300, 1152), (65, 96, 512), (77, 513, 384), (100, 255, 2064), (128, 512, 1024),
          (129, 257, 1040), (200, 384, 256), (256, 256, 128), (257, 640, 1296), (300, 1000, 528), (513, 130, 896), (1, 4096, 18944), (13, 4096, 4096), (7, 8, 16),
          (1030, 520, 272), (48, 3584, 2048), (17, 17, 6464), (30, 400, 8208), (50, 40, 3216), (70, 264, 4112), (70001, 5, 32), (1, 300001, 16), (3, 70000, 48),
-         (33, 1401, 2064), (80, 2047, 256), (200, 850, 1040), (390, 333, 400), (450, 130, 1024), (450, 97, 400), (420, 260, 3216)]
+         (33, 1401, 2064), (80, 2047, 256), (200, 850, 1040), (390, 333, 400), (450, 130, 1024), (450, 97, 400), (420, 260, 3216), (2, 4001, 5520), (7, 1001, 8208), (1, 130, 18944), (12, 2101, 10256), (16, 2050, 10240)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
