@@ -482,8 +482,9 @@ int twm_gemm_tw_marlin_m1_indirect(twm_ctx *ctx, const float *a_dev, const uint8
  *   weights : u8 [N][K] e4m3 codes, as a checkpoint holds a linear layer, f32 scales [ceil(N / 128)][ceil(K / 128)]
  *
  * A last block that K or N cuts short has a scale like any other.  Nothing is repacked and no handle is made.  Pointers are
- * aligned to their elements, the codes of twm_gemm_fp8 to 16 bytes; rows and columns go to 2^24, K to 2^20, M x N to 2^36.  The calls are asynchronous on the
- * context's stream, allocate nothing and can be captured; twm_gemm_fp8 uses the context's scratch like twm_gemm. */
+ * aligned to their elements, the codes of twm_gemm_fp8 to 16 bytes; what a call writes overlaps nothing else that it is given, but where
+ * that is said.  Rows and columns go to 2^24, K to 2^20, M x N to 2^36.  The calls are asynchronous on the context's stream, allocate
+ * nothing and can be captured; twm_gemm_fp8 uses the context's scratch like twm_gemm. */
 
 /* C[m][n] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] * (sum over the block's features of A[m][k] * W[n][k]),
  * C row-major f32 (c_dtype TWM_F32) or f16, rounded at the end (TWM_F16).  K must be a multiple of 16 (TWM_SHAPE_ERROR); M and N
@@ -530,7 +531,7 @@ int twm_add_rms_norm_fp8(twm_ctx *ctx, const void *x_dev, int x_dtype, const flo
  * numbers, so that the result depends neither on the launch nor on other rows; a token of less than half a step is never chosen, nor is
  * one whose distance to the largest logit no f32 holds.
  * -infinity masks a token and NaN counts as that; a row of nothing else yields 0, as do rows without columns.  +infinity shares
- * the choice with its equals.  out [rows] i32. */
+ * the choice with its equals.  out [rows] i32.  A few long rows use the context's scratch and counters, as twm_argmax_f32 does. */
 int twm_sample_f32(twm_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_t cols, const float *uniform_dev,
                    const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev,
                    int32_t *out_dev);
