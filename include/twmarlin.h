@@ -499,8 +499,8 @@ int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, 
  * matrix instructions and the K-split.  Touches no device. */
 int twm_plan_describe_fp8(uint32_t m, uint32_t n, uint32_t k, int c_dtype, char *text, size_t bytes);
 /* Rows of f16 or f32 as e4m3 rows for twm_gemm_fp8: scale = max(max |x| of the row's 128 columns, 1e-30) / 448,
- * code = e4m3_rne(x / scale).  A block with an infinity or a NaN gets a NaN scale.  cols is any size (twm_gemm_fp8 asks for a
- * multiple of 16). */
+ * code = e4m3_rne(x / scale), both quotients rounded to f32 first.  A block with an infinity or a NaN gets a NaN scale.  cols is any size
+ * (twm_gemm_fp8 asks for a multiple of 16). */
 int twm_quantize_rows_fp8(twm_ctx *ctx, const void *x_dev, int x_dtype, uint32_t rows, uint32_t cols, uint8_t *q_dev, float *scales_dev);
 /* twm_swiglu_rows and twm_geglu_rows with f16 or f32 rows in and e4m3 rows out: the gate of fused gate/up rows ahead of a down
  * projection in 8 bits.  gate_up [batch, 2 * dim], paired as in twm_swiglu_rows (dim a multiple of 32 then);
