@@ -9,6 +9,7 @@
 // Sixteen lanes hold a block, eight columns each: the largest magnitude is found by four DPP steps within those lanes, on the
 // bit patterns (which order as the magnitudes do and put NaN above infinity above all numbers).
 #include "twm_device.h"
+#include "twm_slices.h"
 
 #include <type_traits>
 
@@ -256,8 +257,6 @@ __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float
     }
 }
 
-constexpr uint64_t kFp8MostItems = 1ull << 27, kFp8MostRows = 1u << 22;   // of one launch (its threads stay below 2^32)
-
 hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t rows, uint32_t cols, int gate, bool paired, uint8_t *q, float *scales)
 {
     if (rows == 0 || cols == 0) return hipSuccess;
@@ -271,7 +270,7 @@ hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t row
                   : gate == 1 ? kernel_of(std::integral_constant<int, 1>{})
                               : kernel_of(std::integral_constant<int, 2>{});
     const size_t row_bytes = (size_t)cols * (gate ? 2 : 1) * (f16 ? 2 : 4);
-    const uint32_t most = (uint32_t)(kFp8MostItems / blocks);
+    const uint32_t most = most_workgroups(256) * 16u / blocks;   // rows of one launch
     for (uint32_t row = 0; row < rows; row += most) {
         const uint32_t items = (rows - row < most ? rows - row : most) * blocks;
         hipLaunchKernelGGL(kernel, dim3((items + 15) / 16), dim3(256), 0, s, (const char *)in + row * row_bytes, cols, blocks, items, paired ? 1u : 0u,
@@ -298,10 +297,11 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
     auto kernel = wide    ? kernel_of(std::integral_constant<uint32_t, 1024>{}, std::integral_constant<uint32_t, 1>{})
                   : brief ? kernel_of(std::integral_constant<uint32_t, 128>{}, std::integral_constant<uint32_t, 1>{})
                           : kernel_of(std::integral_constant<uint32_t, 256>{}, std::integral_constant<uint32_t, 2>{});
-    for (uint32_t row = 0; row < rows; row += kFp8MostRows) {
-        const uint32_t here = rows - row < kFp8MostRows ? rows - row : (uint32_t)kFp8MostRows;
+    const uint32_t threads = wide ? 1024 : brief ? 128 : 256, most = most_workgroups(threads);
+    for (uint32_t row = 0; row < rows; row += most) {
+        const uint32_t here = rows - row < most ? rows - row : most;
         const size_t at = (size_t)row * cols;
-        hipLaunchKernelGGL(kernel, dim3(here), dim3(wide ? 1024 : brief ? 128 : 256), 0, s, (const char *)x + at * (f16 ? 2 : 4), residual ? residual + at : nullptr, weight, eps, cols, blocks,
+        hipLaunchKernelGGL(kernel, dim3(here), dim3(threads), 0, s, (const char *)x + at * (f16 ? 2 : 4), residual ? residual + at : nullptr, weight, eps, cols, blocks,
                            sum ? sum + at : nullptr, q + at, scales + (size_t)row * blocks, normed ? (_Float16 *)normed + at : nullptr);
     }
     return hipGetLastError();

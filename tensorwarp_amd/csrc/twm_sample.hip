@@ -27,6 +27,7 @@
 // registers over the passes (25.5 us instead of 27.2 with both limits, 24.4 instead of 22.7 without any) and the tokens that are in
 // gathered ahead of their weights (40.1 and 40.3) were not worth their code.
 #include "twm_device.h"
+#include "twm_slices.h"
 
 namespace twm {
 
@@ -969,7 +970,7 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
     }
     // two workgroups a compute unit where there are more rows than those: 4096 rows of 1000 119 us instead of 177, 512 of 32000 65 instead
     // of 74; up to as many rows the registers count, 256 of 32000 39.9 instead of 41.1
-    constexpr uint32_t kMost = 1u << 21;   // rows of one launch (its threads stay below 2^32)
+    constexpr uint32_t kMost = most_workgroups(1024);   // rows of one launch
     for (uint32_t row = 0; row < rows; row += kMost) {
         SampleArgs part = a;
         part.logits = logits + (size_t)row * cols;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import tensorwarp_amd as T
-from test_gpu_fp8 import BLOCK, E4M3, At, Out, blocks
+from test_gpu_fp8 import BLOCK, E4M3, At, Big, Out, blocks, check_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +43,23 @@ def test_codes_are_the_nearest_to_the_quotient_with_the_stored_scale(dev, rows, 
     assert np.array_equal(s, amax / np.float32(448))
     want = nearest_codes(x / np.repeat(s, BLOCK, axis=1)[:, :cols])
     assert np.array_equal(q, want), (q != want).sum()
+
+
+def test_norm_of_more_wide_rows_than_one_launch_takes(dev):
+    # rows of more than 4096 columns take 1024 threads each: 2^22 rows are two launches of 2^31 threads, and three more rows a third
+    rows, cols, at = (1 << 22) + 3, 4104, [0, (1 << 21) - 1, 1 << 21, (1 << 22) - 1, 1 << 22, (1 << 22) + 2]
+    x, q, s = Big(dev, rows * cols * 2), Big(dev, rows * cols), Big(dev, rows * blocks(cols) * 4)
+    some = np.random.default_rng(31).standard_normal((len(at), cols)).astype(np.float16)
+    for r, v in zip(at, some):
+        x.put(r * cols * 2, v)
+    as_array = lambda big, dtype: type("Rows", (), {"ptr": big.ptr, "dtype": dtype})  # noqa: E731
+    T.add_rms_norm_fp8(dev, as_array(x, "f16"), None, At(dev, np.ones(cols, np.float32)), 1e-6, rows, cols, as_array(q, "u8"), as_array(s, "f32"))
+    y = some.astype(np.float64)
+    y = y / np.sqrt((y * y).mean(axis=1, keepdims=True) + 1e-6)
+    codes_ = np.stack([q.take(r * cols, cols, np.uint8) for r in at])
+    scales = np.stack([s.take(r * blocks(cols) * 4, blocks(cols), np.float32) for r in at])
+    check_codes(codes_, scales, y, 2.0 ** -20 * np.abs(y))
+    for r in (1, (1 << 21) + 1, (1 << 22) + 1):   # (rows of zeros beside them)
+        assert (q.take(r * cols, cols, np.uint8) == 0).all() and (s.take(r * blocks(cols) * 4, blocks(cols), np.float32) > 0).all()
+    for big in (x, q, s):
+        big.free()
