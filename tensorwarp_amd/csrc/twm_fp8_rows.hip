@@ -270,13 +270,12 @@ hipError_t launch_fp8_rows(hipStream_t s, const void *in, bool f16, uint32_t row
                   : gate == 1 ? kernel_of(std::integral_constant<int, 1>{})
                               : kernel_of(std::integral_constant<int, 2>{});
     const size_t row_bytes = (size_t)cols * (gate ? 2 : 1) * (f16 ? 2 : 4);
-    const uint32_t most = most_workgroups(256) * 16u / blocks;   // rows of one launch
-    for (uint32_t row = 0; row < rows; row += most) {
-        const uint32_t items = (rows - row < most ? rows - row : most) * blocks;
+    return in_slices(rows, most_workgroups(256) * 16u / blocks, [&](uint32_t row, uint32_t here) {
+        const uint32_t items = here * blocks;
         hipLaunchKernelGGL(kernel, dim3((items + 15) / 16), dim3(256), 0, s, (const char *)in + row * row_bytes, cols, blocks, items, paired ? 1u : 0u,
                            q + (size_t)row * cols, scales + (size_t)row * blocks);
-    }
-    return hipGetLastError();
+        return hipGetLastError();
+    });
 }
 
 hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *residual, const float *weight, float eps, uint32_t rows,
@@ -297,14 +296,13 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
     auto kernel = wide    ? kernel_of(std::integral_constant<uint32_t, 1024>{}, std::integral_constant<uint32_t, 1>{})
                   : brief ? kernel_of(std::integral_constant<uint32_t, 128>{}, std::integral_constant<uint32_t, 1>{})
                           : kernel_of(std::integral_constant<uint32_t, 256>{}, std::integral_constant<uint32_t, 2>{});
-    const uint32_t threads = wide ? 1024 : brief ? 128 : 256, most = most_workgroups(threads);
-    for (uint32_t row = 0; row < rows; row += most) {
-        const uint32_t here = rows - row < most ? rows - row : most;
+    const uint32_t threads = wide ? 1024 : brief ? 128 : 256;
+    return in_slices(rows, most_workgroups(threads), [&](uint32_t row, uint32_t here) {
         const size_t at = (size_t)row * cols;
         hipLaunchKernelGGL(kernel, dim3(here), dim3(threads), 0, s, (const char *)x + at * (f16 ? 2 : 4), residual ? residual + at : nullptr, weight, eps, cols, blocks,
                            sum ? sum + at : nullptr, q + at, scales + (size_t)row * blocks, normed ? (_Float16 *)normed + at : nullptr);
-    }
-    return hipGetLastError();
+        return hipGetLastError();
+    });
 }
 
 }  // namespace twm

@@ -964,14 +964,18 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
         const uint32_t groups = (spans + a.each - 1) / a.each;
         SampleRow *state = (SampleRow *)scratch;
         hipLaunchKernelGGL(k_sample_largest, dim3(groups, rows), dim3(1024), 0, s, a, state);
-        if (top_k || top_p) hipLaunchKernelGGL(k_sample_limits, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
+        hipError_t e = hipGetLastError();
+        if (e == hipSuccess && (top_k || top_p)) {
+            hipLaunchKernelGGL(k_sample_limits, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
+            e = hipGetLastError();
+        }
+        if (e != hipSuccess) return e;
         hipLaunchKernelGGL(k_sample_token, dim3(groups, rows), dim3(1024), 0, s, a, state, counters);
         return hipGetLastError();
     }
     // two workgroups a compute unit where there are more rows than those: 4096 rows of 1000 119 us instead of 177, 512 of 32000 65 instead
     // of 74; up to as many rows the registers count, 256 of 32000 39.9 instead of 41.1
-    constexpr uint32_t kMost = most_workgroups(1024);   // rows of one launch
-    for (uint32_t row = 0; row < rows; row += kMost) {
+    return in_slices(rows, most_workgroups(1024), [&](uint32_t row, uint32_t here) {
         SampleArgs part = a;
         part.logits = logits + (size_t)row * cols;
         part.uniform = uniform + row;
@@ -980,9 +984,9 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
         part.top_p = top_p ? top_p + row : nullptr;
         part.min_p = min_p ? min_p + row : nullptr;
         part.out = out + row;
-        hipLaunchKernelGGL(rows <= kSampleGroups ? k_sample<4> : k_sample<8>, dim3(rows - row < kMost ? rows - row : kMost), dim3(1024), 0, s, part);
-    }
-    return hipGetLastError();
+        hipLaunchKernelGGL(rows <= kSampleGroups ? k_sample<4> : k_sample<8>, dim3(here), dim3(1024), 0, s, part);
+        return hipGetLastError();
+    });
 }
 
 }  // namespace twm

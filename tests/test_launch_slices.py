@@ -24,10 +24,23 @@ def test_a_launch_has_fewer_than_2_to_the_32_threads(tmp_path, threads):
     assert most * threads < 1 << 32 and most >= 1 << 21
 
 
-def test_the_kernels_of_rows_take_their_limits_from_there():
-    for name in ("twm_fp8_rows.hip", "twm_sample.hip"):
+def test_slices_cover_the_rows_and_end_with_the_first_error(tmp_path):
+    # (as the launchers do it: each launch's own error, nothing launched behind one that failed)
+    body = """
+    const unsigned cases[][3] = {{10, 4, 99}, {8, 4, 99}, {3, 4, 99}, {0, 4, 99}, {10, 4, 1}, {10, 4, 0}, {4294967295u, 2147483648u, 99}};
+    for (auto &c : cases) {
+        unsigned calls = 0;
+        const int e = twm::in_slices(c[0], c[1], [&](unsigned row, unsigned count) { printf("%u+%u ", row, count); return calls++ == c[2] ? 7 : 0; });
+        printf("= %d\\n", e);
+    }"""
+    assert run(tmp_path, body) == ["0+4 4+4 8+2 = 0", "0+4 4+4 = 0", "0+3 = 0", "= 0", "0+4 4+4 = 7", "0+4 = 7", "0+2147483648 2147483648+2147483647 = 0"]
+
+
+def test_the_kernels_of_rows_are_launched_so():
+    for name, launchers in (("twm_fp8_rows.hip", 2), ("twm_sample.hip", 1)):
         with open(os.path.join(build.CSRC, name)) as f:
             text = f.read()
-        loops = [line for line in text.split("\n") if "row += " in line]
-        assert loops and all("row += most)" in line or "row += kMost)" in line for line in loops)
-        assert text.count("most_workgroups(") == len(loops)
+        assert text.count("return in_slices(rows, most_workgroups(") == launchers and "row += " not in text
+        # no launch whose error is not asked for before the next one
+        launches = text.split("hipLaunchKernelGGL(")[1:]
+        assert launches and all("hipGetLastError()" in after for after in launches), name
