@@ -63,3 +63,50 @@ def test_norm_of_more_wide_rows_than_one_launch_takes(dev):
         assert (q.take(r * cols, cols, np.uint8) == 0).all() and (s.take(r * blocks(cols) * 4, blocks(cols), np.float32) > 0).all()
     for big in (x, q, s):
         big.free()
+
+
+def gates(act, g, u):
+    """act(g) * u in 64 bits, without a difference of nearly equal numbers and without an overflow on the way."""
+    g, u = g.astype(np.float64), u.astype(np.float64)
+    z2 = g if act == "silu" else 2 * np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3)
+    e = np.exp(-np.abs(z2))
+    return g * u * np.where(z2 > 0, 1.0, e) / (1 + e)
+
+
+def gate_of_single_columns(dev, act, g, u):
+    """|y| as the scales of rows of one column have it, and the codes."""
+    rows = len(g)
+    x = np.stack([g, u], axis=1)
+    q, s = Out(dev, (rows, 1), "u8"), Out(dev, (rows, 1), "f32")
+    (T.swiglu_rows_fp8 if act == "silu" else T.geglu_rows_fp8)(dev, At(dev, x), q, s, 1, rows)
+    return s.get()[:, 0].astype(np.float64) * 448, q.get()[:, 0]
+
+
+def gate_error(act, g):
+    """An exponential and a reciprocal of an ulp each, 2^-23, and four roundings of 2^-24 -- 1 + e, act(g), times u, the exponential's
+    low part -- are 2^-21 of y; the scale's division rounds by 2^-24 again.  gelu's exponent is g (c + d g^2): half an ulp of g^2 and of
+    the bracket, and what f32 leaves of c and d, make as much of e^2z as they are of 2z's logarithm to base two, times ln 2."""
+    error = np.full(g.shape, 2.0 ** -21 + 2.0 ** -24)
+    if act == "gelu":
+        c = 2 * np.sqrt(2 / np.pi) * np.log2(np.e)
+        d, square = 0.044715 * c, np.minimum(g.astype(np.float64) ** 2, 1e4)   # (from g = 100 on 1 + e is one)
+        half = lambda v: np.spacing(v.astype(np.float32)).astype(np.float64) / 2  # noqa: E731
+        bracket = half(c + d * square) + d * half(square) + square * abs(d - float(np.float32(d))) + abs(c - float(np.float32(c)))
+        error += np.log(2) * np.minimum(np.abs(g), 100.0) * bracket * 1.001
+    return error
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_are_as_near_as_their_roundings(dev, act):
+    # relative to the gate itself, also where it is far below zero and its exponent's roundings count most
+    rng = np.random.default_rng(21)
+    g = np.concatenate([rng.uniform(-9, 9, 200000), rng.uniform(-80, -9, 20000) if act == "silu" else rng.uniform(-8.9, -3, 20000),
+                        10.0 ** rng.uniform(-20, 0, 20000), -10.0 ** rng.uniform(-20, 0, 20000), 10.0 ** rng.uniform(1, 15, 2000)]).astype(np.float32)
+    u = rng.uniform(0.5, 2.0, len(g)).astype(np.float32) * np.where(g < -30, np.float32(1e20), np.float32(1))
+    y = gates(act, g, u)
+    seen = np.abs(y) > 1e-29
+    assert seen.sum() > len(g) - 100
+    got, codes_ = gate_of_single_columns(dev, act, g, u)
+    off = (np.abs(got - np.abs(y)) / np.abs(y) / gate_error(act, g))[seen]
+    assert off.max() <= 1, (off.max(), g[seen][off.argmax()])
+    assert np.array_equal(codes_[seen] >> 7, y[seen] < 0)
