@@ -38,23 +38,34 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t v)
 // hardware's exponential and reciprocal, each within a unit in the last place: silu is within 2^-21 of itself.  gelu's t is g times a
 // polynomial of g^2 whose roundings -- of g^2, of the polynomial, of its constants -- count 2z times over: within 2^-21 + 2^-22.7 |2z|
 // (measured 2^-19.6 at g = -5 and 2^-17 at g = -9, where gelu is 5e-8 and 2e-29 of g).  The polynomial in 64 bits would keep it at
-// 2^-21 and takes a 2048 x 11008 f16 gate from 24.2 to 26.4 us.  Below x = -88 the gate is g times less than 2^-126.  (GATE: 1 gelu, 2 silu.)
-template <int GATE> __device__ __forceinline__ float gate_rows(float g, float u)
+// 2^-21 and takes a 2048 x 11008 f16 gate from 24.2 to 26.4 us.  (GATE: 1 gelu, 2 silu; g above far_gate.)
+template <int GATE, bool F16> __device__ __forceinline__ float gate_rows(float g, float u)
 {
-    float t, low;
+    float t, low;   // (finite for any f16 g, and for an f32 one between the limits)
     if constexpr (GATE == 1) {
         constexpr double c = -1.5957691216057308 * 1.4426950408889634;   // -2 sqrt(2 / pi) log2(e)
-        const float x = __builtin_amdgcn_fmed3f(g, -10.0f, 100.0f), p = fmaf(x * x, (float)(0.044715 * c), (float)c);
+        const float x = F16 ? g : __builtin_amdgcn_fmed3f(g, -9.0f, 100.0f), p = fmaf(x * x, (float)(0.044715 * c), (float)c);
         t = x * p;
         low = fmaf(x, p, -t);
     } else {
-        const float x = __builtin_amdgcn_fmed3f(g, -88.0f, 1e4f);
+        const float x = F16 ? g : __builtin_amdgcn_fmed3f(g, -80.0f, 1e4f);
         t = x * -1.44269502f;
         low = fmaf(x, -1.92596303e-8f, fmaf(x, -1.44269502f, -t));
     }
     const float e = __builtin_amdgcn_exp2f(t);
     // (act(g) first: it is small where g u may be beyond f32)
     return g * __builtin_amdgcn_rcpf(fmaf(e, low * 0.693147182f, e) + 1.0f) * u;
+}
+
+// Below this the gate is g e^x and less than 2^-95 of g: 1 / (1 + e^-x) leaves what f32 holds at x = -87, act(g) soon after, while its
+// product with u need not.  There the product is taken in 64 bits, 2^-t as a power of two and the rest.  (One comparison for eight
+// gates: 2048 x 11008 f16 rows 0.3 us, as much as the clamps of t that they no longer need.)
+template <int GATE> constexpr float far_gate = GATE == 1 ? -9.0f : -80.0f;
+template <int GATE> __device__ __forceinline__ float gate_far(float g, float u)
+{
+    const double d = g, x = GATE == 1 ? 1.5957691216057308 * (d + 0.044715 * d * d * d) : d;
+    const double t = fmax(x * 1.4426950408889634, -1000.0), whole = rint(t);   // (g u e^-693 is nothing for any g and u)
+    return (float)(d * u * ldexp((double)__builtin_amdgcn_exp2f((float)(t - whole)), (int)whole));
 }
 
 // Rows begin where the ones before them end, on any element's boundary; the memory takes vectors there too (2048 x 11007 f16 gate
@@ -179,7 +190,13 @@ __global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, u
         load_8<F16, WHOLE>(g, src, in_row ? g_col : 2u * cols, paired ? 2u * cols : cols);
         load_8<F16, WHOLE>(u, src, in_row ? u_col : 2u * cols, 2u * cols);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = gate_rows<GATE>(g[j], u[j]);
+        for (int j = 0; j < 8; j++) v[j] = gate_rows<GATE, F16>(g[j], u[j]);
+        const float least = fminf(fminf(fminf(g[0], g[1]), fminf(g[2], g[3])), fminf(fminf(g[4], g[5]), fminf(g[6], g[7])));
+        if (__builtin_expect(least < far_gate<GATE>, 0)) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (g[j] < far_gate<GATE>) v[j] = gate_far<GATE>(g[j], u[j]);
+        }
     } else {
         load_8<F16, WHOLE>(v, src, col, cols);
     }

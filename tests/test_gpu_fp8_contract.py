@@ -110,3 +110,60 @@ def test_gates_are_as_near_as_their_roundings(dev, act):
     off = (np.abs(got - np.abs(y)) / np.abs(y) / gate_error(act, g))[seen]
     assert off.max() <= 1, (off.max(), g[seen][off.argmax()])
     assert np.array_equal(codes_[seen] >> 7, y[seen] < 0)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_that_vanish(dev, act):
+    # act(g) falls off like e^g beyond what f32 holds: with a large u it still is a number of its own there, and with any other u it
+    # is nothing, not a floor that stays in a block of small values
+    rng = np.random.default_rng(22)
+    least = (-260.0, -20.0)[act == "gelu"]
+    g = np.concatenate([rng.uniform(least, least / 3, 60000), [-1e3, -1e6, -3e38] * 20]).astype(np.float32)
+    u = (10.0 ** rng.uniform(-5, 38.4, len(g)) * rng.choice([-1, 1], len(g))).astype(np.float32)
+    y = gates(act, g, u)
+    got, codes_ = gate_of_single_columns(dev, act, g, u)
+    seen = np.abs(y) > 1.1e-30
+    assert 5000 < seen.sum() < 40000
+    assert (np.abs(got - np.abs(y))[seen] <= gate_error(act, g)[seen] * np.abs(y)[seen]).all()
+    assert np.array_equal(codes_[seen] >> 7, y[seen] < 0)
+    # below 1e-30 the scale is that of 1e-30: half a step of the codes, and y's own error
+    below = np.abs(y) < 0.9e-30
+    v = y[below] / (1e-30 / 448)
+    assert (np.abs(E4M3[codes_[below]] - v) <= np.maximum(2.0 ** -4 * np.abs(v), 2.0 ** -10) + 2.0 ** -19 * np.abs(v) + 1e-12).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_a_gate_that_vanishes_leaves_its_block_alone(dev, act, dtype):
+    rng = np.random.default_rng(23)
+    dim = 256
+    g, u = rng.standard_normal((4, dim)), rng.standard_normal((4, dim))
+    g[:, ::5] = -100.0 if act == "silu" else -30.0
+    u[:, ::5] = 2e38 if dtype == "f32" else 6e4
+    g[3] = -110.0 if act == "silu" else -25.0   # a row of nothing else
+    x = np.concatenate([g, u], axis=1).astype(np.float32 if dtype == "f32" else np.float16)
+    q, s = Out(dev, (4, dim), "u8"), Out(dev, (4, 2), "f32")
+    (T.swiglu_rows_fp8 if act == "silu" else T.geglu_rows_fp8)(dev, At(dev, x), q, s, dim, 4)
+    y = gates(act, x[:, :dim], x[:, dim:])
+    check_codes(q.get(), s.get(), y, 2.0 ** -20 * np.abs(y) + 1e-38)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_that_are_no_numbers_mark_their_own_block(dev, act, dtype):
+    rng = np.random.default_rng(24)
+    dim, rows = 640, 4
+    x = rng.standard_normal((rows, 2 * dim))
+    bad = np.zeros((rows, 5), bool)
+    for r, (b, v) in enumerate(((0, np.inf), (2, -np.inf), (4, np.nan), (1, np.inf))):
+        x[r, b * BLOCK + 9 + (r == 3) * dim] = v   # (the last one is an up value)
+        bad[r, b] = True
+    x = x.astype(np.float32 if dtype == "f32" else np.float16)
+    q, s = Out(dev, (rows, dim), "u8"), Out(dev, (rows, 5), "f32")
+    (T.swiglu_rows_fp8 if act == "silu" else T.geglu_rows_fp8)(dev, At(dev, x), q, s, dim, rows)
+    q, s = q.get(), s.get()
+    assert np.array_equal(np.isnan(s), bad) and (q[np.repeat(bad, BLOCK, axis=1)] & 0x7F == 0x7F).all()
+    y = np.where(np.repeat(bad, BLOCK, axis=1), 1.0, gates(act, np.nan_to_num(x[:, :dim]), np.nan_to_num(x[:, dim:])))
+    for b in range(5):
+        good, at = ~bad[:, b], slice(b * BLOCK, (b + 1) * BLOCK)
+        check_codes(q[good, at], s[good, b:b + 1], y[good, at], 2.0 ** -18 * np.abs(y[good, at]) + 1e-38)
