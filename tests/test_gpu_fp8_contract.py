@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import tensorwarp_amd as T
-from test_gpu_fp8 import BLOCK, E4M3, At, Big, Out, blocks, check_codes
+from test_gpu_fp8 import BLOCK, E4M3, At, Big, Out, blocks, check_codes, gemm_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +167,44 @@ def test_gates_that_are_no_numbers_mark_their_own_block(dev, act, dtype):
     for b in range(5):
         good, at = ~bad[:, b], slice(b * BLOCK, (b + 1) * BLOCK)
         check_codes(q[good, at], s[good, b:b + 1], y[good, at], 2.0 ** -18 * np.abs(y[good, at]) + 1e-38)
+
+
+# (m, n, k, results): ragged everywhere, in each of the tile kernel's forms, with and without ranges of K
+NAN_TILES = [(1030, 517, 272, "f16"), (1030, 517, 272, "f32"), (450, 97, 400, "f32"), (450, 130, 1040, "f16"), (333, 3579, 18880, "f16"), (420, 260, 3216, "f32"),
+             (1500, 9000, 144, "f16"), (200, 9001, 4112, "f16"), (200, 9001, 4112, "f32")]
+
+NAN_FEW = [(9, 200, 400, "f16"), (16, 517, 8208, "f32"), (30, 260, 656, "f32"), (70, 300, 1168, "f16"), (60, 257, 3216, "f32")]
+
+
+def test_the_products_with_nans_reach_every_form_of_the_tile_kernel():
+    plans = {T.plan_fp8(m, n, k, dtype) for m, n, k, dtype in NAN_TILES}
+    assert all(p.startswith("k_fp8_tile") for p in plans), plans
+    shapes = {p.split(", ")[0] + p.split(", ")[2] for p in plans}
+    assert len(shapes) == 5, shapes
+    assert any(p.endswith("splits") for p in plans) and any(p.endswith("1 K-split") for p in plans)
+    assert all(T.plan_fp8(m, n, k, dtype).startswith("k_fp8_rows_few") for m, n, k, dtype in NAN_FEW)
+
+
+@pytest.mark.parametrize("what", ["codes", "row scales", "column scales"])
+@pytest.mark.parametrize("m,n,k,dtype", NAN_TILES + NAN_FEW)
+def test_nans_stay_in_their_rows_and_columns(dev, m, n, k, dtype, what):
+    # a NaN code reaches its row or column, a NaN scale of A its row, one of W its 128 columns, and nothing else; among them the last
+    # row and column, in the last block, which K cuts short
+    a, a_s, w, w_s = gemm_inputs(np.random.default_rng(m + n + k), m, n, k)
+    a_s, w_s = a_s * np.float32(2.0 ** -6), w_s * np.float32(2.0 ** -6)   # (f16 results stay finite)
+    want = np.zeros((m, n), bool)
+    if what == "codes":
+        a[m - 1, k - 1], a[5, 17], w[n - 1, k - 2], w[n // 2, 0] = 0x7F, 0xFF, 0xFF, 0x7F
+        want[[m - 1, 5]] = True
+        want[:, [n - 1, n // 2]] = True
+    elif what == "row scales":
+        a_s[m - 1, -1] = a_s[m // 2, 0] = a_s[7, blocks(k) // 2] = np.nan
+        want[[m - 1, m // 2, 7]] = True
+    else:
+        w_s[-1, -1] = w_s[w_s.shape[0] // 2, 0] = np.nan
+        for b in (w_s.shape[0] - 1, w_s.shape[0] // 2):
+            want[:, b * BLOCK:(b + 1) * BLOCK] = True
+    c = Out(dev, (m, n), dtype)
+    T.gemm_fp8(dev, At(dev, a), At(dev, a_s), At(dev, w), At(dev, w_s), m, n, k, c)
+    got = c.get()
+    assert np.array_equal(np.isnan(got), want) and np.isfinite(got[~want]).all()
