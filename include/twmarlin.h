@@ -489,10 +489,12 @@ int twm_gemm_tw_marlin_m1_indirect(twm_ctx *ctx, const float *a_dev, const uint8
 /* C[m][n] = sum over blocks b of a_scales[m][b] * w_scales[n / 128][b] * (sum over the block's features of A[m][k] * W[n][k]),
  * C row-major f32 (c_dtype TWM_F32) or f16, rounded at the end (TWM_F16).  K must be a multiple of 16 (TWM_SHAPE_ERROR); M and N
  * are any size, from one row on.  K = 0 stores zeros.  Deterministic: the same call gives the same bits.
- * f32 results: every product and every sum in f32.  f16 results of more than 16 rows may use the matrix unit's 8-bit instructions,
- * which add eight neighbouring products (features 8 i .. 8 i + 7) after cutting each off below 2^-13 of the largest one's power
- * of two, and everything else in f32: on bell-shaped values 1.5e-5 of the result's norm, where rounding to f16 costs 2e-4.  A
- * caller to whom that matters asks for f32 results. */
+ * f32 results: every product and every sum in f32, whatever the number of rows.  f16 results of up to 16 rows too.  f16 results of 17 rows
+ * and more may use the matrix unit's 8-bit instructions, which add eight neighbouring products (features 8 i .. 8 i + 7) after cutting
+ * each off below 2^-13 of the largest one's power of two, and everything else in f32: on bell-shaped values 1.5e-5 of the result's norm,
+ * where rounding to f16 costs 2e-4; but where large products of a group cancel, small ones beside them are lost.  So a row's f16
+ * results may differ in their last bits with the number of rows beside it.  A caller to whom that matters asks for f32 results, and rounds
+ * them by twm_cast_f32_to_f16 where f16 rows are wanted.  The two scales of a block are multiplied with each other first. */
 int twm_gemm_fp8(twm_ctx *ctx, const uint8_t *a_dev, const float *a_scales_dev, const uint8_t *w_dev, const float *w_scales_dev,
                  uint32_t m, uint32_t n, uint32_t k, void *c_dev, int c_dtype);
 /* What twm_gemm_fp8 launches for these sizes, as one line of text (see twm_plan_describe): the kernel, its workgroup's shape, the

@@ -22,7 +22,13 @@ def _ptr(t):
 
 
 def gemm_fp8(device, a, a_scales, w, w_scales, m, n, k, c):
-    """C [m, n] (f32 or f16) = A [m, k] x W [n, k]^T, both e4m3; a_scales [m, ceil(k / 128)], w_scales [ceil(n / 128), ceil(k / 128)]."""
+    """C [m, n] (f32 or f16) = A [m, k] x W [n, k]^T, both e4m3; a_scales [m, ceil(k / 128)], w_scales [ceil(n / 128), ceil(k / 128)].
+
+    f32 results come from exact products and f32 sums.  So do f16 results of up to 16 rows; from 17 on they may come from the 8-bit
+    matrix instructions, which cut the products of eight neighbouring features off below 2^-13 of the largest one's power of two before
+    they add them (1.5e-5 of a result's norm; small products beside large ones that cancel are lost).  plan_fp8() says which; f32 results
+    rounded by twm_cast_f32_to_f16 keep the exact ones.
+    """
     _check(device._l.twm_gemm_fp8(device.handle, a.ptr, a_scales.ptr, w.ptr, w_scales.ptr, m, n, k, c.ptr, _dtype(c)))
 
 

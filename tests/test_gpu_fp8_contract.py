@@ -208,3 +208,24 @@ def test_nans_stay_in_their_rows_and_columns(dev, m, n, k, dtype, what):
     T.gemm_fp8(dev, At(dev, a), At(dev, a_s), At(dev, w), At(dev, w_s), m, n, k, c)
     got = c.get()
     assert np.array_equal(np.isnan(got), want) and np.isfinite(got[~want]).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(12, 300, 256), (30, 260, 656), (450, 130, 1040), (1030, 517, 272), (1500, 9000, 144)])
+def test_small_products_beside_large_ones_that_cancel(dev, m, n, k):
+    # eight features of 448 * 448, -448 * 448 and six ones: f32 results have the six, and rounded by the cast they are f16 results with
+    # them; f16 results have them where the plan says f16 instructions, and elsewhere are off by less than 2^-13 of 2^16 a product
+    code = {int(v): c for c, v in enumerate(E4M3) if v in (1.0, 448.0, -448.0)}
+    a, w = np.full((m, k), code[1], np.uint8), np.full((n, k), code[1], np.uint8)
+    a[:, 0::8], a[:, 1::8], w[:, 0::8], w[:, 1::8] = code[448], code[-448], code[448], code[448]
+    a_s, w_s = np.ones((m, blocks(k)), np.float32), np.ones((blocks(n), blocks(k)), np.float32)
+    inputs = [At(dev, v) for v in (a, a_s, w, w_s)]
+    c, half, cast = Out(dev, (m, n), "f32"), Out(dev, (m, n), "f16"), Out(dev, (m, n), "f16")
+    T.gemm_fp8(dev, *inputs, m, n, k, c)
+    T.gemm_fp8(dev, *inputs, m, n, k, half)
+    assert T._lib.load().twm_cast_f32_to_f16(dev.handle, c.ptr, cast.ptr, m * n) == T._lib.OK
+    # (whole numbers below 2^24: no sum of them rounds)
+    assert (c.get() == k // 8 * 6).all() and (cast.get() == k // 8 * 6).all()
+    if "8-bit" in T.plan_fp8(m, n, k, "f16"):
+        assert m > 16 and (np.abs(half.get().astype(np.float64) - k // 8 * 6) <= k * 2.0 ** 3).all()
+    else:
+        assert (half.get() == k // 8 * 6).all()
