@@ -250,12 +250,16 @@ class _Rows:
         self.tensor, self.ptr, self.dtype, self.numel = t, t.data_ptr(), _NAMES[t.dtype], t.numel()
 
 
+_LEGACY_STREAM = 1  # hipStreamLegacy: the null stream as a handle (a null pointer is the context's own stream)
+
+
 def _dev():
-    """The process's one context."""
+    """The process's one context, its work in the order of torch's: on the stream that is torch's current one at the first call."""
     global _device
     if _device is None:
         import tensorwarp_amd as T
         _device = T.WarpDevice(0)
+        _device.with_stream(torch.cuda.current_stream().cuda_stream or _LEGACY_STREAM)
     return _device
 
 
