@@ -93,7 +93,9 @@ void twm_ctx_destroy(twm_ctx *ctx);
 int twm_ctx_sync(twm_ctx *ctx);
 /* WarpDevice::with_stream (device.rs:230-265): run subsequent work on a caller-owned
  * hipStream_t (e.g. the stream a framework already uses).  NULL restores the
- * context's own stream. */
+ * context's own stream, which waits for no other and no other for it: not the null
+ * stream either.  A caller whose arrays are made and read on the null stream passes
+ * hipStreamLegacy (no graph can be captured there). */
 int twm_ctx_set_stream(twm_ctx *ctx, void *hip_stream);
 /* The hipStream_t work is currently issued on. */
 void *twm_ctx_stream(twm_ctx *ctx);
