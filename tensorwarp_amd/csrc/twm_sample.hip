@@ -782,7 +782,8 @@ __device__ __forceinline__ int sample_index(uint64_t key) { return (int)(0xFFFFF
 
 }  // namespace
 
-// A workgroup per row.  WAVES 8: so few registers (64, four of them spilled) that a compute unit holds two workgroups
+// A workgroup per row.  WAVES 8: so few registers (64; eight values of a lane are spilled, 20 bytes at a time) that a compute unit holds
+// two workgroups
 template <int WAVES> __global__ __launch_bounds__(1024, WAVES) void k_sample(const SampleArgs a)
 {
     __shared__ SampleShared sh;
