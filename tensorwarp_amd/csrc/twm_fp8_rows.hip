@@ -9,6 +9,7 @@
 // Sixteen lanes hold a block, eight columns each: the largest magnitude is found by four DPP steps within those lanes, on the
 // bit patterns (which order as the magnitudes do and put NaN above infinity above all numbers).
 #include "twm_device.h"
+#include "twm_e4m3.h"
 #include "twm_slices.h"
 
 #include <type_traits>
@@ -18,7 +19,6 @@ namespace twm {
 namespace {
 
 constexpr uint32_t kFp8Each = 8;       // columns per lane
-constexpr float kFp8Max = 448.0f;
 constexpr float kFp8LeastAmax = 1e-30f;  // (448 / amax stays finite, a block of zeros gets codes of zero)
 
 // the largest of sixteen lanes' values, in each of them
@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t v)
 // hardware's exponential and reciprocal, each within a unit in the last place: silu is within 2^-21 of itself.  gelu's t is g times a
 // polynomial of g^2 whose roundings -- of g^2, of the polynomial, of its constants -- count 2z times over: within 2^-21 + 2^-22.7 |2z|
 // (measured 2^-19.6 at g = -5 and 2^-17 at g = -9, where gelu is 5e-8 and 2e-29 of g).  The polynomial in 64 bits would keep it at
-// 2^-21 and takes a 2048 x 11008 f16 gate from 24.2 to 26.4 us.  (GATE: 1 gelu, 2 silu; g above far_gate.)
+// 2^-21 and takes a 2048 x 11008 f16 gate from 25.6 to 27.8 us.  (GATE: 1 gelu, 2 silu; g above far_gate.)
 template <int GATE, bool F16> __device__ __forceinline__ float gate_rows(float g, float u)
 {
     float t, low;   // (finite for any f16 g, and for an f32 one between the limits)
@@ -59,7 +59,7 @@ template <int GATE, bool F16> __device__ __forceinline__ float gate_rows(float g
 
 // Below this the gate is g e^x and less than 2^-95 of g: 1 / (1 + e^-x) leaves what f32 holds at x = -87, act(g) soon after, while its
 // product with u need not.  There the product is taken in 64 bits, 2^-t as a power of two and the rest.  (One comparison for eight
-// gates: 2048 x 11008 f16 rows 0.3 us, as much as the clamps of t that they no longer need.)
+// gates, and t without clamps in f16: 2048 x 11008 rows 25.2 us, gelu 25.6; clamped and without this 25.5 and 26.0.)
 template <int GATE> constexpr float far_gate = GATE == 1 ? -9.0f : -80.0f;
 template <int GATE> __device__ __forceinline__ float gate_far(float g, float u)
 {
@@ -69,7 +69,7 @@ template <int GATE> __device__ __forceinline__ float gate_far(float g, float u)
 }
 
 // Rows begin where the ones before them end, on any element's boundary; the memory takes vectors there too (2048 x 11007 f16 gate
-// 64.6 us element by element, 28.6 so; 2048 x 4095 f16 norm with every output 68.4 and 29.4)
+// 64.6 us element by element, 27.6 so; 2048 x 4095 f16 norm with every output 68.4 and 31.2)
 typedef half8 half8_any __attribute__((aligned(2)));
 typedef float4v float4v_any __attribute__((aligned(4)));
 typedef uint2v uint2v_any __attribute__((aligned(1)));
@@ -139,21 +139,15 @@ template <bool WHOLE> __device__ __forceinline__ void store_codes(uint8_t *q, fl
     amax = bits >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : amax < kFp8LeastAmax ? kFp8LeastAmax : amax;
     const float block_scale = amax / kFp8Max;
     if (scale && (col & 127u) == 0) *scale = block_scale;
-    // v / block_scale as f32 rounds it, or a neighbour of that on the same side of every border between two codes: the product with the
-    // inverse and one step by its remainder.  (2048 x 11008 f16 gate 23.8 us, with eight divisions 26.3, with the product alone, which put a
-    // code in a few hundred thousand on the wrong side, 23.0.)  Shown by trying it with every mantissa of a scale at every border, on the
-    // f32 values around it: none is off while the remainder is exact, which it is for scales down to 2^-93.
-    const float inverse = 1.0f / block_scale;
+    const float inverse = kFp8Max / amax;   // (not 1 / block_scale, which would wait for it: 1 x 896 norm's kernel 3.1 us, so 3.3)
+    // (2048 x 11008 f16 gate 25.2 us, with eight divisions 27.8, with the product with the inverse alone 24.6)
     float c[8];
-    if (__builtin_expect(block_scale < 0x1p-90f, 0)) {
+    if (__builtin_expect(block_scale < kFp8LeastExact, 0)) {
 #pragma unroll
         for (int j = 0; j < 8; j++) c[j] = v[j] / block_scale;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float near = v[j] * inverse;
-            c[j] = fmaf(fmaf(-near, block_scale, v[j]), inverse, near);
-        }
+        for (int j = 0; j < 8; j++) c[j] = units_of(v[j], block_scale, inverse);
     }
     // (at most 448 and a rounding, which the conversion rounds to 448)
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
@@ -203,8 +197,8 @@ __global__ __launch_bounds__(256) void k_fp8_rows(const void *__restrict__ in, u
     store_codes<WHOLE>(q + (size_t)row * cols, scales + item, col, cols, v);
 }
 
-// A workgroup per row.  Bound: the rows' way through memory (2048 x 4096 f16 rows with every output 22.4 us, 4.9 TB/s; a copy reaches
-// 4.7).  s = x (+ residual) stays in registers up to 8 * THREADS * HELD columns; a longer row is read again for its
+// A workgroup per row.  Bound: the rows' way through memory (2048 x 4096 f16 rows with every output 26.6 us, 4.1 TB/s of four arrays in
+// and out; a copy reaches 4.7).  s = x (+ residual) stays in registers up to 8 * THREADS * HELD columns; a longer row is read again for its
 // second pass.  sum: where s goes, or null; it may be the residual itself, whose elements are read by the lane that writes them.
 template <bool F16, bool WHOLE, uint32_t THREADS, uint32_t HELD>
 __global__ __launch_bounds__(THREADS) void k_fp8_norm(const void *x, const float *residual, const float *__restrict__ weight, float eps,
@@ -313,8 +307,8 @@ hipError_t launch_fp8_norm(hipStream_t s, const void *x, bool f16, const float *
     const uint32_t blocks = (cols + 127u) / 128u;
     const bool whole = cols % 8 == 0;
     // Sixteen waves for a row where four would hold less than all of it, or there are fewer rows than CUs (1024 x 8192 f16 rows with every
-    // output 24.5 us on four, 22.1 on sixteen; 1 x 8192 5.1 and 3.8; but 2048 x 4096 f32 rows 9.2 and 12.1)
-    // and two for short rows (9362 x 896 11.9 us on four, 9.3 on two)
+    // output 26.8 us on four, 24.2 on sixteen; in a graph 1 x 8192 5.6 and 4.1, 1 x 4096 3.5 and 3.1, 256 x 4096 5.2 and 4.9; but 2048 x 4096
+    // f32 rows without a residual 10.0 and 13.7), and two for short rows (9362 x 896 such rows 14.7 us on four, 10.4 on two)
     const bool wide = cols > 4096 || (rows <= 256 && cols > 2048), brief = cols <= 1024;
     auto kernel_of = [&](auto threads, auto held) {
         constexpr uint32_t THREADS = decltype(threads)::value, HELD = decltype(held)::value;
