@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import tensorwarp_amd as T
-from test_gpu_fp8 import BLOCK, E4M3, At, Big, Out, blocks, check_codes, gemm_inputs
+from test_gpu_fp8 import BLOCK, E4M3, At, Big, Out, blocks, check_codes, draw_tokens, gemm_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,55 @@ def test_small_products_beside_large_ones_that_cancel(dev, m, n, k):
         assert m > 16 and (np.abs(half.get().astype(np.float64) - k // 8 * 6) <= k * 2.0 ** 3).all()
     else:
         assert (half.get() == k // 8 * 6).all()
+
+
+# ---- the largest sizes that the header allows --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("m,n", [(1, 40), (16, 5000), (30, 17), (70, 300), (450, 130), (520, 200)])
+def test_products_of_the_deepest_rows(dev, m, n, dtype):
+    # 2^20 features of ones, the last sixteen 448 in the last row of A and the first of W: sums of whole numbers below 2^24 do not round
+    k, code = 1 << 20, {int(v): c for c, v in enumerate(E4M3) if v in (1.0, 448.0)}
+    a, w = np.full((m, k), code[1], np.uint8), np.full((n, k), code[1], np.uint8)
+    a[-1, -16:], w[0, -16:] = code[448], code[448]
+    a_s, w_s = np.full((m, blocks(k)), 2.0 ** -10, np.float32), np.full((blocks(n), blocks(k)), 2.0 ** -10, np.float32)
+    c = Out(dev, (m, n), dtype)
+    T.gemm_fp8(dev, At(dev, a), At(dev, a_s), At(dev, w), At(dev, w_s), m, n, k, c)
+    want = np.ones((m, n))
+    want[-1] += 16 * 447 / k
+    want[:, 0] += 16 * 447 / k
+    want[-1, 0] = 1 + 16 * (448 * 448 - 1) / k
+    assert np.array_equal(c.get().astype(np.float64), want.astype(np.float16 if dtype == "f16" else np.float32).astype(np.float64))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_rows_of_the_most_columns(dev, dtype):
+    rows, cols = 2, (1 << 24) - 5
+    rng = np.random.default_rng(41)
+    x = rng.standard_normal((rows, cols), np.float32).astype(np.float16 if dtype == "f16" else np.float32)
+    w = (1 + 0.3 * rng.standard_normal(cols, np.float32)).astype(np.float32)
+    q, s, total = Out(dev, (rows, cols), "u8"), Out(dev, (rows, blocks(cols)), "f32"), Out(dev, (rows, cols), "f32")
+    T.add_rms_norm_fp8(dev, At(dev, x), None, At(dev, w), 1e-6, rows, cols, q, s, sum=total)
+    y = x.astype(np.float64)
+    y = y / np.sqrt((y * y).mean(axis=1, keepdims=True) + 1e-6) * w
+    q, s = q.get(), s.get()
+    assert np.array_equal(total.get(), x.astype(np.float32))
+    for at in (slice(0, 1 << 15), slice(8 << 20, (8 << 20) + (1 << 15)), slice((cols >> 7) - 300 << 7, cols)):   # (whole blocks from the first)
+        check_codes(q[:, at], s[:, at.start >> 7:blocks(at.stop)], y[:, at], 2.0 ** -20 * np.abs(y[:, at]))
+    dim = cols // 2
+    x = x.reshape(-1)[:rows * 2 * dim].reshape(rows, 2 * dim)
+    q, s = Out(dev, (rows, dim), "u8"), Out(dev, (rows, blocks(dim)), "f32")
+    T.swiglu_rows_fp8(dev, At(dev, x), q, s, dim, rows)
+    q, s = q.get(), s.get()
+    for at in (slice(0, 1 << 15), slice((dim >> 7) - 300 << 7, dim)):
+        y = gates("silu", x[:, at], x[:, dim + at.start:dim + at.stop])
+        check_codes(q[:, at], s[:, at.start >> 7:blocks(at.stop)], y, 2.0 ** -20 * np.abs(y) + 1e-38)
+
+
+def test_sample_of_the_most_columns(dev):
+    rng = np.random.default_rng(42)
+    x = (2 * rng.standard_normal((1, 1 << 24), np.float32)).astype(np.float32)
+    x[0, rng.integers(0, 1 << 24, 24)] = 14.0
+    for limits in (dict(), dict(p=[0.9]), dict(k=[300], p=[0.95]), dict(k=[100000], mp=[0.001])):
+        got, want = draw_tokens(dev, x, rng.random(1), [0.8], **limits)
+        assert np.array_equal(got, want), limits
