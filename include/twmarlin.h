@@ -540,6 +540,65 @@ int twm_sample_f32(twm_ctx *ctx, const float *logits_dev, uint32_t rows, uint32_
                    const float *temperature_dev, const int32_t *top_k_dev, const float *top_p_dev, const float *min_p_dev,
                    int32_t *out_dev);
 
+/* ---- a paged key-value cache, and the attention that reads it ------------------------ */
+
+/* What stands between a layer's fused Q/K/V projection and its output projection, for programs that keep the keys and values of many
+ * sequences in one pool of pages (the reference keeps one contiguous cache per sequence, crates/kernels/src/kv_cache.rs).
+ *
+ * One layer's cache: two arrays of the caller's, [pages][kv_heads][page_tokens][head_dim], f16 or e4m3 codes (dtype TWM_F16 or TWM_U8;
+ * value = scale of the head * code, scales f32 [kv_heads] above zero, NULL: 1).  page_tokens is 16, 32, 64, 128 or 256,
+ * head_dim 64, 128 or 256, the arrays begin at 16 bytes. */
+typedef struct twm_kv_cache {
+    void *k_dev, *v_dev;
+    const float *k_scales_dev, *v_scales_dev;
+    int dtype;
+    uint32_t pages, page_tokens, kv_heads, head_dim;
+} twm_kv_cache;
+/* The sequences of one call.  Token t of sequence s lies in page tables[s][t / page_tokens] of the pool, at t % page_tokens.
+ * lengths[s] counts its tokens in the cache, this call's among them; the call's rows starts[s] .. starts[s + 1] - 1 are the last of
+ * these, in order (starts NULL: row s is sequence s's last token).  All three are i32 arrays on the device, read by the kernels: a
+ * captured call reads what they hold at its replay.  Sequences without rows or tokens are allowed.  Rows of no sequence -- before the
+ * first, behind the last -- stay as they were.  starts do not fall; a length below zero counts as zero, tokens that the table's row does
+ * not reach, or whose page number is outside the pool (-1, say, where a page was freed behind a window), as absent. */
+typedef struct twm_kv_seqs {
+    const int32_t *tables_dev;
+    const int32_t *lengths_dev;
+    const int32_t *starts_dev;
+    uint32_t seqs, table_stride;
+} twm_kv_seqs;
+/* Both structs are read during the call only.  Limits: 2^20 rows and sequences, 2^30 tokens in a table's row, 1024 heads, 2^28 pages;
+ * row strides count elements, rows begin at any element.  What a call writes overlaps nothing else that it is given.  The calls are
+ * asynchronous on the context's stream, allocate nothing and can be captured. */
+
+/* Adds new tokens to the cache.  qkv: `rows` rows of q_heads + 2 * kv_heads heads, [q | k | v], f16 or f32, qkv_stride apart (0: as wide
+ * as they are), as a fused projection stores them.  The first rotary_dim values of every q and k head are rotated by the token's
+ * position p in its sequence: pairs (a, b) of values j and j + rotary_dim / 2 (interleaved != 0: 2 j and 2 j + 1) become
+ * (a cos - b sin, b cos + a sin), cos and sin at cos_sin[p][j] and cos_sin[p][rotary_dim / 2 + j] of an f32 table of `positions` rows, so
+ * that any base and scaling of angles is the caller's.  rotary_dim: 0 (cos_sin may be NULL) or a multiple of 16 up to head_dim.
+ * q goes to q_out [rows][q_heads * head_dim] rounded to f16, k and v to the cache: in f16, or as code = e4m3_rne(x / scale), x / scale
+ * cut off at +-448 (NaN stays).  A position beyond the table makes q and k NaN.  Rows that precede their sequence's first token (more rows
+ * than tokens) are skipped, tokens that count as absent are not stored (their q is).  Two rows of one place in the pool: either's.  */
+int twm_kv_append(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *seqs, const void *qkv_dev, int qkv_dtype, uint32_t rows,
+                  uint32_t qkv_stride, uint32_t q_heads, const float *cos_sin_dev, uint32_t positions, uint32_t rotary_dim, int interleaved,
+                  uint16_t *q_out_dev);
+/* Attention of one new token per sequence: row s of q (f16, q_heads * head_dim values, q_stride apart, 0: dense) against the tokens of
+ * sequence s, the last `window` of them if window is not 0, and out row s likewise:
+ *   out[h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale * q[h] . k_t - max),   k_t and v_t of key-value head h / (q_heads / kv_heads)
+ * q_heads is a multiple of kv_heads; scale is above 0.  A row without tokens is zeros.  Scores, sums and weights are held in 32
+ * bits (the products take the weights as two f16 terms); only what a row sees counts, whatever else the pages hold.  starts_dev is not read.  Uses the
+ * context's scratch.  Deterministic for given lengths and sizes. */
+int twm_attn_decode(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *seqs, const uint16_t *q_dev, uint32_t q_stride,
+                    uint32_t q_heads, float scale, uint32_t window, uint16_t *out_dev, uint32_t out_stride);
+/* The same for several new tokens per sequence -- whole prompts, pieces of them behind what is cached already, drafts to verify --, packed as
+ * seqs->starts_dev says (not NULL): the row at position p sees the tokens up to p, the last `window` of these.  Weights enter the
+ * products rounded to f16; sums are held in 32 bits. */
+int twm_attn_prompt(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *seqs, const uint16_t *q_dev, uint32_t q_stride,
+                    uint32_t rows, uint32_t q_heads, float scale, uint32_t window, uint16_t *out_dev, uint32_t out_stride);
+/* Copies page sources[i] to page targets[i], i < pairs, keys and values, in every one of `count` caches of the same shape and type (a model's
+ * layers): a fork's last page, the moves that compact a pool.  Both are host arrays, as is caches; a captured call copies the same pages
+ * at every replay.  A page outside the pool, a target named twice or named as a source too returns TWM_SHAPE_ERROR. */
+int twm_kv_copy_pages(twm_ctx *ctx, const twm_kv_cache *caches, uint32_t count, const uint32_t *sources, const uint32_t *targets, uint32_t pairs);
+
 /* The library's split-K choice for MI355X (256 CUs) with f16 activations; same role as quantize.rs:1317-1325.
  * 1 where the plan needs no split (among others wherever M <= 16 runs on column sub-tiles). */
 uint32_t twm_pick_splits(uint32_t k, uint32_t n, uint32_t m);

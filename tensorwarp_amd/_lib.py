@@ -14,6 +14,18 @@ F32, F16, I32, I8, U8 = range(5)
 
 _vp, _u32, _sz, _int = C.c_void_p, C.c_uint32, C.c_size_t, C.c_int
 
+
+class KvCacheStruct(C.Structure):
+    """twm_kv_cache"""
+    _fields_ = [("k_dev", _vp), ("v_dev", _vp), ("k_scales_dev", _vp), ("v_scales_dev", _vp), ("dtype", _int), ("pages", _u32),
+                ("page_tokens", _u32), ("kv_heads", _u32), ("head_dim", _u32)]
+
+
+class KvSeqsStruct(C.Structure):
+    """twm_kv_seqs"""
+    _fields_ = [("tables_dev", _vp), ("lengths_dev", _vp), ("starts_dev", _vp), ("seqs", _u32), ("table_stride", _u32)]
+
+
 # name -> (restype, argtypes); the list every symbol of include/twmarlin.h must match
 SIGNATURES = {
     "twm_version": (C.c_char_p, []),
@@ -104,6 +116,10 @@ SIGNATURES = {
     "twm_geglu_rows_fp8": (_int, [_vp, _vp, _int, _u32, _u32, _int, _vp, _vp]),
     "twm_add_rms_norm_fp8": (_int, [_vp, _vp, _int, _vp, _vp, C.c_float, _u32, _u32, _vp, _vp, _vp, _vp]),
     "twm_sample_f32": (_int, [_vp, _vp, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "twm_kv_append": (_int, [_vp, C.POINTER(KvCacheStruct), C.POINTER(KvSeqsStruct), _vp, _int, _u32, _u32, _u32, _vp, _u32, _u32, _int, _vp]),
+    "twm_attn_decode": (_int, [_vp, C.POINTER(KvCacheStruct), C.POINTER(KvSeqsStruct), _vp, _u32, _u32, C.c_float, _u32, _vp, _u32]),
+    "twm_attn_prompt": (_int, [_vp, C.POINTER(KvCacheStruct), C.POINTER(KvSeqsStruct), _vp, _u32, _u32, _u32, C.c_float, _u32, _vp, _u32]),
+    "twm_kv_copy_pages": (_int, [_vp, C.POINTER(KvCacheStruct), _u32, _vp, _vp, _u32]),
     "twm_pick_splits": (_u32, [_u32, _u32, _u32]),
     "twm_graph_begin": (_int, [_vp]),
     "twm_graph_end": (_vp, [_vp]),

@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtwmarlin_hip.so")
 SOURCES = ["twm_kernels.hip", "twm_gemv4.hip", "twm_gemv4s.hip", "twm_gemv4g.hip", "twm_moe.hip", "twm_stream.hip", "twm_batch.hip", "twm_waves.hip", "twm_waves_exact.hip", "twm_batch_range.hip", "twm_splitk.hip", "twm_prefill.hip", "twm_debug_mix.hip", "twm_noalloc.hip", "twm_fp8_rows.hip", "twm_fp8_gemm.hip",
-           "twm_sample.hip", "twm_api.hip", "twm_api_weights.hip", "twm_api_gemm.hip", "twm_api_moe.hip", "twm_api_fp8.hip"]
+           "twm_sample.hip", "twm_kv_cache.hip", "twm_attn_decode.hip", "twm_attn_prompt.hip", "twm_api.hip", "twm_api_weights.hip", "twm_api_gemm.hip", "twm_api_moe.hip", "twm_api_fp8.hip", "twm_api_kv.hip"]
 # The batched-decode kernels read every MFMA result with vector instructions right away (scale, add):
 # with the default choice the results land in AGPRs and each costs a v_accvgpr_read first.
 # The decode kernels' first argument words (thirteen fit the user scalar registers) arrive preloaded (see k_gemv4s).

@@ -6,30 +6,9 @@ using namespace twm;
 
 namespace {
 
-// The context's device is current while one of these lives: a launch takes its code from the current device, which need not be
-// the one that the context's stream belongs to.
-struct DeviceGuard {
-    int before = -1;
-    hipError_t status;
-    explicit DeviceGuard(const twm_ctx *ctx)
-    {
-        int now = -1;
-        status = hipGetDevice(&now);
-        if (status == hipSuccess && now != ctx->ordinal) {
-            status = hipSetDevice(ctx->ordinal);
-            if (status == hipSuccess) before = now;
-        }
-    }
-    ~DeviceGuard()
-    {
-        if (before >= 0) (void)hipSetDevice(before);
-    }
-};
-
 constexpr uint32_t kFp8MostDim = 1u << 24;   // rows and columns of one call
 constexpr uint32_t kFp8MostK = 1u << 20;     // features of a product (256 rows of codes are within a buffer's 32-bit offsets)
 
-bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 bool row_type(int dtype) { return dtype == TWM_F32 || dtype == TWM_F16; }
 
 // what the calls that write e4m3 rows check alike; 1: nothing to do

@@ -4,6 +4,7 @@
 //   twm_api_weights.hip  repacked weight handles and their byte blob
 //   twm_api_gemm.hip     launch planners, the dispatcher of twm_gemm and its variants, measured plans
 //   twm_api_fp8.hip      8-bit floating point: products, the rows that feed them; token sampling
+//   twm_api_kv.hip       the paged key-value cache and the attention that reads it
 //   twm_api_moe.hip      expert banks and the reference's MoE launches on raw slabs
 #pragma once
 #include "../../include/twmarlin.h"
@@ -61,6 +62,28 @@ struct twm_ctx {
     int batch_rounded;    // M = 17 .. 32: 1 = weights rounded to f16 (the reference's dequant-then-FP16-GEMM arithmetic), 0 = exact
     hipDeviceProp_t prop;
 };
+
+// The context's device is current while one of these lives: a launch takes its code from the current device, which need not be
+// the one that the context's stream belongs to.
+struct DeviceGuard {
+    int before = -1;
+    hipError_t status;
+    explicit DeviceGuard(const twm_ctx *ctx)
+    {
+        int now = -1;
+        status = hipGetDevice(&now);
+        if (status == hipSuccess && now != ctx->ordinal) {
+            status = hipSetDevice(ctx->ordinal);
+            if (status == hipSuccess) before = now;
+        }
+    }
+    ~DeviceGuard()
+    {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+inline bool misaligned(const void *p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 
 // A launch form as the option knobs name it (twm_ctx_set_option), measured to be the fastest for one weight and one
 // bucket of row counts by twm_weight_tune: the role of the per-shape table of crates/kernels/src/autotune.rs:254-396.

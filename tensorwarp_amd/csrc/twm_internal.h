@@ -240,4 +240,31 @@ hipError_t launch_sample(hipStream_t s, const float *logits, uint32_t rows, uint
                          const int *top_k, const float *top_p, const float *min_p, int *out, void *scratch, size_t scratch_bytes,
                          unsigned *counters, uint32_t n_counters);
 
+// One layer's paged key-value cache and the sequences of a call (include/twmarlin.h has what they mean)
+struct KvView {
+    void *k, *v;
+    const float *k_scales, *v_scales;
+    uint32_t e4m3, pages, page_shift, kv_heads, dim;   // page_shift: log2 of the tokens in a page
+};
+struct KvSeqs {
+    const int *tables, *lengths, *starts;
+    uint32_t seqs, table_stride;
+};
+hipError_t launch_kv_append(hipStream_t s, const KvView &kv, const KvSeqs &seqs, const void *qkv, bool f16, uint32_t rows, uint32_t qkv_stride,
+                            uint32_t q_heads, const float *cos_sin, uint32_t positions, uint32_t rotary_dim, bool interleaved, _Float16 *q_out);
+// every cache's page sources[i] to its page targets[i]; the caches share one shape
+hipError_t launch_kv_copy_pages(hipStream_t s, const KvView *caches, uint32_t count, const uint32_t *sources, const uint32_t *targets, uint32_t pairs);
+// rows of f16 queries against their sequences' tokens (twm_attn_decode.hip: a row a sequence; twm_attn_prompt.hip: packed rows)
+struct AttnArgs {
+    KvView kv;
+    KvSeqs seqs;
+    const _Float16 *q;
+    _Float16 *out;
+    uint32_t rows, q_stride, out_stride, q_heads, group;   // group = q_heads / kv_heads
+    float scale;
+    uint32_t window;   // 0: none
+};
+hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes);
+hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a);
+
 }  // namespace twm
