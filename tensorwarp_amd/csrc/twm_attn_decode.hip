@@ -1,17 +1,447 @@
 // Attention of one new token per sequence over a paged key-value cache.
-#include "twm_attn_rows.h"
+//
+//   out[h] = sum_t w_t v_t / sum_t w_t,   w_t = 2^(15 + c (s_t - m)),   s_t = q[h] . k_t,   c = scale * log2(e) * the head's scale of keys
+//
+// with m the largest s_t so far; whatever was summed is multiplied by 2^(c (m - m')) when it grows to m'.
+//
+// Keys and values are read once, from memory to registers, whatever the number of query heads that share them: up to sixteen heads are the
+// columns of the matrix instructions (16 x 16 x 32), thirty-two tokens at a time.  Scores come transposed, S^T = K Q^T, which leaves a lane
+// with eight neighbouring tokens of one head: the operand that O^T = V^T P^T asks for, without an exchange between lanes.  The instruction
+// takes the tokens in any order that both operands agree on, so rows 4 g + i of its two blocks are tokens 8 g + i and 8 g + 4 + i.  V^T comes from
+// LDS through the transposing reads; every wave has a buffer of its own there and no other wave is waited for.
+//
+// Weights enter the product as two f16 terms, the first one cut off and the second what it leaves: both are positive, and at least the
+// smallest f16 number where a token is seen (2^-39 of the largest weight), so that an infinite value times its weight is that infinity.
+//
+// All tokens of all sequences and heads, in steps of 128, are dealt out evenly among as many workgroups as the chip holds at once, which
+// find their share from the lengths by themselves: a long sequence is cut into many shares, several short ones make one.  What a share
+// holds of a sequence that others hold too goes to scratch, and a second kernel joins it.
+#include "twm_kv.h"
+
+#include <algorithm>
+#include <cmath>
 
 namespace twm {
 
-template <bool E4M3> __global__ __launch_bounds__(64) void k_attn_decode(const AttnArgs a)
+namespace {
+
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef int int2v __attribute__((ext_vector_type(2)));
+#define TWM_LDS(T) __attribute__((address_space(3))) T
+
+constexpr uint32_t kDecodeHeads = 16;   // query heads of one unit: columns of a matrix instruction
+constexpr uint32_t kDecodeWaves = 4, kDecodeStep = 32 * kDecodeWaves;
+constexpr int kNoScore = 0xFF800000;   // -infinity
+
+struct Decode {
+    AttnArgs a;
+    float *parts;          // [2 * workgroups][heads of a unit][dim]
+    float2 *part_sums;     // [2 * workgroups][heads of a unit]: largest score, sum of weights
+    uint32_t units, tiles;   // per sequence: tiles of up to sixteen heads for each key-value head
+    uint32_t heads;          // of a unit
+    uint32_t shares;         // workgroups of the first kernel
+};
+
+// The tokens that sequence `seq` sees, from `first`, the multiple of 32 at or below the first one, in steps of 128
+struct Span {
+    int lo, hi, first;
+    uint32_t steps;
+};
+__device__ __forceinline__ Span span_of(const Decode &d, int length)
 {
-    attend_row<E4M3>(a, blockIdx.x, blockIdx.y, (int)blockIdx.x, a.seqs.lengths[blockIdx.x] - 1);
+    Span s;
+    s.hi = min(length, (int)(d.a.seqs.table_stride << d.a.kv.page_shift));
+    s.lo = d.a.window ? max(0, length - (int)d.a.window) : 0;
+    s.first = s.lo & ~31;
+    s.steps = s.hi > s.lo && d.a.kv.pages ? (uint32_t)(s.hi - s.first + (int)kDecodeStep - 1) / kDecodeStep : 0u;
+    return s;
 }
 
-hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *, size_t)
+__device__ __forceinline__ uint64_t wave_sum_up_to(uint64_t v)   // of this lane and those before it
 {
-    hipLaunchKernelGGL(a.kv.e4m3 ? k_attn_decode<true> : k_attn_decode<false>, dim3(a.rows, a.q_heads), dim3(64), 0, s, a);
-    return hipGetLastError();
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (uint32_t i = 1; i < 64; i *= 2) {
+        const uint64_t other = __shfl_up((unsigned long long)v, i);
+        if (lane >= i) v += other;
+    }
+    return v;
+}
+
+// Steps of all sequences and units, and of those before sequence `until`
+__device__ __forceinline__ uint64_t all_steps(const Decode &d, uint32_t until, uint64_t *before)
+{
+    uint64_t sum = 0;
+    *before = 0;
+    for (uint32_t base = 0; base < d.a.seqs.seqs; base += 64) {
+        const uint32_t s = base + (threadIdx.x & 63u);
+        const uint64_t up_to = wave_sum_up_to(s < d.a.seqs.seqs ? (uint64_t)span_of(d, d.a.seqs.lengths[s]).steps * d.units : 0u);
+        if (until >= base && until < base + 64) *before = until == base ? sum : sum + __shfl((unsigned long long)up_to, until - base - 1);
+        sum += __shfl((unsigned long long)up_to, 63);
+    }
+    return sum;
+}
+
+// The sequence that step `at` belongs to (there is one); *before: the steps ahead of it
+__device__ __forceinline__ uint32_t sequence_of(const Decode &d, uint64_t at, uint64_t *before)
+{
+    uint64_t sum = 0;
+    for (uint32_t base = 0; base < d.a.seqs.seqs; base += 64) {
+        const uint32_t s = base + (threadIdx.x & 63u);
+        const uint64_t up_to = wave_sum_up_to(s < d.a.seqs.seqs ? (uint64_t)span_of(d, d.a.seqs.lengths[s]).steps * d.units : 0u);
+        const uint64_t past = __ballot(sum + up_to > at);
+        if (past) {
+            const uint32_t lane = (uint32_t)__builtin_ctzll(past);
+            *before = lane == 0 ? sum : sum + __shfl((unsigned long long)up_to, lane - 1);
+            return base + lane;
+        }
+        sum += __shfl((unsigned long long)up_to, 63);
+    }
+    *before = sum;
+    return d.a.seqs.seqs;
+}
+
+// Every share has a step at least
+__device__ __forceinline__ uint32_t shares_of(const Decode &d, uint64_t total) { return (uint32_t)min((uint64_t)d.shares, total); }
+
+// Share w of `total` steps begins here
+__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t w, uint32_t shares) { return total / shares * w + total % shares * w / shares; }
+
+__device__ __forceinline__ float max_over_quarters(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_over_quarters(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// eight codes as f16 (exact)
+__device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
+{
+    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
+    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// 2^(c (m - m')), of sums that hold something
+__device__ __forceinline__ float shrink(float m, float to, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * c); }
+
+// Workgroups of four waves that share a compute unit, by their registers
+template <int D, bool E4M3> constexpr uint32_t kDecodePerUnit = D == 256 ? (E4M3 ? 2 : 1) : D == 128 ? (E4M3 ? 3 : 2) : 3;
+
+}  // namespace
+
+template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D, E4M3>)) void k_attn_decode(const Decode d)
+{
+    constexpr uint32_t kRow = D * (E4M3 ? 1 : 2);          // bytes of a token
+    constexpr uint32_t kStride = kRow + 32;                // in LDS: four rows that are read at once lie in different banks
+    constexpr uint32_t kBuffer = 32 * kStride > kDecodeHeads * D * 4 ? 32 * kStride : kDecodeHeads * D * 4;   // also a wave's results
+    constexpr int NK = kRow / 64, NV = 32 * kRow / 1024;   // loads per lane: of each block of 16 keys, of 32 values
+    constexpr uint32_t kLanesPerRow = kRow / 16, kRowsPerLoad = 64 / kLanesPerRow;
+    __shared__ __align__(16) char buffers[kDecodeWaves][kBuffer];
+    __shared__ half8 queries[D / 32 * 64];
+    __shared__ float tops[kDecodeWaves][kDecodeHeads], sums[kDecodeWaves][kDecodeHeads];
+    const AttnArgs &a = d.a;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, quarter = lane >> 4, col = lane & 15u;
+    char *const buffer = buffers[wave];
+
+    // rows without tokens
+    for (uint32_t s = blockIdx.x; s < a.seqs.seqs; s += gridDim.x)
+        if (span_of(d, a.seqs.lengths[s]).steps == 0)
+            for (uint32_t i = threadIdx.x; i < a.q_heads * D / 8; i += 256) *(half8_any *)(a.out + (size_t)s * a.out_stride + 8u * i) = half8{};
+
+    uint64_t before;
+    const uint64_t total = all_steps(d, 0, &before);
+    const uint32_t shares = shares_of(d, total);
+    if (blockIdx.x >= shares) return;
+    uint64_t at = share_begin(total, blockIdx.x, shares);
+    const uint64_t end = share_begin(total, blockIdx.x + 1, shares);
+    uint32_t seq = __builtin_amdgcn_readfirstlane(sequence_of(d, at, &before));
+    uint32_t part = 2 * blockIdx.x;
+    const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
+    for (bool first_of_share = true; at < end; first_of_share = false) {
+        const Span span = span_of(d, __builtin_amdgcn_readfirstlane(a.seqs.lengths[seq]));
+        if (span.steps == 0) {
+            seq++;
+            continue;
+        }
+        // this share's steps of one unit
+        const uint64_t inside = at - before;
+        const uint32_t unit = (uint32_t)(inside / span.steps), step0 = (uint32_t)(inside - (uint64_t)unit * span.steps);
+        const uint32_t step1 = (uint32_t)min((uint64_t)span.steps, step0 + (end - at));
+        const uint32_t kv_head = unit / d.tiles, head0 = kv_head * a.group + (unit - kv_head * d.tiles) * kDecodeHeads;
+        const uint32_t heads = min(kDecodeHeads, (kv_head + 1) * a.group - head0);
+        const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+
+        // Q^T: a lane's head's values, in the order in which it holds keys
+        for (uint32_t x = threadIdx.x; x < D / 32 * 64; x += 256) {
+            const uint32_t i = x >> 6, head = min(x & 15u, heads - 1), g = x >> 4 & 3u;
+            queries[x] = *(const half8_any *)(a.q + (size_t)seq * a.q_stride + (head0 + head) * D + (E4M3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8));
+        }
+
+        float top = -INFINITY, sum = 0.f;
+        float4v o[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
+
+        const TWM_CONSTANT int *table = (const TWM_CONSTANT int *)(a.seqs.tables + (size_t)seq * a.seqs.table_stride);
+        const char *const k_base = (const char *)a.kv.k, *const v_base = (const char *)a.kv.v;
+        int page0, page1;   // of this wave's next 32 tokens' halves
+        auto pages_of = [&](int t) {
+            page0 = table[(uint32_t)t >> a.kv.page_shift];
+            page1 = t + 16 < span.hi ? table[(uint32_t)(t + 16) >> a.kv.page_shift] : -1;
+        };
+        uint4v k[2][NK], v[NV];
+        bool k_there = false;   // whether both pages are inside the pool
+        auto load = [&](int t) {
+            const bool in0 = (uint32_t)page0 < a.kv.pages, in1 = (uint32_t)page1 < a.kv.pages;
+            k_there = in0 && in1;
+            // what lies outside is read from the pool's first page, and left out
+            const size_t chunk0 = kv_chunk(a.kv, in0 ? (uint32_t)page0 : 0u, kv_head) + ((uint32_t)t & page_mask) * D;
+            const size_t chunk1 = kv_chunk(a.kv, in1 ? (uint32_t)page1 : 0u, kv_head) + ((uint32_t)(t + 16) & page_mask) * D;
+            const size_t bytes0 = chunk0 * (E4M3 ? 1 : 2), bytes1 = chunk1 * (E4M3 ? 1 : 2);
+            const char *key = k_base + (col < 8 ? bytes0 : bytes1) + (8u * ((col >> 2) & 1u) + (col & 3u)) * kRow + quarter * 16u;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < NK; i++) k[b][i] = *(const uint4v *)(key + b * 4 * kRow + i * 64);
+            const uint32_t v_off = lane / kLanesPerRow * kRow + lane % kLanesPerRow * 16u;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const uint32_t row = i * kRowsPerLoad;   // (a load's rows lie in one half)
+                v[i] = *(const uint4v *)(v_base + (row < 16 ? bytes0 + row * kRow : bytes1 + (row - 16) * kRow) + v_off);
+            }
+        };
+        const int stop = min(span.hi, span.first + (int)(step1 * kDecodeStep));
+        int t = span.first + (int)(step0 * kDecodeStep + wave * 32u);
+        if (t < stop) {
+            pages_of(t);
+            load(t);
+        }
+        __syncthreads();
+        for (; t < stop; t += (int)kDecodeStep) {
+            const bool whole = k_there && t >= span.lo && t + 32 <= span.hi;
+            const bool in0 = (uint32_t)page0 < a.kv.pages, in1 = (uint32_t)page1 < a.kv.pages;
+            // values to LDS; what is not seen is zeros there, whatever it may be in memory
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const uint32_t row = i * kRowsPerLoad + lane / kLanesPerRow;
+                if (!whole) {
+                    const int token = t + (int)row;
+                    const bool seen = token >= span.lo && token < span.hi && (row < 16 ? in0 : in1);
+                    v[i] = seen ? v[i] : uint4v{0u, 0u, 0u, 0u};
+                }
+                *(uint4v *)(buffer + row * kStride + lane % kLanesPerRow * 16u) = v[i];
+            }
+            float4v s[2];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                s[b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) {
+                    half8 key;
+                    if constexpr (E4M3)
+                        key = to_f16(k[b][i / 2][(i % 2) * 2], k[b][i / 2][(i % 2) * 2 + 1]);
+                    else
+                        key = __builtin_bit_cast(half8, k[b][i]);
+                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, queries[i * 64 + lane], s[b], 0, 0, 0);
+                }
+            }
+            const int next = t + (int)kDecodeStep;
+            if (next < stop) {
+                pages_of(next);
+                load(next);
+            }
+            // scores of tokens t + 8 quarter + 4 b + i
+            uint32_t seen = 0xFFu;
+            if (!whole) {
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int token = t + 8 * (int)quarter + i;
+                    const bool one = token >= span.lo && token < span.hi && (quarter < 2 ? in0 : in1);
+                    seen |= one ? 1u << i : 0u;
+                    s[i / 4][i % 4] = one ? s[i / 4][i % 4] : __int_as_float(kNoScore);
+                }
+            }
+            float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            most = fmaxf(top, max_over_quarters(most));
+            if (__any(most > top)) {
+                const float by = shrink(top, most, c);
+                sum *= by;
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) o[i] *= by;
+                top = most;
+            }
+            const float base = 15.0f - (top == -INFINITY ? 0.f : top) * c;
+            half2v p_hi[4], p_lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4], c, base)), y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4 + 1], c, base));
+                sum += x + y;
+                p_hi[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
+                p_lo[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x - (float)p_hi[i][0], y - (float)p_hi[i][1]));
+                const uint32_t least = (seen >> (2 * i) & 1u) | (seen >> (2 * i + 1) & 1u) << 16;   // 2^-24
+                p_hi[i] = __builtin_elementwise_max(p_hi[i], __builtin_bit_cast(half2v, least));
+                p_lo[i] = __builtin_elementwise_max(p_lo[i], __builtin_bit_cast(half2v, least));
+            }
+            const half8 hi = {p_hi[0][0], p_hi[0][1], p_hi[1][0], p_hi[1][1], p_hi[2][0], p_hi[2][1], p_hi[3][0], p_hi[3][1]};
+            const half8 lo = {p_lo[0][0], p_lo[0][1], p_lo[1][0], p_lo[1][1], p_lo[2][0], p_lo[2][1], p_lo[3][0], p_lo[3][1]};
+            // (the wave's own stores have reached LDS: its reads come after them, in order)
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                half8 value;
+                if constexpr (E4M3) {
+                    const int2v codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (TWM_LDS(int2v) *)(buffer + (8u * quarter + (col >> 1)) * kStride + 16u * i + 8u * (col & 1u)));
+                    value = to_f16((unsigned)codes[0], (unsigned)codes[1]);
+                } else {
+                    const char *from = buffer + (8u * quarter + (col >> 2)) * kStride + 32u * i + 8u * (col & 3u);
+                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)from));
+                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(from + 4 * kStride)));
+                    value = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                }
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, hi, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, lo, o[i], 0, 0, 0);
+            }
+        }
+
+        // the waves' sums, brought to the largest score of all and added in wave order
+        sum = sum_over_quarters(sum);
+        if (lane < 16) {
+            tops[wave][col] = top;
+            sums[wave][col] = sum;
+        }
+        __syncthreads();
+        float most = top;
+#pragma unroll
+        for (uint32_t w = 0; w < kDecodeWaves; w++) most = fmaxf(most, tops[w][col]);
+        const float by = shrink(top, most, c);
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) *(float4v *)(buffer + (col * D + 16 * i + 4 * quarter) * 4) = o[i] * by;
+        __syncthreads();
+        const bool all = step0 == 0 && step1 == span.steps;
+        const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
+        for (uint32_t i = threadIdx.x; i < heads * (D / 4); i += 256) {
+            const uint32_t h = i / (D / 4), x = i % (D / 4) * 4;
+            float4v r = *(const float4v *)(buffers[0] + (h * D + x) * 4);
+#pragma unroll
+            for (uint32_t w = 1; w < kDecodeWaves; w++) r += *(const float4v *)(buffers[w] + (h * D + x) * 4);
+            float m = tops[0][h], l = 0.f;
+#pragma unroll
+            for (uint32_t w = 1; w < kDecodeWaves; w++) m = fmaxf(m, tops[w][h]);
+#pragma unroll
+            for (uint32_t w = 0; w < kDecodeWaves; w++) l += sums[w][h] * shrink(tops[w][h], m, c);
+            if (all) {
+                const float to = l == 0.f ? 0.f : v_scale / l;
+                typedef half4 half4_any __attribute__((aligned(2)));
+                *(half4_any *)(a.out + (size_t)seq * a.out_stride + (head0 + h) * D + x) =
+                    half4{(_Float16)(r[0] * to), (_Float16)(r[1] * to), (_Float16)(r[2] * to), (_Float16)(r[3] * to)};
+            } else {
+                // a share holds at most two parts: of the unit in which it begins, and of the one in which it ends
+                const size_t slot = (size_t)(first_of_share ? part : part + 1) * d.heads + h;
+                *(float4v *)(d.parts + slot * D + x) = r;
+                if (x == 0) d.part_sums[slot] = float2{m, l};
+            }
+        }
+        __syncthreads();   // (the buffers are the waves' own again)
+        at += step1 - step0;
+        if (at - before == (uint64_t)span.steps * d.units) {
+            before = at;
+            seq++;
+        }
+    }
+}
+
+// Joins what several shares hold of a unit: a workgroup per query head and sequence, its waves every fourth share.
+template <int D> __global__ __launch_bounds__(256) void k_attn_join(const Decode d)
+{
+    __shared__ float tops[4], totals[4], results[4][D];
+    const AttnArgs &a = d.a;
+    const uint32_t seq = blockIdx.x, head = blockIdx.y, kv_head = head / a.group, in_group = head - kv_head * a.group;
+    const uint32_t unit = kv_head * d.tiles + in_group / kDecodeHeads, h = in_group % kDecodeHeads;
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const uint32_t steps = span_of(d, a.seqs.lengths[seq]).steps;
+    uint64_t before;
+    const uint64_t total = all_steps(d, seq, &before);
+    if (steps == 0) return;
+    const uint64_t begin = before + (uint64_t)unit * steps, end = begin + steps;
+    const uint32_t shares = shares_of(d, total);
+    // the shares that hold its first and its last step
+    auto share_of = [&](uint64_t at) {
+        uint32_t w = (uint32_t)min((uint64_t)(shares - 1), (uint64_t)((double)at / (double)total * shares));
+        while (share_begin(total, w, shares) > at) w--;
+        while (share_begin(total, w + 1, shares) <= at) w++;
+        return w;
+    };
+    const uint32_t first = share_of(begin), last = share_of(end - 1);
+    if (first == last) return;
+    const uint32_t first_slot = 2 * first + (share_begin(total, first, shares) < begin ? 1u : 0u);
+    auto slot_of = [&](uint32_t w) { return (size_t)(w == first ? first_slot : 2 * w) * d.heads + h; };
+    const float c = a.scale * 1.44269504f * (a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f), v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
+    float top = -INFINITY;
+    for (uint32_t w = first + threadIdx.x; w <= last; w += 256) top = fmaxf(top, d.part_sums[slot_of(w)].x);
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    float l = 0.f, r[D / 64] = {};
+    for (uint32_t w = first + wave; w <= last; w += 4) {
+        const size_t slot = slot_of(w);
+        const float2 ml = d.part_sums[slot];
+        const float by = shrink(ml.x, top, c);
+        l += ml.y * by;
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) r[i] += d.parts[slot * D + 64 * i + lane] * by;
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) results[wave][64 * i + lane] = r[i];
+    if (lane == 0) totals[wave] = l;
+    __syncthreads();
+    l = totals[0] + totals[1] + totals[2] + totals[3];
+    const float to = l == 0.f ? 0.f : v_scale / l;
+    for (uint32_t i = threadIdx.x; i < D; i += 256)
+        a.out[(size_t)seq * a.out_stride + head * D + i] = (_Float16)((results[0][i] + results[1][i] + results[2][i] + results[3][i]) * to);
+}
+
+hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes)
+{
+    Decode d;
+    d.a = a;
+    d.tiles = (a.group + kDecodeHeads - 1) / kDecodeHeads;
+    d.units = a.kv.kv_heads * d.tiles;
+    d.heads = std::min(a.group, kDecodeHeads);
+    const uint32_t per_unit = a.kv.dim == 64    ? kDecodePerUnit<64, false>
+                              : a.kv.dim == 128 ? (a.kv.e4m3 ? kDecodePerUnit<128, true> : kDecodePerUnit<128, false>)
+                                                : (a.kv.e4m3 ? kDecodePerUnit<256, true> : kDecodePerUnit<256, false>);
+    // as many workgroups as the chip holds at once, or as there may be steps
+    const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
+    const uint64_t most_steps = (std::min(capacity, a.window ? (uint64_t)a.window + 31 : capacity) + kDecodeStep - 1) / kDecodeStep;
+    d.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 * per_unit, most_steps * d.units * a.seqs.seqs));
+    const size_t slots = 2 * (size_t)d.shares * d.heads;
+    d.part_sums = (float2 *)scratch;
+    d.parts = (float *)((char *)scratch + (slots * sizeof(float2) + 255) / 256 * 256);
+    if ((size_t)((char *)(d.parts + slots * a.kv.dim) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 25 MB of 256)
+    auto kernels = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_decode<D, true> : k_attn_decode<D, false>), dim3(d.shares), dim3(256), 0, s, d);
+        hipError_t error = hipGetLastError();
+        if (error != hipSuccess || most_steps <= 1) return error;   // (a step is never cut)
+        hipLaunchKernelGGL(k_attn_join<D>, dim3(a.seqs.seqs, a.q_heads), dim3(256), 0, s, d);
+        return hipGetLastError();
+    };
+    return a.kv.dim == 64    ? kernels(std::integral_constant<int, 64>{})
+           : a.kv.dim == 128 ? kernels(std::integral_constant<int, 128>{})
+                             : kernels(std::integral_constant<int, 256>{});
 }
 
 }  // namespace twm
