@@ -1,22 +1,375 @@
 // Causal attention of packed rows over a paged key-value cache.
-#include "twm_attn_rows.h"
+//
+//   out[row][h] = sum_t w_t v_t / sum_t w_t,   w_t = 2^(c s_t - r),   s_t = q . k_t,   c = scale * log2(e) * the head's scale of keys
+//
+// over the tokens t that the row sees, r a reference for the row's exponents: 8 below the largest one when it was set, moved (and the sums with
+// it) only where a weight would pass 2^15, so that sums are rarely touched again and f16 holds the weights with all of its digits down to 2^-22
+// of the largest.
+//
+// A workgroup takes 128 queries of one key-value head -- tokens times the query heads that share it, so that short prompts fill
+// tiles too -- and its four waves 32 each.  Keys and values come through LDS, tile by tile, the next tile on its way while this one is worked on;
+// f16 ones directly, 16 bytes a lane, e4m3 ones through registers, where they become f16.  Scores are transposed, S^T = K Q^T: a
+// lane then holds the scores of one query, row maxima need one exchange between lanes, and the weights already lie as O^T = V^T P^T wants
+// its operand (the product takes tokens in any order that both operands agree on).  V^T comes from LDS through the transposing reads.
+// Units of 16 bytes are stored at their place XOR their row's number, so that the rows which one instruction reads lie in different banks.
+//
+// Where a tile holds tokens that some of the queries do not see, weights alone would not keep an infinity or a NaN away from these (0 times
+// either is NaN): there values are looked through first, rows that nobody sees become zeros, and if anything not finite is left, the tile's
+// products are made one token at a time, for those who see it.
+#include "twm_kv.h"
+#include "twm_slices.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace twm {
 
-template <bool E4M3> __global__ __launch_bounds__(64) void k_attn_prompt(const AttnArgs a)
+namespace {
+
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef half4 half4_any __attribute__((aligned(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+#define TWM_LDS(T) __attribute__((address_space(3))) T
+
+constexpr uint32_t kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
+
+// Workgroups of one key-value head: 128 rows each, token by token
+__device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, uint32_t seq)
 {
-    const int row = (int)blockIdx.x;
-    int seq = -1;
-    for (uint32_t s = 0; s < a.seqs.seqs; s++)
-        if (a.seqs.starts[s] <= row && row < a.seqs.starts[s + 1]) seq = (int)s;
-    if (seq < 0) return;
-    attend_row<E4M3>(a, blockIdx.x, blockIdx.y, seq, a.seqs.lengths[seq] - (a.seqs.starts[seq + 1] - row));
+    const int first = max(a.seqs.starts[seq], 0), end = min(a.seqs.starts[seq + 1], (int)a.rows);
+    return end > first ? ((uint32_t)(end - first) * a.group + kPromptRows - 1) / kPromptRows : 0u;
+}
+
+__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)   // of this lane and those before it
+{
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (uint32_t i = 1; i < 64; i *= 2) {
+        const uint32_t other = __shfl_up(v, i);
+        if (lane >= i) v += other;
+    }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t prompt_tiles_of_all(const AttnArgs &a)
+{
+    uint32_t sum = 0;
+    for (uint32_t s = threadIdx.x & 63u; s < a.seqs.seqs; s += 64) sum += prompt_tiles(a, s);
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
+    return sum;
+}
+
+// the sequence of tile `at` of a key-value head, and its place among the sequence's
+__device__ __forceinline__ uint32_t prompt_sequence_of(const AttnArgs &a, uint32_t at, uint32_t *inside)
+{
+    uint32_t sum = 0;
+    for (uint32_t base = 0; base < a.seqs.seqs; base += 64) {
+        const uint32_t s = base + (threadIdx.x & 63u);
+        const uint32_t up_to = wave_sum_up_to(s < a.seqs.seqs ? prompt_tiles(a, s) : 0u);
+        const uint64_t past = __ballot(sum + up_to > at);
+        if (past) {
+            const uint32_t lane = (uint32_t)__builtin_ctzll(past);
+            *inside = at - (lane == 0 ? sum : sum + __shfl(up_to, lane - 1));
+            return base + lane;
+        }
+        sum += __shfl(up_to, 63);
+    }
+    *inside = 0;
+    return 0;
+}
+
+__device__ __forceinline__ float max_of_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// eight codes as f16 (exact)
+__device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
+{
+    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
+    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+__device__ __forceinline__ bool not_finite(uint4v v)
+{
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) found |= (v[i] & 0x7C00u) == 0x7C00u || (v[i] & 0x7C000000u) == 0x7C000000u;
+    return found;
+}
+
+// tokens of a tile
+template <int D> constexpr int kPromptTile = D == 256 ? 32 : 64;
+
+}  // namespace
+
+template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(const AttnArgs a, uint32_t first_tile)
+{
+    constexpr int KT = kPromptTile<D>, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
+    constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
+    constexpr uint32_t kTile = KT * kRow;
+    constexpr uint32_t kWaveRows = KT / kPromptWaves;       // rows that a wave brings in
+    constexpr uint32_t kWeights = D == 64 ? KT * 32 * 2 * kPromptWaves : 16;   // room for the waves' weights where a tile of keys is too small
+    __shared__ __align__(16) char keys[2][kTile], values[2][kTile];
+    __shared__ __align__(16) char more_weights[kWeights];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
+
+    // the last tiles first: they have the most tokens to look at
+    const uint32_t total = prompt_tiles_of_all(a), local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads, back = first_tile + local;
+    if (back >= total) return;
+    uint32_t tile_in_seq;
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, &tile_in_seq));
+    tile_in_seq = __builtin_amdgcn_readfirstlane(tile_in_seq);
+    const int start = max(a.seqs.starts[seq], 0), tokens = min(a.seqs.starts[seq + 1], (int)a.rows) - start, length = a.seqs.lengths[seq];
+    if (tokens <= 0) return;
+    const int before = (length < 0 ? 0 : length) - (a.seqs.starts[seq + 1] - start);   // position of the sequence's first row here
+    const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
+    const uint32_t row0 = tile_in_seq * kPromptRows, rows = (uint32_t)tokens * a.group;
+
+    auto begin_of = [&](int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; };
+    // this lane's query: a row behind the last one repeats it and is not stored
+    const uint32_t row = row0 + wave * 32u + col, my_row = min(row, rows - 1);
+    const uint32_t my_token = my_row / a.group, my_head = kv_head * a.group + (my_row - my_token * a.group);
+    const int my_position = before + (int)my_token, my_begin = begin_of(my_position), my_end = min(my_position + 1, capacity);
+    // the workgroup's and the wave's first and last ones
+    const int low = before + (int)(row0 / a.group), high = before + (int)(min(row0 + kPromptRows, rows) - 1) / (int)a.group;
+    const uint32_t wave_row = row0 + wave * 32u;
+    const int wave_low = before + (int)(min(wave_row, rows - 1) / a.group), wave_high = before + (int)(min(wave_row + 31u, rows - 1) / a.group);
+    const int first = begin_of(low), last = min(high + 1, capacity);   // tokens that anyone sees: first .. last - 1
+
+    half8 q[D / 16];
+    {
+        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + 8u * half;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
+    }
+    const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+    float reference = -INFINITY, sum = 0.f;
+    float16v o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+
+    auto swizzled = [](uint32_t r, uint32_t unit) { return r * kRow + ((unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4); };
+    const TWM_CONSTANT int *table = (const TWM_CONSTANT int *)(a.seqs.tables + (size_t)seq * a.seqs.table_stride);
+    const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
+    int pages[kGroups];   // of the tile that is brought in next
+    auto find_pages = [&](int t0) {
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) pages[g] = t0 + 16 * g < last ? table[(uint32_t)(t0 + 16 * g) >> a.kv.page_shift] : -1;
+    };
+    // groups of a tile whose pages are inside the pool
+    auto present = [&]() {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) bits |= (uint32_t)pages[g] < a.kv.pages ? 1u << g : 0u;
+        return bits;
+    };
+    // This wave's rows of a tile: kWaveRows (16, or 8) neighbours, which lie in one page.  Those of a page outside the pool are read from its
+    // first one.
+    constexpr int kLoads = E4M3 ? (int)(kWaveRows * D / 1024) : (int)(kWaveRows * D * 2 / 1024);   // 1 KB each
+    constexpr uint32_t kLoadRow = E4M3 ? D : D * 2, kLoadUnits = kLoadRow / 16, kRowsPerLoad = 64 / kLoadUnits;
+    constexpr int kHeld = E4M3 ? (kLoads ? kLoads : 1) : 1;
+    uint4v k_held[kHeld], v_held[kHeld];
+    auto bring = [&](int t0, uint32_t buf) {
+        const uint32_t r0 = wave * kWaveRows;
+        int page = pages[0];
+#pragma unroll
+        for (int g = 1; g < kGroups; g++) page = r0 >= 16u * g ? pages[g] : page;
+        const size_t at = (kv_chunk(a.kv, (uint32_t)page < a.kv.pages ? (uint32_t)page : 0u, kv_head) + ((uint32_t)(t0 + (int)r0) & page_mask) * D) * (E4M3 ? 1 : 2);
+        const char *k_from = (const char *)a.kv.k + at, *v_from = (const char *)a.kv.v + at;
+        if constexpr (E4M3) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                k_held[i] = *(const uint4v *)(k_from + i * 1024 + lane * 16u);
+                v_held[i] = *(const uint4v *)(v_from + i * 1024 + lane * 16u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const uint32_t r = r0 + i * kRowsPerLoad + lane / kUnits;   // the row in the tile, and the unit that this lane's place holds
+                const uint32_t off = i * 1024u + lane / kUnits * kRow + ((lane % kUnits ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4);
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + off), (TWM_LDS(void) *)(keys[buf] + (r0 + i * kRowsPerLoad) * kRow), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + off), (TWM_LDS(void) *)(values[buf] + (r0 + i * kRowsPerLoad) * kRow), 16, 0, 0);
+            }
+        }
+    };
+    // e4m3: what has arrived in registers becomes f16 in LDS
+    auto keep = [&](uint32_t buf) {
+        if constexpr (E4M3) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const uint32_t r = wave * kWaveRows + i * kRowsPerLoad + lane / kLoadUnits, unit = lane % kLoadUnits * 2;
+                *(half8 *)(keys[buf] + swizzled(r, unit)) = to_f16(k_held[i][0], k_held[i][1]);
+                *(half8 *)(keys[buf] + swizzled(r, unit + 1)) = to_f16(k_held[i][2], k_held[i][3]);
+                *(half8 *)(values[buf] + swizzled(r, unit)) = to_f16(v_held[i][0], v_held[i][1]);
+                *(half8 *)(values[buf] + swizzled(r, unit + 1)) = to_f16(v_held[i][2], v_held[i][3]);
+            }
+        }
+    };
+
+    const int t_begin = first & ~(KT - 1);
+    uint32_t there = 0, there_next = 0, buf = 0;
+    if (t_begin < last) {
+        find_pages(t_begin);
+        there = present();
+        bring(t_begin, 0);
+        keep(0);
+        find_pages(t_begin + KT);
+        there_next = present();
+    }
+    __syncthreads();
+    for (int t0 = t_begin; t0 < last; t0 += KT) {
+        if (t0 + KT < last) bring(t0 + KT, buf ^ 1u);
+        const uint32_t there_now = there;
+        there = there_next;
+        find_pages(t0 + 2 * KT);
+        there_next = present();
+        // whether some token of the tile is not for every row
+        const bool edge = t0 + KT > low + 1 || t0 + KT > last || t0 < begin_of(high) || there_now != (1u << kGroups) - 1u;
+        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
+        const char *const k_tile = keys[buf], *const v_tile = values[buf];
+
+        half8 p[KT / 16];
+        if (!idle) {
+            float16v s[KT / 32];
+#pragma unroll
+            for (int b = 0; b < KT / 32; b++) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[b][j] = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 16; i++)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(k_tile + swizzled(32u * b + col, 2u * i + half)), q[i], s[b], 0, 0, 0);
+            }
+            // element j of block b: token t0 + 32 b + 8 (j / 4) + 4 half + j % 4
+            if (edge) {
+#pragma unroll
+                for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int token = t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4;
+                        const bool seen = token >= my_begin && token < my_end && (there_now >> (2 * b + j / 8) & 1u);
+                        s[b][j] = seen ? s[b][j] : -INFINITY;
+                    }
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) most = fmaxf(most, s[b][j]);
+            most = max_of_halves(most) * c;
+            if (__any(most > reference + 15.0f)) {
+                const float next = fmaxf(reference, most - 8.0f);
+                const float by = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - next);
+                sum *= by;
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) o[i] *= by;
+                reference = next;
+            }
+            const float base = reference == -INFINITY ? 0.f : -reference;
+#pragma unroll
+            for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s[b][j], c, base));
+                    sum += w;
+                    p[2 * b + j / 8][j % 8] = (_Float16)w;
+                }
+        }
+        bool single = false;   // the tile's products token by token
+        if (edge) {
+            // values: rows that nobody sees become zeros, the others are looked through
+            constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
+            const uint32_t r = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
+            const int token = t0 + (int)r;
+            const bool dead = token < first || token >= last || !(there_now >> (r / 16) & 1u);
+            bool bad = false;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) {
+                uint4v *at = (uint4v *)(values[buf] + swizzled(r, unit + i));
+                if (dead)
+                    *at = uint4v{0u, 0u, 0u, 0u};
+                else
+                    bad |= not_finite(*at);
+            }
+            single = __syncthreads_or(bad);
+        }
+        if (!idle && !single) {
+#pragma unroll
+            for (int i = 0; i < D / 32; i++)
+#pragma unroll
+                for (int b = 0; b < KT / 16; b++) {
+                    // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
+                    const uint32_t r = 16u * b + 4u * half + (lane >> 2 & 3u), unit = 4u * i + (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u), piece = (lane & 1u) * 8u;
+                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(v_tile + swizzled(r, unit) + piece)));
+                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(v_tile + swizzled(r + 8u, unit) + piece)));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[b], o[i], 0, 0, 0);
+                }
+        } else if (!idle) {
+            // the wave's weights to LDS (every wave is done with the tile's keys), then one token after the other
+            _Float16 *weights = (_Float16 *)(D == 64 ? more_weights : keys[buf]) + wave * (KT * 32);
+#pragma unroll
+            for (int b = 0; b < KT / 16; b++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) weights[(16 * b + 8 * (j / 4) + 4 * (int)half + j % 4) * 32 + (int)col] = p[b][j];
+            for (int r = 0; r < KT; r++) {
+                const int token = t0 + r;
+                if (token < first || token >= last || !(there_now >> (r / 16) & 1u)) continue;
+                const bool seen = token >= my_begin && token < my_end;
+                const float w = (float)weights[r * 32 + (int)col];
+#pragma unroll
+                for (int i = 0; i < D / 32; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const half4 x = *(const half4 *)(v_tile + swizzled((uint32_t)r, 4u * i + j) + 8u * half);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
+                    }
+            }
+        }
+        if (t0 + KT < last) keep(buf ^ 1u);
+        buf ^= 1u;
+        __syncthreads();   // (what this wave brought in has arrived too: the compiler waits for all of its loads ahead of a barrier)
+    }
+
+    sum = sum_of_halves(sum);
+    if (row < rows) {
+        const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
+        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + 4u * half;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *(half4_any *)(out + 32 * i + 8 * j) = half4{(_Float16)(o[i][4 * j] * to), (_Float16)(o[i][4 * j + 1] * to), (_Float16)(o[i][4 * j + 2] * to),
+                                                             (_Float16)(o[i][4 * j + 3] * to)};
+    }
 }
 
 hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a)
 {
-    hipLaunchKernelGGL(a.kv.e4m3 ? k_attn_prompt<true> : k_attn_prompt<false>, dim3(a.rows, a.q_heads), dim3(64), 0, s, a);
-    return hipGetLastError();
+    // every sequence begins a tile of its own
+    const uint64_t tiles = (uint64_t)a.rows * a.group / kPromptRows + std::min(a.seqs.seqs, a.rows);
+    auto launch = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        return in_slices((uint32_t)tiles, most_workgroups(256) / a.kv.kv_heads, [&](uint32_t tile, uint32_t here) {
+            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads), dim3(256), 0, s, a, tile);
+            return hipGetLastError();
+        });
+    };
+    return a.kv.dim == 64    ? launch(std::integral_constant<int, 64>{})
+           : a.kv.dim == 128 ? launch(std::integral_constant<int, 128>{})
+                             : launch(std::integral_constant<int, 256>{});
 }
 
 }  // namespace twm
