@@ -117,11 +117,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 {
     constexpr int KT = kPromptTile<D>, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
     constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
-    constexpr uint32_t kTile = KT * kRow;
-    constexpr uint32_t kWaveRows = KT / kPromptWaves;       // rows that a wave brings in
-    constexpr uint32_t kWeights = D == 64 ? KT * 32 * 2 * kPromptWaves : 16;   // room for the waves' weights where a tile of keys is too small
-    __shared__ __align__(16) char keys[2][kTile], values[2][kTile];
-    __shared__ __align__(16) char more_weights[kWeights];
+    constexpr uint32_t kTile = KT * kRow, kWaveRows = KT / kPromptWaves;   // bytes of a tile's keys; rows that a wave brings in
+    // two buffers of keys, then two of values (and room for the waves' weights where a tile of keys is too small for them)
+    extern __shared__ __align__(16) char lds[];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
 
     // the last tiles first: they have the most tokens to look at
@@ -164,44 +162,41 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
     auto swizzled = [](uint32_t r, uint32_t unit) { return r * kRow + ((unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4); };
     const TWM_CONSTANT int *table = (const TWM_CONSTANT int *)(a.seqs.tables + (size_t)seq * a.seqs.table_stride);
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
-    int pages[kGroups];   // of the tile that is brought in next
+    // A tile's pages: this wave's rows are kWaveRows (16, or 8) neighbours, which lie in one; bit g: the page of tokens 16 g .. is in the pool
+    struct Pages {
+        int mine;
+        uint32_t there;
+    };
     auto find_pages = [&](int t0) {
+        Pages p{-1, 0};
 #pragma unroll
-        for (int g = 0; g < kGroups; g++) pages[g] = t0 + 16 * g < last ? table[(uint32_t)(t0 + 16 * g) >> a.kv.page_shift] : -1;
+        for (int g = 0; g < kGroups; g++) {
+            const int page = t0 + 16 * g < last ? table[(uint32_t)(t0 + 16 * g) >> a.kv.page_shift] : -1;
+            p.there |= (uint32_t)page < a.kv.pages ? 1u << g : 0u;
+            p.mine = wave * kWaveRows / 16u == (uint32_t)g ? page : p.mine;
+        }
+        return p;
     };
-    // groups of a tile whose pages are inside the pool
-    auto present = [&]() {
-        uint32_t bits = 0;
-#pragma unroll
-        for (int g = 0; g < kGroups; g++) bits |= (uint32_t)pages[g] < a.kv.pages ? 1u << g : 0u;
-        return bits;
-    };
-    // This wave's rows of a tile: kWaveRows (16, or 8) neighbours, which lie in one page.  Those of a page outside the pool are read from its
-    // first one.
-    constexpr int kLoads = E4M3 ? (int)(kWaveRows * D / 1024) : (int)(kWaveRows * D * 2 / 1024);   // 1 KB each
-    constexpr uint32_t kLoadRow = E4M3 ? D : D * 2, kLoadUnits = kLoadRow / 16, kRowsPerLoad = 64 / kLoadUnits;
-    constexpr int kHeld = E4M3 ? (kLoads ? kLoads : 1) : 1;
-    uint4v k_held[kHeld], v_held[kHeld];
-    auto bring = [&](int t0, uint32_t buf) {
+    constexpr int kLoads = (int)(kWaveRows * D * (E4M3 ? 1 : 2) / 1024);   // 1 KB each
+    constexpr uint32_t kLoadUnits = D * (E4M3 ? 1 : 2) / 16, kRowsPerLoad = 64 / kLoadUnits;
+    uint4v k_held[kLoads], v_held[kLoads];   // e4m3 only
+    auto bring = [&](int t0, const Pages &pages, uint32_t buf) {
         const uint32_t r0 = wave * kWaveRows;
-        int page = pages[0];
-#pragma unroll
-        for (int g = 1; g < kGroups; g++) page = r0 >= 16u * g ? pages[g] : page;
-        const size_t at = (kv_chunk(a.kv, (uint32_t)page < a.kv.pages ? (uint32_t)page : 0u, kv_head) + ((uint32_t)(t0 + (int)r0) & page_mask) * D) * (E4M3 ? 1 : 2);
+        // rows of a page outside the pool are read from its first one
+        const uint32_t page = (uint32_t)pages.mine < a.kv.pages ? (uint32_t)pages.mine : 0u;
+        const size_t at = (kv_chunk(a.kv, page, kv_head) + ((uint32_t)(t0 + (int)r0) & page_mask) * D) * (E4M3 ? 1 : 2);
         const char *k_from = (const char *)a.kv.k + at, *v_from = (const char *)a.kv.v + at;
-        if constexpr (E4M3) {
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) {
+        for (int i = 0; i < kLoads; i++) {
+            if constexpr (E4M3) {
                 k_held[i] = *(const uint4v *)(k_from + i * 1024 + lane * 16u);
                 v_held[i] = *(const uint4v *)(v_from + i * 1024 + lane * 16u);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; i++) {
+            } else {
                 const uint32_t r = r0 + i * kRowsPerLoad + lane / kUnits;   // the row in the tile, and the unit that this lane's place holds
                 const uint32_t off = i * 1024u + lane / kUnits * kRow + ((lane % kUnits ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4);
-                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + off), (TWM_LDS(void) *)(keys[buf] + (r0 + i * kRowsPerLoad) * kRow), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + off), (TWM_LDS(void) *)(values[buf] + (r0 + i * kRowsPerLoad) * kRow), 16, 0, 0);
+                char *to = lds + buf * kTile + (r0 + i * kRowsPerLoad) * kRow;
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + off), (TWM_LDS(void) *)to, 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + off), (TWM_LDS(void) *)(to + 2 * kTile), 16, 0, 0);
             }
         }
     };
@@ -211,80 +206,91 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
                 const uint32_t r = wave * kWaveRows + i * kRowsPerLoad + lane / kLoadUnits, unit = lane % kLoadUnits * 2;
-                *(half8 *)(keys[buf] + swizzled(r, unit)) = to_f16(k_held[i][0], k_held[i][1]);
-                *(half8 *)(keys[buf] + swizzled(r, unit + 1)) = to_f16(k_held[i][2], k_held[i][3]);
-                *(half8 *)(values[buf] + swizzled(r, unit)) = to_f16(v_held[i][0], v_held[i][1]);
-                *(half8 *)(values[buf] + swizzled(r, unit + 1)) = to_f16(v_held[i][2], v_held[i][3]);
+                char *to = lds + buf * kTile;
+                *(half8 *)(to + swizzled(r, unit)) = to_f16(k_held[i][0], k_held[i][1]);
+                *(half8 *)(to + swizzled(r, unit + 1)) = to_f16(k_held[i][2], k_held[i][3]);
+                *(half8 *)(to + 2 * kTile + swizzled(r, unit)) = to_f16(v_held[i][0], v_held[i][1]);
+                *(half8 *)(to + 2 * kTile + swizzled(r, unit + 1)) = to_f16(v_held[i][2], v_held[i][3]);
             }
         }
     };
+    // everything that this wave has brought in and kept has arrived, and that of the other waves
+    auto arrived = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+        __syncthreads();
+    };
 
-    const int t_begin = first & ~(KT - 1);
-    uint32_t there = 0, there_next = 0, buf = 0;
+    const int t_begin = first & ~(KT - 1), high_begin = begin_of(high);
+    uint32_t there = 0, buf = 0;
+    Pages next{-1, 0};
     if (t_begin < last) {
-        find_pages(t_begin);
-        there = present();
-        bring(t_begin, 0);
+        const Pages pages = find_pages(t_begin);
+        there = pages.there;
+        bring(t_begin, pages, 0);
         keep(0);
-        find_pages(t_begin + KT);
-        there_next = present();
+        next = find_pages(t_begin + KT);
     }
-    __syncthreads();
+    // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
+    const uint32_t k_at = swizzled(col, half), v_row = 4u * half + (lane >> 2 & 3u), v_unit = (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u);
+    const uint32_t v_at = 2 * kTile + swizzled(v_row, v_unit) + (lane & 1u) * 8u, v_at_8 = 2 * kTile + swizzled(v_row + 8u, v_unit) + (lane & 1u) * 8u;
+    arrived();
     for (int t0 = t_begin; t0 < last; t0 += KT) {
-        if (t0 + KT < last) bring(t0 + KT, buf ^ 1u);
+        if (t0 + KT < last) bring(t0 + KT, next, buf ^ 1u);
         const uint32_t there_now = there;
-        there = there_next;
-        find_pages(t0 + 2 * KT);
-        there_next = present();
-        // whether some token of the tile is not for every row
-        const bool edge = t0 + KT > low + 1 || t0 + KT > last || t0 < begin_of(high) || there_now != (1u << kGroups) - 1u;
-        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
-        const char *const k_tile = keys[buf], *const v_tile = values[buf];
-
+        there = next.there;
+        next = find_pages(t0 + 2 * KT);
+        // whether the tile holds tokens that some of the workgroup's rows do not see
+        const bool edge = t0 + KT > min(low + 1, last) || t0 < high_begin || there_now != (1u << kGroups) - 1u;
+        const bool idle = edge && (t0 > wave_high || t0 + KT <= begin_of(wave_low));   // nothing for this wave
+        const char *const tile = lds + buf * kTile;
         half8 p[KT / 16];
         if (!idle) {
             float16v s[KT / 32];
 #pragma unroll
-            for (int b = 0; b < KT / 32; b++) {
+            for (int b = 0; b < KT / 32; b++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) s[b][j] = 0.f;
 #pragma unroll
-                for (int i = 0; i < D / 16; i++)
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(k_tile + swizzled(32u * b + col, 2u * i + half)), q[i], s[b], 0, 0, 0);
-            }
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int b = 0; b < KT / 32; b++)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
             // element j of block b: token t0 + 32 b + 8 (j / 4) + 4 half + j % 4
             if (edge) {
 #pragma unroll
-                for (int b = 0; b < KT / 32; b++)
+                for (int b = 0; b < KT / 32; b++) {
+                    asm volatile("" : "+v"(s[b]));   // (a branch, not a selection in every tile)
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         const int token = t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4;
                         const bool seen = token >= my_begin && token < my_end && (there_now >> (2 * b + j / 8) & 1u);
                         s[b][j] = seen ? s[b][j] : -INFINITY;
                     }
+                }
             }
-            float most = -INFINITY;
+            float most = s[0][0];
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) most = fmaxf(most, s[b][j]);
             most = max_of_halves(most) * c;
             if (__any(most > reference + 15.0f)) {
-                const float next = fmaxf(reference, most - 8.0f);
-                const float by = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - next);
+                const float raised = fmaxf(reference, most - 8.0f);
+                const float by = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - raised);
                 sum *= by;
 #pragma unroll
                 for (int i = 0; i < D / 32; i++) o[i] *= by;
-                reference = next;
+                reference = raised;
             }
             const float base = reference == -INFINITY ? 0.f : -reference;
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(s[b][j], c, base));
-                    sum += w;
-                    p[2 * b + j / 8][j % 8] = (_Float16)w;
+                for (int j = 0; j < 16; j += 2) {
+                    const half2v w = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j], c, base)), (_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j + 1], c, base))};
+                    sum = __builtin_amdgcn_fdot2(w, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                    p[2 * b + j / 8][j % 8] = w[0];
+                    p[2 * b + j / 8][j % 8 + 1] = w[1];
                 }
         }
         bool single = false;   // the tile's products token by token
@@ -297,7 +303,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
             bool bad = false;
 #pragma unroll
             for (uint32_t i = 0; i < kEach; i++) {
-                uint4v *at = (uint4v *)(values[buf] + swizzled(r, unit + i));
+                uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + swizzled(r, unit + i));
                 if (dead)
                     *at = uint4v{0u, 0u, 0u, 0u};
                 else
@@ -307,18 +313,17 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         }
         if (!idle && !single) {
 #pragma unroll
-            for (int i = 0; i < D / 32; i++)
+            for (int b = 0; b < KT / 16; b++)
 #pragma unroll
-                for (int b = 0; b < KT / 16; b++) {
+                for (int i = 0; i < D / 32; i++) {
                     // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
-                    const uint32_t r = 16u * b + 4u * half + (lane >> 2 & 3u), unit = 4u * i + (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u), piece = (lane & 1u) * 8u;
-                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(v_tile + swizzled(r, unit) + piece)));
-                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(v_tile + swizzled(r + 8u, unit) + piece)));
+                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + b * 16 * kRow)));
+                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at_8 ^ i << 6) + b * 16 * kRow)));
                     o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[b], o[i], 0, 0, 0);
                 }
         } else if (!idle) {
             // the wave's weights to LDS (every wave is done with the tile's keys), then one token after the other
-            _Float16 *weights = (_Float16 *)(D == 64 ? more_weights : keys[buf]) + wave * (KT * 32);
+            _Float16 *weights = (_Float16 *)(lds + (D == 64 ? 4 * kTile : buf * kTile)) + wave * (KT * 32);
 #pragma unroll
             for (int b = 0; b < KT / 16; b++)
 #pragma unroll
@@ -332,7 +337,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
                 for (int i = 0; i < D / 32; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(v_tile + swizzled((uint32_t)r, 4u * i + j) + 8u * half);
+                        const half4 x = *(const half4 *)(tile + 2 * kTile + swizzled((uint32_t)r, 4u * i + j) + 8u * half);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
                     }
@@ -340,7 +345,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         }
         if (t0 + KT < last) keep(buf ^ 1u);
         buf ^= 1u;
-        __syncthreads();   // (what this wave brought in has arrived too: the compiler waits for all of its loads ahead of a barrier)
+        arrived();
     }
 
     sum = sum_of_halves(sum);
@@ -356,6 +361,24 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
     }
 }
 
+// LDS of a workgroup
+template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile<D> * D * 2 + (D == 64 ? kPromptTile<D> * 2 * kPromptRows : 0);
+
+hipError_t init_attn_prompt()
+{
+    hipError_t e = hipSuccess;
+    auto ask = [&](auto kernel, uint32_t bytes) {
+        if (e == hipSuccess) e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    };
+    ask(k_attn_prompt<64, false>, kPromptLds<64>);
+    ask(k_attn_prompt<64, true>, kPromptLds<64>);
+    ask(k_attn_prompt<128, false>, kPromptLds<128>);
+    ask(k_attn_prompt<128, true>, kPromptLds<128>);
+    ask(k_attn_prompt<256, false>, kPromptLds<256>);
+    ask(k_attn_prompt<256, true>, kPromptLds<256>);
+    return e;
+}
+
 hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a)
 {
     // every sequence begins a tile of its own
@@ -363,7 +386,7 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a)
     auto launch = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         return in_slices((uint32_t)tiles, most_workgroups(256) / a.kv.kv_heads, [&](uint32_t tile, uint32_t here) {
-            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads), dim3(256), 0, s, a, tile);
+            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads), dim3(256), kPromptLds<D>, s, a, tile);
             return hipGetLastError();
         });
     };

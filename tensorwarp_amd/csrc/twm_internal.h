@@ -266,5 +266,6 @@ struct AttnArgs {
 };
 hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes);
 hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a);
+hipError_t init_attn_prompt();
 
 }  // namespace twm
