@@ -159,23 +159,29 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
-    auto swizzled = [](uint32_t r, uint32_t unit) { return r * kRow + ((unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4); };
-    const TWM_CONSTANT int *table = (const TWM_CONSTANT int *)(a.seqs.tables + (size_t)seq * a.seqs.table_stride);
+    // The place of a unit in its row of keys (of which 16 rows are read at once) and of values (four rows, four units of each)
+    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
+    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); };
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
-    // A tile's pages: this wave's rows are kWaveRows (16, or 8) neighbours, which lie in one; bit g: the page of tokens 16 g .. is in the pool
+    // A tile's pages: this wave's rows are kWaveRows (16, or 8) neighbours, which lie in one; bit g: the page of tokens 16 g .. is in the pool.
+    // A lane looks the pages of sixteen tokens up, the wave those of 1024 at once.
     struct Pages {
         int mine;
         uint32_t there;
     };
+    const int t_begin = first & ~(KT - 1);
+    int looked_up = t_begin, page_of = -1;
+    uint64_t page_there = 0;
+    auto look_up = [&](int t0) {
+        looked_up = t0;
+        const int token = t0 + 16 * (int)lane;
+        page_of = token < last ? a.seqs.tables[(size_t)seq * a.seqs.table_stride + ((uint32_t)token >> a.kv.page_shift)] : -1;
+        page_there = __ballot((uint32_t)page_of < a.kv.pages);
+    };
     auto find_pages = [&](int t0) {
-        Pages p{-1, 0};
-#pragma unroll
-        for (int g = 0; g < kGroups; g++) {
-            const int page = t0 + 16 * g < last ? table[(uint32_t)(t0 + 16 * g) >> a.kv.page_shift] : -1;
-            p.there |= (uint32_t)page < a.kv.pages ? 1u << g : 0u;
-            p.mine = wave * kWaveRows / 16u == (uint32_t)g ? page : p.mine;
-        }
-        return p;
+        if (t0 - looked_up >= 1024) look_up(t0);
+        const uint32_t group = (uint32_t)(t0 - looked_up) >> 4;
+        return Pages{__builtin_amdgcn_readlane(page_of, group + wave * kWaveRows / 16u), (uint32_t)(page_there >> group) & ((1u << kGroups) - 1u)};
     };
     constexpr int kLoads = (int)(kWaveRows * D * (E4M3 ? 1 : 2) / 1024);   // 1 KB each
     constexpr uint32_t kLoadUnits = D * (E4M3 ? 1 : 2) / 16, kRowsPerLoad = 64 / kLoadUnits;
@@ -193,10 +199,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
                 v_held[i] = *(const uint4v *)(v_from + i * 1024 + lane * 16u);
             } else {
                 const uint32_t r = r0 + i * kRowsPerLoad + lane / kUnits;   // the row in the tile, and the unit that this lane's place holds
-                const uint32_t off = i * 1024u + lane / kUnits * kRow + ((lane % kUnits ^ (D == 64 ? (r >> 1) & 7u : r & 15u)) << 4);
+                const uint32_t row_off = i * 1024u + lane / kUnits * kRow, k_off = row_off + (key_place(r, lane % kUnits) << 4),
+                               v_off = row_off + (value_place(r, lane % kUnits) << 4);
                 char *to = lds + buf * kTile + (r0 + i * kRowsPerLoad) * kRow;
-                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + off), (TWM_LDS(void) *)to, 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + off), (TWM_LDS(void) *)(to + 2 * kTile), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + k_off), (TWM_LDS(void) *)to, 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + v_off), (TWM_LDS(void) *)(to + 2 * kTile), 16, 0, 0);
             }
         }
     };
@@ -206,11 +213,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
                 const uint32_t r = wave * kWaveRows + i * kRowsPerLoad + lane / kLoadUnits, unit = lane % kLoadUnits * 2;
-                char *to = lds + buf * kTile;
-                *(half8 *)(to + swizzled(r, unit)) = to_f16(k_held[i][0], k_held[i][1]);
-                *(half8 *)(to + swizzled(r, unit + 1)) = to_f16(k_held[i][2], k_held[i][3]);
-                *(half8 *)(to + 2 * kTile + swizzled(r, unit)) = to_f16(v_held[i][0], v_held[i][1]);
-                *(half8 *)(to + 2 * kTile + swizzled(r, unit + 1)) = to_f16(v_held[i][2], v_held[i][3]);
+                char *to = lds + buf * kTile + r * kRow;
+                *(half8 *)(to + (key_place(r, unit) << 4)) = to_f16(k_held[i][0], k_held[i][1]);
+                *(half8 *)(to + (key_place(r, unit + 1) << 4)) = to_f16(k_held[i][2], k_held[i][3]);
+                *(half8 *)(to + 2 * kTile + (value_place(r, unit) << 4)) = to_f16(v_held[i][0], v_held[i][1]);
+                *(half8 *)(to + 2 * kTile + (value_place(r, unit + 1) << 4)) = to_f16(v_held[i][2], v_held[i][3]);
             }
         }
     };
@@ -220,10 +227,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         __syncthreads();
     };
 
-    const int t_begin = first & ~(KT - 1), high_begin = begin_of(high);
+    const int high_begin = begin_of(high);
     uint32_t there = 0, buf = 0;
     Pages next{-1, 0};
     if (t_begin < last) {
+        look_up(t_begin);
         const Pages pages = find_pages(t_begin);
         there = pages.there;
         bring(t_begin, pages, 0);
@@ -231,96 +239,145 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         next = find_pages(t_begin + KT);
     }
     // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
-    const uint32_t k_at = swizzled(col, half), v_row = 4u * half + (lane >> 2 & 3u), v_unit = (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u);
-    const uint32_t v_at = 2 * kTile + swizzled(v_row, v_unit) + (lane & 1u) * 8u, v_at_8 = 2 * kTile + swizzled(v_row + 8u, v_unit) + (lane & 1u) * 8u;
+    const uint32_t k_at = col * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
+    // S^T of the tile in buffer `tile`; element j of block b: token 32 b + 8 (j / 4) + 4 half + j % 4
+    auto scores = [&](const char *tile, float16v (&s)[KT / 32]) {
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[b][j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int b = 0; b < KT / 32; b++)
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
+    };
+    // the largest score, as an exponent; it sets the reference where there is none yet, and nothing is summed
+    auto largest = [&](const float16v (&s)[KT / 32]) {
+        float most = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) most = fmaxf(most, s[b][j]);
+        most = max_of_halves(most) * c;
+        reference = reference == -INFINITY ? most - 8.0f : reference;
+        return most;
+    };
+    // a weight would pass 2^15: the reference moves, and what is summed with it
+    auto raise = [&](float most) {
+        const float raised = fmaxf(reference, most - 8.0f), by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(reference - raised);
+        sum *= by;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) o[i] *= by;
+        reference = raised;
+    };
+    auto weigh = [&](const float16v (&s)[KT / 32], half8 (&p)[KT / 16]) {
+        const float base = reference == -INFINITY ? 0.f : -reference;
+#pragma unroll
+        for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const half2v w = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j], c, base)), (_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j + 1], c, base))};
+                sum = __builtin_amdgcn_fdot2(w, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                p[2 * b + j / 8][j % 8] = w[0];
+                p[2 * b + j / 8][j % 8 + 1] = w[1];
+            }
+    };
+    auto add_values = [&](const char *tile, const half8 (&p)[KT / 16]) {
+#pragma unroll
+        for (int b = 0; b < KT / 16; b++)
+#pragma unroll
+            for (int i = 0; i < D / 32; i++) {
+                // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
+                const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + b * 16 * kRow)));
+                const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[b], o[i], 0, 0, 0);
+            }
+    };
+    // the last tile that everyone sees whole ends here
+    const int whole_end = min(low + 1, last);
     arrived();
-    for (int t0 = t_begin; t0 < last; t0 += KT) {
+    int t0 = t_begin;
+    bool advanced = false;
+    uint32_t there_now = 0;
+    auto advance = [&]() {   // once a tile: the one behind it begins its way, and the pages of the one after that are known
+        if (advanced) return;
         if (t0 + KT < last) bring(t0 + KT, next, buf ^ 1u);
-        const uint32_t there_now = there;
         there = next.there;
         next = find_pages(t0 + 2 * KT);
-        // whether the tile holds tokens that some of the workgroup's rows do not see
-        const bool edge = t0 + KT > min(low + 1, last) || t0 < high_begin || there_now != (1u << kGroups) - 1u;
-        const bool idle = edge && (t0 > wave_high || t0 + KT <= begin_of(wave_low));   // nothing for this wave
+        advanced = true;
+    };
+    auto turn = [&]() {
+        if (t0 + KT < last) keep(buf ^ 1u);
+        buf ^= 1u;
+        t0 += KT;
+        there_now = there;
+        advanced = false;
+        arrived();
+    };
+    there_now = there;
+    while (t0 < last) {
+        // tiles that every row of the workgroup sees whole
+        float raise_to = -INFINITY;
+        while (t0 >= high_begin && t0 + KT <= whole_end && there_now == (1u << kGroups) - 1u) {
+            const char *const tile = lds + buf * kTile;
+            advance();
+            float16v s[KT / 32];
+            half8 p[KT / 16];
+            scores(tile, s);
+            const float most = largest(s);
+            if (__any(most > reference + 15.0f)) {   // (rare; outside of this loop, so that the sums never move within it)
+                raise_to = most;
+                break;
+            }
+            weigh(s, p);
+            add_values(tile, p);
+            turn();
+        }
+        if (__any(raise_to > -INFINITY)) {
+            raise(raise_to);
+            continue;
+        }
+        if (t0 >= last) break;
+        // one that some do not, or that lacks pages
         const char *const tile = lds + buf * kTile;
+        const uint32_t present = there_now;
+        advance();
+        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
         half8 p[KT / 16];
         if (!idle) {
             float16v s[KT / 32];
+            scores(tile, s);
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) s[b][j] = 0.f;
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int b = 0; b < KT / 32; b++)
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
-            // element j of block b: token t0 + 32 b + 8 (j / 4) + 4 half + j % 4
-            if (edge) {
-#pragma unroll
-                for (int b = 0; b < KT / 32; b++) {
-                    asm volatile("" : "+v"(s[b]));   // (a branch, not a selection in every tile)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int token = t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4;
-                        const bool seen = token >= my_begin && token < my_end && (there_now >> (2 * b + j / 8) & 1u);
-                        s[b][j] = seen ? s[b][j] : -INFINITY;
-                    }
+                for (int j = 0; j < 16; j++) {
+                    const int token = t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4;
+                    const bool seen = token >= my_begin && token < my_end && (present >> (2 * b + j / 8) & 1u);
+                    s[b][j] = seen ? s[b][j] : -INFINITY;
                 }
-            }
-            float most = s[0][0];
-#pragma unroll
-            for (int b = 0; b < KT / 32; b++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) most = fmaxf(most, s[b][j]);
-            most = max_of_halves(most) * c;
-            if (__any(most > reference + 15.0f)) {
-                const float raised = fmaxf(reference, most - 8.0f);
-                const float by = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - raised);
-                sum *= by;
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) o[i] *= by;
-                reference = raised;
-            }
-            const float base = reference == -INFINITY ? 0.f : -reference;
-#pragma unroll
-            for (int b = 0; b < KT / 32; b++)
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const half2v w = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j], c, base)), (_Float16)__builtin_amdgcn_exp2f(fmaf(s[b][j + 1], c, base))};
-                    sum = __builtin_amdgcn_fdot2(w, half2v{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
-                    p[2 * b + j / 8][j % 8] = w[0];
-                    p[2 * b + j / 8][j % 8 + 1] = w[1];
-                }
+            const float most = largest(s);
+            if (__any(most > reference + 15.0f)) raise(most);
+            weigh(s, p);
         }
-        bool single = false;   // the tile's products token by token
-        if (edge) {
-            // values: rows that nobody sees become zeros, the others are looked through
-            constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
-            const uint32_t r = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
-            const int token = t0 + (int)r;
-            const bool dead = token < first || token >= last || !(there_now >> (r / 16) & 1u);
-            bool bad = false;
+        // values: rows that nobody sees become zeros, the others are looked through
+        constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
+        const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
+        const int token = t0 + (int)looked;
+        const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
+        bool bad = false;
 #pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) {
-                uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + swizzled(r, unit + i));
-                if (dead)
-                    *at = uint4v{0u, 0u, 0u, 0u};
-                else
-                    bad |= not_finite(*at);
-            }
-            single = __syncthreads_or(bad);
+        for (uint32_t i = 0; i < kEach; i++) {
+            uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
+            if (dead)
+                *at = uint4v{0u, 0u, 0u, 0u};
+            else
+                bad |= not_finite(*at);
         }
+        const bool single = __syncthreads_or(bad);
         if (!idle && !single) {
-#pragma unroll
-            for (int b = 0; b < KT / 16; b++)
-#pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
-                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + b * 16 * kRow)));
-                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at_8 ^ i << 6) + b * 16 * kRow)));
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[b], o[i], 0, 0, 0);
-                }
+            add_values(tile, p);
         } else if (!idle) {
             // the wave's weights to LDS (every wave is done with the tile's keys), then one token after the other
             _Float16 *weights = (_Float16 *)(lds + (D == 64 ? 4 * kTile : buf * kTile)) + wave * (KT * 32);
@@ -329,23 +386,21 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 #pragma unroll
                 for (int j = 0; j < 8; j++) weights[(16 * b + 8 * (j / 4) + 4 * (int)half + j % 4) * 32 + (int)col] = p[b][j];
             for (int r = 0; r < KT; r++) {
-                const int token = t0 + r;
-                if (token < first || token >= last || !(there_now >> (r / 16) & 1u)) continue;
-                const bool seen = token >= my_begin && token < my_end;
+                const int at = t0 + r;
+                if (at < first || at >= last || !(present >> (r / 16) & 1u)) continue;
+                const bool seen = at >= my_begin && at < my_end;
                 const float w = (float)weights[r * 32 + (int)col];
 #pragma unroll
                 for (int i = 0; i < D / 32; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(tile + 2 * kTile + swizzled((uint32_t)r, 4u * i + j) + 8u * half);
+                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
                     }
             }
         }
-        if (t0 + KT < last) keep(buf ^ 1u);
-        buf ^= 1u;
-        arrived();
+        turn();
     }
 
     sum = sum_of_halves(sum);
