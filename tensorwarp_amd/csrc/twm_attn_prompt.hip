@@ -33,13 +33,16 @@ typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 #define TWM_LDS(T) __attribute__((address_space(3))) T
 
-constexpr uint32_t kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
+constexpr uint32_t kPromptWaves = 4;
+// Waves that share 32 queries: of 256 values each holds half, which is what registers hold (the whole of it in one wave: 2.2 times slower)
+template <int D> constexpr uint32_t kPromptShared = D == 256 ? 2 : 1;
+template <int D> constexpr uint32_t kPromptRows = 32 * kPromptWaves / kPromptShared<D>;
 
-// Workgroups of one key-value head: 128 rows each, token by token
-__device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, uint32_t seq)
+// Workgroups of one key-value head: `each` rows per one, token by token
+__device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, uint32_t seq, uint32_t each)
 {
     const int first = max(a.seqs.starts[seq], 0), end = min(a.seqs.starts[seq + 1], (int)a.rows);
-    return end > first ? ((uint32_t)(end - first) * a.group + kPromptRows - 1) / kPromptRows : 0u;
+    return end > first ? ((uint32_t)(end - first) * a.group + each - 1) / each : 0u;
 }
 
 __device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)   // of this lane and those before it
@@ -53,22 +56,22 @@ __device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)   // of this lane
     return v;
 }
 
-__device__ __forceinline__ uint32_t prompt_tiles_of_all(const AttnArgs &a)
+__device__ __forceinline__ uint32_t prompt_tiles_of_all(const AttnArgs &a, uint32_t each)
 {
     uint32_t sum = 0;
-    for (uint32_t s = threadIdx.x & 63u; s < a.seqs.seqs; s += 64) sum += prompt_tiles(a, s);
+    for (uint32_t s = threadIdx.x & 63u; s < a.seqs.seqs; s += 64) sum += prompt_tiles(a, s, each);
 #pragma unroll
     for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
     return sum;
 }
 
 // the sequence of tile `at` of a key-value head, and its place among the sequence's
-__device__ __forceinline__ uint32_t prompt_sequence_of(const AttnArgs &a, uint32_t at, uint32_t *inside)
+__device__ __forceinline__ uint32_t prompt_sequence_of(const AttnArgs &a, uint32_t at, uint32_t each, uint32_t *inside)
 {
     uint32_t sum = 0;
     for (uint32_t base = 0; base < a.seqs.seqs; base += 64) {
         const uint32_t s = base + (threadIdx.x & 63u);
-        const uint32_t up_to = wave_sum_up_to(s < a.seqs.seqs ? prompt_tiles(a, s) : 0u);
+        const uint32_t up_to = wave_sum_up_to(s < a.seqs.seqs ? prompt_tiles(a, s, each) : 0u);
         const uint64_t past = __ballot(sum + up_to > at);
         if (past) {
             const uint32_t lane = (uint32_t)__builtin_ctzll(past);
@@ -110,52 +113,56 @@ __device__ __forceinline__ bool not_finite(uint4v v)
 
 // tokens of a tile
 template <int D> constexpr int kPromptTile = D == 256 ? 32 : 64;
+// LDS of a workgroup
+template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile<D> * D * 2 + (D == 256 ? kPromptWaves * 32 * 32 * 4 : D == 64 ? kPromptWaves * 64 * 32 * 2 + 16 : 16);
 
 }  // namespace
 
-template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(const AttnArgs a, uint32_t first_tile)
+template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt(const AttnArgs a, uint32_t first_tile)
 {
     constexpr int KT = kPromptTile<D>, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
     constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
     constexpr uint32_t kTile = KT * kRow, kWaveRows = KT / kPromptWaves;   // bytes of a tile's keys; rows that a wave brings in
-    // two buffers of keys, then two of values (and room for the waves' weights where a tile of keys is too small for them)
+    constexpr uint32_t kShared = kPromptShared<D>, kRows = kPromptRows<D>, kHalf = D / kShared;   // values of a head that a wave holds
+    // two buffers of keys, then two of values; behind them room for the waves' weights, where a tile of keys is too small for them, or for
+    // their parts of the scores, and a flag for each
     extern __shared__ __align__(16) char lds[];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
 
     // the last tiles first: they have the most tokens to look at
-    const uint32_t total = prompt_tiles_of_all(a), local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads, back = first_tile + local;
+    const uint32_t total = prompt_tiles_of_all(a, kRows), local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads, back = first_tile + local;
     if (back >= total) return;
     uint32_t tile_in_seq;
-    const uint32_t seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, &tile_in_seq));
+    const uint32_t seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, kRows, &tile_in_seq));
     tile_in_seq = __builtin_amdgcn_readfirstlane(tile_in_seq);
     const int start = max(a.seqs.starts[seq], 0), tokens = min(a.seqs.starts[seq + 1], (int)a.rows) - start, length = a.seqs.lengths[seq];
     if (tokens <= 0) return;
     const int before = (length < 0 ? 0 : length) - (a.seqs.starts[seq + 1] - start);   // position of the sequence's first row here
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
-    const uint32_t row0 = tile_in_seq * kPromptRows, rows = (uint32_t)tokens * a.group;
+    const uint32_t row0 = tile_in_seq * kRows, rows = (uint32_t)tokens * a.group;
 
     auto begin_of = [&](int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; };
     // this lane's query: a row behind the last one repeats it and is not stored
-    const uint32_t row = row0 + wave * 32u + col, my_row = min(row, rows - 1);
+    const uint32_t sharer = wave % kShared, wave_row = row0 + wave / kShared * 32u;
+    const uint32_t row = wave_row + col, my_row = min(row, rows - 1);
     const uint32_t my_token = my_row / a.group, my_head = kv_head * a.group + (my_row - my_token * a.group);
     const int my_position = before + (int)my_token, my_begin = begin_of(my_position), my_end = min(my_position + 1, capacity);
     // the workgroup's and the wave's first and last ones
-    const int low = before + (int)(row0 / a.group), high = before + (int)(min(row0 + kPromptRows, rows) - 1) / (int)a.group;
-    const uint32_t wave_row = row0 + wave * 32u;
+    const int low = before + (int)(row0 / a.group), high = before + (int)(min(row0 + kRows, rows) - 1) / (int)a.group;
     const int wave_low = before + (int)(min(wave_row, rows - 1) / a.group), wave_high = before + (int)(min(wave_row + 31u, rows - 1) / a.group);
     const int first = begin_of(low), last = min(high + 1, capacity);   // tokens that anyone sees: first .. last - 1
 
-    half8 q[D / 16];
+    half8 q[kHalf / 16];
     {
-        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + 8u * half;
+        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + sharer * kHalf + 8u * half;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
+        for (int i = 0; i < (int)kHalf / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
     const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
     float reference = -INFINITY, sum = 0.f;
-    float16v o[D / 32];
+    float16v o[kHalf / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; i++)
+    for (int i = 0; i < (int)kHalf / 32; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
@@ -239,19 +246,33 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         next = find_pages(t_begin + KT);
     }
     // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
-    const uint32_t k_at = col * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
-    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
+    const uint32_t k_at = (col * kRow + (key_place(col, half) << 4)) ^ sharer * kHalf * 2u, v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u + sharer * kHalf * 2u;
     // S^T of the tile in buffer `tile`; element j of block b: token 32 b + 8 (j / 4) + 4 half + j % 4
+    // (waves that share queries add their parts of the sums over a head's values)
     auto scores = [&](const char *tile, float16v (&s)[KT / 32]) {
 #pragma unroll
         for (int b = 0; b < KT / 32; b++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[b][j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++)
+        for (int i = 0; i < (int)kHalf / 16; i++)
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
+        if constexpr (kShared > 1) {
+            static_assert(KT == 32, "a wave's part is one block");
+            float4v *const parts = (float4v *)(lds + 4 * kTile);
+#pragma unroll
+            for (int j = 0; j < 4; j++) parts[(wave * 4u + j) * 64u + lane] = float4v{s[0][4 * j], s[0][4 * j + 1], s[0][4 * j + 2], s[0][4 * j + 3]};
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float4v other = parts[((wave ^ 1u) * 4u + j) * 64u + lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[0][4 * j + e] += other[e];
+            }
+        }
     };
     // the largest score, as an exponent; it sets the reference where there is none yet, and nothing is summed
     auto largest = [&](const float16v (&s)[KT / 32]) {
@@ -269,7 +290,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         const float raised = fmaxf(reference, most - 8.0f), by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(reference - raised);
         sum *= by;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) o[i] *= by;
+        for (int i = 0; i < (int)kHalf / 32; i++) o[i] *= by;
         reference = raised;
     };
     auto weigh = [&](const float16v (&s)[KT / 32], half8 (&p)[KT / 16]) {
@@ -288,7 +309,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
 #pragma unroll
         for (int b = 0; b < KT / 16; b++)
 #pragma unroll
-            for (int i = 0; i < D / 32; i++) {
+            for (int i = 0; i < (int)kHalf / 32; i++) {
                 // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
                 const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + b * 16 * kRow)));
                 const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
@@ -327,9 +348,12 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
             half8 p[KT / 16];
             scores(tile, s);
             const float most = largest(s);
-            if (__any(most > reference + 15.0f)) {   // (rare; outside of this loop, so that the sums never move within it)
-                raise_to = most;
-                break;
+            if (__any(most > reference + 15.0f)) {
+                if constexpr (kShared == 1) {   // (rare; outside of this loop, so that the sums never move within it)
+                    raise_to = most;
+                    break;
+                }
+                raise(most);
             }
             weigh(s, p);
             add_values(tile, p);
@@ -344,7 +368,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
         const char *const tile = lds + buf * kTile;
         const uint32_t present = there_now;
         advance();
-        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
+        // nothing for this wave (waves that share queries meet in every tile)
+        const bool idle = kShared == 1 && (t0 > wave_high || t0 + KT <= begin_of(wave_low));
         half8 p[KT / 16];
         if (!idle) {
             float16v s[KT / 32];
@@ -375,7 +400,13 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
             else
                 bad |= not_finite(*at);
         }
-        const bool single = __syncthreads_or(bad);
+        // (waves that share queries have met since they read the tile's keys, so that flags and weights may take their place)
+        uint32_t *const flags = (uint32_t *)(lds + (D == 256 ? buf * kTile : kPromptLds<D> - 16));
+        bad = __any(bad);
+        if (lane == 0) flags[wave] = bad;
+        __syncthreads();
+        const bool single = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+        if (single) __syncthreads();   // (flags are read)
         if (!idle && !single) {
             add_values(tile, p);
         } else if (!idle) {
@@ -391,10 +422,10 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
                 const bool seen = at >= my_begin && at < my_end;
                 const float w = (float)weights[r * 32 + (int)col];
 #pragma unroll
-                for (int i = 0; i < D / 32; i++)
+                for (int i = 0; i < (int)kHalf / 32; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
+                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
                     }
@@ -406,18 +437,15 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) 
     sum = sum_of_halves(sum);
     if (row < rows) {
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
-        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + 4u * half;
+        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + sharer * kHalf + 4u * half;
 #pragma unroll
-        for (int i = 0; i < D / 32; i++)
+        for (int i = 0; i < (int)kHalf / 32; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 *(half4_any *)(out + 32 * i + 8 * j) = half4{(_Float16)(o[i][4 * j] * to), (_Float16)(o[i][4 * j + 1] * to), (_Float16)(o[i][4 * j + 2] * to),
                                                              (_Float16)(o[i][4 * j + 3] * to)};
     }
 }
-
-// LDS of a workgroup
-template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile<D> * D * 2 + (D == 64 ? kPromptTile<D> * 2 * kPromptRows : 0);
 
 hipError_t init_attn_prompt()
 {
@@ -436,10 +464,10 @@ hipError_t init_attn_prompt()
 
 hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a)
 {
-    // every sequence begins a tile of its own
-    const uint64_t tiles = (uint64_t)a.rows * a.group / kPromptRows + std::min(a.seqs.seqs, a.rows);
     auto launch = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
+        // every sequence begins a tile of its own
+        const uint64_t tiles = (uint64_t)a.rows * a.group / kPromptRows<D> + std::min(a.seqs.seqs, a.rows);
         return in_slices((uint32_t)tiles, most_workgroups(256) / a.kv.kv_heads, [&](uint32_t tile, uint32_t here) {
             hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads), dim3(256), kPromptLds<D>, s, a, tile);
             return hipGetLastError();
