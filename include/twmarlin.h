@@ -591,7 +591,7 @@ int twm_attn_decode(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *
                     uint32_t q_heads, float scale, uint32_t window, uint16_t *out_dev, uint32_t out_stride);
 /* The same for several new tokens per sequence -- whole prompts, pieces of them behind what is cached already, drafts to verify --, packed as
  * seqs->starts_dev says (not NULL): the row at position p sees the tokens up to p, the last `window` of these.  Weights enter the
- * products rounded to f16; sums are held in 32 bits. */
+ * products rounded to f16; sums are held in 32 bits.  Uses the context's scratch. */
 int twm_attn_prompt(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *seqs, const uint16_t *q_dev, uint32_t q_stride,
                     uint32_t rows, uint32_t q_heads, float scale, uint32_t window, uint16_t *out_dev, uint32_t out_stride);
 /* Copies page sources[i] to page targets[i], i < pairs, keys and values, in every one of `count` caches of the same shape and type (a model's

@@ -79,7 +79,7 @@ int attention(const char *who, twm_ctx *ctx, const twm_kv_cache *cache, const tw
     a.window = std::min(window, 0x7FFFFFFFu);   // (as far as a position goes)
     DeviceGuard on(ctx);
     HIP_TRY(on.status, TWM_DEVICE_ERROR, who);
-    HIP_TRY(prompt ? launch_attn_prompt(ctx->stream, a) : launch_attn_decode(ctx->stream, a, ctx->ws, ctx->ws_bytes), TWM_DEVICE_ERROR, who);
+    HIP_TRY((prompt ? launch_attn_prompt : launch_attn_decode)(ctx->stream, a, ctx->ws, ctx->ws_bytes), TWM_DEVICE_ERROR, who);
     return TWM_OK;
 }
 

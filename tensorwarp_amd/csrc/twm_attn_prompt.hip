@@ -111,6 +111,46 @@ __device__ __forceinline__ bool not_finite(uint4v v)
     return found;
 }
 
+struct Prompt {
+    AttnArgs a;
+    float4v *parts;       // [workgroups][dim / 4][rows of a workgroup], for rows that several workgroups share the tokens of
+    float2 *part_sums;    // [workgroups][rows]: reference, sum of weights
+    uint32_t splits, first_tile;   // splits: the most workgroups that share a tile of rows
+};
+
+// What a workgroup works on: `rows` rows (tokens times heads of a group) of sequence seq, of which it has those from row0 on
+struct Rows {
+    uint32_t seq, row0, rows;
+    int start, before, first, last;   // the sequence's first row and its position; tokens that any of the workgroup's rows sees: first .. last - 1
+};
+__device__ __forceinline__ int prompt_begin(const AttnArgs &a, int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; }
+// Tile `back` from the end; false: there is none.
+__device__ __forceinline__ bool find_rows(const AttnArgs &a, uint32_t back, uint32_t each, Rows *r)
+{
+    const uint32_t total = prompt_tiles_of_all(a, each);
+    if (back >= total) return false;
+    uint32_t inside;
+    r->seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, each, &inside));
+    r->row0 = __builtin_amdgcn_readfirstlane(inside) * each;
+    const int end = a.seqs.starts[r->seq + 1], length = max(a.seqs.lengths[r->seq], 0);
+    r->start = max(a.seqs.starts[r->seq], 0);
+    const int tokens = min(end, (int)a.rows) - r->start;
+    if (tokens <= 0) return false;
+    r->rows = (uint32_t)tokens * a.group;
+    r->before = length - (end - r->start);
+    r->first = prompt_begin(a, r->before + (int)(r->row0 / a.group));
+    r->last = min(r->before + (int)((min(r->row0 + each, r->rows) - 1) / a.group) + 1, a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0);
+    return true;
+}
+// How many workgroups share these rows' tokens: each has kLeastPart tiles at least
+constexpr int kLeastPart = 6;
+__device__ __forceinline__ uint32_t parts_of(const Rows &r, uint32_t splits, int tile, uint32_t *tiles)
+{
+    const int begin = r.first & ~(tile - 1);
+    *tiles = r.last > begin ? (uint32_t)(r.last - begin + tile - 1) / (uint32_t)tile : 0u;
+    return max(1u, min(splits, *tiles / kLeastPart));
+}
+
 // tokens of a tile
 template <int D> constexpr int kPromptTile = D == 256 ? 32 : 64;
 // LDS of a workgroup
@@ -118,7 +158,7 @@ template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile<D> * D * 2 + (D
 
 }  // namespace
 
-template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt(const AttnArgs a, uint32_t first_tile)
+template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt(const Prompt job)
 {
     constexpr int KT = kPromptTile<D>, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
     constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
@@ -127,21 +167,21 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     // two buffers of keys, then two of values; behind them room for the waves' weights, where a tile of keys is too small for them, or for
     // their parts of the scores, and a flag for each
     extern __shared__ __align__(16) char lds[];
+    const AttnArgs &a = job.a;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
 
     // the last tiles first: they have the most tokens to look at
-    const uint32_t total = prompt_tiles_of_all(a, kRows), local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads, back = first_tile + local;
-    if (back >= total) return;
-    uint32_t tile_in_seq;
-    const uint32_t seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, kRows, &tile_in_seq));
-    tile_in_seq = __builtin_amdgcn_readfirstlane(tile_in_seq);
-    const int start = max(a.seqs.starts[seq], 0), tokens = min(a.seqs.starts[seq + 1], (int)a.rows) - start, length = a.seqs.lengths[seq];
-    if (tokens <= 0) return;
-    const int before = (length < 0 ? 0 : length) - (a.seqs.starts[seq + 1] - start);   // position of the sequence's first row here
+    const uint32_t pair = blockIdx.x / job.splits, split = blockIdx.x - pair * job.splits, local = pair / a.kv.kv_heads, kv_head = pair - local * a.kv.kv_heads;
+    Rows mine;
+    if (!find_rows(a, job.first_tile + local, kRows, &mine)) return;
+    const uint32_t seq = mine.seq, row0 = mine.row0, rows = mine.rows;
+    const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
-    const uint32_t row0 = tile_in_seq * kRows, rows = (uint32_t)tokens * a.group;
+    uint32_t key_tiles;
+    const uint32_t parts = parts_of(mine, job.splits, KT, &key_tiles);
+    if (split >= parts) return;
 
-    auto begin_of = [&](int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; };
+    auto begin_of = [&](int position) { return prompt_begin(a, position); };
     // this lane's query: a row behind the last one repeats it and is not stored
     const uint32_t sharer = wave % kShared, wave_row = row0 + wave / kShared * 32u;
     const uint32_t row = wave_row + col, my_row = min(row, rows - 1);
@@ -150,7 +190,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     // the workgroup's and the wave's first and last ones
     const int low = before + (int)(row0 / a.group), high = before + (int)(min(row0 + kRows, rows) - 1) / (int)a.group;
     const int wave_low = before + (int)(min(wave_row, rows - 1) / a.group), wave_high = before + (int)(min(wave_row + 31u, rows - 1) / a.group);
-    const int first = begin_of(low), last = min(high + 1, capacity);   // tokens that anyone sees: first .. last - 1
+    // the tokens that anyone sees, or this part of them
+    const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * key_tiles / parts) * KT);
+    const int last = min(mine.last, all_begin + (int)((split + 1) * key_tiles / parts) * KT);
 
     half8 q[kHalf / 16];
     {
@@ -435,7 +477,17 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     }
 
     sum = sum_of_halves(sum);
-    if (row < rows) {
+    if (parts > 1) {
+        // to scratch, rows beside each other
+        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + wave_row - row0 + col;
+#pragma unroll
+        for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (row < rows)
+                    to[(sharer * (kHalf / 4) + 8u * i + 2u * j + half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        if (row < rows && sharer == 0 && half == 0) job.part_sums[(size_t)blockIdx.x * kRows + wave_row - row0 + col] = float2{reference, sum};
+    } else if (row < rows) {
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
         _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + sharer * kHalf + 4u * half;
 #pragma unroll
@@ -445,6 +497,64 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
                 *(half4_any *)(out + 32 * i + 8 * j) = half4{(_Float16)(o[i][4 * j] * to), (_Float16)(o[i][4 * j + 1] * to), (_Float16)(o[i][4 * j + 2] * to),
                                                              (_Float16)(o[i][4 * j + 3] * to)};
     }
+}
+
+// Joins what several workgroups hold of rows: 256 / (D / 4) rows of a tile and key-value head a workgroup, or a fourth of that where parts
+// are many and each wave takes every fourth.
+template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_prompt_join(const Prompt job)
+{
+    constexpr uint32_t kRows = kPromptRows<D>, kEach = 256 / SLICES, kHere = kEach / (D / 4);   // threads of a slice, rows of a workgroup
+    __shared__ float4v sums_of[SLICES][kEach];
+    __shared__ float2 tops_of[SLICES][kEach];
+    const AttnArgs &a = job.a;
+    const uint32_t local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads;
+    Rows mine;
+    if (!find_rows(a, job.first_tile + local, kRows, &mine)) return;
+    uint32_t key_tiles;
+    const uint32_t parts = parts_of(mine, job.splits, kPromptTile<D>, &key_tiles);
+    const uint32_t first_row = blockIdx.y * kHere;
+    if (parts == 1 || mine.row0 + first_row >= mine.rows) return;
+    const uint32_t slice = threadIdx.x / kEach, x = threadIdx.x % kEach, r = first_row + x % kHere, quad = x / kHere;   // (rows lie beside each other)
+    const float2 *sums = job.part_sums + (size_t)blockIdx.x * job.splits * kRows + r;
+    const float4v *from = job.parts + (size_t)blockIdx.x * job.splits * (D / 4 * kRows) + quad * kRows + r;
+    float top = -INFINITY, sum = 0.f;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const float2 &s, const float4v &part) {
+        const float raised = fmaxf(top, s.x), keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - raised), by = s.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.x - raised);
+        sum = sum * keep + s.y * by;
+        o = o * keep + part * by;
+        top = raised;
+    };
+    if (mine.row0 + r < mine.rows) {
+        constexpr uint32_t kAhead = 4;
+        for (uint32_t p = slice; p < parts; p += SLICES * kAhead) {
+            float2 s[kAhead];
+            float4v part[kAhead];
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; i++) {
+                const uint32_t q = min(p + SLICES * i, parts - 1);
+                s[i] = sums[q * kRows];
+                part[i] = from[(size_t)q * (D / 4 * kRows)];
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; i++)
+                if (p + SLICES * i < parts) add(s[i], part[i]);
+        }
+    }
+    if constexpr (SLICES > 1) {
+        sums_of[slice][x] = o;
+        tops_of[slice][x] = float2{top, sum};
+        __syncthreads();
+        if (slice != 0) return;
+#pragma unroll
+        for (uint32_t i = 1; i < SLICES; i++) add(tops_of[i][x], sums_of[i][x]);
+    }
+    const uint32_t row = mine.row0 + r;
+    if (row >= mine.rows) return;
+    const float v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
+    const uint32_t token = row / a.group, head = kv_head * a.group + (row - token * a.group);
+    *(half4_any *)(a.out + (size_t)(mine.start + (int)token) * a.out_stride + head * D + 4u * quad) =
+        half4{(_Float16)(o[0] * to), (_Float16)(o[1] * to), (_Float16)(o[2] * to), (_Float16)(o[3] * to)};
 }
 
 hipError_t init_attn_prompt()
@@ -462,16 +572,34 @@ hipError_t init_attn_prompt()
     return e;
 }
 
-hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a)
+hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes)
 {
     auto launch = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
+        constexpr uint32_t kRows = kPromptRows<D>;
         // every sequence begins a tile of its own
-        const uint64_t tiles = (uint64_t)a.rows * a.group / kPromptRows<D> + std::min(a.seqs.seqs, a.rows);
-        return in_slices((uint32_t)tiles, most_workgroups(256) / a.kv.kv_heads, [&](uint32_t tile, uint32_t here) {
-            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads), dim3(256), kPromptLds<D>, s, a, tile);
+        const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + std::min(a.seqs.seqs, a.rows), workgroups = tiles * a.kv.kv_heads;
+        // Tokens are shared out where rows alone leave most of the chip without work (two workgroups a compute unit), as far as there may be some
+        const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
+        const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile<D> * kLeastPart);
+        Prompt job;
+        job.a = a;
+        job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / workgroups, most));
+        job.parts = (float4v *)scratch;
+        job.part_sums = (float2 *)((char *)scratch + (size_t)workgroups * job.splits * kRows * D * 4);
+        if (job.splits > 1 && (size_t)workgroups * job.splits * kRows * (D * 4 + 8) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
+        const hipError_t error = in_slices((uint32_t)tiles, most_workgroups(256) / (a.kv.kv_heads * job.splits), [&](uint32_t tile, uint32_t here) {
+            job.first_tile = tile;
+            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads * job.splits), dim3(256), kPromptLds<D>, s, job);
             return hipGetLastError();
         });
+        if (error != hipSuccess || job.splits == 1) return error;
+        // (one slice: at most 512 workgroups)
+        if (job.splits >= 8)
+            hipLaunchKernelGGL((k_attn_prompt_join<D, 4>), dim3((uint32_t)workgroups, kRows / (64 / (D / 4))), dim3(256), 0, s, job);
+        else
+            hipLaunchKernelGGL((k_attn_prompt_join<D, 1>), dim3((uint32_t)workgroups, kRows / (256 / (D / 4))), dim3(256), 0, s, job);
+        return hipGetLastError();
     };
     return a.kv.dim == 64    ? launch(std::integral_constant<int, 64>{})
            : a.kv.dim == 128 ? launch(std::integral_constant<int, 128>{})

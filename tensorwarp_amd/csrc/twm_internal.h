@@ -265,7 +265,7 @@ struct AttnArgs {
     uint32_t window;   // 0: none
 };
 hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes);
-hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a);
+hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes);
 hipError_t init_attn_prompt();
 
 }  // namespace twm

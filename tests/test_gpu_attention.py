@@ -122,6 +122,17 @@ def test_prompt_looks_back_a_window(dev, window, cache):
     run_prompt(dev, pool, table, lengths, new, 8, window=window)
 
 
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kv,window", [(64, 14, 2, 0), (128, 7, 1, 0), (128, 4, 4, 2500), (256, 4, 2, 0)])
+@pytest.mark.parametrize("new,lengths", [([1], [6000]), ([5], [4003]), ([40, 2, 1], [3000, 90, 5001]), ([150], [4500])])
+def test_few_rows_behind_many_tokens(dev, new, lengths, dim, heads, kv, window, cache):
+    # shared out among workgroups by their tokens, in as many parts as a sequence has tiles for
+    pool = Pool(np.random.default_rng(sum(new) + dim), sum(-(-n // 64) for n in lengths) + 3, kv, 64, dim, cache)
+    table = pool.fill(lengths)
+    table[0, 20:25] = -1   # (absent pages, and rows whose parts lack them all or see none of theirs)
+    run_prompt(dev, pool, table, lengths, new, heads, window=window)
+
+
 def test_rows_of_no_sequence_stay_as_they_were(dev):
     pool = Pool(np.random.default_rng(8), 40, 2, 16, 64)
     run_prompt(dev, pool, pool.fill([40, 3, 70]), [40, 3, 70], [33, 0, 70], 6, first=5, spare=150)
