@@ -13,8 +13,8 @@
 // Weights enter the product as two f16 terms, the first one cut off and the second what it leaves: both are positive, and at least the
 // smallest f16 number where a token is seen (2^-39 of the largest weight), so that an infinite value times its weight is that infinity.
 //
-// All tokens of all sequences and heads, in steps of 128, are dealt out evenly among as many workgroups as the chip holds at once, which
-// find their share from the lengths by themselves: a long sequence is cut into many shares, several short ones make one.  What a share
+// All tokens of all sequences, in steps of 128, are dealt out evenly among as many workgroups for each key-value head as the chip holds at once,
+// which find their share from the lengths by themselves: a long sequence is cut into many shares, several short ones make one.  What a share
 // holds of a sequence that others hold too goes to scratch, and a second kernel joins it.
 #include "twm_kv.h"
 
@@ -26,6 +26,7 @@ namespace twm {
 namespace {
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef half4 half4_any __attribute__((aligned(2)));
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef int int2v __attribute__((ext_vector_type(2)));
 #define TWM_LDS(T) __attribute__((address_space(3))) T
@@ -38,12 +39,13 @@ struct Decode {
     AttnArgs a;
     float *parts;          // [2 * workgroups][heads of a unit][dim]
     float2 *part_sums;     // [2 * workgroups][heads of a unit]: largest score, sum of weights
-    uint32_t units, tiles;   // per sequence: tiles of up to sixteen heads for each key-value head
+    uint32_t units, tiles;   // units: tiles of up to sixteen heads for each key-value head
     uint32_t heads;          // of a unit
-    uint32_t shares;         // workgroups of the first kernel
+    uint32_t shares;         // of each unit: workgroup unit * shares + share of the first kernel
+    Divisor by_shares, by_tiles, by_group;
 };
 
-// The tokens that sequence `seq` sees, from `first`, the multiple of 32 at or below the first one, in steps of 128
+// The tokens that a sequence sees, from `first`, the multiple of 32 at or below the first one, in steps of 128
 struct Span {
     int lo, hi, first;
     uint32_t steps;
@@ -58,55 +60,30 @@ __device__ __forceinline__ Span span_of(const Decode &d, int length)
     return s;
 }
 
-__device__ __forceinline__ uint64_t wave_sum_up_to(uint64_t v)   // of this lane and those before it
+// The steps of 64 sequences, a lane each, and the sums up to it (64 sequences have less than 2^29)
+struct Lengths {
+    int length;
+    uint32_t steps, up_to, all;
+};
+__device__ __forceinline__ Lengths lengths_from(const Decode &d, uint32_t base)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t i = 1; i < 64; i *= 2) {
-        const uint64_t other = __shfl_up((unsigned long long)v, i);
-        if (lane >= i) v += other;
-    }
-    return v;
+    const uint32_t s = base + (threadIdx.x & 63u);
+    Lengths l;
+    l.length = s < d.a.seqs.seqs ? d.a.seqs.lengths[s] : 0;
+    l.steps = span_of(d, l.length).steps;
+    l.up_to = wave_sum_up_to(l.steps);
+    l.all = __builtin_amdgcn_readlane(l.up_to, 63);
+    return l;
 }
 
-// Steps of all sequences and units, and of those before sequence `until`
-__device__ __forceinline__ uint64_t all_steps(const Decode &d, uint32_t until, uint64_t *before)
+// Share w of a unit's `total` steps begins here; every share has a step at least, where there are as many.  (In 64 bits beyond 2^20: any
+// rounding would do that is the same for all who ask.)
+__device__ __forceinline__ uint64_t share_begin(const Decode &d, uint64_t total, uint32_t w)
 {
-    uint64_t sum = 0;
-    *before = 0;
-    for (uint32_t base = 0; base < d.a.seqs.seqs; base += 64) {
-        const uint32_t s = base + (threadIdx.x & 63u);
-        const uint64_t up_to = wave_sum_up_to(s < d.a.seqs.seqs ? (uint64_t)span_of(d, d.a.seqs.lengths[s]).steps * d.units : 0u);
-        if (until >= base && until < base + 64) *before = until == base ? sum : sum + __shfl((unsigned long long)up_to, until - base - 1);
-        sum += __shfl((unsigned long long)up_to, 63);
-    }
-    return sum;
+    if (total <= d.shares) return min((uint64_t)w, total);
+    if (total < 1u << 20) return d.by_shares((uint32_t)total * w);
+    return w == d.shares ? total : (uint64_t)((double)total * w / d.shares);
 }
-
-// The sequence that step `at` belongs to (there is one); *before: the steps ahead of it
-__device__ __forceinline__ uint32_t sequence_of(const Decode &d, uint64_t at, uint64_t *before)
-{
-    uint64_t sum = 0;
-    for (uint32_t base = 0; base < d.a.seqs.seqs; base += 64) {
-        const uint32_t s = base + (threadIdx.x & 63u);
-        const uint64_t up_to = wave_sum_up_to(s < d.a.seqs.seqs ? (uint64_t)span_of(d, d.a.seqs.lengths[s]).steps * d.units : 0u);
-        const uint64_t past = __ballot(sum + up_to > at);
-        if (past) {
-            const uint32_t lane = (uint32_t)__builtin_ctzll(past);
-            *before = lane == 0 ? sum : sum + __shfl((unsigned long long)up_to, lane - 1);
-            return base + lane;
-        }
-        sum += __shfl((unsigned long long)up_to, 63);
-    }
-    *before = sum;
-    return d.a.seqs.seqs;
-}
-
-// Every share has a step at least
-__device__ __forceinline__ uint32_t shares_of(const Decode &d, uint64_t total) { return (uint32_t)min((uint64_t)d.shares, total); }
-
-// Share w of `total` steps begins here
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t w, uint32_t shares) { return total / shares * w + total % shares * w / shares; }
 
 __device__ __forceinline__ float max_over_quarters(float v)
 {
@@ -153,32 +130,49 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, quarter = lane >> 4, col = lane & 15u;
     char *const buffer = buffers[wave];
 
-    // rows without tokens
-    for (uint32_t s = blockIdx.x; s < a.seqs.seqs; s += gridDim.x)
+    const uint32_t unit = d.by_shares(blockIdx.x), share = blockIdx.x - unit * d.shares;
+    const uint32_t kv_head = d.by_tiles(unit), head0 = kv_head * a.group + (unit - kv_head * d.tiles) * kDecodeHeads;
+    const uint32_t heads = min(kDecodeHeads, (kv_head + 1) * a.group - head0);
+    // Up to 64 sequences are looked up once
+    Lengths l = lengths_from(d, 0);
+    uint64_t total = l.all;
+    for (uint32_t base = 64; base < a.seqs.seqs; base += 64) total += lengths_from(d, base).all;
+    // rows without tokens: every share clears some
+    for (uint32_t s = share; s < a.seqs.seqs; s += d.shares)
         if (span_of(d, a.seqs.lengths[s]).steps == 0)
-            for (uint32_t i = threadIdx.x; i < a.q_heads * D / 8; i += 256) *(half8_any *)(a.out + (size_t)s * a.out_stride + 8u * i) = half8{};
-
-    uint64_t before;
-    const uint64_t total = all_steps(d, 0, &before);
-    const uint32_t shares = shares_of(d, total);
-    if (blockIdx.x >= shares) return;
-    uint64_t at = share_begin(total, blockIdx.x, shares);
-    const uint64_t end = share_begin(total, blockIdx.x + 1, shares);
-    uint32_t seq = __builtin_amdgcn_readfirstlane(sequence_of(d, at, &before));
-    uint32_t part = 2 * blockIdx.x;
+            for (uint32_t i = threadIdx.x; i < heads * D / 8; i += 256) *(half8_any *)(a.out + (size_t)s * a.out_stride + head0 * D + 8u * i) = half8{};
+    uint64_t at = share_begin(d, total, share);
+    const uint64_t end = share_begin(d, total, share + 1);
+    if (at >= end) return;
+    // the sequence in which the share begins
+    uint64_t before = 0;
+    uint32_t base = 0, seq;
+    for (;;) {
+        const uint64_t past = __ballot(before + l.up_to > at);
+        if (past) {
+            const uint32_t lane_of = (uint32_t)__builtin_ctzll(past);
+            seq = base + lane_of;
+            before += lane_of == 0 ? 0u : (uint32_t)__builtin_amdgcn_readlane(l.up_to, lane_of - 1);
+            break;
+        }
+        before += l.all;
+        base += 64;
+        l = lengths_from(d, base);
+    }
+    const uint32_t part = 2 * blockIdx.x;
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
     for (bool first_of_share = true; at < end; first_of_share = false) {
-        const Span span = span_of(d, __builtin_amdgcn_readfirstlane(a.seqs.lengths[seq]));
+        if (seq - base >= 64) {
+            base += 64;
+            l = lengths_from(d, base);
+        }
+        const Span span = span_of(d, __builtin_amdgcn_readlane(l.length, seq - base));
         if (span.steps == 0) {
             seq++;
             continue;
         }
-        // this share's steps of one unit
-        const uint64_t inside = at - before;
-        const uint32_t unit = (uint32_t)(inside / span.steps), step0 = (uint32_t)(inside - (uint64_t)unit * span.steps);
-        const uint32_t step1 = (uint32_t)min((uint64_t)span.steps, step0 + (end - at));
-        const uint32_t kv_head = unit / d.tiles, head0 = kv_head * a.group + (unit - kv_head * d.tiles) * kDecodeHeads;
-        const uint32_t heads = min(kDecodeHeads, (kv_head + 1) * a.group - head0);
+        // this share's steps of the sequence
+        const uint32_t step0 = (uint32_t)(at - before), step1 = (uint32_t)min((uint64_t)span.steps, step0 + (end - at));
         const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
 
         // Q^T: a lane's head's values, in the order in which it holds keys
@@ -342,7 +336,6 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
             for (uint32_t w = 0; w < kDecodeWaves; w++) l += sums[w][h] * shrink(tops[w][h], m, c);
             if (all) {
                 const float to = l == 0.f ? 0.f : v_scale / l;
-                typedef half4 half4_any __attribute__((aligned(2)));
                 *(half4_any *)(a.out + (size_t)seq * a.out_stride + (head0 + h) * D + x) =
                     half4{(_Float16)(r[0] * to), (_Float16)(r[1] * to), (_Float16)(r[2] * to), (_Float16)(r[3] * to)};
             } else {
@@ -354,63 +347,77 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
         }
         __syncthreads();   // (the buffers are the waves' own again)
         at += step1 - step0;
-        if (at - before == (uint64_t)span.steps * d.units) {
-            before = at;
-            seq++;
-        }
+        before += span.steps;
+        seq++;
     }
 }
 
-// Joins what several shares hold of a unit: a workgroup per query head and sequence, its waves every fourth share.
-template <int D> __global__ __launch_bounds__(256) void k_attn_join(const Decode d)
+// Joins what several shares hold of a unit: a workgroup per query head and sequence.  D / 4 lanes hold a part, 2048 / D of them at a time, four
+// on their way.
+constexpr uint32_t kJoinThreads = 512;
+template <int D> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const Decode d)
 {
-    __shared__ float tops[4], totals[4], results[4][D];
+    constexpr uint32_t kLanes = D / 4, kAtOnce = kJoinThreads / kLanes, kAhead = 4;
+    __shared__ float4v results[kAtOnce][kLanes];
+    __shared__ float2 sums[kAtOnce];
     const AttnArgs &a = d.a;
-    const uint32_t seq = blockIdx.x, head = blockIdx.y, kv_head = head / a.group, in_group = head - kv_head * a.group;
+    const uint32_t seq = blockIdx.x, head = blockIdx.y, kv_head = d.by_group(head), in_group = head - kv_head * a.group;
     const uint32_t unit = kv_head * d.tiles + in_group / kDecodeHeads, h = in_group % kDecodeHeads;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u;
-    const uint32_t steps = span_of(d, a.seqs.lengths[seq]).steps;
-    uint64_t before;
-    const uint64_t total = all_steps(d, seq, &before);
+    uint64_t total = 0, begin = 0;
+    uint32_t steps = 0;
+    for (uint32_t base = 0; base < a.seqs.seqs; base += 64) {
+        const Lengths l = lengths_from(d, base);
+        if (seq - base < 64u) {
+            steps = __builtin_amdgcn_readlane(l.steps, seq - base);
+            begin = total + __builtin_amdgcn_readlane(l.up_to, seq - base) - steps;
+        }
+        total += l.all;
+    }
     if (steps == 0) return;
-    const uint64_t begin = before + (uint64_t)unit * steps, end = begin + steps;
-    const uint32_t shares = shares_of(d, total);
+    const uint64_t end = begin + steps;
     // the shares that hold its first and its last step
     auto share_of = [&](uint64_t at) {
-        uint32_t w = (uint32_t)min((uint64_t)(shares - 1), (uint64_t)((double)at / (double)total * shares));
-        while (share_begin(total, w, shares) > at) w--;
-        while (share_begin(total, w + 1, shares) <= at) w++;
+        uint32_t w = (uint32_t)min((uint64_t)(d.shares - 1), (uint64_t)((float)at / (float)total * d.shares));
+        while (share_begin(d, total, w) > at) w--;
+        while (share_begin(d, total, w + 1) <= at) w++;
         return w;
     };
     const uint32_t first = share_of(begin), last = share_of(end - 1);
     if (first == last) return;
-    const uint32_t first_slot = 2 * first + (share_begin(total, first, shares) < begin ? 1u : 0u);
-    auto slot_of = [&](uint32_t w) { return (size_t)(w == first ? first_slot : 2 * w) * d.heads + h; };
+    const uint32_t first_slot = 2 * (unit * d.shares + first) + (share_begin(d, total, first) < begin ? 1u : 0u);
+    auto slot_of = [&](uint32_t w) { return (size_t)(w == first ? first_slot : 2 * (unit * d.shares + w)) * d.heads + h; };
     const float c = a.scale * 1.44269504f * (a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f), v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
-    float top = -INFINITY;
-    for (uint32_t w = first + threadIdx.x; w <= last; w += 256) top = fmaxf(top, d.part_sums[slot_of(w)].x);
+    const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
+    float top = -INFINITY, sum = 0.f;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](const float2 &s, const float4v &part) {
+        const float most = fmaxf(top, s.x), keep = shrink(top, most, c), by = shrink(s.x, most, c);
+        sum = sum * keep + s.y * by;
+        o = o * keep + part * by;
+        top = most;
+    };
+    for (uint32_t w = first + group; w <= last; w += kAtOnce * kAhead) {
+        float2 s[kAhead];
+        float4v part[kAhead];
 #pragma unroll
-    for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    float l = 0.f, r[D / 64] = {};
-    for (uint32_t w = first + wave; w <= last; w += 4) {
-        const size_t slot = slot_of(w);
-        const float2 ml = d.part_sums[slot];
-        const float by = shrink(ml.x, top, c);
-        l += ml.y * by;
+        for (uint32_t i = 0; i < kAhead; i++) {
+            const size_t slot = slot_of(min(w + kAtOnce * i, last));
+            s[i] = d.part_sums[slot];
+            part[i] = *(const float4v *)(d.parts + slot * D + 4u * lane);
+        }
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) r[i] += d.parts[slot * D + 64 * i + lane] * by;
+        for (uint32_t i = 0; i < kAhead; i++)
+            if (w + kAtOnce * i <= last) add(s[i], part[i]);
     }
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) results[wave][64 * i + lane] = r[i];
-    if (lane == 0) totals[wave] = l;
+    results[group][lane] = o;
+    if (lane == 0) sums[group] = float2{top, sum};
     __syncthreads();
-    l = totals[0] + totals[1] + totals[2] + totals[3];
-    const float to = l == 0.f ? 0.f : v_scale / l;
-    for (uint32_t i = threadIdx.x; i < D; i += 256)
-        a.out[(size_t)seq * a.out_stride + head * D + i] = (_Float16)((results[0][i] + results[1][i] + results[2][i] + results[3][i]) * to);
+    if (group != 0) return;
+#pragma unroll 4
+    for (uint32_t g = 1; g < kAtOnce; g++) add(sums[g], results[g][lane]);
+    const float to = sum == 0.f ? 0.f : v_scale / sum;
+    *(half4_any *)(a.out + (size_t)seq * a.out_stride + head * D + 4u * lane) =
+        half4{(_Float16)(o[0] * to), (_Float16)(o[1] * to), (_Float16)(o[2] * to), (_Float16)(o[3] * to)};
 }
 
 hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, size_t scratch_bytes)
@@ -426,17 +433,20 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
     // as many workgroups as the chip holds at once, or as there may be steps
     const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
     const uint64_t most_steps = (std::min(capacity, a.window ? (uint64_t)a.window + 31 : capacity) + kDecodeStep - 1) / kDecodeStep;
-    d.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 * per_unit, most_steps * d.units * a.seqs.seqs));
-    const size_t slots = 2 * (size_t)d.shares * d.heads;
+    d.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 * per_unit / d.units, most_steps * a.seqs.seqs));
+    d.by_shares = Divisor(d.shares);
+    d.by_tiles = Divisor(d.tiles);
+    d.by_group = Divisor(a.group);
+    const size_t slots = 2 * (size_t)d.shares * d.units * d.heads;
     d.part_sums = (float2 *)scratch;
     d.parts = (float *)((char *)scratch + (slots * sizeof(float2) + 255) / 256 * 256);
     if ((size_t)((char *)(d.parts + slots * a.kv.dim) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 25 MB of 256)
     auto kernels = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_decode<D, true> : k_attn_decode<D, false>), dim3(d.shares), dim3(256), 0, s, d);
+        hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_decode<D, true> : k_attn_decode<D, false>), dim3(d.shares * d.units), dim3(256), 0, s, d);
         hipError_t error = hipGetLastError();
         if (error != hipSuccess || most_steps <= 1) return error;   // (a step is never cut)
-        hipLaunchKernelGGL(k_attn_join<D>, dim3(a.seqs.seqs, a.q_heads), dim3(256), 0, s, d);
+        hipLaunchKernelGGL(k_attn_join<D>, dim3(a.seqs.seqs, a.q_heads), dim3(kJoinThreads), 0, s, d);
         return hipGetLastError();
     };
     return a.kv.dim == 64    ? kernels(std::integral_constant<int, 64>{})

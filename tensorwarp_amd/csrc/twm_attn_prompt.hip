@@ -38,52 +38,6 @@ constexpr uint32_t kPromptWaves = 4;
 template <int D> constexpr uint32_t kPromptShared = D == 256 ? 2 : 1;
 template <int D> constexpr uint32_t kPromptRows = 32 * kPromptWaves / kPromptShared<D>;
 
-// Workgroups of one key-value head: `each` rows per one, token by token
-__device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, uint32_t seq, uint32_t each)
-{
-    const int first = max(a.seqs.starts[seq], 0), end = min(a.seqs.starts[seq + 1], (int)a.rows);
-    return end > first ? ((uint32_t)(end - first) * a.group + each - 1) / each : 0u;
-}
-
-__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)   // of this lane and those before it
-{
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t i = 1; i < 64; i *= 2) {
-        const uint32_t other = __shfl_up(v, i);
-        if (lane >= i) v += other;
-    }
-    return v;
-}
-
-__device__ __forceinline__ uint32_t prompt_tiles_of_all(const AttnArgs &a, uint32_t each)
-{
-    uint32_t sum = 0;
-    for (uint32_t s = threadIdx.x & 63u; s < a.seqs.seqs; s += 64) sum += prompt_tiles(a, s, each);
-#pragma unroll
-    for (int i = 1; i < 64; i *= 2) sum += __shfl_xor(sum, i);
-    return sum;
-}
-
-// the sequence of tile `at` of a key-value head, and its place among the sequence's
-__device__ __forceinline__ uint32_t prompt_sequence_of(const AttnArgs &a, uint32_t at, uint32_t each, uint32_t *inside)
-{
-    uint32_t sum = 0;
-    for (uint32_t base = 0; base < a.seqs.seqs; base += 64) {
-        const uint32_t s = base + (threadIdx.x & 63u);
-        const uint32_t up_to = wave_sum_up_to(s < a.seqs.seqs ? prompt_tiles(a, s, each) : 0u);
-        const uint64_t past = __ballot(sum + up_to > at);
-        if (past) {
-            const uint32_t lane = (uint32_t)__builtin_ctzll(past);
-            *inside = at - (lane == 0 ? sum : sum + __shfl(up_to, lane - 1));
-            return base + lane;
-        }
-        sum += __shfl(up_to, 63);
-    }
-    *inside = 0;
-    return 0;
-}
-
 __device__ __forceinline__ float max_of_halves(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -116,6 +70,7 @@ struct Prompt {
     float4v *parts;       // [workgroups][dim / 4][rows of a workgroup], for rows that several workgroups share the tokens of
     float2 *part_sums;    // [workgroups][rows]: reference, sum of weights
     uint32_t splits, first_tile;   // splits: the most workgroups that share a tile of rows
+    Divisor by_group, by_kv_heads, by_splits;
 };
 
 // What a workgroup works on: `rows` rows (tokens times heads of a group) of sequence seq, of which it has those from row0 on
@@ -124,22 +79,53 @@ struct Rows {
     int start, before, first, last;   // the sequence's first row and its position; tokens that any of the workgroup's rows sees: first .. last - 1
 };
 __device__ __forceinline__ int prompt_begin(const AttnArgs &a, int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; }
-// Tile `back` from the end; false: there is none.
-__device__ __forceinline__ bool find_rows(const AttnArgs &a, uint32_t back, uint32_t each, Rows *r)
+
+// A sequence, as a lane looks it up
+struct Sequence {
+    int start, end, length;
+};
+__device__ __forceinline__ Sequence sequence_at(const AttnArgs &a, uint32_t s)
 {
-    const uint32_t total = prompt_tiles_of_all(a, each);
+    Sequence q{0, 0, 0};
+    if (s < a.seqs.seqs) q = Sequence{a.seqs.starts[s], a.seqs.starts[s + 1], a.seqs.lengths[s]};
+    return q;
+}
+// Workgroups of one key-value head that a sequence's rows take, EACH of them one
+template <uint32_t EACH> __device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, const Sequence &q)
+{
+    const int first = max(q.start, 0), end = min(q.end, (int)a.rows);
+    return end > first ? ((uint32_t)(end - first) * a.group + EACH - 1) / EACH : 0u;
+}
+// Tile `back` from the end; false: there is none.  (Up to 64 sequences are looked up once.)
+template <uint32_t EACH> __device__ __forceinline__ bool find_rows(const Prompt &job, uint32_t back, Rows *r)
+{
+    const AttnArgs &a = job.a;
+    const uint32_t lane = threadIdx.x & 63u;
+    Sequence q = sequence_at(a, lane);
+    uint32_t up_to = wave_sum_up_to(prompt_tiles<EACH>(a, q)), total = __builtin_amdgcn_readlane(up_to, 63);
+    for (uint32_t base = 64; base < a.seqs.seqs; base += 64) total += __builtin_amdgcn_readlane(wave_sum_up_to(prompt_tiles<EACH>(a, sequence_at(a, base + lane))), 63);
     if (back >= total) return false;
-    uint32_t inside;
-    r->seq = __builtin_amdgcn_readfirstlane(prompt_sequence_of(a, total - 1 - back, each, &inside));
-    r->row0 = __builtin_amdgcn_readfirstlane(inside) * each;
-    const int end = a.seqs.starts[r->seq + 1], length = max(a.seqs.lengths[r->seq], 0);
-    r->start = max(a.seqs.starts[r->seq], 0);
+    const uint32_t at = total - 1 - back;
+    uint32_t sum = 0, base = 0;
+    uint64_t past;
+    while ((past = __ballot(sum + up_to > at)) == 0) {
+        sum += __builtin_amdgcn_readlane(up_to, 63);
+        base += 64;
+        if (base >= a.seqs.seqs) return false;   // (starts that fall)
+        q = sequence_at(a, base + lane);
+        up_to = wave_sum_up_to(prompt_tiles<EACH>(a, q));
+    }
+    const uint32_t found = (uint32_t)__builtin_ctzll(past);
+    r->seq = base + found;
+    r->row0 = (at - sum - (found == 0 ? 0u : (uint32_t)__builtin_amdgcn_readlane(up_to, found - 1))) * EACH;
+    const int end = __builtin_amdgcn_readlane(q.end, found), length = max(__builtin_amdgcn_readlane(q.length, found), 0);
+    r->start = max(__builtin_amdgcn_readlane(q.start, found), 0);
     const int tokens = min(end, (int)a.rows) - r->start;
     if (tokens <= 0) return false;
     r->rows = (uint32_t)tokens * a.group;
     r->before = length - (end - r->start);
-    r->first = prompt_begin(a, r->before + (int)(r->row0 / a.group));
-    r->last = min(r->before + (int)((min(r->row0 + each, r->rows) - 1) / a.group) + 1, a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0);
+    r->first = prompt_begin(a, r->before + (int)job.by_group(r->row0));
+    r->last = min(r->before + (int)job.by_group(min(r->row0 + EACH, r->rows) - 1) + 1, a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0);
     return true;
 }
 // How many workgroups share these rows' tokens: each has kLeastPart tiles at least
@@ -171,9 +157,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
 
     // the last tiles first: they have the most tokens to look at
-    const uint32_t pair = blockIdx.x / job.splits, split = blockIdx.x - pair * job.splits, local = pair / a.kv.kv_heads, kv_head = pair - local * a.kv.kv_heads;
+    const uint32_t pair = job.by_splits(blockIdx.x), split = blockIdx.x - pair * job.splits, local = job.by_kv_heads(pair), kv_head = pair - local * a.kv.kv_heads;
     Rows mine;
-    if (!find_rows(a, job.first_tile + local, kRows, &mine)) return;
+    if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
     const uint32_t seq = mine.seq, row0 = mine.row0, rows = mine.rows;
     const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
@@ -185,11 +171,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     // this lane's query: a row behind the last one repeats it and is not stored
     const uint32_t sharer = wave % kShared, wave_row = row0 + wave / kShared * 32u;
     const uint32_t row = wave_row + col, my_row = min(row, rows - 1);
-    const uint32_t my_token = my_row / a.group, my_head = kv_head * a.group + (my_row - my_token * a.group);
+    const uint32_t my_token = job.by_group(my_row), my_head = kv_head * a.group + (my_row - my_token * a.group);
     const int my_position = before + (int)my_token, my_begin = begin_of(my_position), my_end = min(my_position + 1, capacity);
     // the workgroup's and the wave's first and last ones
-    const int low = before + (int)(row0 / a.group), high = before + (int)(min(row0 + kRows, rows) - 1) / (int)a.group;
-    const int wave_low = before + (int)(min(wave_row, rows - 1) / a.group), wave_high = before + (int)(min(wave_row + 31u, rows - 1) / a.group);
+    const int low = before + (int)job.by_group(row0), high = before + (int)job.by_group(min(row0 + kRows, rows) - 1);
+    const int wave_low = __builtin_amdgcn_readfirstlane(my_position), wave_high = __builtin_amdgcn_readlane(my_position, 31);
     // the tokens that anyone sees, or this part of them
     const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * key_tiles / parts) * KT);
     const int last = min(mine.last, all_begin + (int)((split + 1) * key_tiles / parts) * KT);
@@ -420,9 +406,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
             for (int b = 0; b < KT / 32; b++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
-                    const int token = t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4;
-                    const bool seen = token >= my_begin && token < my_end && (present >> (2 * b + j / 8) & 1u);
-                    s[b][j] = seen ? s[b][j] : -INFINITY;
+                    // (tokens from the first seen one on, as unsigned numbers, against their number: none where the page is absent)
+                    const uint32_t seen = present >> (2 * b + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
+                    s[b][j] = (uint32_t)(t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[b][j] : -INFINITY;
                 }
             const float most = largest(s);
             if (__any(most > reference + 15.0f)) raise(most);
@@ -507,9 +493,9 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     __shared__ float4v sums_of[SLICES][kEach];
     __shared__ float2 tops_of[SLICES][kEach];
     const AttnArgs &a = job.a;
-    const uint32_t local = blockIdx.x / a.kv.kv_heads, kv_head = blockIdx.x - local * a.kv.kv_heads;
+    const uint32_t local = job.by_kv_heads(blockIdx.x), kv_head = blockIdx.x - local * a.kv.kv_heads;
     Rows mine;
-    if (!find_rows(a, job.first_tile + local, kRows, &mine)) return;
+    if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
     uint32_t key_tiles;
     const uint32_t parts = parts_of(mine, job.splits, kPromptTile<D>, &key_tiles);
     const uint32_t first_row = blockIdx.y * kHere;
@@ -552,7 +538,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     const uint32_t row = mine.row0 + r;
     if (row >= mine.rows) return;
     const float v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
-    const uint32_t token = row / a.group, head = kv_head * a.group + (row - token * a.group);
+    const uint32_t token = job.by_group(row), head = kv_head * a.group + (row - token * a.group);
     *(half4_any *)(a.out + (size_t)(mine.start + (int)token) * a.out_stride + head * D + 4u * quad) =
         half4{(_Float16)(o[0] * to), (_Float16)(o[1] * to), (_Float16)(o[2] * to), (_Float16)(o[3] * to)};
 }
@@ -584,7 +570,10 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile<D> * kLeastPart);
         Prompt job;
         job.a = a;
+        job.by_group = Divisor(a.group);
+        job.by_kv_heads = Divisor(a.kv.kv_heads);
         job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / workgroups, most));
+        job.by_splits = Divisor(job.splits);
         job.parts = (float4v *)scratch;
         job.part_sums = (float2 *)((char *)scratch + (size_t)workgroups * job.splits * kRows * D * 4);
         if (job.splits > 1 && (size_t)workgroups * job.splits * kRows * (D * 4 + 8) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)

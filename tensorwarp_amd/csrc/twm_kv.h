@@ -14,4 +14,34 @@ __device__ __forceinline__ size_t kv_chunk(const KvView &kv, uint32_t page, uint
     return (((size_t)page * kv.kv_heads + head) << kv.page_shift) * kv.dim;
 }
 
+// v of this lane and of those before it, added up (by moves within rows of sixteen lanes, then across them)
+__device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)
+{
+#define TWM_ADD_STEP(CONTROL, ROWS) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, ROWS, 0xf, false)
+    TWM_ADD_STEP(0x111, 0xf);   // row_shr:1, 2, 4, 8
+    TWM_ADD_STEP(0x112, 0xf);
+    TWM_ADD_STEP(0x114, 0xf);
+    TWM_ADD_STEP(0x118, 0xf);
+    TWM_ADD_STEP(0x142, 0xa);   // row_bcast:15 to rows 1 and 3, row_bcast:31 to rows 2 and 3
+    TWM_ADD_STEP(0x143, 0xc);
+#undef TWM_ADD_STEP
+    return v;
+}
+
+// Division by a number that a launch knows: n / d for n below 2^31 as (n * factor) >> shift, factor = ceil(2^shift / d) with
+// shift = 31 + ceil(log2 d).  (factor d is less than 2^shift + d, so that n factor / 2^shift is less than n / d + n / 2^shift, and the
+// last term is at most 1 / d.)
+struct Divisor {
+    uint32_t d, factor, shift;
+    explicit __host__ Divisor(uint32_t by) : d(by)
+    {
+        uint32_t log = 0;
+        while ((1ull << log) < by) log++;
+        shift = 31 + log;
+        factor = (uint32_t)(((1ull << shift) + by - 1) / by);
+    }
+    Divisor() = default;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)((uint64_t)n * factor >> shift); }
+};
+
 }  // namespace twm
