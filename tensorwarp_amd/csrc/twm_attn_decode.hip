@@ -15,11 +15,19 @@
 //
 // All tokens of all sequences, in steps of 128, are dealt out evenly among as many workgroups for each key-value head as the chip holds at once,
 // which find their share from the lengths by themselves: a long sequence is cut into many shares, several short ones make one.  What a share
-// holds of a sequence that others hold too goes to scratch, and a second kernel joins it.
+// holds of a sequence that others hold too goes to scratch, and a second kernel joins it.  (Joining by the last workgroup to arrive cost the same
+// 5 us.)  Where no sequence is long, each sequence and unit has a workgroup of more waves to itself and nothing is joined.
+//
+// Bound by the reading of the cache where it is long: 32 sequences of up to 8192 tokens, 28 heads on 4 of 128 f16 values, 60.5 us (4.5 TB/s; a copy
+// reaches 5.1); 48 of up to 4096, 32 heads on 32, e4m3, 155 us (4.9 TB/s); one sequence of 131072 59 us, of 32768 21 (3.2 TB/s: two launches and
+// eight steps a share are what is left), and of 777 tokens, 14 heads of 64 values, 9.2 us, which are the chain from the length by the table and the
+// keys to the sums.
 #include "twm_kv.h"
+#include "twm_slices.h"
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace twm {
 
@@ -32,7 +40,7 @@ typedef int int2v __attribute__((ext_vector_type(2)));
 #define TWM_LDS(T) __attribute__((address_space(3))) T
 
 constexpr uint32_t kDecodeHeads = 16;   // query heads of one unit: columns of a matrix instruction
-constexpr uint32_t kDecodeWaves = 4, kDecodeStep = 32 * kDecodeWaves;
+constexpr uint32_t kDecodeWaves = 4, kDecodeStep = 32 * kDecodeWaves;   // of shares
 constexpr int kNoScore = 0xFF800000;   // -infinity
 
 struct Decode {
@@ -111,63 +119,77 @@ __device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
 // 2^(c (m - m')), of sums that hold something
 __device__ __forceinline__ float shrink(float m, float to, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * c); }
 
-// Workgroups of four waves that share a compute unit, by their registers
+// Workgroups of four waves that share a compute unit, by their registers; waves of a workgroup that has a sequence to itself
 template <int D, bool E4M3> constexpr uint32_t kDecodePerUnit = D == 256 ? (E4M3 ? 2 : 1) : D == 128 ? (E4M3 ? 3 : 2) : 3;
+template <int D, bool E4M3> constexpr uint32_t kDecodeWholeWaves = D == 64 ? 16 : D == 128 || E4M3 ? 8 : 4;
 
 }  // namespace
 
-template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D, E4M3>)) void k_attn_decode(const Decode d)
+// WHOLE: a workgroup has a sequence and unit to itself, sequence first_seq + blockIdx.x / units
+template <int D, bool E4M3, uint32_t WAVES, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, E4M3>)) void k_attn_decode(const Decode d, uint32_t first_seq)
 {
+    constexpr uint32_t THREADS = 64 * WAVES, STEP = 32 * WAVES;
     constexpr uint32_t kRow = D * (E4M3 ? 1 : 2);          // bytes of a token
     constexpr uint32_t kStride = kRow + 32;                // in LDS: four rows that are read at once lie in different banks
     constexpr uint32_t kBuffer = 32 * kStride > kDecodeHeads * D * 4 ? 32 * kStride : kDecodeHeads * D * 4;   // also a wave's results
     constexpr int NK = kRow / 64, NV = 32 * kRow / 1024;   // loads per lane: of each block of 16 keys, of 32 values
     constexpr uint32_t kLanesPerRow = kRow / 16, kRowsPerLoad = 64 / kLanesPerRow;
-    __shared__ __align__(16) char buffers[kDecodeWaves][kBuffer];
+    __shared__ __align__(16) char buffers[WAVES][kBuffer];
     __shared__ half8 queries[D / 32 * 64];
-    __shared__ float tops[kDecodeWaves][kDecodeHeads], sums[kDecodeWaves][kDecodeHeads];
+    __shared__ float tops[WAVES][kDecodeHeads], sums[WAVES][kDecodeHeads];
     const AttnArgs &a = d.a;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, quarter = lane >> 4, col = lane & 15u;
     char *const buffer = buffers[wave];
 
-    const uint32_t unit = d.by_shares(blockIdx.x), share = blockIdx.x - unit * d.shares;
+    const uint32_t pair = d.by_shares(blockIdx.x), unit = WHOLE ? blockIdx.x - pair * d.shares : pair, share = WHOLE ? 0u : blockIdx.x - unit * d.shares;
     const uint32_t kv_head = d.by_tiles(unit), head0 = kv_head * a.group + (unit - kv_head * d.tiles) * kDecodeHeads;
     const uint32_t heads = min(kDecodeHeads, (kv_head + 1) * a.group - head0);
-    // Up to 64 sequences are looked up once
-    Lengths l = lengths_from(d, 0);
-    uint64_t total = l.all;
-    for (uint32_t base = 64; base < a.seqs.seqs; base += 64) total += lengths_from(d, base).all;
-    // rows without tokens: every share clears some
-    for (uint32_t s = share; s < a.seqs.seqs; s += d.shares)
-        if (span_of(d, a.seqs.lengths[s]).steps == 0)
-            for (uint32_t i = threadIdx.x; i < heads * D / 8; i += 256) *(half8_any *)(a.out + (size_t)s * a.out_stride + head0 * D + 8u * i) = half8{};
-    uint64_t at = share_begin(d, total, share);
-    const uint64_t end = share_begin(d, total, share + 1);
-    if (at >= end) return;
-    // the sequence in which the share begins
-    uint64_t before = 0;
-    uint32_t base = 0, seq;
-    for (;;) {
-        const uint64_t past = __ballot(before + l.up_to > at);
-        if (past) {
-            const uint32_t lane_of = (uint32_t)__builtin_ctzll(past);
-            seq = base + lane_of;
-            before += lane_of == 0 ? 0u : (uint32_t)__builtin_amdgcn_readlane(l.up_to, lane_of - 1);
-            break;
+    auto clear = [&](uint32_t s) {   // a row without tokens
+        for (uint32_t i = threadIdx.x; i < heads * D / 8; i += THREADS) *(half8_any *)(a.out + (size_t)s * a.out_stride + head0 * D + 8u * i) = half8{};
+    };
+    Lengths l;
+    uint64_t total = 0, at = 0, end = 1, before = 0;
+    uint32_t base = 0, seq = first_seq + pair;
+    if constexpr (WHOLE) {
+        l.length = a.seqs.lengths[seq];
+        if (span_of(d, l.length).steps == 0) {
+            clear(seq);
+            return;
         }
-        before += l.all;
-        base += 64;
-        l = lengths_from(d, base);
+    } else {
+        // Up to 64 sequences are looked up once
+        l = lengths_from(d, 0);
+        total = l.all;
+        for (uint32_t b = 64; b < a.seqs.seqs; b += 64) total += lengths_from(d, b).all;
+        for (uint32_t s = share; s < a.seqs.seqs; s += d.shares)   // (every share sees to some)
+            if (span_of(d, a.seqs.lengths[s]).steps == 0) clear(s);
+        at = share_begin(d, total, share);
+        end = share_begin(d, total, share + 1);
+        if (at >= end) return;
+        // the sequence in which the share begins
+        for (;;) {
+            const uint64_t past = __ballot(before + l.up_to > at);
+            if (past) {
+                const uint32_t lane_of = (uint32_t)__builtin_ctzll(past);
+                seq = base + lane_of;
+                before += lane_of == 0 ? 0u : (uint32_t)__builtin_amdgcn_readlane(l.up_to, lane_of - 1);
+                break;
+            }
+            before += l.all;
+            base += 64;
+            l = lengths_from(d, base);
+        }
     }
     const uint32_t part = 2 * blockIdx.x;
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
     for (bool first_of_share = true; at < end; first_of_share = false) {
-        if (seq - base >= 64) {
+        if (!WHOLE && seq - base >= 64) {
             base += 64;
             l = lengths_from(d, base);
         }
-        const Span span = span_of(d, __builtin_amdgcn_readlane(l.length, seq - base));
-        if (span.steps == 0) {
+        const Span span = span_of(d, WHOLE ? l.length : __builtin_amdgcn_readlane(l.length, seq - base));
+        if (!WHOLE && span.steps == 0) {
             seq++;
             continue;
         }
@@ -176,7 +198,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
         const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
 
         // Q^T: a lane's head's values, in the order in which it holds keys
-        for (uint32_t x = threadIdx.x; x < D / 32 * 64; x += 256) {
+        for (uint32_t x = threadIdx.x; x < D / 32 * 64; x += THREADS) {
             const uint32_t i = x >> 6, head = min(x & 15u, heads - 1), g = x >> 4 & 3u;
             queries[x] = *(const half8_any *)(a.q + (size_t)seq * a.q_stride + (head0 + head) * D + (E4M3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8));
         }
@@ -186,12 +208,19 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
 #pragma unroll
         for (int i = 0; i < D / 16; i++) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
 
-        const TWM_CONSTANT int *table = (const TWM_CONSTANT int *)(a.seqs.tables + (size_t)seq * a.seqs.table_stride);
+        // Pages of this wave's tokens, 32 a step: a lane looks one of a step's halves up, the wave those of 32 steps at once
+        const int *table = a.seqs.tables + (size_t)seq * a.seqs.table_stride;
         const char *const k_base = (const char *)a.kv.k, *const v_base = (const char *)a.kv.v;
-        int page0, page1;   // of this wave's next 32 tokens' halves
+        int page_of = -1, page0 = -1, page1 = -1;
+        uint32_t looked_up = 0;
         auto pages_of = [&](int t) {
-            page0 = table[(uint32_t)t >> a.kv.page_shift];
-            page1 = t + 16 < span.hi ? table[(uint32_t)(t + 16) >> a.kv.page_shift] : -1;
+            if ((looked_up & 31u) == 0) {
+                const int64_t token = t + (int64_t)(lane >> 1) * (int)STEP + (int)(lane & 1u) * 16;
+                page_of = token < span.hi ? table[(uint32_t)token >> a.kv.page_shift] : -1;
+            }
+            page0 = __builtin_amdgcn_readlane(page_of, 2 * (looked_up & 31u));
+            page1 = __builtin_amdgcn_readlane(page_of, 2 * (looked_up & 31u) + 1);
+            looked_up++;
         };
         uint4v k[2][NK], v[NV];
         bool k_there = false;   // whether both pages are inside the pool
@@ -214,14 +243,14 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
                 v[i] = *(const uint4v *)(v_base + (row < 16 ? bytes0 + row * kRow : bytes1 + (row - 16) * kRow) + v_off);
             }
         };
-        const int stop = min(span.hi, span.first + (int)(step1 * kDecodeStep));
-        int t = span.first + (int)(step0 * kDecodeStep + wave * 32u);
+        const int stop = WHOLE ? span.hi : min(span.hi, span.first + (int)(step1 * STEP));
+        int t = span.first + (int)(step0 * STEP + wave * 32u);
         if (t < stop) {
             pages_of(t);
             load(t);
         }
         __syncthreads();
-        for (; t < stop; t += (int)kDecodeStep) {
+        for (; t < stop; t += (int)STEP) {
             const bool whole = k_there && t >= span.lo && t + 32 <= span.hi;
             const bool in0 = (uint32_t)page0 < a.kv.pages, in1 = (uint32_t)page1 < a.kv.pages;
             // values to LDS; what is not seen is zeros there, whatever it may be in memory
@@ -249,7 +278,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
                     s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, queries[i * 64 + lane], s[b], 0, 0, 0);
                 }
             }
-            const int next = t + (int)kDecodeStep;
+            const int next = t + (int)STEP;
             if (next < stop) {
                 pages_of(next);
                 load(next);
@@ -317,23 +346,23 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
         __syncthreads();
         float most = top;
 #pragma unroll
-        for (uint32_t w = 0; w < kDecodeWaves; w++) most = fmaxf(most, tops[w][col]);
+        for (uint32_t w = 0; w < WAVES; w++) most = fmaxf(most, tops[w][col]);
         const float by = shrink(top, most, c);
 #pragma unroll
         for (int i = 0; i < D / 16; i++) *(float4v *)(buffer + (col * D + 16 * i + 4 * quarter) * 4) = o[i] * by;
         __syncthreads();
-        const bool all = step0 == 0 && step1 == span.steps;
+        const bool all = WHOLE || (step0 == 0 && step1 == span.steps);
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
-        for (uint32_t i = threadIdx.x; i < heads * (D / 4); i += 256) {
+        for (uint32_t i = threadIdx.x; i < heads * (D / 4); i += THREADS) {
             const uint32_t h = i / (D / 4), x = i % (D / 4) * 4;
             float4v r = *(const float4v *)(buffers[0] + (h * D + x) * 4);
 #pragma unroll
-            for (uint32_t w = 1; w < kDecodeWaves; w++) r += *(const float4v *)(buffers[w] + (h * D + x) * 4);
+            for (uint32_t w = 1; w < WAVES; w++) r += *(const float4v *)(buffers[w] + (h * D + x) * 4);
             float m = tops[0][h], l = 0.f;
 #pragma unroll
-            for (uint32_t w = 1; w < kDecodeWaves; w++) m = fmaxf(m, tops[w][h]);
+            for (uint32_t w = 1; w < WAVES; w++) m = fmaxf(m, tops[w][h]);
 #pragma unroll
-            for (uint32_t w = 0; w < kDecodeWaves; w++) l += sums[w][h] * shrink(tops[w][h], m, c);
+            for (uint32_t w = 0; w < WAVES; w++) l += sums[w][h] * shrink(tops[w][h], m, c);
             if (all) {
                 const float to = l == 0.f ? 0.f : v_scale / l;
                 *(half4_any *)(a.out + (size_t)seq * a.out_stride + (head0 + h) * D + x) =
@@ -345,6 +374,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
                 if (x == 0) d.part_sums[slot] = float2{m, l};
             }
         }
+        if (WHOLE) return;
         __syncthreads();   // (the buffers are the waves' own again)
         at += step1 - step0;
         before += span.steps;
@@ -352,12 +382,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (kDecodePerUnit<D,
     }
 }
 
-// Joins what several shares hold of a unit: a workgroup per query head and sequence.  D / 4 lanes hold a part, 2048 / D of them at a time, four
+// Joins what several shares hold of a unit: a workgroup per query head and sequence.  D / 4 lanes hold a part, as many at a time as THREADS do, four
 // on their way.
-constexpr uint32_t kJoinThreads = 512;
-template <int D> __global__ __launch_bounds__(kJoinThreads) void k_attn_join(const Decode d)
+template <int D, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void k_attn_join(const Decode d)
 {
-    constexpr uint32_t kLanes = D / 4, kAtOnce = kJoinThreads / kLanes, kAhead = 4;
+    constexpr uint32_t kLanes = D / 4, kAtOnce = THREADS / kLanes, kAhead = 4;
     __shared__ float4v results[kAtOnce][kLanes];
     __shared__ float2 sums[kAtOnce];
     const AttnArgs &a = d.a;
@@ -427,31 +456,46 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
     d.tiles = (a.group + kDecodeHeads - 1) / kDecodeHeads;
     d.units = a.kv.kv_heads * d.tiles;
     d.heads = std::min(a.group, kDecodeHeads);
-    const uint32_t per_unit = a.kv.dim == 64    ? kDecodePerUnit<64, false>
-                              : a.kv.dim == 128 ? (a.kv.e4m3 ? kDecodePerUnit<128, true> : kDecodePerUnit<128, false>)
-                                                : (a.kv.e4m3 ? kDecodePerUnit<256, true> : kDecodePerUnit<256, false>);
-    // as many workgroups as the chip holds at once, or as there may be steps
-    const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
-    const uint64_t most_steps = (std::min(capacity, a.window ? (uint64_t)a.window + 31 : capacity) + kDecodeStep - 1) / kDecodeStep;
-    d.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 * per_unit / d.units, most_steps * a.seqs.seqs));
-    d.by_shares = Divisor(d.shares);
     d.by_tiles = Divisor(d.tiles);
     d.by_group = Divisor(a.group);
-    const size_t slots = 2 * (size_t)d.shares * d.units * d.heads;
-    d.part_sums = (float2 *)scratch;
-    d.parts = (float *)((char *)scratch + (slots * sizeof(float2) + 255) / 256 * 256);
-    if ((size_t)((char *)(d.parts + slots * a.kv.dim) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 25 MB of 256)
-    auto kernels = [&](auto dim) {
+    const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift, seen = std::min(capacity, a.window ? (uint64_t)a.window + 31 : capacity);
+    auto launch = [&](auto dim, auto e4m3) {
         constexpr int D = decltype(dim)::value;
-        hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_decode<D, true> : k_attn_decode<D, false>), dim3(d.shares * d.units), dim3(256), 0, s, d);
-        hipError_t error = hipGetLastError();
-        if (error != hipSuccess || most_steps <= 1) return error;   // (a step is never cut)
-        hipLaunchKernelGGL(k_attn_join<D>, dim3(a.seqs.seqs, a.q_heads), dim3(kJoinThreads), 0, s, d);
+        constexpr bool E4M3 = decltype(e4m3)::value;
+        constexpr uint32_t WHOLE_WAVES = kDecodeWholeWaves<D, E4M3>;
+        // No shares, and nothing to join, where no sequence is long, by as much more as there are many.  28 heads on 4 of 128 values, up to 512 tokens:
+        // one sequence 9.8 us, 10.8 in shares; 32 sequences 11.1 and 17.4; 200 sequences 34 and 38.  Up to 2048, 200 sequences 91 and 97, but up to
+        // 4096 166 either way, and one of 1024 tokens, four steps of its eight waves, takes 14.4 and 10.6 in shares.
+        if (seen <= std::min<uint64_t>(16, 2 + (uint64_t)a.seqs.seqs * d.units / 64) * (32 * WHOLE_WAVES)) {
+            d.shares = d.units;
+            d.by_shares = Divisor(d.units);
+            return in_slices(a.seqs.seqs, most_workgroups(64 * WHOLE_WAVES) / d.units, [&](uint32_t seq, uint32_t here) {
+                hipLaunchKernelGGL((k_attn_decode<D, E4M3, WHOLE_WAVES, true>), dim3(here * d.units), dim3(64 * WHOLE_WAVES), 0, s, d, seq);
+                return hipGetLastError();
+            });
+        }
+        // as many workgroups as the chip holds at once, or as there may be steps
+        const uint64_t most_steps = (seen + kDecodeStep - 1) / kDecodeStep * a.seqs.seqs;
+        d.shares = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 * kDecodePerUnit<D, E4M3> / d.units, most_steps));
+        d.by_shares = Divisor(d.shares);
+        const size_t slots = 2 * (size_t)d.shares * d.units * d.heads;
+        d.part_sums = (float2 *)scratch;
+        d.parts = (float *)((char *)scratch + (slots * sizeof(float2) + 255) / 256 * 256);
+        if ((size_t)((char *)(d.parts + slots * D) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
+        hipLaunchKernelGGL((k_attn_decode<D, E4M3, kDecodeWaves, false>), dim3(d.shares * d.units), dim3(64 * kDecodeWaves), 0, s, d, 0u);
+        if (const hipError_t error = hipGetLastError(); error != hipSuccess) return error;
+        // sixteen parts of 128 values at once for few sequences, which have many, four otherwise (32 sequences up to 1024 tokens 20.7 us with
+        // sixteen, 18.9 with four; one of 32768 21.3 and 25.3)
+        if (a.seqs.seqs < 8)
+            hipLaunchKernelGGL((k_attn_join<D, 512>), dim3(a.seqs.seqs, a.q_heads), dim3(512), 0, s, d);
+        else
+            hipLaunchKernelGGL((k_attn_join<D, 128>), dim3(a.seqs.seqs, a.q_heads), dim3(128), 0, s, d);
         return hipGetLastError();
     };
-    return a.kv.dim == 64    ? kernels(std::integral_constant<int, 64>{})
-           : a.kv.dim == 128 ? kernels(std::integral_constant<int, 128>{})
-                             : kernels(std::integral_constant<int, 256>{});
+    auto of_type = [&](auto dim) { return a.kv.e4m3 ? launch(dim, std::true_type{}) : launch(dim, std::false_type{}); };
+    return a.kv.dim == 64    ? of_type(std::integral_constant<int, 64>{})
+           : a.kv.dim == 128 ? of_type(std::integral_constant<int, 128>{})
+                             : of_type(std::integral_constant<int, 256>{});
 }
 
 }  // namespace twm
