@@ -87,16 +87,20 @@ class Pool:
 
     def tokens(self, name, row, count):
         """[kv_heads, count, dim] of a table's row; absent pages are NaN."""
-        values, pages = self.values(name), self.shape[0]
         out = np.full((self.shape[1], count, self.shape[3]), np.nan)
-        for t in range(count):
-            page = row[t // self.page] if t // self.page < len(row) else -1
-            if 0 <= page < pages:
-                out[:, t] = values[page, :, t % self.page]
+        at = np.flatnonzero(self.present(row, count))
+        places = np.asarray(row)[at // self.page], slice(None), at % self.page
+        bits = self.bits[name][places]
+        values = bits.view(np.float16).astype(np.float64) if self.cache == "f16" else E4M3[bits]
+        if self.scales[name] is not None:
+            values = values * self.scales[name].astype(np.float64)[:, None]
+        out[:, at] = values.transpose(1, 0, 2)
         return out
 
     def present(self, row, count):
-        return np.array([t // self.page < len(row) and 0 <= row[t // self.page] < self.shape[0] for t in range(count)], bool)
+        at = np.arange(count) // self.page
+        pages = np.concatenate([np.asarray(row, np.int64), [-1]])[np.minimum(at, len(row))]
+        return (pages >= 0) & (pages < self.shape[0])
 
     def upload(self, dev):
         self.dev = {name: T.GpuTensor.from_host(dev, self.bits[name], "f16" if self.cache == "f16" else "u8") for name in "kv"}
