@@ -61,7 +61,10 @@ def kv_layers(caches):
 
 def kv_copy_pages(device, layers, sources, targets):
     """Page sources[i] to page targets[i] in every layer (kv_layers())."""
-    sources, targets = np.ascontiguousarray(sources, np.uint32), np.ascontiguousarray(targets, np.uint32)
+    sources, targets = np.asarray(sources, np.int64), np.asarray(targets, np.int64)
     if sources.shape != targets.shape or sources.ndim != 1:
         raise ValueError("kv_copy_pages: as many targets as sources")
+    if sources.size and (min(sources.min(), targets.min()) < 0 or max(sources.max(), targets.max()) > 0xFFFFFFFF):
+        raise ValueError("kv_copy_pages: a page's number is outside the pool")
+    sources, targets = sources.astype(np.uint32), targets.astype(np.uint32)
     _check(device._l.twm_kv_copy_pages(device.handle, layers, len(layers), sources.ctypes.data, targets.ctypes.data, sources.size))

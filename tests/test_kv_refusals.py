@@ -2,8 +2,10 @@
 is nothing but zeros will do."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
+import tensorwarp_amd as T
 from tensorwarp_amd import _lib
 
 A, B = 0x1000, 0x2000   # addresses that are never read: every call here is refused, or has nothing to do
@@ -136,3 +138,12 @@ def test_copies(ctx):
     refused(copy(ctx, caches=[cache(), cache(k_dev=None)]), _lib.INVALID_HANDLE, b"null pointer")
     refused(copy(ctx, count=(1 << 20) + 1), _lib.SHAPE_ERROR, b"beyond 2^20")
     assert copy(ctx, sources=(), targets=()) == _lib.OK and copy(ctx, caches=[]) == _lib.OK
+
+
+@pytest.mark.parametrize("page", [-1, 1 << 32, -(1 << 32), 1 << 40])
+def test_page_numbers_that_32_bits_do_not_hold(page):
+    # (refused before anything is asked of a device)
+    layers = T.kv_layers([])
+    for sources, targets in (([page], [1]), ([1], [page]), (np.array([0, page]), np.array([1, 2]))):
+        with pytest.raises(ValueError, match="outside the pool"):
+            T.kv_copy_pages(None, layers, sources, targets)
