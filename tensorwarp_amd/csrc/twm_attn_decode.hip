@@ -62,7 +62,7 @@ __device__ __forceinline__ Span span_of(const Decode &d, int length)
 {
     Span s;
     s.hi = min(length, (int)(d.a.seqs.table_stride << d.a.kv.page_shift));
-    s.lo = d.a.window ? max(0, length - (int)d.a.window) : 0;
+    s.lo = d.a.window ? max(0, max(length, 0) - (int)d.a.window) : 0;
     s.first = s.lo & ~31;
     s.steps = s.hi > s.lo && d.a.kv.pages ? (uint32_t)(s.hi - s.first + (int)kDecodeStep - 1) / kDecodeStep : 0u;
     return s;
@@ -464,9 +464,11 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
         constexpr bool E4M3 = decltype(e4m3)::value;
         constexpr uint32_t WHOLE_WAVES = kDecodeWholeWaves<D, E4M3>;
         // No shares, and nothing to join, where no sequence is long, by as much more as there are many.  28 heads on 4 of 128 values, up to 512 tokens:
-        // one sequence 9.8 us, 10.8 in shares; 32 sequences 11.1 and 17.4; 200 sequences 34 and 38.  Up to 2048, 200 sequences 91 and 97, but up to
-        // 4096 166 either way, and one of 1024 tokens, four steps of its eight waves, takes 14.4 and 10.6 in shares.
-        if (seen <= std::min<uint64_t>(16, 2 + (uint64_t)a.seqs.seqs * d.units / 64) * (32 * WHOLE_WAVES)) {
+        // one sequence 9.8 us, 10.8 in shares; 32 sequences 11.1 and 17.4; 200 sequences 34 and 38.  Up to 2048, 200 sequences 91 and 97; but up to
+        // 4096 166 either way, 48 of 32 heads in e4m3 160 and 155, and one of 1024 tokens, four steps of its eight waves, 14.4 and 10.6.  And none among
+        // so many sequences that each share's way through their lengths costs more than a long one's wait: 1024 up to 512 tokens 154 us, 188 in
+        // shares, up to 8192 1433 and 1495, 16384 up to 64 (7 heads on one) 342 and 2384.
+        if (seen <= std::min<uint64_t>(8, 2 + (uint64_t)a.seqs.seqs * d.units / 64) * (32 * WHOLE_WAVES) || a.seqs.seqs >= 1024) {
             d.shares = d.units;
             d.by_shares = Divisor(d.units);
             return in_slices(a.seqs.seqs, most_workgroups(64 * WHOLE_WAVES) / d.units, [&](uint32_t seq, uint32_t here) {

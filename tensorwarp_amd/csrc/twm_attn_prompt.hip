@@ -69,7 +69,7 @@ struct Prompt {
     AttnArgs a;
     float4v *parts;       // [workgroups][dim / 4][rows of a workgroup], for rows that several workgroups share the tokens of
     float2 *part_sums;    // [workgroups][rows]: reference, sum of weights
-    uint32_t splits, first_tile;   // splits: the most workgroups that share a tile of rows
+    uint32_t tiles, splits, first_tile;   // splits: the most workgroups that share a tile of rows
     Divisor by_group, by_kv_heads, by_splits;
 };
 
@@ -78,52 +78,42 @@ struct Rows {
     uint32_t seq, row0, rows;
     int start, before, first, last;   // the sequence's first row and its position; tokens that any of the workgroup's rows sees: first .. last - 1
 };
-__device__ __forceinline__ int prompt_begin(const AttnArgs &a, int position) { return a.window ? max(0, position + 1 - (int)a.window) : 0; }
+__device__ __forceinline__ int prompt_begin(const AttnArgs &a, int position) { return a.window ? max(0, max(position, -1) + 1 - (int)a.window) : 0; }
 
-// A sequence, as a lane looks it up
-struct Sequence {
-    int start, end, length;
-};
-__device__ __forceinline__ Sequence sequence_at(const AttnArgs &a, uint32_t s)
-{
-    Sequence q{0, 0, 0};
-    if (s < a.seqs.seqs) q = Sequence{a.seqs.starts[s], a.seqs.starts[s + 1], a.seqs.lengths[s]};
-    return q;
-}
-// Workgroups of one key-value head that a sequence's rows take, EACH of them one
-template <uint32_t EACH> __device__ __forceinline__ uint32_t prompt_tiles(const AttnArgs &a, const Sequence &q)
-{
-    const int first = max(q.start, 0), end = min(q.end, (int)a.rows);
-    return end > first ? ((uint32_t)(end - first) * a.group + EACH - 1) / EACH : 0u;
-}
-// Tile `back` from the end; false: there is none.  (Up to 64 sequences are looked up once.)
+// What a sequence takes of the tiles: those of EACH rows that its rows make begin at tile start * group / EACH + s, which leaves each sequence as
+// many as it has, or one more, and needs no sum over those before it.  Tile `back` from the end: its sequence is the last one that begins at or before
+// it, found among 64 at once; false: nothing is there.
 template <uint32_t EACH> __device__ __forceinline__ bool find_rows(const Prompt &job, uint32_t back, Rows *r)
 {
     const AttnArgs &a = job.a;
-    const uint32_t lane = threadIdx.x & 63u;
-    Sequence q = sequence_at(a, lane);
-    uint32_t up_to = wave_sum_up_to(prompt_tiles<EACH>(a, q)), total = __builtin_amdgcn_readlane(up_to, 63);
-    for (uint32_t base = 64; base < a.seqs.seqs; base += 64) total += __builtin_amdgcn_readlane(wave_sum_up_to(prompt_tiles<EACH>(a, sequence_at(a, base + lane))), 63);
-    if (back >= total) return false;
-    const uint32_t at = total - 1 - back;
-    uint32_t sum = 0, base = 0;
-    uint64_t past;
-    while ((past = __ballot(sum + up_to > at)) == 0) {
-        sum += __builtin_amdgcn_readlane(up_to, 63);
-        base += 64;
-        if (base >= a.seqs.seqs) return false;   // (starts that fall)
-        q = sequence_at(a, base + lane);
-        up_to = wave_sum_up_to(prompt_tiles<EACH>(a, q));
+    const uint32_t lane = threadIdx.x & 63u, at = job.tiles - 1 - back;
+    auto rows_before = [&](int start) { return (uint32_t)min(max(start, 0), (int)a.rows) * a.group; };
+    uint32_t base = 0, among = a.seqs.seqs;
+    int end_of, length_of;
+    for (;;) {
+        const uint32_t stride = (among + 63u) / 64u, s = base + min(lane * stride, among - 1);
+        const int start = a.seqs.starts[s], end = a.seqs.starts[s + 1], length = a.seqs.lengths[s];
+        asm volatile("" : : "v"(start), "v"(end), "v"(length));   // (three loads on their way, not one after the other)
+        const uint32_t tiles_before = rows_before(start) / EACH + s;
+        const uint64_t begun = __ballot(lane * stride < among && tiles_before <= at);
+        if (begun == 0) return false;
+        const uint32_t found = 63u - (uint32_t)__builtin_clzll(begun);
+        base += found * stride;
+        among = min(stride, among - found * stride);
+        if (stride == 1) {
+            r->start = max(__builtin_amdgcn_readlane(start, found), 0);
+            r->row0 = (at - (uint32_t)__builtin_amdgcn_readlane(tiles_before, found)) * EACH;
+            end_of = __builtin_amdgcn_readlane(end, found);
+            length_of = max(__builtin_amdgcn_readlane(length, found), 0);
+            break;
+        }
     }
-    const uint32_t found = (uint32_t)__builtin_ctzll(past);
-    r->seq = base + found;
-    r->row0 = (at - sum - (found == 0 ? 0u : (uint32_t)__builtin_amdgcn_readlane(up_to, found - 1))) * EACH;
-    const int end = __builtin_amdgcn_readlane(q.end, found), length = max(__builtin_amdgcn_readlane(q.length, found), 0);
-    r->start = max(__builtin_amdgcn_readlane(q.start, found), 0);
-    const int tokens = min(end, (int)a.rows) - r->start;
+    r->seq = base;
+    const int tokens = min(end_of, (int)a.rows) - r->start;
     if (tokens <= 0) return false;
     r->rows = (uint32_t)tokens * a.group;
-    r->before = length - (end - r->start);
+    if (r->row0 >= r->rows) return false;
+    r->before = length_of - (end_of - r->start);
     r->first = prompt_begin(a, r->before + (int)job.by_group(r->row0));
     r->last = min(r->before + (int)job.by_group(min(r->row0 + EACH, r->rows) - 1) + 1, a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0);
     return true;
@@ -177,8 +167,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     const int low = before + (int)job.by_group(row0), high = before + (int)job.by_group(min(row0 + kRows, rows) - 1);
     const int wave_low = __builtin_amdgcn_readfirstlane(my_position), wave_high = __builtin_amdgcn_readlane(my_position, 31);
     // the tokens that anyone sees, or this part of them
-    const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * key_tiles / parts) * KT);
-    const int last = min(mine.last, all_begin + (int)((split + 1) * key_tiles / parts) * KT);
+    const uint32_t each_part = key_tiles / parts, one_more = key_tiles - each_part * parts;
+    const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * each_part + min(split, one_more)) * KT);
+    const int last = min(mine.last, all_begin + (int)((split + 1) * each_part + min(split + 1, one_more)) * KT);
 
     half8 q[kHalf / 16];
     {
@@ -564,12 +555,13 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         constexpr int D = decltype(dim)::value;
         constexpr uint32_t kRows = kPromptRows<D>;
         // every sequence begins a tile of its own
-        const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + std::min(a.seqs.seqs, a.rows), workgroups = tiles * a.kv.kv_heads;
+        const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + a.seqs.seqs, workgroups = tiles * a.kv.kv_heads;
         // Tokens are shared out where rows alone leave most of the chip without work (two workgroups a compute unit), as far as there may be some
         const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
         const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile<D> * kLeastPart);
         Prompt job;
         job.a = a;
+        job.tiles = (uint32_t)tiles;
         job.by_group = Divisor(a.group);
         job.by_kv_heads = Divisor(a.kv.kv_heads);
         job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / workgroups, most));

@@ -60,25 +60,26 @@ __device__ __forceinline__ uint2v codes_8(const float (&v)[8], float scale)
 }  // namespace
 
 // A workgroup per row.  A thread holds sixteen values of one head: the two runs of eight that a rotation of halves turns into each other,
-// or sixteen neighbours.  The row's sequence is the number of starts up to it, counted by all threads at once, while its values are on
-// their way.
+// or sixteen neighbours.  The row's sequence is the last one that starts up to it, found among as many at once as there are threads.
 template <bool F16> __global__ void k_kv_append(const Append a)
 {
     const uint32_t row = blockIdx.x, dim = a.kv.dim, each = dim >> 4, units = (a.q_heads + 2u * a.kv.kv_heads) * each;
     int seq = (int)row, behind = 0;   // behind: the rows of the sequence from this one on
     if (a.seqs.starts) {
-        int before = 0;
-        for (uint32_t base = 0; base < a.seqs.seqs; base += blockDim.x) {
-            const uint32_t s = base + threadIdx.x;
-            before += __syncthreads_count(s < a.seqs.seqs && a.seqs.starts[s] <= (int)row);
+        uint32_t base = 0, among = a.seqs.seqs;
+        for (uint32_t stride = 0; stride != 1; among = min(stride, a.seqs.seqs - base)) {
+            stride = (among + blockDim.x - 1) / blockDim.x;
+            const uint32_t s = threadIdx.x * stride;
+            const uint32_t begun = (uint32_t)__syncthreads_count(s < among && a.seqs.starts[base + s] <= (int)row);
+            if (begun == 0) return;
+            base += (begun - 1) * stride;
         }
-        if (before == 0) return;
-        seq = before - 1;
+        seq = (int)base;
         behind = a.seqs.starts[seq + 1] - (int)row;
     } else {
         behind = 1;
     }
-    const int position = a.seqs.lengths[seq] - behind;
+    const int position = max(a.seqs.lengths[seq], 0) - behind;
     if (behind <= 0 || position < 0) return;
     const uint32_t in_table = (uint32_t)position >> a.kv.page_shift;
     const int page = in_table < a.seqs.table_stride ? a.seqs.tables[(size_t)seq * a.seqs.table_stride + in_table] : -1;

@@ -62,7 +62,7 @@ def test_decode_of_many_sequences(dev, seqs, longest, wide):
 
 
 @pytest.mark.parametrize("dim", [64, 256])
-@pytest.mark.parametrize("seqs,most,behind", [(64, 4, 30), (65, 4, 30), (300, 3, 100), (1100, 2, 5), (130, 40, 0)])
+@pytest.mark.parametrize("seqs,most,behind", [(64, 4, 30), (4097, 1, 3), (65, 4, 30), (300, 3, 100), (1100, 2, 5), (130, 40, 0)])
 def test_prompts_of_many_sequences(dev, seqs, most, behind, dim):
     rng = np.random.default_rng(seqs)
     new = list(rng.integers(0, most + 1, seqs))
@@ -112,6 +112,23 @@ def test_thousands_of_rows_against_their_single_tokens(dev, dim, heads, kv, cach
     # the first rows see few tokens, where a bound is as good as the sums
     want, exact_tol, _ = attend_rows(pool, table, [70], [70], q[:70], dim ** -0.5, window, PROMPT_STEP)
     check(a.get()[:70], want, exact_tol)
+
+
+def test_all_rows_in_the_last_of_many_sequences(dev):
+    new = [0] * 4100 + [70] + [0] * 200
+    lengths = [0] * 4100 + [90] + [7] * 200
+    pool = Pool(np.random.default_rng(7), 300, 2, 16, 64)
+    run_prompt(dev, pool, pool.fill(lengths), lengths, new, 4, first=3, spare=2)
+
+
+@pytest.mark.parametrize("least", [-1, -(1 << 31)])
+def test_lengths_below_zero(dev, least):
+    pool = Pool(np.random.default_rng(8), 10, 2, 16, 64)
+    table = pool.fill([40, 0, 0])
+    lengths = [40, least, least]
+    for window in (0, 1, 30, 0xFFFFFFFF):
+        run_decode(dev, pool, table, lengths, 4, window=window)
+        run_prompt(dev, pool, table, lengths, [20, 0, 3], 4, window=window)
 
 
 class Large:

@@ -156,6 +156,23 @@ def test_many_sequences(dev):
     run_append(dev, pool, pool.fill(lengths), lengths, new, 1, "f32")
 
 
+def test_thousands_of_sequences(dev):
+    # more than the square of a workgroup's threads would hold in one look, and rows of one among empty ones
+    rng = np.random.default_rng(9)
+    new = list(rng.integers(0, 2, 5000))
+    lengths = [n + int(rng.integers(0, 3)) for n in new]
+    pool = Pool(rng, sum(-(-n // 16) for n in lengths) + 1, 1, 16, 64)
+    run_append(dev, pool, pool.fill(lengths), lengths, new, 1, "f32")
+    new, lengths = [0] * 4500 + [30] + [0] * 77, [0] * 4500 + [50] + [2] * 77
+    run_append(dev, pool := Pool(rng, 90, 1, 16, 64), pool.fill(lengths), lengths, new, 1)
+
+
+@pytest.mark.parametrize("least", [-1, -(1 << 31)])
+def test_rows_of_lengths_below_zero_are_not_stored(dev, least):
+    pool = Pool(np.random.default_rng(10), 8, 2, 16, 64)
+    run_append(dev, pool, pool.fill([20, 0, 0]), [20, least, least], [5, 2, 1], 4)
+
+
 def test_values_beyond_f16_and_e4m3(dev):
     for cache in ("f16", "e4m3"):
         pool = Pool(np.random.default_rng(8), 4, 1, 16, 64, cache, scales=False)
