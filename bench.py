@@ -180,6 +180,63 @@ def trace_decode(T, dev, layers):
         print("%s: %.1f MB in a span of %.2f us = %.2f TB/s inside the kernel" % (name, algo_bytes(k, n) / 1e6, m[7], algo_bytes(k, n) / m[7] / 1e6))
 
 
+def attention_layers(T, dev, layers, capture, graphs_done, reps, log):
+    """The layer's four projections with what stands between the first two of them: rows into a paged key-value cache
+    (28 query heads on 4 of 128 values, f16, pages of 16 tokens, a cache per layer), and one new token's attention per sequence, whose rows the
+    second projection takes.  And a prompt's rows into the same cache with their attention, without projections."""
+    heads, kv, dim, page = 28, 4, 128, 16
+    rng, out = np.random.default_rng(7), {}
+    half = dim // 2
+    for seqs, tokens, prompt in ((1, 512, False), (1, 4096, False), (1, 32768, False), (16, 2048, False), (1, 2048, True), (1, 8192, True)):
+        label = "prompt_%d" % tokens if prompt else "M%d_context_%d" % (seqs, tokens)
+        log("attention: " + label)
+        per_seq = -(-tokens // page)
+        angle = np.arange(tokens)[:, None] * 1e6 ** (-np.arange(half) / half)
+        cos_sin = T.GpuTensor.from_host(dev, np.concatenate([np.cos(angle), np.sin(angle)], axis=1).astype(np.float32))
+        table = rng.permutation(seqs * per_seq).astype(np.int32).reshape(seqs, per_seq)
+        rows = tokens if prompt else seqs
+        seqs_dev = T.KvSequences(T.GpuTensor.from_host(dev, table), T.GpuTensor.from_host(dev, np.full(seqs, tokens, np.int32)), seqs, per_seq,
+                                 starts=T.GpuTensor.from_host(dev, np.array([0, rows], np.int32)) if prompt else None)
+        values = rng.standard_normal((seqs * per_seq, kv, page, dim), dtype=np.float32).astype(np.float16)
+        caches = [T.KvCache(T.GpuTensor.from_host(dev, values), T.GpuTensor.from_host(dev, values), page, kv, dim) for _ in range(1 if prompt else len(layers))]
+        bufs = {name: (T.GpuTensor.from_host(dev, rng.standard_normal((rows, k), dtype=np.float32).astype(np.float16)),
+                       T.GpuTensor.zeros(dev, (rows, n), "f32")) for name, k, n in LAYER_7B if not prompt or name == "o"}
+        qkv = T.GpuTensor.from_host(dev, rng.standard_normal((rows, (heads + 2 * kv) * dim), dtype=np.float32)) if prompt else bufs["qkv"][1]
+        q, attended = T.GpuTensor.zeros(dev, (rows, heads * dim), "f16"), bufs["o"][0]
+
+        def between(cache):
+            T.kv_append(dev, cache, seqs_dev, qkv, rows, heads, q, cos_sin=cos_sin, positions=tokens, rotary_dim=dim)
+            if prompt:
+                T.attention_prompt(dev, cache, seqs_dev, q, rows, heads, attended)
+            else:
+                T.attention_decode(dev, cache, seqs_dev, q, heads, attended)
+
+        def attention_only():
+            for cache in caches:
+                between(cache)
+
+        def whole():
+            for layer, cache in zip(layers, caches):
+                for name, _k, _n in LAYER_7B:
+                    T.gemm(dev, layer[name][0], bufs[name][0], rows, bufs[name][1])
+                    if name == "qkv":
+                        between(cache)
+        figures = {}
+        for key, fn in (("us_append_and_attention", attention_only),) + (() if prompt else (("us_layer", whole),)):
+            fn()
+            dev.synchronize()
+            graph = capture(fn)
+            figures[key] = round(time_launches(dev, lambda i: graph.replay(), reps) / len(caches) * 1e3, 2)
+            graphs_done.append(graph)
+        read = 2 * seqs * tokens * kv * dim * 2
+        if prompt:
+            figures["attention_TFLOPs"] = round(4 * heads * dim * tokens * (tokens + 1) / 2 / figures["us_append_and_attention"] / 1e6, 1)
+        else:
+            figures["cache_GBps"] = round(read / figures["us_append_and_attention"] / 1e3, 1)
+        out[label] = figures
+    return out
+
+
 def mfma_mix(dev):
     """FP16 matrix throughput under the instruction mixes of a W4A16 prefill block (twm_debug_mfma_mix): the ceilings
     the prefill kernel's arrangement was chosen against.  Median of five timed launches per line."""
@@ -307,6 +364,8 @@ def main():
     ap.add_argument("--sweep-models", action="store_true",
                     help="also time the projections of other model sizes (Llama-3-8B, 13B, 70B, Qwen-1.5B shapes) at "
                          "M = 1, 4, 8, 16 with the library's plan against the 64-column / streaming kernels alone")
+    ap.add_argument("--attention", action="store_true",
+                    help="also time the decode layer with a paged key-value cache and attention between its projections, and prompts' attention")
     ap.add_argument("--pmc-copy", action="store_true",
                     help="also run four 64 MiB device-to-device copies: a kernel of known traffic to scale rocprofv3 "
                          "FETCH_SIZE / WRITE_SIZE readings by")
@@ -552,6 +611,10 @@ def main():
             lb = sum(algo_bytes(k, n, m) for _, k, n in LAYER_7B)
             extra["layer_M%d" % m] = {"us": round(ms * 1e3, 2), "GBps": round(lb / (ms * 1e-3) / 1e9, 1),
                                       "frac_hbm": round(lb / (ms * 1e-3) / 1e9 / HBM_PEAK_GBS, 4)}
+
+    attention = None
+    if args.attention:
+        attention = attention_layers(T, dev, layers, capture, graphs_done, max(4, steps // L // 4), log)
 
     # the same layer once more with measured plans: twm_weight_tune times the launch forms per weight and row count and
     # keeps what beats the planners' choice by more than 2 % (the role of the reference's autotune table)
@@ -1028,6 +1091,8 @@ def main():
                                    "all_m2048_shapes": {key: v["frac_mfma_f16_peak"] for key, v in m2048.items()}}
     if extra:
         out["batched_decode"] = extra
+    if attention is not None:
+        out["layer_with_attention"] = attention
     if tuned is not None:
         out["decode_with_measured_plans"] = tuned
     if sweep:
