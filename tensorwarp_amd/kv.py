@@ -3,7 +3,7 @@ arrays and what the calls do with them are described in include/twmarlin.h.
 
 Arrays are GpuTensors, or anything with .ptr, .dtype ("f32", "f16", "i32", "u8" for e4m3 codes) and .numel.
 """
-import ctypes as C
+import array
 
 import numpy as np
 
@@ -59,12 +59,26 @@ def kv_layers(caches):
     return layers
 
 
+def _page_numbers(pages):
+    """Page numbers for the library, an address and how many; what keeps them alive comes first."""
+    try:
+        if not isinstance(pages, np.ndarray):
+            numbers = array.array("I", pages)
+            return (numbers,) + numbers.buffer_info()
+        if pages.ndim != 1 or pages.dtype.kind not in "iu":
+            raise ValueError("kv_copy_pages: pages are a list of whole numbers")
+        if pages.size == 0 or (pages.min() >= 0 and pages.max() <= 0xFFFFFFFF):
+            numbers = np.ascontiguousarray(pages, np.uint32)
+            return numbers, numbers.ctypes.data, numbers.size
+    except OverflowError:
+        pass
+    raise ValueError("kv_copy_pages: a page's number is outside the pool")
+
+
 def kv_copy_pages(device, layers, sources, targets):
     """Page sources[i] to page targets[i] in every layer (kv_layers())."""
-    sources, targets = np.asarray(sources, np.int64), np.asarray(targets, np.int64)
-    if sources.shape != targets.shape or sources.ndim != 1:
+    _from, source, count = _page_numbers(sources)
+    _to, target, targeted = _page_numbers(targets)
+    if count != targeted:
         raise ValueError("kv_copy_pages: as many targets as sources")
-    if sources.size and (min(sources.min(), targets.min()) < 0 or max(sources.max(), targets.max()) > 0xFFFFFFFF):
-        raise ValueError("kv_copy_pages: a page's number is outside the pool")
-    sources, targets = sources.astype(np.uint32), targets.astype(np.uint32)
-    _check(device._l.twm_kv_copy_pages(device.handle, layers, len(layers), sources.ctypes.data, targets.ctypes.data, sources.size))
+    _check(device._l.twm_kv_copy_pages(device.handle, layers, len(layers), source, target, count))

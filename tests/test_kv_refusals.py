@@ -147,3 +147,12 @@ def test_page_numbers_that_32_bits_do_not_hold(page):
     for sources, targets in (([page], [1]), ([1], [page]), (np.array([0, page]), np.array([1, 2]))):
         with pytest.raises(ValueError, match="outside the pool"):
             T.kv_copy_pages(None, layers, sources, targets)
+
+
+def test_what_is_no_list_of_pages():
+    layers = T.kv_layers([])
+    for sources, targets in ((np.zeros((1, 1), np.int32), [1]), (np.array([0.5]), [1]), ([0], np.array([1.0])), ([0, 1], [2]), (np.arange(2), [5])):
+        with pytest.raises(ValueError):
+            T.kv_copy_pages(None, layers, sources, targets)
+    with pytest.raises(TypeError):
+        T.kv_copy_pages(None, layers, [0.5], [1])
