@@ -279,6 +279,16 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
+        // keys of two steps ahead of the products, where the compiler would read those of one and wait (8192 rows 522 -> 518 us, 2048 in seven
+        // prompts 25.1 -> 24.1)
+        constexpr int kReads = (int)kHalf / 16 * (KT / 32), kAhead = 4;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < kReads - kAhead; i += 2) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
         if constexpr (kShared > 1) {
             static_assert(KT == 32, "a wave's part is one block");
             float4v *const parts = (float4v *)(lds + 4 * kTile);
