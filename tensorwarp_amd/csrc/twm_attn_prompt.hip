@@ -16,6 +16,14 @@
 // Where a tile holds tokens that some of the queries do not see, weights alone would not keep an infinity or a NaN away from these (0 times
 // either is NaN): there values are looked through first, rows that nobody sees become zeros, and if anything not finite is left, the tile's
 // products are made one token at a time, for those who see it.
+//
+// Bound by no single unit where prompts are long: a wave's 32 queries read as many bytes of keys and values from LDS (128 a cycle and compute unit) as
+// keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
+// 128 f16 values, 510 - 525 us (920 - 940 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
+// that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
+// registers (579).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
+// heads of 64, 5.7 us; 2048 rows in seven prompts 23 us, of which the longest's eleven tiles are half.  Heads of 256 values meet twice a tile of 32
+// tokens: 1500 rows behind 5000 tokens, 16 heads on 8, window 1024, e4m3, 80 us (f16 72).
 #include "twm_kv.h"
 #include "twm_slices.h"
 
