@@ -21,9 +21,10 @@
 // keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
 // 128 f16 values, 510 - 525 us (920 - 940 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
 // that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
-// registers (579).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
-// heads of 64, 5.7 us; 2048 rows in seven prompts 23 us, of which the longest's eleven tiles are half.  Heads of 256 values meet twice a tile of 32
-// tokens: 1500 rows behind 5000 tokens, 16 heads on 8, window 1024, e4m3, 80 us (f16 72).
+// registers (579), and 64 queries a wave with the next tile's scores beside this one's exponentials leave one wave a SIMD (heads of 64: 376, with 32 queries
+// 309; of 128 they spill).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
+// heads of 64, 5.7 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.  Heads of 256 values meet twice a tile of 32
+// tokens: 1500 rows behind 5000 tokens, 16 heads on 8, window 1024, e4m3, 79 - 82 us (f16 72).
 #include "twm_kv.h"
 #include "twm_slices.h"
 
@@ -65,12 +66,15 @@ __device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-__device__ __forceinline__ bool not_finite(uint4v v)
+// What is not finite times 0 is NaN, and stays in the sum
+__device__ __forceinline__ half2v times_0(uint4v v, half2v sum)
 {
-    bool found = false;
 #pragma unroll
-    for (int i = 0; i < 4; i++) found |= (v[i] & 0x7C00u) == 0x7C00u || (v[i] & 0x7C000000u) == 0x7C000000u;
-    return found;
+    for (int i = 0; i < 4; i++) {
+        const uint32_t pair = v[i];   // (a cast of v[i] itself would take the first one's bits)
+        sum = __builtin_elementwise_fma(__builtin_bit_cast(half2v, pair), half2v{(_Float16)0.f, (_Float16)0.f}, sum);
+    }
+    return sum;
 }
 
 struct Prompt {
@@ -411,14 +415,22 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         if (!idle) {
             float16v s[KT / 32];
             scores(tile, s);
+            if (t0 >= high_begin && present == (1u << kGroups) - 1u) {   // (everyone sees its beginning)
+                const int seen = my_end - t0 - 4 * (int)half;
 #pragma unroll
-            for (int b = 0; b < KT / 32; b++)
+                for (int b = 0; b < KT / 32; b++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    // (tokens from the first seen one on, as unsigned numbers, against their number: none where the page is absent)
-                    const uint32_t seen = present >> (2 * b + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
-                    s[b][j] = (uint32_t)(t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[b][j] : -INFINITY;
-                }
+                    for (int j = 0; j < 16; j++) s[b][j] = 32 * b + 8 * (j / 4) + j % 4 < seen ? s[b][j] : -INFINITY;
+            } else {
+#pragma unroll
+                for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        // (tokens from the first seen one on, as unsigned numbers, against their number: none where the page is absent)
+                        const uint32_t seen = present >> (2 * b + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
+                        s[b][j] = (uint32_t)(t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[b][j] : -INFINITY;
+                    }
+            }
             const float most = largest(s);
             if (__any(most > reference + 15.0f)) raise(most);
             weigh(s, p);
@@ -428,18 +440,18 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
         const int token = t0 + (int)looked;
         const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
-        bool bad = false;
+        half2v found = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
         for (uint32_t i = 0; i < kEach; i++) {
             uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
             if (dead)
                 *at = uint4v{0u, 0u, 0u, 0u};
             else
-                bad |= not_finite(*at);
+                found = times_0(*at, found);
         }
         // (waves that share queries have met since they read the tile's keys, so that flags and weights may take their place)
         uint32_t *const flags = (uint32_t *)(lds + (D == 256 ? buf * kTile : kPromptLds<D> - 16));
-        bad = __any(bad);
+        const bool bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
         if (lane == 0) flags[wave] = bad;
         __syncthreads();
         const bool single = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;

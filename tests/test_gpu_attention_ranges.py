@@ -88,6 +88,24 @@ def test_hundreds_of_thousands_of_tokens(dev, cache):
     run_prompt(dev, pool, table, lengths, [2, 1], 3)
 
 
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+def test_hundreds_of_millions_of_tokens(dev, cache):
+    # one page of 256 tokens named a million times is that page's attention.  Every token is one of 2^28 and no more than (2^28 / 2048 waves + 64)
+    # f32 additions stand behind a sum, of products and of weights
+    pool = Pool(np.random.default_rng(9), 3, 1, 256, 64, cache)
+    table = np.full((2, 1 << 20), pool.fill([256])[0, 0], np.int32)
+    lengths, heads = [1 << 28, 256], 2
+    q = queries(np.random.default_rng(10), 2, heads, 64)
+    kc, seqs = pool.upload(dev), sequences(dev, table, lengths, [1, 1])
+    for call, more in ((T.attention_decode, []), (T.attention_prompt, [2])):
+        out = Out(dev, q.shape, "f16")
+        call(dev, kc, seqs, At(dev, q), *more, heads, out)
+        want, tol, _ = attend_rows(pool, table[:, :1], [256, 256], [1, 1], q, 0.125, 0, PROMPT_STEP)
+        most = np.abs(pool.tokens("v", table[0, :1], 256)).max(1)[None]
+        tol[0] += 2 * (131072 + 64) * 2.0 ** -23 * most[0]
+        check(out.get(), want, tol)
+
+
 @pytest.mark.parametrize("dim,heads,kv,cache", [(64, 2, 1, "f16"), (128, 2, 2, "e4m3"), (256, 2, 1, "f16")])
 @pytest.mark.parametrize("window", [0, 777])
 def test_thousands_of_rows_against_their_single_tokens(dev, dim, heads, kv, cache, window):
@@ -129,6 +147,29 @@ def test_lengths_below_zero(dev, least):
     for window in (0, 1, 30, 0xFFFFFFFF):
         run_decode(dev, pool, table, lengths, 4, window=window)
         run_prompt(dev, pool, table, lengths, [20, 0, 3], 4, window=window)
+
+
+@pytest.mark.parametrize("dim,cache", [(64, "f16"), (128, "f16"), (256, "f16"), (128, "e4m3")])
+def test_one_infinity_in_any_column_does_not_reach_the_rows_before_it(dev, dim, cache):
+    n = 40
+    pool = Pool(np.random.default_rng(11), 4, 1, 16, dim, cache, scales=False)
+    table, q = pool.fill([n]), queries(np.random.default_rng(12), n, 1, dim)
+    clean = run_prompt(dev, pool, table, [n], [n], 1, q=q)
+    want, tol, _ = attend_rows(pool, table, [n], [n], q, dim ** -0.5, 0, PROMPT_STEP)
+    bad = (0x7F, np.uint8) if cache == "e4m3" else (0x7C00, np.uint16)   # (e4m3 has no infinity: NaN)
+    for column in range(dim):
+        token = 1 + column % (n - 1)
+        at = table[0, token // 16], 0, token % 16, column
+        kept = pool.bits["v"][at]
+        pool.bits["v"][at] = bad[0]
+        out = Out(dev, q.shape, "f16")
+        T.attention_prompt(dev, pool.upload(dev), sequences(dev, table, [n], [n]), At(dev, q), n, 1, out)
+        pool.bits["v"][at] = kept
+        got, others = out.get(), np.arange(dim) != column
+        assert not np.isfinite(got[token:, 0, column]).any()
+        check(got[:token], want[:token], tol[:token])
+        check(got[token:][:, :, others], want[token:][:, :, others], tol[token:][:, :, others])
+    assert np.array_equal(run_prompt(dev, pool, table, [n], [n], 1, q=q).view(np.uint16), clean.view(np.uint16))
 
 
 class Large:

@@ -224,6 +224,29 @@ def test_copies(dev, layers, pairs, pages, kv, page, dim, cache):
     run_copy(dev, layers, pairs, pages, kv, page, dim, cache)
 
 
+def test_a_captured_copy_copies_what_is_there_at_its_replay(dev):
+    rng = np.random.default_rng(12)
+    pools = [Pool(rng, 9, 2, 16, 64) for _ in range(3)]
+    layers = T.kv_layers([p.upload(dev) for p in pools])
+    sources, targets = [4, 4, 0], np.array([1, 8, 3])
+    T.kv_copy_pages(dev, layers, sources, targets)   # (once before)
+    graph = T.GraphCapture.record_with_device(dev, lambda: T.kv_copy_pages(dev, layers, sources, targets))
+    for _ in range(4):
+        for p in pools:
+            for name in "kv":
+                p.bits[name] = rng.integers(0, 1 << 16, p.shape).astype(np.uint16)
+                p.dev[name].copy_from_host(p.bits[name])
+        graph.replay()
+        dev.synchronize()
+        for p in pools:
+            before = {name: p.bits[name].copy() for name in "kv"}
+            p.download()
+            for name in "kv":
+                before[name][targets] = before[name][sources]
+                assert np.array_equal(p.bits[name], before[name])
+        T.kv_copy_pages(dev, layers, [2], [5])   # eager work in between
+
+
 # ---- together ----------------------------------------------------------------------------------------------------------
 
 
