@@ -82,6 +82,7 @@ struct Prompt {
     float4v *parts;       // [workgroups][dim / 4][rows of a workgroup], for rows that several workgroups share the tokens of
     float2 *part_sums;    // [workgroups][rows]: reference, sum of weights
     uint32_t tiles, splits, first_tile;   // splits: the most workgroups that share a tile of rows
+    float balance;                        // 5120 / dim / workgroups
     Divisor by_group, by_kv_heads, by_splits;
 };
 
@@ -130,13 +131,16 @@ template <uint32_t EACH> __device__ __forceinline__ bool find_rows(const Prompt 
     r->last = min(r->before + (int)job.by_group(min(r->row0 + EACH, r->rows) - 1) + 1, a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0);
     return true;
 }
-// How many workgroups share these rows' tokens: each has kLeastPart tiles at least
-constexpr int kLeastPart = 6;
-__device__ __forceinline__ uint32_t parts_of(const Rows &r, uint32_t splits, int tile, uint32_t *tiles)
+// How many workgroups share these rows' tokens: kLeastPart tiles each at least, and as many as balance the tiles' time with that of the parts on their way
+// to the join, which reads 4 D bytes of each row and part; both are p = sqrt(5120 / D * tiles / workgroups) apart.  Heads of 128: 100 rows behind 600
+// tokens on 8 key-value heads in 2 parts 16.1 us, whole 20.4; 1024 rows of one key-value head in 4 20.2, in 2 23.6, whole 25.0; but of four (240
+// workgroups) whole 28.1, in 2 30.2, and 512 rows of four whole 17.6, in 2 19.9.  300 rows of 256 values behind 2000 tokens, on 2, in 6 parts 34, in 12 39.
+constexpr int kLeastPart = 4;
+__device__ __forceinline__ uint32_t parts_of(const Rows &r, const Prompt &job, int tile, uint32_t *tiles)
 {
     const int begin = r.first & ~(tile - 1);
     *tiles = r.last > begin ? (uint32_t)(r.last - begin + tile - 1) / (uint32_t)tile : 0u;
-    return max(1u, min(splits, *tiles / kLeastPart));
+    return max(1u, min(min(job.splits, *tiles / kLeastPart), (uint32_t)sqrtf((float)*tiles * job.balance)));
 }
 
 // tokens of a tile
@@ -166,7 +170,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
     uint32_t key_tiles;
-    const uint32_t parts = parts_of(mine, job.splits, KT, &key_tiles);
+    const uint32_t parts = parts_of(mine, job, KT, &key_tiles);
     if (split >= parts) return;
 
     auto begin_of = [&](int position) { return prompt_begin(a, position); };
@@ -518,7 +522,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     Rows mine;
     if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
     uint32_t key_tiles;
-    const uint32_t parts = parts_of(mine, job.splits, kPromptTile<D>, &key_tiles);
+    const uint32_t parts = parts_of(mine, job, kPromptTile<D>, &key_tiles);
     const uint32_t first_row = blockIdx.y * kHere;
     if (parts == 1 || mine.row0 + first_row >= mine.rows) return;
     const uint32_t slice = threadIdx.x / kEach, x = threadIdx.x % kEach, r = first_row + x % kHere, quad = x / kHere;   // (rows lie beside each other)
@@ -594,7 +598,9 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         job.tiles = (uint32_t)tiles;
         job.by_group = Divisor(a.group);
         job.by_kv_heads = Divisor(a.kv.kv_heads);
-        job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(512 / workgroups, most));
+        job.balance = 5120.0f / D / (float)workgroups;
+        const float balanced = std::sqrt((float)(seen / kPromptTile<D> + 1) * job.balance);   // of the most tiles that there may be
+        job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(512 / workgroups, most), (uint64_t)balanced));
         job.by_splits = Divisor(job.splits);
         job.parts = (float4v *)scratch;
         job.part_sums = (float2 *)((char *)scratch + (size_t)workgroups * job.splits * kRows * D * 4);

@@ -172,6 +172,19 @@ def test_one_infinity_in_any_column_does_not_reach_the_rows_before_it(dev, dim, 
     assert np.array_equal(run_prompt(dev, pool, table, [n], [n], 1, q=q).view(np.uint16), clean.view(np.uint16))
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_rows_of_nothing_but_infinitely_low_scores_are_zeros(dev, dim):
+    n = 70
+    pool = Pool(np.random.default_rng(13), 6, 1, 16, dim)
+    table = pool.fill([n])
+    q = np.abs(queries(np.random.default_rng(14), n, 2, dim)) + np.float16(0.25)
+    pool.bits["k"][:, :, :, 3] = np.float16(-np.inf).view(np.uint16)
+    kc, out, one = pool.upload(dev), Out(dev, q.shape, "f16"), Out(dev, (1, 2, dim), "f16")
+    T.attention_prompt(dev, kc, sequences(dev, table, [n], [n]), At(dev, q), n, 2, out)
+    T.attention_decode(dev, kc, sequences(dev, table, [n]), At(dev, q[:1]), 2, one)
+    assert (out.get() == 0).all() and (one.get() == 0).all()
+
+
 class Large:
     """A device array that no host array stands behind, cleared page by page."""
 
