@@ -6,7 +6,7 @@
 // it) only where a weight would pass 2^15, so that sums are rarely touched again and f16 holds the weights with all of its digits down to 2^-22
 // of the largest.
 //
-// A workgroup takes 128 queries of one key-value head -- tokens times the query heads that share it, so that short prompts fill
+// A workgroup takes 128 queries (of 256 values 64) of one key-value head -- tokens times the query heads that share it, so that short prompts fill
 // tiles too -- and its four waves 32 each.  Keys and values come through LDS, tile by tile, the next tile on its way while this one is worked on;
 // f16 ones directly, 16 bytes a lane, e4m3 ones through registers, where they become f16.  Scores are transposed, S^T = K Q^T: a
 // lane then holds the scores of one query, row maxima need one exchange between lanes, and the weights already lie as O^T = V^T P^T wants
@@ -23,8 +23,7 @@
 // that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
 // registers (579), and 64 queries a wave with the next tile's scores beside this one's exponentials leave one wave a SIMD (heads of 64: 376, with 32 queries
 // 309; of 128 they spill).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
-// heads of 64, 5.7 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.  Heads of 256 values meet twice a tile of 32
-// tokens: 1500 rows behind 5000 tokens, 16 heads on 8, window 1024, e4m3, 79 - 82 us (f16 72).
+// heads of 64, 5.7 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.
 #include "twm_kv.h"
 #include "twm_slices.h"
 
@@ -43,9 +42,8 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 #define TWM_LDS(T) __attribute__((address_space(3))) T
 
 constexpr uint32_t kPromptWaves = 4;
-// Waves that share 32 queries: of 256 values each holds half, which is what registers hold (the whole of it in one wave: 2.2 times slower)
-template <int D> constexpr uint32_t kPromptShared = D == 256 ? 2 : 1;
-template <int D> constexpr uint32_t kPromptRows = 32 * kPromptWaves / kPromptShared<D>;
+template <int D> constexpr uint32_t kPromptRows = D == 256 ? 64 : 128;   // of a workgroup
+constexpr int kPromptTile = 64;                                          // tokens of a tile
 
 __device__ __forceinline__ float max_of_halves(float v)
 {
@@ -143,21 +141,20 @@ __device__ __forceinline__ uint32_t parts_of(const Rows &r, const Prompt &job, i
     return max(1u, min(min(job.splits, *tiles / kLeastPart), (uint32_t)sqrtf((float)*tiles * job.balance)));
 }
 
-// tokens of a tile
-template <int D> constexpr int kPromptTile = D == 256 ? 32 : 64;
 // LDS of a workgroup
-template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile<D> * D * 2 + (D == 256 ? kPromptWaves * 32 * 32 * 4 : D == 64 ? kPromptWaves * 64 * 32 * 2 + 16 : 16);
+template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile * D * 2 + (D == 64 ? kPromptWaves * 64 * 32 * 2 + 16 : 16);
+constexpr uint32_t kPairsLds = 2 * kPromptTile * 512 + kPromptWaves * 2048 + kPromptWaves * 32 * 4 + 16;
 
 }  // namespace
 
 template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt(const Prompt job)
 {
-    constexpr int KT = kPromptTile<D>, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
+    constexpr int KT = kPromptTile, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
     constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
     constexpr uint32_t kTile = KT * kRow, kWaveRows = KT / kPromptWaves;   // bytes of a tile's keys; rows that a wave brings in
-    constexpr uint32_t kShared = kPromptShared<D>, kRows = kPromptRows<D>, kHalf = D / kShared;   // values of a head that a wave holds
-    // two buffers of keys, then two of values; behind them room for the waves' weights, where a tile of keys is too small for them, or for
-    // their parts of the scores, and a flag for each
+    constexpr uint32_t kRows = kPromptRows<D>;
+    // two buffers of keys, then two of values; behind them room for the waves' weights, where a tile of keys is too small for them, and a flag
+    // for each
     extern __shared__ __align__(16) char lds[];
     const AttnArgs &a = job.a;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
@@ -175,7 +172,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
 
     auto begin_of = [&](int position) { return prompt_begin(a, position); };
     // this lane's query: a row behind the last one repeats it and is not stored
-    const uint32_t sharer = wave % kShared, wave_row = row0 + wave / kShared * 32u;
+    const uint32_t wave_row = row0 + wave * 32u;
     const uint32_t row = wave_row + col, my_row = min(row, rows - 1);
     const uint32_t my_token = job.by_group(my_row), my_head = kv_head * a.group + (my_row - my_token * a.group);
     const int my_position = before + (int)my_token, my_begin = begin_of(my_position), my_end = min(my_position + 1, capacity);
@@ -187,17 +184,17 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * each_part + min(split, one_more)) * KT);
     const int last = min(mine.last, all_begin + (int)((split + 1) * each_part + min(split + 1, one_more)) * KT);
 
-    half8 q[kHalf / 16];
+    half8 q[D / 16];
     {
-        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + sharer * kHalf + 8u * half;
+        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + 8u * half;
 #pragma unroll
-        for (int i = 0; i < (int)kHalf / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
+        for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
     const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
     float reference = -INFINITY, sum = 0.f;
-    float16v o[kHalf / 32];
+    float16v o[D / 32];
 #pragma unroll
-    for (int i = 0; i < (int)kHalf / 32; i++)
+    for (int i = 0; i < D / 32; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
@@ -281,23 +278,22 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         next = find_pages(t_begin + KT);
     }
     // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
-    const uint32_t k_at = (col * kRow + (key_place(col, half) << 4)) ^ sharer * kHalf * 2u, v_row = 4u * half + (lane >> 2 & 3u);
-    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u + sharer * kHalf * 2u;
+    const uint32_t k_at = col * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
     // S^T of the tile in buffer `tile`; element j of block b: token 32 b + 8 (j / 4) + 4 half + j % 4
-    // (waves that share queries add their parts of the sums over a head's values)
     auto scores = [&](const char *tile, float16v (&s)[KT / 32]) {
 #pragma unroll
         for (int b = 0; b < KT / 32; b++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[b][j] = 0.f;
 #pragma unroll
-        for (int i = 0; i < (int)kHalf / 16; i++)
+        for (int i = 0; i < D / 16; i++)
 #pragma unroll
             for (int b = 0; b < KT / 32; b++)
                 s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(tile + (k_at ^ i << 5) + b * 32 * kRow), q[i], s[b], 0, 0, 0);
         // keys of two steps ahead of the products, where the compiler would read those of one and wait (8192 rows 522 -> 518 us, 2048 in seven
         // prompts 25.1 -> 24.1)
-        constexpr int kReads = (int)kHalf / 16 * (KT / 32), kAhead = 4;
+        constexpr int kReads = D / 16 * (KT / 32), kAhead = 4;
         __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
         for (int i = 0; i < kReads - kAhead; i += 2) {
@@ -305,19 +301,6 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
             __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x8, kAhead, 0);
-        if constexpr (kShared > 1) {
-            static_assert(KT == 32, "a wave's part is one block");
-            float4v *const parts = (float4v *)(lds + 4 * kTile);
-#pragma unroll
-            for (int j = 0; j < 4; j++) parts[(wave * 4u + j) * 64u + lane] = float4v{s[0][4 * j], s[0][4 * j + 1], s[0][4 * j + 2], s[0][4 * j + 3]};
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float4v other = parts[((wave ^ 1u) * 4u + j) * 64u + lane];
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[0][4 * j + e] += other[e];
-            }
-        }
     };
     // the largest score, as an exponent; it sets the reference where there is none yet, and nothing is summed
     auto largest = [&](const float16v (&s)[KT / 32]) {
@@ -335,7 +318,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         const float raised = fmaxf(reference, most - 8.0f), by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(reference - raised);
         sum *= by;
 #pragma unroll
-        for (int i = 0; i < (int)kHalf / 32; i++) o[i] *= by;
+        for (int i = 0; i < D / 32; i++) o[i] *= by;
         reference = raised;
     };
     auto weigh = [&](const float16v (&s)[KT / 32], half8 (&p)[KT / 16]) {
@@ -354,7 +337,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
 #pragma unroll
         for (int b = 0; b < KT / 16; b++)
 #pragma unroll
-            for (int i = 0; i < (int)kHalf / 32; i++) {
+            for (int i = 0; i < D / 32; i++) {
                 // tokens 16 b + 4 half .. + 3 and 8 further, of which a lane is given one value each
                 const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + b * 16 * kRow)));
                 const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(tile + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
@@ -394,11 +377,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
             scores(tile, s);
             const float most = largest(s);
             if (__any(most > reference + 15.0f)) {
-                if constexpr (kShared == 1) {   // (rare; outside of this loop, so that the sums never move within it)
-                    raise_to = most;
-                    break;
-                }
-                raise(most);
+                raise_to = most;   // (rare; outside of this loop, so that the sums never move within it)
+                break;
             }
             weigh(s, p);
             add_values(tile, p);
@@ -413,8 +393,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         const char *const tile = lds + buf * kTile;
         const uint32_t present = there_now;
         advance();
-        // nothing for this wave (waves that share queries meet in every tile)
-        const bool idle = kShared == 1 && (t0 > wave_high || t0 + KT <= begin_of(wave_low));
+        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
         half8 p[KT / 16];
         if (!idle) {
             float16v s[KT / 32];
@@ -453,8 +432,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
             else
                 found = times_0(*at, found);
         }
-        // (waves that share queries have met since they read the tile's keys, so that flags and weights may take their place)
-        uint32_t *const flags = (uint32_t *)(lds + (D == 256 ? buf * kTile : kPromptLds<D> - 16));
+        uint32_t *const flags = (uint32_t *)(lds + kPromptLds<D> - 16);
         const bool bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
         if (lane == 0) flags[wave] = bad;
         __syncthreads();
@@ -475,10 +453,10 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
                 const bool seen = at >= my_begin && at < my_end;
                 const float w = (float)weights[r * 32 + (int)col];
 #pragma unroll
-                for (int i = 0; i < (int)kHalf / 32; i++)
+                for (int i = 0; i < D / 32; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
+                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
 #pragma unroll
                         for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
                     }
@@ -488,6 +466,289 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     }
 
     sum = sum_of_halves(sum);
+    if (parts > 1) {
+        // to scratch, rows beside each other
+        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + wave_row - row0 + col;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (row < rows)
+                    to[(8u * i + 2u * j + half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        if (row < rows && half == 0) job.part_sums[(size_t)blockIdx.x * kRows + wave_row - row0 + col] = float2{reference, sum};
+    } else if (row < rows) {
+        const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
+        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + 4u * half;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                *(half4_any *)(out + 32 * i + 8 * j) = half4{(_Float16)(o[i][4 * j] * to), (_Float16)(o[i][4 * j + 1] * to), (_Float16)(o[i][4 * j + 2] * to),
+                                                             (_Float16)(o[i][4 * j + 3] * to)};
+    }
+}
+
+// Heads of 256 values: two waves share 32 queries.  Each takes half of a tile's tokens for the scores, with all of a head's values, and half of
+// a head's values for the sums, with all of the tile's tokens; weights change hands in LDS, and with them whether a reference must move, which both do
+// alike.  One buffer of keys and one of values: the next tile's keys come while values are summed, its values while keys are scored.  Half of a
+// head's values a wave for the scores too, whose parts were added through LDS in tiles of 32, took 1.2 - 1.3 times as long (8192 rows, 16 heads on 8: f16
+// 866 us, now 734; e4m3 909, now 694; 1500 rows behind 5000, window 1024, e4m3 82, now 69), and every lane's sixteen addresses, if held, spill
+// (e4m3 99).  f16 values wait for the next keys, which go to LDS directly; through registers, as e4m3 does, they spill (854).
+template <bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt_pairs(const Prompt job)
+{
+    constexpr int D = 256, KT = kPromptTile, kGroups = KT / 16;
+    constexpr uint32_t kUnits = D / 8, kRow = D * 2, kTile = KT * kRow, kWaveRows = KT / kPromptWaves, kRows = kPromptRows<D>, kHalf = D / 2;
+    extern __shared__ __align__(16) char lds[];
+    half8 *const weights = (half8 *)(lds + 2 * kTile);              // [wave][two runs of 16 tokens][lane]
+    float *const tops = (float *)(lds + 2 * kTile + 4 * 2048);      // [wave][query]
+    uint32_t *const flags = (uint32_t *)(lds + kPairsLds - 16);     // [wave]: 1: a weight would pass 2^15, 2: a value is not finite
+    const AttnArgs &a = job.a;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
+
+    const uint32_t pair = job.by_splits(blockIdx.x), split = blockIdx.x - pair * job.splits, local = job.by_kv_heads(pair), kv_head = pair - local * a.kv.kv_heads;
+    Rows mine;
+    if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
+    const uint32_t seq = mine.seq, row0 = mine.row0, rows = mine.rows;
+    const int start = mine.start, before = mine.before;
+    const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
+    uint32_t key_tiles;
+    const uint32_t parts = parts_of(mine, job, KT, &key_tiles);
+    if (split >= parts) return;
+
+    const uint32_t sharer = wave & 1u, wave_row = row0 + wave / 2u * 32u;
+    const uint32_t row = wave_row + col, my_row = min(row, rows - 1);
+    const uint32_t my_token = job.by_group(my_row), my_head = kv_head * a.group + (my_row - my_token * a.group);
+    const int my_position = before + (int)my_token, my_begin = prompt_begin(a, my_position), my_end = min(my_position + 1, capacity);
+    const int low = before + (int)job.by_group(row0), high = before + (int)job.by_group(min(row0 + kRows, rows) - 1);
+    const uint32_t each_part = key_tiles / parts, one_more = key_tiles - each_part * parts;
+    const int all_begin = mine.first & ~(KT - 1), first = max(mine.first, all_begin + (int)(split * each_part + min(split, one_more)) * KT);
+    const int last = min(mine.last, all_begin + (int)((split + 1) * each_part + min(split + 1, one_more)) * KT);
+
+    half8 q[D / 16];
+    {
+        const _Float16 *from = a.q + (size_t)(start + (int)my_token) * a.q_stride + my_head * D + 8u * half;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
+    }
+    const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+    float reference = -INFINITY, sum = 0.f;
+    float16v o[kHalf / 32];
+#pragma unroll
+    for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+
+    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (r & 15u); };
+    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (r & 3u) << 2; };
+    const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
+    struct Pages {
+        int mine;
+        uint32_t there;
+    };
+    const int t_begin = first & ~(KT - 1);
+    int looked_up = t_begin, page_of = -1;
+    uint64_t page_there = 0;
+    auto look_up = [&](int t0) {
+        looked_up = t0;
+        const int token = t0 + 16 * (int)lane;
+        page_of = token < last ? a.seqs.tables[(size_t)seq * a.seqs.table_stride + ((uint32_t)token >> a.kv.page_shift)] : -1;
+        page_there = __ballot((uint32_t)page_of < a.kv.pages);
+    };
+    auto find_pages = [&](int t0) {
+        if (t0 - looked_up >= 1024) look_up(t0);
+        const uint32_t group = (uint32_t)(t0 - looked_up) >> 4;
+        return Pages{__builtin_amdgcn_readlane(page_of, group + wave), (uint32_t)(page_there >> group) & ((1u << kGroups) - 1u)};
+    };
+    constexpr int kLoads = (int)(kWaveRows * D * (E4M3 ? 1 : 2) / 1024);   // 1 KB each
+    constexpr uint32_t kLoadUnits = D * (E4M3 ? 1 : 2) / 16, kRowsPerLoad = 64 / kLoadUnits;
+    uint4v held[kLoads];   // e4m3 only: keys or values on their way
+    const uint32_t r0 = wave * kWaveRows;
+    auto bring = [&](int t0, int of, bool value) {
+        // rows of a page outside the pool are read from its first one
+        const uint32_t page = (uint32_t)of < a.kv.pages ? (uint32_t)of : 0u;
+        const size_t at = (kv_chunk(a.kv, page, kv_head) + ((uint32_t)(t0 + (int)r0) & page_mask) * D) * (E4M3 ? 1 : 2);
+        const char *from = (const char *)(value ? a.kv.v : a.kv.k) + at;
+        uint32_t me = lane;
+        asm volatile("" : "+v"(me));
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            if constexpr (E4M3) {
+                held[i] = *(const uint4v *)(from + i * 1024 + me * 16u);
+            } else {
+                const uint32_t r = r0 + i * kRowsPerLoad + me / kUnits;
+                const uint32_t off = i * 1024u + me / kUnits * kRow + ((value ? value_place(r, me % kUnits) : key_place(r, me % kUnits)) << 4);
+                char *to = lds + (value ? kTile : 0u) + (r0 + i * kRowsPerLoad) * kRow;
+                __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(from + off), (TWM_LDS(void) *)to, 16, 0, 0);
+            }
+        }
+    };
+    auto keep = [&](bool value) {
+        if constexpr (E4M3) {
+            uint32_t me = lane;
+            asm volatile("" : "+v"(me));
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const uint32_t r = r0 + i * kRowsPerLoad + me / kLoadUnits, unit = me % kLoadUnits * 2;
+                char *to = lds + (value ? kTile : 0u) + r * kRow;
+                *(half8 *)(to + ((value ? value_place(r, unit) : key_place(r, unit)) << 4)) = to_f16(held[i][0], held[i][1]);
+                *(half8 *)(to + ((value ? value_place(r, unit + 1) : key_place(r, unit + 1)) << 4)) = to_f16(held[i][2], held[i][3]);
+            }
+        }
+    };
+    auto arrived = [&]() {
+        if constexpr (!E4M3) __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+        __syncthreads();
+    };
+
+    const int high_begin = prompt_begin(a, high), whole_end = min(low + 1, last);
+    const uint32_t k_at = (32u * sharer + col) * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u + sharer * kHalf * 2u;
+    const half8 *const pair_weights = weights + (wave & ~1u) * 128u + lane;
+    float16v s;
+    float added;
+    auto weigh = [&]() {
+        const float base = reference == -INFINITY ? 0.f : -reference;
+        half8 p[2];
+        added = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const half2v w = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[j], c, base)), (_Float16)__builtin_amdgcn_exp2f(fmaf(s[j + 1], c, base))};
+            added = __builtin_amdgcn_fdot2(w, half2v{(_Float16)1.0f, (_Float16)1.0f}, added, false);
+            p[j / 8][j % 8] = w[0];
+            p[j / 8][j % 8 + 1] = w[1];
+        }
+        weights[wave * 128u + lane] = p[0];
+        weights[wave * 128u + 64u + lane] = p[1];
+    };
+
+    int t0 = t_begin;
+    uint32_t there = 0;
+    Pages next{-1, 0};
+    if (t0 < last) {
+        look_up(t0);
+        const Pages now = find_pages(t0);
+        there = now.there;
+        bring(t0, now.mine, false);
+        keep(false);
+        bring(t0, now.mine, true);
+        next = find_pages(t0 + KT);
+        arrived();
+    }
+    while (t0 < last) {
+        const bool more = t0 + KT < last;
+        if constexpr (E4M3) {
+            // values of this tile to LDS; the next one begins its way
+            keep(true);
+            if (more) bring(t0 + KT, next.mine, false);
+        }
+        uint32_t keys_at = k_at;
+        asm volatile("" : "+v"(keys_at));   // (sixteen addresses that are made anew, not held)
+#pragma unroll
+        for (int j = 0; j < 16; j++) s[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(lds + (keys_at ^ i << 5)), q[i], s, 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < D / 16 - 4; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+        const bool whole = t0 >= high_begin && t0 + KT <= whole_end && there == (1u << kGroups) - 1u;
+        bool bad = false;
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                const uint32_t seen = there >> (2 * sharer + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
+                s[j] = (uint32_t)(t0 + 32 * (int)sharer + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[j] : -INFINITY;
+            }
+            // values that this wave has brought: rows that nobody sees become zeros, the others are looked through
+            if constexpr (!E4M3) __builtin_amdgcn_s_waitcnt(0x0F70);
+            uint32_t me = lane;
+            asm volatile("" : "+v"(me));
+            const uint32_t looked = r0 + me / 4, unit = me % 4 * 8;
+            const int token = t0 + (int)looked;
+            const bool dead = token < first || token >= last || !(there >> (looked / 16) & 1u);
+            half2v found = {(_Float16)0.f, (_Float16)0.f};
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                uint4v *at = (uint4v *)(lds + kTile + looked * kRow + (value_place(looked, unit + i) << 4));
+                if (dead)
+                    *at = uint4v{0u, 0u, 0u, 0u};
+                else
+                    found = times_0(*at, found);
+            }
+            bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);
+        }
+        float most = s[0];
+#pragma unroll
+        for (int j = 0; j < 16; j++) most = fmaxf(most, s[j]);
+        most = max_of_halves(most) * c;
+        weigh();
+        if (half == 0) tops[wave * 32u + col] = most;
+        const bool over = __any(most > reference + 15.0f);
+        if (lane == 0) flags[wave] = (over ? 1u : 0u) | (bad ? 2u : 0u);
+        arrived();
+        const uint32_t flag = flags[0] | flags[1] | flags[2] | flags[3];
+        if (flag & 1u) {
+            // the reference moves, for both waves of a pair alike, and what is summed with it
+            most = fmaxf(most, tops[(wave ^ 1u) * 32u + col]);
+            const float raised = most > reference + 15.0f ? most - 8.0f : reference;
+            const float by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(reference - raised);
+            sum *= by;
+#pragma unroll
+            for (int i = 0; i < (int)kHalf / 32; i++) o[i] *= by;
+            reference = raised;
+            weigh();
+            __syncthreads();
+        }
+        sum += added;
+        // every wave is done with the tile's keys
+        if (more) {
+            if constexpr (E4M3) keep(false);
+            bring(t0 + KT, next.mine, E4M3);
+        }
+        if (!(flag & 2u)) {
+#pragma unroll
+            for (int b = 0; b < KT / 16; b++) {
+                const half8 p = pair_weights[b * 64];
+#pragma unroll
+                for (int i = 0; i < (int)kHalf / 32; i++) {
+                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + b * 16 * kRow)));
+                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p, o[i], 0, 0, 0);
+                }
+            }
+        } else {
+            // one token after the other
+            for (int r = 0; r < KT; r++) {
+                const int at = t0 + r;
+                if (at < first || at >= last || !(there >> (r / 16) & 1u)) continue;
+                const bool seen = at >= my_begin && at < my_end;
+                const float w = (float)((const _Float16 *)(weights + ((wave & ~1u) + r / 32u) * 128u + r % 32 / 16 * 64 + r / 4 % 2 * 32 + col))[r / 8 % 2 * 4 + r % 4];
+#pragma unroll
+                for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const half4 x = *(const half4 *)(lds + kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
+                    }
+            }
+        }
+        arrived();
+        if constexpr (!E4M3) {
+            if (more) bring(t0 + KT, next.mine, true);
+        }
+        t0 += KT;
+        there = next.there;
+        next = find_pages(t0 + KT);
+    }
+
+    sum = sum_of_halves(sum);
+    if (half == 0) tops[wave * 32u + col] = sum;
+    __syncthreads();
+    sum += tops[(wave ^ 1u) * 32u + col];
     if (parts > 1) {
         // to scratch, rows beside each other
         float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + wave_row - row0 + col;
@@ -522,7 +783,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     Rows mine;
     if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
     uint32_t key_tiles;
-    const uint32_t parts = parts_of(mine, job, kPromptTile<D>, &key_tiles);
+    const uint32_t parts = parts_of(mine, job, kPromptTile, &key_tiles);
     const uint32_t first_row = blockIdx.y * kHere;
     if (parts == 1 || mine.row0 + first_row >= mine.rows) return;
     const uint32_t slice = threadIdx.x / kEach, x = threadIdx.x % kEach, r = first_row + x % kHere, quad = x / kHere;   // (rows lie beside each other)
@@ -578,8 +839,8 @@ hipError_t init_attn_prompt()
     ask(k_attn_prompt<64, true>, kPromptLds<64>);
     ask(k_attn_prompt<128, false>, kPromptLds<128>);
     ask(k_attn_prompt<128, true>, kPromptLds<128>);
-    ask(k_attn_prompt<256, false>, kPromptLds<256>);
-    ask(k_attn_prompt<256, true>, kPromptLds<256>);
+    ask(k_attn_prompt_pairs<false>, kPairsLds);
+    ask(k_attn_prompt_pairs<true>, kPairsLds);
     return e;
 }
 
@@ -592,14 +853,14 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + a.seqs.seqs, workgroups = tiles * a.kv.kv_heads;
         // Tokens are shared out where rows alone leave most of the chip without work (two workgroups a compute unit), as far as there may be some
         const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
-        const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile<D> * kLeastPart);
+        const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile * kLeastPart);
         Prompt job;
         job.a = a;
         job.tiles = (uint32_t)tiles;
         job.by_group = Divisor(a.group);
         job.by_kv_heads = Divisor(a.kv.kv_heads);
         job.balance = 5120.0f / D / (float)workgroups;
-        const float balanced = std::sqrt((float)(seen / kPromptTile<D> + 1) * job.balance);   // of the most tiles that there may be
+        const float balanced = std::sqrt((float)(seen / kPromptTile + 1) * job.balance);   // of the most tiles that there may be
         job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(512 / workgroups, most), (uint64_t)balanced));
         job.by_splits = Divisor(job.splits);
         job.parts = (float4v *)scratch;
@@ -607,7 +868,11 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         if (job.splits > 1 && (size_t)workgroups * job.splits * kRows * (D * 4 + 8) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
         const hipError_t error = in_slices((uint32_t)tiles, most_workgroups(256) / (a.kv.kv_heads * job.splits), [&](uint32_t tile, uint32_t here) {
             job.first_tile = tile;
-            hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), dim3(here * a.kv.kv_heads * job.splits), dim3(256), kPromptLds<D>, s, job);
+            const dim3 grid(here * a.kv.kv_heads * job.splits);
+            if constexpr (D == 256)
+                hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt_pairs<true> : k_attn_prompt_pairs<false>), grid, dim3(256), kPairsLds, s, job);
+            else
+                hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), grid, dim3(256), kPromptLds<D>, s, job);
             return hipGetLastError();
         });
         if (error != hipSuccess || job.splits == 1) return error;
