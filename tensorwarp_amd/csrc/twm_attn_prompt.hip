@@ -19,7 +19,7 @@
 //
 // Bound by no single unit where prompts are long: a wave's 32 queries read as many bytes of keys and values from LDS (128 a cycle and compute unit) as
 // keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
-// 128 f16 values, 510 - 525 us (920 - 940 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
+// 128 f16 values, 504 - 525 us (920 - 950 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
 // that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
 // registers (579), and 64 queries a wave with the next tile's scores beside this one's exponentials leave one wave a SIMD (heads of 64: 376, with 32 queries
 // 309; of 128 they spill).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
@@ -80,7 +80,7 @@ struct Prompt {
     float4v *parts;       // [workgroups][dim / 4][rows of a workgroup], for rows that several workgroups share the tokens of
     float2 *part_sums;    // [workgroups][rows]: reference, sum of weights
     uint32_t tiles, splits, first_tile;   // splits: the most workgroups that share a tile of rows
-    float balance;                        // 5120 / dim / workgroups
+    float balance;                        // (see parts_of)
     Divisor by_group, by_kv_heads, by_splits;
 };
 
@@ -130,9 +130,10 @@ template <uint32_t EACH> __device__ __forceinline__ bool find_rows(const Prompt 
     return true;
 }
 // How many workgroups share these rows' tokens: kLeastPart tiles each at least, and as many as balance the tiles' time with that of the parts on their way
-// to the join, which reads 4 D bytes of each row and part; both are p = sqrt(5120 / D * tiles / workgroups) apart.  Heads of 128: 100 rows behind 600
-// tokens on 8 key-value heads in 2 parts 16.1 us, whole 20.4; 1024 rows of one key-value head in 4 20.2, in 2 23.6, whole 25.0; but of four (240
-// workgroups) whole 28.1, in 2 30.2, and 512 rows of four whole 17.6, in 2 19.9.  300 rows of 256 values behind 2000 tokens, on 2, in 6 parts 34, in 12 39.
+// to the join, which reads 4 D bytes of each row and part: p = sqrt(k tiles / workgroups), k = 80, 40 and 48 for heads of 64, 128 and 256.  Heads of 128:
+// 100 rows behind 600 tokens on 8 key-value heads in 2 parts 16.1 us, whole 20.4; 1024 rows of one key-value head in 4 20.2, in 2 23.6, whole 25.0; but of
+// four (240 workgroups) whole 28.1, in 2 30.2, and 512 rows of four whole 17.6, in 2 19.9.  300 rows of 256 values behind 2000 tokens, on 2: in 6 parts
+// 30.1, in 4 35.7, in 7 36.0.
 constexpr int kLeastPart = 4;
 __device__ __forceinline__ uint32_t parts_of(const Rows &r, const Prompt &job, int tile, uint32_t *tiles)
 {
@@ -859,7 +860,7 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         job.tiles = (uint32_t)tiles;
         job.by_group = Divisor(a.group);
         job.by_kv_heads = Divisor(a.kv.kv_heads);
-        job.balance = 5120.0f / D / (float)workgroups;
+        job.balance = (D == 64 ? 80.0f : D == 128 ? 40.0f : 48.0f) / (float)workgroups;
         const float balanced = std::sqrt((float)(seen / kPromptTile + 1) * job.balance);   // of the most tiles that there may be
         job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(512 / workgroups, most), (uint64_t)balanced));
         job.by_splits = Divisor(job.splits);
