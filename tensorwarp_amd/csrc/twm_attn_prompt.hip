@@ -144,7 +144,7 @@ __device__ __forceinline__ uint32_t parts_of(const Rows &r, const Prompt &job, i
 
 // LDS of a workgroup
 template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile * D * 2 + (D == 64 ? kPromptWaves * 64 * 32 * 2 + 16 : 16);
-constexpr uint32_t kPairsLds = 2 * kPromptTile * 512 + kPromptWaves * 2048 + kPromptWaves * 32 * 4 + 16;
+template <int D> constexpr uint32_t kPairsLds = 2 * kPromptTile * D * 2 + kPromptWaves * 2048 + kPromptWaves * 32 * 4 + 16;
 
 }  // namespace
 
@@ -489,26 +489,26 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     }
 }
 
-// Heads of 256 values: two waves share 32 queries.  Each takes half of a tile's tokens for the scores, with all of a head's values, and half of
+// Heads of 256 values, and short sequences: two waves share 32 queries.  Each takes half of a tile's tokens for the scores, with all of a head's values, and half of
 // a head's values for the sums, with all of the tile's tokens; weights change hands in LDS, and with them whether a reference must move, which both do
 // alike.  One buffer of keys and one of values: the next tile's keys come while values are summed, its values while keys are scored.  Half of a
 // head's values a wave for the scores too, whose parts were added through LDS in tiles of 32, took 1.2 - 1.3 times as long (8192 rows, 16 heads on 8: f16
 // 866 us, now 734; e4m3 909, now 694; 1500 rows behind 5000, window 1024, e4m3 82, now 69), and every lane's sixteen addresses, if held, spill
 // (e4m3 99).  f16 values wait for the next keys, which go to LDS directly; through registers, as e4m3 does, they spill (854).
-template <bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt_pairs(const Prompt job)
+template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)) void k_attn_prompt_pairs(const Prompt job)
 {
-    constexpr int D = 256, KT = kPromptTile, kGroups = KT / 16;
-    constexpr uint32_t kUnits = D / 8, kRow = D * 2, kTile = KT * kRow, kWaveRows = KT / kPromptWaves, kRows = kPromptRows<D>, kHalf = D / 2;
+    constexpr int KT = kPromptTile, kGroups = KT / 16;
+    constexpr uint32_t kUnits = D / 8, kRow = D * 2, kTile = KT * kRow, kWaveRows = KT / kPromptWaves, kRows = 64, kHalf = D / 2;
     extern __shared__ __align__(16) char lds[];
     half8 *const weights = (half8 *)(lds + 2 * kTile);              // [wave][two runs of 16 tokens][lane]
     float *const tops = (float *)(lds + 2 * kTile + 4 * 2048);      // [wave][query]
-    uint32_t *const flags = (uint32_t *)(lds + kPairsLds - 16);     // [wave]: 1: a weight would pass 2^15, 2: a value is not finite
+    uint32_t *const flags = (uint32_t *)(lds + kPairsLds<D> - 16);     // [wave]: 1: a weight would pass 2^15, 2: a value is not finite
     const AttnArgs &a = job.a;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, half = lane >> 5, col = lane & 31u;
 
     const uint32_t pair = job.by_splits(blockIdx.x), split = blockIdx.x - pair * job.splits, local = job.by_kv_heads(pair), kv_head = pair - local * a.kv.kv_heads;
     Rows mine;
-    if (!find_rows<kRows>(job, job.first_tile + local, &mine)) return;
+    if (!find_rows<64>(job, job.first_tile + local, &mine)) return;
     const uint32_t seq = mine.seq, row0 = mine.row0, rows = mine.rows;
     const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
@@ -539,8 +539,8 @@ template <bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt_pai
 #pragma unroll
         for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
-    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (r & 15u); };
-    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (r & 3u) << 2; };
+    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
+    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); };
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
     struct Pages {
         int mine;
@@ -603,7 +603,7 @@ template <bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt_pai
 
     const int high_begin = prompt_begin(a, high), whole_end = min(low + 1, last);
     const uint32_t k_at = (32u * sharer + col) * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
-    const uint32_t v_at = kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u + sharer * kHalf * 2u;
+    const uint32_t v_at = (kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u) ^ sharer * kHalf * 2u;
     const half8 *const pair_weights = weights + (wave & ~1u) * 128u + lane;
     float16v s;
     float added;
@@ -667,12 +667,12 @@ template <bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt_pai
             if constexpr (!E4M3) __builtin_amdgcn_s_waitcnt(0x0F70);
             uint32_t me = lane;
             asm volatile("" : "+v"(me));
-            const uint32_t looked = r0 + me / 4, unit = me % 4 * 8;
+            const uint32_t looked = r0 + me / 4, unit = me % 4 * (kUnits / 4);
             const int token = t0 + (int)looked;
             const bool dead = token < first || token >= last || !(there >> (looked / 16) & 1u);
             half2v found = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
+            for (uint32_t i = 0; i < kUnits / 4; i++) {
                 uint4v *at = (uint4v *)(lds + kTile + looked * kRow + (value_place(looked, unit + i) << 4));
                 if (dead)
                     *at = uint4v{0u, 0u, 0u, 0u};
@@ -840,8 +840,12 @@ hipError_t init_attn_prompt()
     ask(k_attn_prompt<64, true>, kPromptLds<64>);
     ask(k_attn_prompt<128, false>, kPromptLds<128>);
     ask(k_attn_prompt<128, true>, kPromptLds<128>);
-    ask(k_attn_prompt_pairs<false>, kPairsLds);
-    ask(k_attn_prompt_pairs<true>, kPairsLds);
+    ask(k_attn_prompt_pairs<256, false>, kPairsLds<256>);
+    ask(k_attn_prompt_pairs<256, true>, kPairsLds<256>);
+    ask(k_attn_prompt_pairs<128, false>, kPairsLds<128>);
+    ask(k_attn_prompt_pairs<128, true>, kPairsLds<128>);
+    ask(k_attn_prompt_pairs<64, false>, kPairsLds<64>);
+    ask(k_attn_prompt_pairs<64, true>, kPairsLds<64>);
     return e;
 }
 
@@ -849,12 +853,18 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
 {
     auto launch = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        constexpr uint32_t kRows = kPromptRows<D>;
-        // every sequence begins a tile of its own
-        const uint64_t tiles = (uint64_t)a.rows * a.group / kRows + a.seqs.seqs, workgroups = tiles * a.kv.kv_heads;
-        // Tokens are shared out where rows alone leave most of the chip without work (two workgroups a compute unit), as far as there may be some
         const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
-        const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + kRows : capacity), most = seen / (kPromptTile * kLeastPart);
+        // Waves in pairs for heads of 256 values, and where no sequence is longer than eight tiles and the chip is not full of them: tiles of 64 rows and
+        // half of a tile's tokens a wave take less time each, if more together.  28 heads on 4 of 128: 128 rows 8.2 us, 9.8 in the other form, 512
+        // 16.9 and 17.4, 1000 in twenty prompts 11.7 and 12.6; 200 rows of 32 heads on 32 in e4m3 10.0 and 12.8; but 1000 rows in five prompts 17.8 and
+        // 16.1, 4000 in twenty 40 and 34, 8192 in one 670 and 500.
+        const uint64_t pairs_tiles = (uint64_t)a.rows * a.group / 64 + a.seqs.seqs;
+        const bool pairs = D == 256 || (capacity <= 512 && pairs_tiles * a.kv.kv_heads * capacity <= 2048 * kPromptTile);
+        const uint32_t each = pairs ? 64 : 128;
+        // every sequence begins a tile of its own
+        const uint64_t tiles = (uint64_t)a.rows * a.group / each + a.seqs.seqs, workgroups = tiles * a.kv.kv_heads;
+        // Tokens are shared out where rows alone leave most of the chip without work (two workgroups a compute unit), as far as there may be some
+        const uint64_t seen = std::min(capacity, a.window ? (uint64_t)a.window + each : capacity);
         Prompt job;
         job.a = a;
         job.tiles = (uint32_t)tiles;
@@ -862,26 +872,28 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
         job.by_kv_heads = Divisor(a.kv.kv_heads);
         job.balance = (D == 64 ? 80.0f : D == 128 ? 40.0f : 48.0f) / (float)workgroups;
         const float balanced = std::sqrt((float)(seen / kPromptTile + 1) * job.balance);   // of the most tiles that there may be
-        job.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(512 / workgroups, most), (uint64_t)balanced));
+        job.splits = each != kPromptRows<D> ? 1u
+                                            : (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(512 / workgroups, seen / (kPromptTile * kLeastPart)),
+                                                                                                 (uint64_t)balanced));
         job.by_splits = Divisor(job.splits);
         job.parts = (float4v *)scratch;
-        job.part_sums = (float2 *)((char *)scratch + (size_t)workgroups * job.splits * kRows * D * 4);
-        if (job.splits > 1 && (size_t)workgroups * job.splits * kRows * (D * 4 + 8) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
+        job.part_sums = (float2 *)((char *)scratch + (size_t)workgroups * job.splits * each * D * 4);
+        if (job.splits > 1 && (size_t)workgroups * job.splits * each * (D * 4 + 8) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
         const hipError_t error = in_slices((uint32_t)tiles, most_workgroups(256) / (a.kv.kv_heads * job.splits), [&](uint32_t tile, uint32_t here) {
             job.first_tile = tile;
             const dim3 grid(here * a.kv.kv_heads * job.splits);
-            if constexpr (D == 256)
-                hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt_pairs<true> : k_attn_prompt_pairs<false>), grid, dim3(256), kPairsLds, s, job);
-            else
+            if (pairs)
+                hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt_pairs<D, true> : k_attn_prompt_pairs<D, false>), grid, dim3(256), kPairsLds<D>, s, job);
+            else if constexpr (D != 256)
                 hipLaunchKernelGGL((a.kv.e4m3 ? k_attn_prompt<D, true> : k_attn_prompt<D, false>), grid, dim3(256), kPromptLds<D>, s, job);
             return hipGetLastError();
         });
         if (error != hipSuccess || job.splits == 1) return error;
         // (one slice: at most 512 workgroups)
         if (job.splits >= 8)
-            hipLaunchKernelGGL((k_attn_prompt_join<D, 4>), dim3((uint32_t)workgroups, kRows / (64 / (D / 4))), dim3(256), 0, s, job);
+            hipLaunchKernelGGL((k_attn_prompt_join<D, 4>), dim3((uint32_t)workgroups, each / (64 / (D / 4))), dim3(256), 0, s, job);
         else
-            hipLaunchKernelGGL((k_attn_prompt_join<D, 1>), dim3((uint32_t)workgroups, kRows / (256 / (D / 4))), dim3(256), 0, s, job);
+            hipLaunchKernelGGL((k_attn_prompt_join<D, 1>), dim3((uint32_t)workgroups, each / (256 / (D / 4))), dim3(256), 0, s, job);
         return hipGetLastError();
     };
     return a.kv.dim == 64    ? launch(std::integral_constant<int, 64>{})

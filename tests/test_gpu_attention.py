@@ -162,13 +162,14 @@ def test_absent_pages_take_no_part(dev, cache, dim):
     run_prompt(dev, pool, np.ascontiguousarray(table[:, :4]), lengths, [150, 90, 5, 30], 6)
 
 
+@pytest.mark.parametrize("width", [None, 40])
 @pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_what_a_row_does_not_see_does_not_reach_it(dev, dim, bad):
+def test_what_a_row_does_not_see_does_not_reach_it(dev, dim, bad, width):
     # later tokens of the same prompt, earlier ones behind the window, other sequences' pages: infinities and NaN in all of them
     new = lengths = [150, 40]
     pool = Pool(np.random.default_rng(11), 30, 2, 16, dim)
-    table = pool.fill(lengths)
+    table = pool.fill(lengths, width)
     for name, tokens in (("v", (70, 149)), ("k", (90,)), ("v", (10,))):
         for t in tokens:
             pool.bits[name][table[0, t // 16], 1, t % 16, 5::17] = np.float16(bad).view(np.uint16)
@@ -179,11 +180,12 @@ def test_what_a_row_does_not_see_does_not_reach_it(dev, dim, bad):
     assert np.isfinite(got.astype(np.float64)).all()
 
 
-@pytest.mark.parametrize("dim", [64, 128])
-def test_infinite_scores_and_values_are_as_the_formula_has_them(dev, dim):
+@pytest.mark.parametrize("width", [None, 40])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_infinite_scores_and_values_are_as_the_formula_has_them(dev, dim, width):
     pool = Pool(np.random.default_rng(12), 30, 1, 16, dim)
     lengths = [100, 100, 100]
-    table = pool.fill(lengths)
+    table = pool.fill(lengths, width)
     pool.bits["v"][table[0, 2], 0, 3, 7] = np.float16(np.inf).view(np.uint16)    # one value: that column is infinite
     pool.bits["v"][table[1, 2], 0, 3, 7] = np.float16(np.nan).view(np.uint16)
     pool.bits["k"][table[2, 2], 0, 3, 7] = np.float16(np.nan).view(np.uint16)    # a score: the whole row is NaN
@@ -192,21 +194,25 @@ def test_infinite_scores_and_values_are_as_the_formula_has_them(dev, dim):
     run_prompt(dev, pool, table, lengths, [100, 100, 100], 2)
 
 
+@pytest.mark.parametrize("width", [None, 40])
+@pytest.mark.parametrize("dim", [64, 256])
 @pytest.mark.parametrize("scale", [1e-3, 1.0, 30.0])
-def test_scales_and_large_scores(dev, scale):
+def test_scales_and_large_scores(dev, scale, dim, width):
     # scores of thousands: one token takes all the weight; far apart from one another in the order that raises the maximum most often
-    pool = Pool(np.random.default_rng(13), 60, 2, 16, 64)
+    pool = Pool(np.random.default_rng(13), 60, 2, 16, dim)
     lengths = [400, 33, 200]
-    table = pool.fill(lengths, spread=4.0)
+    table = pool.fill(lengths, width, spread=4.0)
     run_decode(dev, pool, table, lengths, 4, scale=scale)
     run_prompt(dev, pool, table, lengths, [300, 33, 1], 4, scale=scale)
 
 
-def test_rising_scores(dev):
+@pytest.mark.parametrize("width", [None, 40])
+@pytest.mark.parametrize("dim", [128, 256])
+def test_rising_scores(dev, dim, width):
     # every token outweighs the ones before it, by up to 2^20
-    dim, n = 128, 500
+    n = 500
     pool = Pool(np.random.default_rng(14), 40, 1, 16, dim)
-    table = pool.fill([n])
+    table = pool.fill([n], width)
     q = np.ones((n, 1, dim), np.float16)
     for t in range(n):
         pool.bits["k"][table[0, t // 16], 0, t % 16] = np.float16(t * 0.11).view(np.uint16)

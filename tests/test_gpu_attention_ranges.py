@@ -61,22 +61,39 @@ def test_decode_of_many_sequences(dev, seqs, longest, wide):
     run_decode(dev, pool, widened(table, 500) if wide else table, lengths, 4)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dim", [64, 256])
 @pytest.mark.parametrize("seqs,most,behind", [(64, 4, 30), (4097, 1, 3), (65, 4, 30), (300, 3, 100), (1100, 2, 5), (130, 40, 0)])
-def test_prompts_of_many_sequences(dev, seqs, most, behind, dim):
+def test_prompts_of_many_sequences(dev, seqs, most, behind, dim, wide):
     rng = np.random.default_rng(seqs)
     new = list(rng.integers(0, most + 1, seqs))
     lengths = [n + int(rng.integers(0, behind + 1)) for n in new]
     pool = Pool(rng, sum(-(-n // 16) for n in lengths) + 1, 1, 16, dim)
-    run_prompt(dev, pool, pool.fill(lengths), lengths, new, 3, first=2, spare=9)
+    table = pool.fill(lengths)
+    run_prompt(dev, pool, widened(table, 40) if wide else table, lengths, new, 3, first=2, spare=9)
 
 
+# (tables of 512 tokens and wider ones: waves in pairs, and not)
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim,heads,kv,page", [(64, 6, 2, 16), (128, 7, 1, 64), (128, 4, 4, 16)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_prompts_with_short_and_wide_tables(dev, dim, heads, kv, page, cache, window, wide):
+    new, lengths = [3, 0, 70, 1, 130, 64], [3, 5, 200, 450, 130, 512]
+    pool = Pool(np.random.default_rng(dim + heads), 1400 // page + 8, kv, page, dim, cache)
+    table = pool.fill(lengths)
+    table[2, 1] = -1
+    run_prompt(dev, pool, widened(table, 2000 // page) if wide else table, lengths, new, heads, window=window, first=1, spare=4)
+
+
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("heads,kv", [(17, 1), (130, 1), (66, 2)])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_prompt_with_heads_across_the_rows_of_a_workgroup(dev, heads, kv, dim):
+def test_prompt_with_heads_across_the_rows_of_a_workgroup(dev, heads, kv, dim, wide):
     new, lengths = [5, 30, 1], [5, 90, 70]
     pool = Pool(np.random.default_rng(heads), 16, kv, 16, dim)
-    run_prompt(dev, pool, pool.fill(lengths), lengths, new, heads)
+    table = pool.fill(lengths)
+    run_prompt(dev, pool, widened(table, 50) if wide else table, lengths, new, heads)
 
 
 @pytest.mark.parametrize("cache", ["f16", "e4m3"])
@@ -149,11 +166,12 @@ def test_lengths_below_zero(dev, least):
         run_prompt(dev, pool, table, lengths, [20, 0, 3], 4, window=window)
 
 
-@pytest.mark.parametrize("dim,cache", [(64, "f16"), (128, "f16"), (256, "f16"), (128, "e4m3")])
-def test_one_infinity_in_any_column_does_not_reach_the_rows_before_it(dev, dim, cache):
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("dim,cache", [(64, "f16"), (128, "f16"), (256, "f16"), (128, "e4m3"), (256, "e4m3")])
+def test_one_infinity_in_any_column_does_not_reach_the_rows_before_it(dev, dim, cache, wide):
     n = 40
     pool = Pool(np.random.default_rng(11), 4, 1, 16, dim, cache, scales=False)
-    table, q = pool.fill([n]), queries(np.random.default_rng(12), n, 1, dim)
+    table, q = pool.fill([n], width=40 if wide else None), queries(np.random.default_rng(12), n, 1, dim)
     clean = run_prompt(dev, pool, table, [n], [n], 1, q=q)
     want, tol, _ = attend_rows(pool, table, [n], [n], q, dim ** -0.5, 0, PROMPT_STEP)
     bad = (0x7F, np.uint8) if cache == "e4m3" else (0x7C00, np.uint16)   # (e4m3 has no infinity: NaN)
@@ -172,11 +190,12 @@ def test_one_infinity_in_any_column_does_not_reach_the_rows_before_it(dev, dim, 
     assert np.array_equal(run_prompt(dev, pool, table, [n], [n], 1, q=q).view(np.uint16), clean.view(np.uint16))
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-def test_rows_of_nothing_but_infinitely_low_scores_are_zeros(dev, dim):
+def test_rows_of_nothing_but_infinitely_low_scores_are_zeros(dev, dim, wide):
     n = 70
     pool = Pool(np.random.default_rng(13), 6, 1, 16, dim)
-    table = pool.fill([n])
+    table = pool.fill([n], width=40 if wide else None)
     q = np.abs(queries(np.random.default_rng(14), n, 2, dim)) + np.float16(0.25)
     pool.bits["k"][:, :, :, 3] = np.float16(-np.inf).view(np.uint16)
     kc, out, one = pool.upload(dev), Out(dev, q.shape, "f16"), Out(dev, (1, 2, dim), "f16")

@@ -29,7 +29,7 @@ def kernels():
 
 
 def test_every_form_is_there_and_none_spills(kernels):
-    for kernel, forms in (("k_kv_appendI", 2), ("k_kv_copy_pagesE", 1), ("k_attn_decodeI", 12), ("k_attn_joinI", 6), ("k_attn_promptI", 4), ("k_attn_prompt_pairsI", 2),
+    for kernel, forms in (("k_kv_appendI", 2), ("k_kv_copy_pagesE", 1), ("k_attn_decodeI", 12), ("k_attn_joinI", 6), ("k_attn_promptI", 4), ("k_attn_prompt_pairsI", 6),
                           ("k_attn_prompt_joinI", 6)):
         assert sum("%d%s" % (len(kernel) - 1, kernel) in name for name in kernels) == forms, kernel
     for name, (_, scratch) in kernels.items():
