@@ -19,11 +19,11 @@
 //
 // Bound by no single unit where prompts are long: a wave's 32 queries read as many bytes of keys and values from LDS (128 a cycle and compute unit) as
 // keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
-// 128 f16 values, 504 - 525 us (920 - 950 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
+// 128 f16 values, 500 - 525 us (920 - 960 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
 // that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
 // registers (579), and 64 queries a wave with the next tile's scores beside this one's exponentials leave one wave a SIMD (heads of 64: 376, with 32 queries
 // 309; of 128 they spill).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
-// heads of 64, 5.7 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.
+// heads of 64, 5.3 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.
 #include "twm_kv.h"
 #include "twm_slices.h"
 
