@@ -19,7 +19,7 @@
 // 5 us.)  Where no sequence is long, each sequence and unit has a workgroup of more waves to itself and nothing is joined.
 //
 // Bound by the reading of the cache where it is long: 32 sequences of up to 8192 tokens, 28 heads on 4 of 128 f16 values, 60.5 us (4.5 TB/s; a copy
-// reaches 5.1); 48 of up to 4096, 32 heads on 32, e4m3, 155 us (4.9 TB/s); one sequence of 131072 59 us, of 32768 21 (3.2 TB/s: two launches and
+// reaches 5.1); 48 of up to 4096, 32 heads on 32, e4m3, 155 us (4.9 TB/s); one sequence of 131072 58 us, of 32768 20.8 (3.2 TB/s: two launches and
 // eight steps a share are what is left), and of 777 tokens, 14 heads of 64 values, 9.2 us, which are the chain from the length by the table and the
 // keys to the sums.
 #include "twm_kv.h"
@@ -438,12 +438,17 @@ template <int D, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void k_
         for (uint32_t i = 0; i < kAhead; i++)
             if (w + kAtOnce * i <= last) add(s[i], part[i]);
     }
-    results[group][lane] = o;
-    if (lane == 0) sums[group] = float2{top, sum};
-    __syncthreads();
+    // the upper half of those that hold something joins the lower one (one after the other: 32768 tokens 21.4 us, now 20.8, of heads of 64 15.2 and 13.3)
+#pragma unroll
+    for (uint32_t half = kAtOnce / 2; half != 0; half /= 2) {
+        if (group >= half && group < 2 * half) {
+            results[group][lane] = o;
+            if (lane == 0) sums[group] = float2{top, sum};
+        }
+        __syncthreads();
+        if (group < half) add(sums[group + half], results[group + half][lane]);
+    }
     if (group != 0) return;
-#pragma unroll 4
-    for (uint32_t g = 1; g < kAtOnce; g++) add(sums[g], results[g][lane]);
     const float to = sum == 0.f ? 0.f : v_scale / sum;
     *(half4_any *)(a.out + (size_t)seq * a.out_stride + head * D + 4u * lane) =
         half4{(_Float16)(o[0] * to), (_Float16)(o[1] * to), (_Float16)(o[2] * to), (_Float16)(o[3] * to)};
@@ -487,7 +492,7 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
         hipLaunchKernelGGL((k_attn_decode<D, E4M3, kDecodeWaves, false>), dim3(d.shares * d.units), dim3(64 * kDecodeWaves), 0, s, d, 0u);
         if (const hipError_t error = hipGetLastError(); error != hipSuccess) return error;
         // sixteen parts of 128 values at once for few sequences, which have many, four otherwise (32 sequences up to 1024 tokens 20.7 us with
-        // sixteen, 18.9 with four; one of 32768 21.3 and 25.3)
+        // sixteen, 18.9 with four; one of 32768 21.3 and 25.3; both before the halves joined)
         if (a.seqs.seqs < 8)
             hipLaunchKernelGGL((k_attn_join<D, 512>), dim3(a.seqs.seqs, a.q_heads), dim3(512), 0, s, d);
         else
