@@ -2,7 +2,8 @@
 //
 //   out[h] = sum_t w_t v_t / sum_t w_t,   w_t = 2^(15 + c (s_t - m)),   s_t = q[h] . k_t,   c = scale * log2(e) * the head's scale of keys
 //
-// with m the largest s_t so far; whatever was summed is multiplied by 2^(c (m - m')) when it grows to m'.
+// with m the largest s_t so far; whatever was summed is multiplied by 2^(c (m - m')) when it grows to m'.  (The difference comes before the
+// product: c m by itself would be rounded, and where scores are large its rounding would be a power of two in the weight.)
 //
 // Keys and values are read once, from memory to registers, whatever the number of query heads that share them: up to sixteen heads are the
 // columns of the matrix instructions (16 x 16 x 32), thirty-two tokens at a time.  Scores come transposed, S^T = K Q^T, which leaves a lane
@@ -304,11 +305,11 @@ __global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, 
                 for (int i = 0; i < D / 16; i++) o[i] *= by;
                 top = most;
             }
-            const float base = 15.0f - (top == -INFINITY ? 0.f : top) * c;
+            const float from = top == -INFINITY ? 0.f : top;
             half2v p_hi[4], p_lo[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4], c, base)), y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4 + 1], c, base));
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4] - from, c, 15.0f)), y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4 + 1] - from, c, 15.0f));
                 sum += x + y;
                 p_hi[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
                 p_lo[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x - (float)p_hi[i][0], y - (float)p_hi[i][1]));

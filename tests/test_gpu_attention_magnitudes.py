@@ -1,0 +1,128 @@
+"""Attention over a paged key-value cache whose scores are large, up to the largest that finite f16 queries and keys make.  What a row comes to is
+known there whatever a score's own roundings are: one token's value where it sees one, or where one outweighs all others by far; the mean where
+all scores are the same sum of the same products; the formula on differences where every partial sum of the scores is exact."""
+import numpy as np
+import pytest
+
+import tensorwarp_amd as T
+from kv_oracle import DECODE_STEP, PROMPT_STEP, Pool, half_step_f16
+from test_gpu_attention import sequences
+from test_gpu_fp8 import At, Out
+
+pytestmark = pytest.mark.gpu
+
+# a short table and a wide one: a workgroup for each sequence or shares of all, waves in pairs or not (heads of 256 values are always in pairs)
+WIDTHS = [None, 400]
+TINY = 2.0 ** -20   # roundings in 32 bits: of the scale of values, of the weights' exponential, of the division by their sum
+
+
+@pytest.fixture(scope="module")
+def dev():
+    with T.WarpDevice(0) as d:
+        yield d
+
+
+def run(dev, kc, seqs, q, heads, **more):
+    out = Out(dev, q.shape, "f16")
+    if seqs.starts is None:
+        T.attention_decode(dev, kc, seqs, At(dev, q), heads, out, **more)
+    else:
+        T.attention_prompt(dev, kc, seqs, At(dev, q), q.shape[0], heads, out, **more)
+    return out.get().astype(np.float64)
+
+
+def near(got, want, tol):
+    assert np.isfinite(got).all()
+    off = np.abs(got - want) / (tol + half_step_f16(want))
+    assert off.max() <= 1.0, (off.max(), (off > 1).sum(), off.size)
+
+
+def filled(seed, dim, cache, n, width, keys):
+    """One sequence of n tokens whose values are random and whose keys (f16) `keys` gives, of one key-value head with pages of 16."""
+    pool = Pool(np.random.default_rng(seed), -(-n // 16) + 2, 1, 16, dim, cache, scales=False)
+    table = pool.fill([n], width)
+    if cache == "f16":
+        for t in range(n):
+            pool.bits["k"][table[0, t // 16], 0, t % 16] = keys[t].astype(np.float16).view(np.uint16)
+    return pool, table
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [700.0, 2000.0, 3001.0, 4000.0, 10007.0, 40000.0, 65504.0])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_a_row_that_sees_one_token_is_its_value(dev, size, sign, dim, cache, width):
+    # every row of 70 looks back one token.  e4m3 keys are as large as they come with the scales that make them so
+    n, heads = 70, 2
+    rng = np.random.default_rng(int(size) + dim)
+    pool, table = filled(int(size) + dim, dim, cache, n, width, np.full((n, dim), size))
+    if cache == "e4m3":
+        pool.bits["k"][:, 0] = np.where(rng.random((pool.shape[0], 16, dim)) < 0.5, 0x7E, 0x7D)   # 448 and 416
+        pool.scales = {"k": np.full(1, size / 448.0, np.float32), "v": np.full(1, 0.0371, np.float32)}
+    q = (sign * size * rng.choice([1.0, 1.0, 0.75], (n, heads, dim))).astype(np.float16)
+    v = np.repeat(pool.tokens("v", table[0], n).transpose(1, 0, 2), heads, axis=1)
+    kc = pool.upload(dev)
+    near(run(dev, kc, sequences(dev, table, [n], [n]), q, heads, window=1), v, TINY * np.abs(v))
+    each = np.arange(1, n + 1)
+    near(run(dev, kc, sequences(dev, np.repeat(table, n, axis=0), each), q, heads, window=1), v, TINY * np.abs(v))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [700.0, 2000.0, -3001.0, 10007.0, -40000.0, 65504.0])
+def test_equal_scores_are_the_mean(dev, size, dim, width):
+    # (the same products in the same order: scores are equal to the bit whatever their roundings are)
+    n, heads = 200, 3
+    pool, table = filled(3, dim, "f16", n, width, np.full((n, dim), abs(size)))
+    q = np.full((n, heads, dim), size, np.float16)
+    v = pool.tokens("v", table[0], n)[0]
+    counts = np.arange(1, n + 1)[:, None]
+    mean, magnitude = v.cumsum(0) / counts, np.abs(v).cumsum(0) / counts
+    for rows, seqs in ((slice(None), sequences(dev, table, [n], [n])), (slice(n - 1, n), sequences(dev, table, [n]))):
+        got = run(dev, pool.upload(dev), seqs, q[rows], heads)
+        near(got, np.repeat(mean[rows, None], heads, 1), np.repeat((((n + 16) * 2.0 ** -23 + TINY) * magnitude)[rows, None], heads, 1))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("size", [200.0, 2000.0, 4000.0, 40000.0])
+@pytest.mark.parametrize("at", [0, 63, 64, 130, 399])
+def test_one_token_that_outweighs_all_others(dev, at, size, dim, width):
+    # others score 0, or a tenth of it; the one comes first, later in the first tile, in later ones and last
+    n, heads = 400, 2
+    rng = np.random.default_rng(at)
+    keys = np.where(rng.random((n, 1)) < 0.5, 0.0, size / 10) * np.ones((n, dim))
+    keys[at] = size
+    pool, table = filled(at, dim, "f16", n, width, keys)
+    q = np.full((n - at, heads, dim), size, np.float16)
+    v = pool.tokens("v", table[0], n)[0, at]
+    for rows, seqs in ((n - at, sequences(dev, table, [n], [n - at])), (1, sequences(dev, table, [n]))):
+        got = run(dev, pool.upload(dev), seqs, q[:rows], heads)
+        near(got, np.broadcast_to(v, got.shape), TINY * np.abs(v))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("offset", [0, 1 << 10, 1 << 12, 1 << 13, 1 << 16, 1 << 19, 1 << 22, 1 << 25, -(1 << 16), -(1 << 25)])
+def test_differences_beside_a_large_sum_of_products(dev, offset, dim, width):
+    # scores offset + gap, gaps whole multiples of 4 from -60 to 60: every sum is exact in 32 bits.  Scaled, they are up to 15 apart and come in an
+    # order that raises the maximum now and then
+    n, heads, group = 333, 2, 16
+    rng = np.random.default_rng(abs(offset) % 1000 + dim)
+    gaps = 4.0 * rng.integers(0, group, n) - 60.0 * (np.arange(n) < 250) * (rng.random(n) < 0.9)
+    keys = np.zeros((n, dim))
+    keys[:, 0], keys[:, dim - 3] = abs(offset) / 4096.0 if offset else 0.0, gaps
+    pool, table = filled(dim, dim, "f16", n, width, keys)
+    q = np.zeros((n, heads, dim), np.float16)
+    q[:, :, 0], q[:, :, dim - 3] = np.sign(offset) * 4096.0, 1.0
+    v = pool.tokens("v", table[0], n)[0]
+    p = np.exp(0.125 * (gaps - gaps.max()))
+    total = p.cumsum()[:, None]
+    want, magnitude = (p[:, None] * v).cumsum(0) / total, (p[:, None] * np.abs(v)).cumsum(0) / total
+    # an exponent of up to 21.7 in base 2: half a step (2^-20) of its own, 2^-23 of it from the scale's roundings, as much again where the maximum was raised,
+    # together below 2^-17; twice over, for the weight and the sum, and the exponential's own: 2^-16.  In f16 2^-25 at least, of a weight 2^8
+    for rows, seqs, step in ((slice(None), sequences(dev, table, [n], [n]), PROMPT_STEP), (slice(n - 1, n), sequences(dev, table, [n]), DECODE_STEP)):
+        got = run(dev, pool.upload(dev), seqs, q[rows], heads, scale=0.125)
+        tol = ((step + 2.0 ** -16 + (n + 16) * 2.0 ** -23) * magnitude + 2.0 ** -33 * np.abs(v).sum(0))[rows]
+        near(got, np.repeat(want[rows, None], heads, 1), np.repeat(tol[:, None], heads, 1))
