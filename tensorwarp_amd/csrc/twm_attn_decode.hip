@@ -196,7 +196,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, 
         }
         // this share's steps of the sequence
         const uint32_t step0 = (uint32_t)(at - before), step1 = (uint32_t)min((uint64_t)span.steps, step0 + (end - at));
-        const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+        const float c = exponent_factor(a.kv, a.scale, kv_head);
 
         // Q^T: a lane's head's values, in the order in which it holds keys
         for (uint32_t x = threadIdx.x; x < D / 32 * 64; x += THREADS) {
@@ -416,7 +416,7 @@ template <int D, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void k_
     if (first == last) return;
     const uint32_t first_slot = 2 * (unit * d.shares + first) + (share_begin(d, total, first) < begin ? 1u : 0u);
     auto slot_of = [&](uint32_t w) { return (size_t)(w == first ? first_slot : 2 * (unit * d.shares + w)) * d.heads + h; };
-    const float c = a.scale * 1.44269504f * (a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f), v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
+    const float c = exponent_factor(a.kv, a.scale, kv_head), v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f;
     const uint32_t group = threadIdx.x / kLanes, lane = threadIdx.x % kLanes;
     float top = -INFINITY, sum = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};

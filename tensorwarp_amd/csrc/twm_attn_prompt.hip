@@ -191,7 +191,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
 #pragma unroll
         for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
-    const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+    const float c = exponent_factor(a.kv, a.scale, kv_head);
     float reference = -INFINITY, sum = 0.f;
     float16v o[D / 32];
 #pragma unroll
@@ -536,7 +536,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
 #pragma unroll
         for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
-    const float c = a.scale * 1.44269504f * (E4M3 && a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+    const float c = exponent_factor(a.kv, a.scale, kv_head);
     float reference = -INFINITY, sum = 0.f;
     float16v o[kHalf / 32];
 #pragma unroll
@@ -795,7 +795,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     const uint32_t slice = threadIdx.x / kEach, x = threadIdx.x % kEach, r = first_row + x % kHere, quad = x / kHere;   // (rows lie beside each other)
     const float2 *sums = job.part_sums + (size_t)blockIdx.x * job.splits * kRows + r;
     const float4v *from = job.parts + (size_t)blockIdx.x * job.splits * (D / 4 * kRows) + quad * kRows + r;
-    const float c = a.scale * 1.44269504f * (a.kv.k_scales ? a.kv.k_scales[kv_head] : 1.0f);
+    const float c = exponent_factor(a.kv, a.scale, kv_head);
     float top = -INFINITY, sum = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
     auto add = [&](const float2 &s, const float4v &part) {

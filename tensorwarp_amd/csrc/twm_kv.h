@@ -2,6 +2,8 @@
 #pragma once
 #include "twm_device.h"
 
+#include <cfloat>
+
 namespace twm {
 
 // Rows of queries and of fused projections begin at any element; the memory takes vectors there too
@@ -12,6 +14,15 @@ typedef float4v float4v_any __attribute__((aligned(4)));
 __device__ __forceinline__ size_t kv_chunk(const KvView &kv, uint32_t page, uint32_t head)
 {
     return (((size_t)page * kv.kv_heads + head) << kv.page_shift) * kv.dim;
+}
+
+// What a difference of scores is multiplied by, to base 2.  The product of three numbers passes what f32 holds although the two on the host's side
+// are finite: it is made in 64 bits, and kept within f32's range, where no weight differs from what lies beyond it (at the largest, the least
+// difference of two f16 rows' scores is 2^80 of an exponent, at the least the largest one 2^-80), and where it times -infinity is that.
+__device__ __forceinline__ float exponent_factor(const KvView &kv, float scale, uint32_t head)
+{
+    const float c = (float)((double)scale * 1.4426950408889634 * (kv.k_scales ? (double)kv.k_scales[head] : 1.0));
+    return c > FLT_MAX ? FLT_MAX : c < FLT_MIN ? FLT_MIN : c;   // (a NaN stays)
 }
 
 // v of this lane and of those before it, added up (by moves within rows of sixteen lanes, then across them)

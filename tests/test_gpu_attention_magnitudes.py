@@ -126,3 +126,53 @@ def test_differences_beside_a_large_sum_of_products(dev, offset, dim, width):
         got = run(dev, pool.upload(dev), seqs, q[rows], heads, scale=0.125)
         tol = ((step + 2.0 ** -16 + (n + 16) * 2.0 ** -23) * magnitude + 2.0 ** -33 * np.abs(v).sum(0))[rows]
         near(got, np.repeat(want[rows, None], heads, 1), np.repeat(tol[:, None], heads, 1))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale,k_scale", [(3.0e38, 1.0), (3.4e38, 0.03), (1.0e-38, 1.0), (1.5e-45, 1.0), (1.0, 3.0e38), (1.0e-30, 1.0e-30)])
+def test_the_largest_and_the_smallest_scales(dev, scale, k_scale, dim, cache, width):
+    # whole scores, so that differences are at least 1 or none: of the largest scales only the largest scores count, alike, of the smallest all do
+    n, heads = 150, 2
+    rng = np.random.default_rng(dim)
+    scores = rng.integers(-8, 4, n)
+    keys = np.zeros((n, dim))
+    keys[:, dim - 5] = scores
+    pool, table = filled(dim, dim, cache, n, width, keys)
+    if cache == "e4m3":
+        pool.scales["k"] = np.full(1, k_scale, np.float32)
+        codes = {0: 0, 1: 0x38, 2: 0x40, 3: 0x44, 4: 0x48, 5: 0x4A, 6: 0x4C, 7: 0x4E, 8: 0x50}   # e4m3 of the whole numbers up to 8
+        for t in range(n):
+            pool.bits["k"][table[0, t // 16], 0, t % 16] = 0
+            pool.bits["k"][table[0, t // 16], 0, t % 16, dim - 5] = codes[abs(scores[t])] | (0x80 if scores[t] < 0 else 0)
+    elif k_scale != 1.0:
+        return
+    q = np.zeros((n, heads, dim), np.float16)
+    q[:, :, dim - 5] = 1.0
+    v = pool.tokens("v", table[0], n)[0]
+    want, magnitude = np.zeros((n, dim)), np.zeros((n, dim))
+    for row in range(n):
+        seen = scores[:row + 1]
+        of = v[:row + 1][seen == seen.max()] if scale * k_scale > 1.0 else v[:row + 1]
+        want[row], magnitude[row] = of.mean(0), np.abs(of).mean(0)
+    for rows, seqs in ((slice(None), sequences(dev, table, [n], [n])), (slice(n - 1, n), sequences(dev, table, [n]))):
+        got = run(dev, pool.upload(dev), seqs, q[rows], heads, scale=scale)
+        near(got, np.repeat(want[rows, None], heads, 1), np.repeat((((n + 16) * 2.0 ** -23 + TINY) * magnitude)[rows, None], heads, 1))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("up", [100, -100])
+def test_a_scale_of_scores_and_one_of_keys_that_meet_in_the_middle(dev, up, dim, width):
+    # 2^up times 2^-up of both: the same bits as without
+    n, heads = 90, 4
+    pool, table = filled(1, dim, "e4m3", n, width, None)
+    q = (1.5 * np.random.default_rng(2).standard_normal((n, heads, dim))).astype(np.float16)
+    results = []
+    for scale, k_scale in ((0.125, 0.03125), (0.125 * 2.0 ** up, 0.03125 * 2.0 ** -up)):
+        pool.scales["k"] = np.full(1, k_scale, np.float32)
+        kc = pool.upload(dev)
+        results.append([run(dev, kc, s, rows, heads, scale=scale) for s, rows in ((sequences(dev, table, [n], [n]), q), (sequences(dev, table, [n]), q[:1]))])
+    for a, b in zip(*results):
+        assert np.isfinite(a).all() and np.array_equal(a, b)
