@@ -11,8 +11,9 @@
 // takes the tokens in any order that both operands agree on, so rows 4 g + i of its two blocks are tokens 8 g + i and 8 g + 4 + i.  V^T comes from
 // LDS through the transposing reads; every wave has a buffer of its own there and no other wave is waited for.
 //
-// Weights enter the product as two f16 terms, the first one cut off and the second what it leaves: both are positive, and at least the
-// smallest f16 number where a token is seen (2^-39 of the largest weight), so that an infinite value times its weight is that infinity.
+// Weights enter the product as two f16 terms, the first one cut off and the second what it leaves.  A term that is 0 times an infinite value is NaN,
+// where the formula has that infinity: a wave whose sums have come to NaN goes over its tokens once more with terms of at least the smallest f16 number
+// (both 2^-38 of the largest weight; what is not seen has values of 0).
 //
 // All tokens of all sequences, in steps of 128, are dealt out evenly among as many workgroups for each key-value head as the chip holds at once,
 // which find their share from the lengths by themselves: a long sequence is cut into many shares, several short ones make one.  What a share
@@ -117,8 +118,8 @@ __device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
     return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// 2^(c (m - m')), of sums that hold something
-__device__ __forceinline__ float shrink(float m, float to, float c) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - to) * c); }
+// 2^(c (m - m')); never 0, so that an infinite sum stays one (and 2^-126 of nothing is nothing where m is -infinity)
+__device__ __forceinline__ float shrink(float m, float to, float c) { return __builtin_amdgcn_exp2f(fmaxf((m - to) * c, -126.0f)); }
 
 // Workgroups of four waves that share a compute unit, by their registers; waves of a workgroup that has a sequence to itself
 template <int D, bool E4M3> constexpr uint32_t kDecodePerUnit = D == 256 ? (E4M3 ? 2 : 1) : D == 128 ? (E4M3 ? 3 : 2) : 3;
@@ -204,16 +205,14 @@ __global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, 
             queries[x] = *(const half8_any *)(a.q + (size_t)seq * a.q_stride + (head0 + head) * D + (E4M3 ? (i / 2) * 64 + g * 16 + (i % 2) * 8 : i * 32 + g * 8));
         }
 
-        float top = -INFINITY, sum = 0.f;
+        float top, sum;
         float4v o[D / 16];
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
 
         // Pages of this wave's tokens, 32 a step: a lane looks one of a step's halves up, the wave those of 32 steps at once
         const int *table = a.seqs.tables + (size_t)seq * a.seqs.table_stride;
         const char *const k_base = (const char *)a.kv.k, *const v_base = (const char *)a.kv.v;
         int page_of = -1, page0 = -1, page1 = -1;
-        uint32_t looked_up = 0;
+        uint32_t looked_up;
         auto pages_of = [&](int t) {
             if ((looked_up & 31u) == 0) {
                 const int64_t token = t + (int64_t)(lane >> 1) * (int)STEP + (int)(lane & 1u) * 16;
@@ -245,97 +244,108 @@ __global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, 
             }
         };
         const int stop = WHOLE ? span.hi : min(span.hi, span.first + (int)(step1 * STEP));
-        int t = span.first + (int)(step0 * STEP + wave * 32u);
-        if (t < stop) {
-            pages_of(t);
-            load(t);
-        }
-        __syncthreads();
-        for (; t < stop; t += (int)STEP) {
-            const bool whole = k_there && t >= span.lo && t + 32 <= span.hi;
-            const bool in0 = (uint32_t)page0 < a.kv.pages, in1 = (uint32_t)page1 < a.kv.pages;
-            // values to LDS; what is not seen is zeros there, whatever it may be in memory
+        for (uint32_t least = 0;; least = 0x00010001u) {   // the least of two f16 terms: 0, or 2^-24
+            top = -INFINITY;
+            sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const uint32_t row = i * kRowsPerLoad + lane / kLanesPerRow;
+            for (int i = 0; i < D / 16; i++) o[i] = float4v{0.f, 0.f, 0.f, 0.f};
+            looked_up = 0;
+            int t = span.first + (int)(step0 * STEP + wave * 32u);
+            if (t < stop) {
+                pages_of(t);
+                load(t);
+            }
+            if (least == 0) __syncthreads();
+            for (; t < stop; t += (int)STEP) {
+                const bool whole = k_there && t >= span.lo && t + 32 <= span.hi;
+                const bool in0 = (uint32_t)page0 < a.kv.pages, in1 = (uint32_t)page1 < a.kv.pages;
+                // values to LDS; what is not seen is zeros there, whatever it may be in memory
+#pragma unroll
+                for (int i = 0; i < NV; i++) {
+                    const uint32_t row = i * kRowsPerLoad + lane / kLanesPerRow;
+                    if (!whole) {
+                        const int token = t + (int)row;
+                        const bool seen = token >= span.lo && token < span.hi && (row < 16 ? in0 : in1);
+                        v[i] = seen ? v[i] : uint4v{0u, 0u, 0u, 0u};
+                    }
+                    *(uint4v *)(buffer + row * kStride + lane % kLanesPerRow * 16u) = v[i];
+                }
+                float4v s[2];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    s[b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) {
+                        half8 key;
+                        if constexpr (E4M3)
+                            key = to_f16(k[b][i / 2][(i % 2) * 2], k[b][i / 2][(i % 2) * 2 + 1]);
+                        else
+                            key = __builtin_bit_cast(half8, k[b][i]);
+                        s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, queries[i * 64 + lane], s[b], 0, 0, 0);
+                    }
+                }
+                const int next = t + (int)STEP;
+                if (next < stop) {
+                    pages_of(next);
+                    load(next);
+                }
+                // scores of tokens t + 8 quarter + 4 b + i
                 if (!whole) {
-                    const int token = t + (int)row;
-                    const bool seen = token >= span.lo && token < span.hi && (row < 16 ? in0 : in1);
-                    v[i] = seen ? v[i] : uint4v{0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int token = t + 8 * (int)quarter + i;
+                        const bool one = token >= span.lo && token < span.hi && (quarter < 2 ? in0 : in1);
+                        s[i / 4][i % 4] = one ? s[i / 4][i % 4] : __int_as_float(kNoScore);
+                    }
                 }
-                *(uint4v *)(buffer + row * kStride + lane % kLanesPerRow * 16u) = v[i];
-            }
-            float4v s[2];
+                float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+                most = fmaxf(top, max_over_quarters(most));
+                if (__any(most > top)) {
+                    const float by = shrink(top, most, c);
+                    sum *= by;
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                s[b] = float4v{0.f, 0.f, 0.f, 0.f};
+                    for (int i = 0; i < D / 16; i++) o[i] *= by;
+                    top = most;
+                }
+                const float from = top == -INFINITY ? 0.f : top;
+                half2v p_hi[4], p_lo[4];
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) {
-                    half8 key;
-                    if constexpr (E4M3)
-                        key = to_f16(k[b][i / 2][(i % 2) * 2], k[b][i / 2][(i % 2) * 2 + 1]);
-                    else
-                        key = __builtin_bit_cast(half8, k[b][i]);
-                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, queries[i * 64 + lane], s[b], 0, 0, 0);
+                for (int i = 0; i < 4; i++) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4] - from, c, 15.0f)), y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4 + 1] - from, c, 15.0f));
+                    sum += x + y;
+                    p_hi[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
+                    p_lo[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x - (float)p_hi[i][0], y - (float)p_hi[i][1]));
+                    if constexpr (!E4M3) {
+                        p_hi[i] = __builtin_elementwise_max(p_hi[i], __builtin_bit_cast(half2v, least));
+                        p_lo[i] = __builtin_elementwise_max(p_lo[i], __builtin_bit_cast(half2v, least));
+                    }
+                }
+                const half8 hi = {p_hi[0][0], p_hi[0][1], p_hi[1][0], p_hi[1][1], p_hi[2][0], p_hi[2][1], p_hi[3][0], p_hi[3][1]};
+                const half8 lo = {p_lo[0][0], p_lo[0][1], p_lo[1][0], p_lo[1][1], p_lo[2][0], p_lo[2][1], p_lo[3][0], p_lo[3][1]};
+                // (the wave's own stores have reached LDS: its reads come after them, in order)
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    half8 value;
+                    if constexpr (E4M3) {
+                        const int2v codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                            (TWM_LDS(int2v) *)(buffer + (8u * quarter + (col >> 1)) * kStride + 16u * i + 8u * (col & 1u)));
+                        value = to_f16((unsigned)codes[0], (unsigned)codes[1]);
+                    } else {
+                        const char *from = buffer + (8u * quarter + (col >> 2)) * kStride + 32u * i + 8u * (col & 3u);
+                        const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)from));
+                        const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(from + 4 * kStride)));
+                        value = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                    }
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, hi, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, lo, o[i], 0, 0, 0);
                 }
             }
-            const int next = t + (int)STEP;
-            if (next < stop) {
-                pages_of(next);
-                load(next);
-            }
-            // scores of tokens t + 8 quarter + 4 b + i
-            uint32_t seen = 0xFFu;
-            if (!whole) {
-                seen = 0;
+            if (E4M3 || least != 0) break;   // (e4m3 has no infinity)
+            float4v all = o[0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int token = t + 8 * (int)quarter + i;
-                    const bool one = token >= span.lo && token < span.hi && (quarter < 2 ? in0 : in1);
-                    seen |= one ? 1u << i : 0u;
-                    s[i / 4][i % 4] = one ? s[i / 4][i % 4] : __int_as_float(kNoScore);
-                }
-            }
-            float most = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            most = fmaxf(top, max_over_quarters(most));
-            if (__any(most > top)) {
-                const float by = shrink(top, most, c);
-                sum *= by;
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) o[i] *= by;
-                top = most;
-            }
-            const float from = top == -INFINITY ? 0.f : top;
-            half2v p_hi[4], p_lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4] - from, c, 15.0f)), y = __builtin_amdgcn_exp2f(fmaf(s[i / 2][(2 * i) % 4 + 1] - from, c, 15.0f));
-                sum += x + y;
-                p_hi[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x, y));
-                p_lo[i] = __builtin_bit_cast(half2v, __builtin_amdgcn_cvt_pkrtz(x - (float)p_hi[i][0], y - (float)p_hi[i][1]));
-                const uint32_t least = (seen >> (2 * i) & 1u) | (seen >> (2 * i + 1) & 1u) << 16;   // 2^-24
-                p_hi[i] = __builtin_elementwise_max(p_hi[i], __builtin_bit_cast(half2v, least));
-                p_lo[i] = __builtin_elementwise_max(p_lo[i], __builtin_bit_cast(half2v, least));
-            }
-            const half8 hi = {p_hi[0][0], p_hi[0][1], p_hi[1][0], p_hi[1][1], p_hi[2][0], p_hi[2][1], p_hi[3][0], p_hi[3][1]};
-            const half8 lo = {p_lo[0][0], p_lo[0][1], p_lo[1][0], p_lo[1][1], p_lo[2][0], p_lo[2][1], p_lo[3][0], p_lo[3][1]};
-            // (the wave's own stores have reached LDS: its reads come after them, in order)
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                half8 value;
-                if constexpr (E4M3) {
-                    const int2v codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                        (TWM_LDS(int2v) *)(buffer + (8u * quarter + (col >> 1)) * kStride + 16u * i + 8u * (col & 1u)));
-                    value = to_f16((unsigned)codes[0], (unsigned)codes[1]);
-                } else {
-                    const char *from = buffer + (8u * quarter + (col >> 2)) * kStride + 32u * i + 8u * (col & 3u);
-                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)from));
-                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(from + 4 * kStride)));
-                    value = half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-                }
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, hi, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value, lo, o[i], 0, 0, 0);
-            }
+            for (int i = 1; i < D / 16; i++) all += o[i];
+            const float one = (all[0] + all[1]) + (all[2] + all[3]);
+            if (!__any(one != one)) break;
         }
 
         // the waves' sums, brought to the largest score of all and added in wave order

@@ -176,3 +176,39 @@ def test_a_scale_of_scores_and_one_of_keys_that_meet_in_the_middle(dev, up, dim,
         results.append([run(dev, kc, s, rows, heads, scale=scale) for s, rows in ((sequences(dev, table, [n], [n]), q), (sequences(dev, table, [n]), q[:1]))])
     for a, b in zip(*results):
         assert np.isfinite(a).all() and np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("value", [3.0, 60000.0])
+@pytest.mark.parametrize("infinite", [False, True])
+def test_tokens_without_weight_add_nothing(dev, infinite, value, dim, width):
+    # one token, the second, outweighs a thousand others by e^200: 0 in 32 bits.  Its value is the result, zeros in all but one column, however large the others' are.
+    # With an infinite one among them, in a column of its own and with a weight of its own, rows that do not see it stay as they are
+    n, heads = 1000, 2
+    pool = Pool(np.random.default_rng(1), 70, 1, 16, dim)
+    table = pool.fill([n], width)
+    bits = lambda x: np.float16(x).view(np.uint16)
+    at = lambda t: (table[0, t // 16], 0, t % 16)
+    for t in range(n):
+        pool.bits["k"][at(t)], pool.bits["v"][at(t)] = 0, bits(value)
+    pool.bits["k"][at(1)][7], pool.bits["v"][at(1)] = bits(200.0), 0
+    pool.bits["v"][at(1)][9] = bits(0.375)
+    if infinite:
+        pool.bits["k"][at(600)][7], pool.bits["v"][at(600)][11] = bits(198.0), bits(np.inf)
+        pool.bits["v"][at(600)][12] = 0
+    q = np.zeros((n - 1, heads, dim), np.float16)
+    q[:, :, 7] = 1.0
+    want = np.zeros(dim)
+    want[9] = 0.375
+    for rows, seqs in ((n - 1, sequences(dev, table, [n], [n - 1])), (1, sequences(dev, table, [n]))):
+        got = run(dev, pool.upload(dev), seqs, q[:rows], heads, scale=1.0)
+        if not infinite:
+            assert np.array_equal(got, np.broadcast_to(want, got.shape))
+            continue
+        # rows from the infinite token on: its column is infinite; column 12, which it and the first have zeros in, has 2^-38 of the others' at most
+        behind = slice(599, None) if rows > 1 else slice(None)
+        assert np.isposinf(got[behind, :, 11]).all()
+        assert np.abs(got[behind, :, 12]).max() <= n * 2.0 ** -38 * value + 2.0 ** -25
+        if rows > 1:
+            assert np.array_equal(got[:599], np.broadcast_to(want, got[:599].shape))
