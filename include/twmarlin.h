@@ -585,7 +585,8 @@ int twm_kv_append(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *se
  * sequence s, the last `window` of them if window is not 0, and out row s likewise:
  *   out[h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale * q[h] . k_t - max),   k_t and v_t of key-value head h / (q_heads / kv_heads)
  * q_heads is a multiple of kv_heads; scale is above 0.  A row without tokens, or whose scores are all -infinity, is zeros.  Scores, sums and weights are held in 32
- * bits (the products take the weights as two f16 terms); only what a row sees counts, whatever else the pages hold.  starts_dev is not read.  Uses the
+ * bits (the products take the weights as two f16 terms); only what a row sees counts, whatever else the pages hold.  An infinite value that a row sees
+ * makes its column that infinity, however little it weighs, or NaN beside the other one.  starts_dev is not read.  Uses the
  * context's scratch.  Deterministic for given lengths and sizes. */
 int twm_attn_decode(twm_ctx *ctx, const twm_kv_cache *cache, const twm_kv_seqs *seqs, const uint16_t *q_dev, uint32_t q_stride,
                     uint32_t q_heads, float scale, uint32_t window, uint16_t *out_dev, uint32_t out_stride);

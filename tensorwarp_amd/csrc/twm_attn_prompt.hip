@@ -15,7 +15,8 @@
 //
 // Where a tile holds tokens that some of the queries do not see, weights alone would not keep an infinity or a NaN away from these (0 times
 // either is NaN): there values are looked through first, rows that nobody sees become zeros, and if anything not finite is left, the tile's
-// products are made one token at a time, for those who see it.
+// products are made one token at a time, for those who see it.  So they are once more in all tiles where sums came to NaN: an infinite value times a weight
+// that f16 rounds to 0 is NaN in a matrix product, where the formula has that infinity.
 //
 // Bound by no single unit where prompts are long: a wave's 32 queries read as many bytes of keys and values from LDS (128 a cycle and compute unit) as
 // keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
@@ -28,6 +29,7 @@
 #include "twm_slices.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -55,6 +57,10 @@ __device__ __forceinline__ float sum_of_halves(float v)
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+
+// What sums are multiplied by where the reference moves: 2^(c (from - to)), never 0, so that an infinite sum stays one (of nothing, from = -infinity,
+// nothing is left)
+__device__ __forceinline__ float shrink(float from, float to, float c) { return __builtin_amdgcn_exp2f(fmaxf((from - to) * c, -126.0f)); }
 
 // eight codes as f16 (exact)
 __device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
@@ -148,7 +154,8 @@ template <int D> constexpr uint32_t kPairsLds = 2 * kPromptTile * D * 2 + kPromp
 
 }  // namespace
 
-template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_prompt(const Prompt job)
+// Two workgroups a compute unit; of heads of 64 f16 values three, whose registers just suffice (8192 rows of 28 heads on 4 297 us, with two 308)
+template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 ? 3 : 2)) void k_attn_prompt(const Prompt job)
 {
     constexpr int KT = kPromptTile, kGroups = KT / 16;   // tokens of a tile; runs of 16, each within a page
     constexpr uint32_t kUnits = D / 8, kRow = D * 2;        // of 16 bytes, bytes of a row in LDS
@@ -168,7 +175,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
     uint32_t key_tiles;
-    const uint32_t parts = parts_of(mine, job, KT, &key_tiles);
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(parts_of(mine, job, KT, &key_tiles));
     if (split >= parts) return;
 
     auto begin_of = [&](int position) { return prompt_begin(a, position); };
@@ -192,12 +199,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
     const float c = exponent_factor(a.kv, a.scale, kv_head);
-    float reference = -INFINITY, sum = 0.f;
+    float reference, sum;
     float16v o[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
     // The place of a unit in its row of keys (of which 16 rows are read at once) and of values (four rows, four units of each)
     auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
@@ -261,6 +264,14 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
             }
         }
     };
+    // whether it holds for any lane of any wave; not again before another meeting of the waves
+    uint32_t *const flags = (uint32_t *)(lds + kPromptLds<D> - 16);
+    auto any_wave = [&](bool mine) {
+        const bool any = __any(mine);
+        if (lane == 0) flags[wave] = any;
+        __syncthreads();
+        return (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
+    };
     // everything that this wave has brought in and kept has arrived, and that of the other waves
     auto arrived = [&]() {
         __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
@@ -268,16 +279,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     };
 
     const int high_begin = begin_of(high);
-    uint32_t there = 0, buf = 0;
-    Pages next{-1, 0};
-    if (t_begin < last) {
-        look_up(t_begin);
-        const Pages pages = find_pages(t_begin);
-        there = pages.there;
-        bring(t_begin, pages, 0);
-        keep(0);
-        next = find_pages(t_begin + KT);
-    }
+    uint32_t there, buf;
+    Pages next;
     // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
     const uint32_t k_at = col * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
     const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
@@ -316,7 +319,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
     };
     // a weight would pass 2^15: the reference moves, and what is summed with it
     auto raise = [&](float most) {
-        const float raised = fmaxf(reference, most), by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((reference - raised) * c);
+        const float raised = fmaxf(reference, most), by = shrink(reference, raised, c);
         sum *= by;
 #pragma unroll
         for (int i = 0; i < D / 32; i++) o[i] *= by;
@@ -350,12 +353,10 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
                 o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p[b], o[i], 0, 0, 0);
             }
     };
-    // the last tile that everyone sees whole ends here
-    const int whole_end = min(low + 1, last);
-    arrived();
-    int t0 = t_begin;
-    bool advanced = false;
-    uint32_t there_now = 0;
+    int whole_end = min(low + 1, last);   // the last tile that everyone sees whole ends here
+    int t0;
+    bool advanced;
+    uint32_t there_now;
     auto advance = [&]() {   // once a tile: the one behind it begins its way, and the pages of the one after that are known
         if (advanced) return;
         if (t0 + KT < last) bring(t0 + KT, next, buf ^ 1u);
@@ -371,120 +372,151 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, 2) void k_attn_pro
         advanced = false;
         arrived();
     };
-    there_now = there;
-    while (t0 < last) {
-        // tiles that every row of the workgroup sees whole
-        float raise_to = -INFINITY;
-        while (t0 >= high_begin && t0 + KT <= whole_end && there_now == (1u << kGroups) - 1u) {
-            const char *const tile = lds + buf * kTile;
-            advance();
-            float16v s[KT / 32];
-            half8 p[KT / 16];
-            scores(tile, s);
-            const float most = largest(s);
-            if (__any((most - reference) * c > 7.0f || fabsf(reference) * c > 1024.0f)) {
-                raise_to = most;   // (rare; outside of this loop, so that the sums never move within it)
-                break;
+    for (;;) {
+        reference = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+        there = buf = 0;
+        next = Pages{-1, 0};
+        if (t_begin < last) {
+            look_up(t_begin);
+            const Pages pages = find_pages(t_begin);
+            there = pages.there;
+            bring(t_begin, pages, 0);
+            keep(0);
+            next = find_pages(t_begin + KT);
+        }
+        arrived();
+        t0 = t_begin;
+        advanced = false;
+        there_now = there;
+        while (t0 < last) {
+            // tiles that every row of the workgroup sees whole
+            float raise_to = -INFINITY;
+            while (t0 >= high_begin && t0 + KT <= whole_end && there_now == (1u << kGroups) - 1u) {
+                const char *const tile = lds + buf * kTile;
+                advance();
+                float16v s[KT / 32];
+                half8 p[KT / 16];
+                scores(tile, s);
+                const float most = largest(s);
+                if (__any((most - reference) * c > 7.0f || fabsf(reference) * c > 1024.0f)) {
+                    raise_to = most;   // (rare; outside of this loop, so that the sums never move within it)
+                    break;
+                }
+                weigh(std::true_type{}, s, p);
+                add_values(tile, p);
+                turn();
             }
-            weigh(std::true_type{}, s, p);
-            add_values(tile, p);
+            if (__any((raise_to - reference) * c > 7.0f)) {
+                raise(raise_to);
+                continue;
+            }
+            if (t0 >= last) break;
+            // one that some do not, or that lacks pages, or one of large scores
+            const char *const tile = lds + buf * kTile;
+            const uint32_t present = there_now;
+            advance();
+            const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
+            half8 p[KT / 16];
+            if (!idle) {
+                float16v s[KT / 32];
+                scores(tile, s);
+                if (t0 >= high_begin && present == (1u << kGroups) - 1u) {   // (everyone sees its beginning)
+                    const int seen = my_end - t0 - 4 * (int)half;
+#pragma unroll
+                    for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) s[b][j] = 32 * b + 8 * (j / 4) + j % 4 < seen ? s[b][j] : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int b = 0; b < KT / 32; b++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            // (tokens from the first seen one on, as unsigned numbers, against their number: none where the page is absent)
+                            const uint32_t seen = present >> (2 * b + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
+                            s[b][j] = (uint32_t)(t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[b][j] : -INFINITY;
+                        }
+                }
+                const float most = largest(s);
+                if (__any((most - reference) * c > 7.0f)) raise(most);
+                weigh(std::false_type{}, s, p);
+            }
+            // values: rows that nobody sees become zeros, the others are looked through
+            constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
+            const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
+            const int token = t0 + (int)looked;
+            const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
+            half2v found = {(_Float16)0.f, (_Float16)0.f};
+#pragma unroll
+            for (uint32_t i = 0; i < kEach; i++) {
+                uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
+                if (dead)
+                    *at = uint4v{0u, 0u, 0u, 0u};
+                else
+                    found = times_0(*at, found);
+            }
+            const bool single = any_wave((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
+            if (single) __syncthreads();   // (flags are read)
+            if (!idle && !single) {
+                add_values(tile, p);
+            } else if (!idle) {
+                // the wave's weights to LDS (every wave is done with the tile's keys), then one token after the other
+                _Float16 *weights = (_Float16 *)(lds + (D == 64 ? 4 * kTile : buf * kTile)) + wave * (KT * 32);
+#pragma unroll
+                for (int b = 0; b < KT / 16; b++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) weights[(16 * b + 8 * (j / 4) + 4 * (int)half + j % 4) * 32 + (int)col] = p[b][j];
+                for (int r = 0; r < KT; r++) {
+                    const int at = t0 + r;
+                    if (at < first || at >= last || !(present >> (r / 16) & 1u)) continue;
+                    const bool seen = at >= my_begin && at < my_end;
+                    const float w = fmaxf((float)weights[r * 32 + (int)col], FLT_MIN);   // (an infinite value times 0 would be NaN)
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
+                        }
+                }
+            }
             turn();
         }
-        if (__any((raise_to - reference) * c > 7.0f)) {
-            raise(raise_to);
-            continue;
-        }
-        if (t0 >= last) break;
-        // one that some do not, or that lacks pages, or one of large scores
-        const char *const tile = lds + buf * kTile;
-        const uint32_t present = there_now;
-        advance();
-        const bool idle = t0 > wave_high || t0 + KT <= begin_of(wave_low);   // nothing for this wave
-        half8 p[KT / 16];
-        if (!idle) {
-            float16v s[KT / 32];
-            scores(tile, s);
-            if (t0 >= high_begin && present == (1u << kGroups) - 1u) {   // (everyone sees its beginning)
-                const int seen = my_end - t0 - 4 * (int)half;
+        if (E4M3 || max(t_begin, high_begin) + KT > whole_end) break;   // (no tile was taken as whole; e4m3 has no infinity)
+        // Sums that are NaN may be an infinite value times a weight that f16 holds as 0, which is that infinity: once more, with no tile taken as whole
+        float one = 0.f;
 #pragma unroll
-                for (int b = 0; b < KT / 32; b++)
+        for (int i = 0; i < D / 32; i++)
 #pragma unroll
-                    for (int j = 0; j < 16; j++) s[b][j] = 32 * b + 8 * (j / 4) + j % 4 < seen ? s[b][j] : -INFINITY;
-            } else {
-#pragma unroll
-                for (int b = 0; b < KT / 32; b++)
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        // (tokens from the first seen one on, as unsigned numbers, against their number: none where the page is absent)
-                        const uint32_t seen = present >> (2 * b + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
-                        s[b][j] = (uint32_t)(t0 + 32 * b + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[b][j] : -INFINITY;
-                    }
-            }
-            const float most = largest(s);
-            if (__any((most - reference) * c > 7.0f)) raise(most);
-            weigh(std::false_type{}, s, p);
-        }
-        // values: rows that nobody sees become zeros, the others are looked through
-        constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
-        const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
-        const int token = t0 + (int)looked;
-        const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
-        half2v found = {(_Float16)0.f, (_Float16)0.f};
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; i++) {
-            uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
-            if (dead)
-                *at = uint4v{0u, 0u, 0u, 0u};
-            else
-                found = times_0(*at, found);
-        }
-        uint32_t *const flags = (uint32_t *)(lds + kPromptLds<D> - 16);
-        const bool bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
-        if (lane == 0) flags[wave] = bad;
-        __syncthreads();
-        const bool single = (flags[0] | flags[1] | flags[2] | flags[3]) != 0;
-        if (single) __syncthreads();   // (flags are read)
-        if (!idle && !single) {
-            add_values(tile, p);
-        } else if (!idle) {
-            // the wave's weights to LDS (every wave is done with the tile's keys), then one token after the other
-            _Float16 *weights = (_Float16 *)(lds + (D == 64 ? 4 * kTile : buf * kTile)) + wave * (KT * 32);
-#pragma unroll
-            for (int b = 0; b < KT / 16; b++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) weights[(16 * b + 8 * (j / 4) + 4 * (int)half + j % 4) * 32 + (int)col] = p[b][j];
-            for (int r = 0; r < KT; r++) {
-                const int at = t0 + r;
-                if (at < first || at >= last || !(present >> (r / 16) & 1u)) continue;
-                const bool seen = at >= my_begin && at < my_end;
-                const float w = (float)weights[r * 32 + (int)col];
-#pragma unroll
-                for (int i = 0; i < D / 32; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
-                    }
-            }
-        }
-        turn();
+            for (int j = 0; j < 16; j++) one += o[i][j];
+        if (!any_wave(one != one)) break;
+        whole_end = t_begin;
     }
 
     sum = sum_of_halves(sum);
+    // (where results go is made anew: held all along it would take the registers that a third workgroup of heads of 64 needs)
+    uint32_t me = lane;
+    asm volatile("" : "+v"(me));
+    const uint32_t out_row = wave_row + (me & 31u), out_half = me >> 5;
     if (parts > 1) {
         // to scratch, rows beside each other
-        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + wave_row - row0 + col;
+        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + out_row - row0;
 #pragma unroll
         for (int i = 0; i < D / 32; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (row < rows)
-                    to[(8u * i + 2u * j + half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-        if (row < rows && half == 0) job.part_sums[(size_t)blockIdx.x * kRows + wave_row - row0 + col] = float2{reference, sum};
-    } else if (row < rows) {
+                if (out_row < rows)
+                    to[(8u * i + 2u * j + out_half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        if (out_row < rows && out_half == 0) job.part_sums[(size_t)blockIdx.x * kRows + out_row - row0] = float2{reference, sum};
+    } else if (out_row < rows) {
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
-        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + 4u * half;
+        const uint32_t token = job.by_group(out_row), head = kv_head * a.group + (out_row - token * a.group);
+        _Float16 *out = a.out + (size_t)(start + (int)token) * a.out_stride + head * D + 4u * out_half;
 #pragma unroll
         for (int i = 0; i < D / 32; i++)
 #pragma unroll
@@ -518,7 +550,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
     const int start = mine.start, before = mine.before;
     const int capacity = a.kv.pages ? (int)(a.seqs.table_stride << a.kv.page_shift) : 0;
     uint32_t key_tiles;
-    const uint32_t parts = parts_of(mine, job, KT, &key_tiles);
+    const uint32_t parts = __builtin_amdgcn_readfirstlane(parts_of(mine, job, KT, &key_tiles));
     if (split >= parts) return;
 
     const uint32_t sharer = wave & 1u, wave_row = row0 + wave / 2u * 32u;
@@ -537,12 +569,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
         for (int i = 0; i < D / 16; i++) q[i] = *(const half8_any *)(from + 16 * i);
     }
     const float c = exponent_factor(a.kv, a.scale, kv_head);
-    float reference = -INFINITY, sum = 0.f;
+    float reference, sum;
     float16v o[kHalf / 32];
-#pragma unroll
-    for (int i = 0; i < (int)kHalf / 32; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) o[i][j] = 0.f;
 
     auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
     auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); };
@@ -606,7 +634,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
         __syncthreads();
     };
 
-    const int high_begin = prompt_begin(a, high), whole_end = min(low + 1, last);
+    const int high_begin = prompt_begin(a, high);
+    int whole_end = min(low + 1, last);
     const uint32_t k_at = (32u * sharer + col) * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
     const uint32_t v_at = (kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u) ^ sharer * kHalf * 2u;
     const half8 *const pair_weights = weights + (wave & ~1u) * 128u + lane;
@@ -627,128 +656,148 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
         weights[wave * 128u + 64u + lane] = p[1];
     };
 
-    int t0 = t_begin;
-    uint32_t there = 0;
-    Pages next{-1, 0};
-    if (t0 < last) {
-        look_up(t0);
-        const Pages now = find_pages(t0);
-        there = now.there;
-        bring(t0, now.mine, false);
-        keep(false);
-        bring(t0, now.mine, true);
-        next = find_pages(t0 + KT);
-        arrived();
-    }
-    while (t0 < last) {
-        const bool more = t0 + KT < last;
-        if constexpr (E4M3) {
-            // values of this tile to LDS; the next one begins its way
-            keep(true);
-            if (more) bring(t0 + KT, next.mine, false);
+    for (;;) {
+        reference = -INFINITY;
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+        int t0 = t_begin;
+        uint32_t there = 0;
+        Pages next{-1, 0};
+        if (t0 < last) {
+            look_up(t0);
+            const Pages now = find_pages(t0);
+            there = now.there;
+            bring(t0, now.mine, false);
+            keep(false);
+            bring(t0, now.mine, true);
+            next = find_pages(t0 + KT);
+            arrived();
         }
-        uint32_t keys_at = k_at;
-        asm volatile("" : "+v"(keys_at));   // (sixteen addresses that are made anew, not held)
-#pragma unroll
-        for (int j = 0; j < 16; j++) s[j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 16; i++) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(lds + (keys_at ^ i << 5)), q[i], s, 0, 0, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int i = 0; i < D / 16 - 4; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
-        const bool whole = t0 >= high_begin && t0 + KT <= whole_end && there == (1u << kGroups) - 1u;
-        bool bad = false;
-        if (!whole) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const uint32_t seen = there >> (2 * sharer + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
-                s[j] = (uint32_t)(t0 + 32 * (int)sharer + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[j] : -INFINITY;
+        while (t0 < last) {
+            const bool more = t0 + KT < last;
+            if constexpr (E4M3) {
+                // values of this tile to LDS; the next one begins its way
+                keep(true);
+                if (more) bring(t0 + KT, next.mine, false);
             }
-            // values that this wave has brought: rows that nobody sees become zeros, the others are looked through
-            if constexpr (!E4M3) __builtin_amdgcn_s_waitcnt(0x0F70);
-            uint32_t me = lane;
-            asm volatile("" : "+v"(me));
-            const uint32_t looked = r0 + me / 4, unit = me % 4 * (kUnits / 4);
-            const int token = t0 + (int)looked;
-            const bool dead = token < first || token >= last || !(there >> (looked / 16) & 1u);
-            half2v found = {(_Float16)0.f, (_Float16)0.f};
+            uint32_t keys_at = k_at;
+            asm volatile("" : "+v"(keys_at));   // (sixteen addresses that are made anew, not held)
 #pragma unroll
-            for (uint32_t i = 0; i < kUnits / 4; i++) {
-                uint4v *at = (uint4v *)(lds + kTile + looked * kRow + (value_place(looked, unit + i) << 4));
-                if (dead)
-                    *at = uint4v{0u, 0u, 0u, 0u};
-                else
-                    found = times_0(*at, found);
+            for (int j = 0; j < 16; j++) s[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8 *)(lds + (keys_at ^ i << 5)), q[i], s, 0, 0, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < D / 16 - 4; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);
-        }
-        float most = s[0];
+            __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+            const bool whole = t0 >= high_begin && t0 + KT <= whole_end && there == (1u << kGroups) - 1u;
+            bool bad = false;
+            if (!whole) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) most = fmaxf(most, s[j]);
-        most = max_of_halves(most);
-        weigh();
-        if (half == 0) tops[wave * 32u + col] = most;
-        const bool over = __any((most - reference) * c > 7.0f);
-        if (lane == 0) flags[wave] = (over ? 1u : 0u) | (bad ? 2u : 0u);
-        arrived();
-        const uint32_t flag = flags[0] | flags[1] | flags[2] | flags[3];
-        if (flag & 1u) {
-            // the reference moves, for both waves of a pair alike, and what is summed with it
-            most = fmaxf(most, tops[(wave ^ 1u) * 32u + col]);
-            const float raised = (most - reference) * c > 7.0f ? most : reference;
-            const float by = reference == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((reference - raised) * c);
-            sum *= by;
+                for (int j = 0; j < 16; j++) {
+                    const uint32_t seen = there >> (2 * sharer + j / 8) & 1u ? (uint32_t)max(0, my_end - my_begin) : 0u;
+                    s[j] = (uint32_t)(t0 + 32 * (int)sharer + 8 * (j / 4) + 4 * (int)half + j % 4 - my_begin) < seen ? s[j] : -INFINITY;
+                }
+                // values that this wave has brought: rows that nobody sees become zeros, the others are looked through
+                if constexpr (!E4M3) __builtin_amdgcn_s_waitcnt(0x0F70);
+                uint32_t me = lane;
+                asm volatile("" : "+v"(me));
+                const uint32_t looked = r0 + me / 4, unit = me % 4 * (kUnits / 4);
+                const int token = t0 + (int)looked;
+                const bool dead = token < first || token >= last || !(there >> (looked / 16) & 1u);
+                half2v found = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
-            for (int i = 0; i < (int)kHalf / 32; i++) o[i] *= by;
-            reference = raised;
+                for (uint32_t i = 0; i < kUnits / 4; i++) {
+                    uint4v *at = (uint4v *)(lds + kTile + looked * kRow + (value_place(looked, unit + i) << 4));
+                    if (dead)
+                        *at = uint4v{0u, 0u, 0u, 0u};
+                    else
+                        found = times_0(*at, found);
+                }
+                bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);
+            }
+            float most = s[0];
+#pragma unroll
+            for (int j = 0; j < 16; j++) most = fmaxf(most, s[j]);
+            most = max_of_halves(most);
             weigh();
-            __syncthreads();
-        }
-        sum += added;
-        // every wave is done with the tile's keys
-        if (more) {
-            if constexpr (E4M3) keep(false);
-            bring(t0 + KT, next.mine, E4M3);
-        }
-        if (!(flag & 2u)) {
+            if (half == 0) tops[wave * 32u + col] = most;
+            const bool over = __any((most - reference) * c > 7.0f);
+            if (lane == 0) flags[wave] = (over ? 1u : 0u) | (bad ? 2u : 0u);
+            arrived();
+            const uint32_t flag = flags[0] | flags[1] | flags[2] | flags[3];
+            if (flag & 1u) {
+                // the reference moves, for both waves of a pair alike, and what is summed with it
+                most = fmaxf(most, tops[(wave ^ 1u) * 32u + col]);
+                const float raised = (most - reference) * c > 7.0f ? most : reference;
+                const float by = shrink(reference, raised, c);
+                sum *= by;
 #pragma unroll
-            for (int b = 0; b < KT / 16; b++) {
-                const half8 p = pair_weights[b * 64];
+                for (int i = 0; i < (int)kHalf / 32; i++) o[i] *= by;
+                reference = raised;
+                weigh();
+                __syncthreads();
+            }
+            sum += added;
+            // every wave is done with the tile's keys
+            if (more) {
+                if constexpr (E4M3) keep(false);
+                bring(t0 + KT, next.mine, E4M3);
+            }
+            if (!(flag & 2u)) {
 #pragma unroll
-                for (int i = 0; i < (int)kHalf / 32; i++) {
-                    const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + b * 16 * kRow)));
-                    const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p, o[i], 0, 0, 0);
+                for (int b = 0; b < KT / 16; b++) {
+                    const half8 p = pair_weights[b * 64];
+#pragma unroll
+                    for (int i = 0; i < (int)kHalf / 32; i++) {
+                        const half4 x = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + b * 16 * kRow)));
+                        const half4 y = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((TWM_LDS(short4v) *)(lds + (v_at ^ i << 6) + (b * 16 + 8) * kRow)));
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}, p, o[i], 0, 0, 0);
+                    }
+                }
+            } else {
+                // one token after the other
+                for (int r = 0; r < KT; r++) {
+                    const int at = t0 + r;
+                    if (at < first || at >= last || !(there >> (r / 16) & 1u)) continue;
+                    const bool seen = at >= my_begin && at < my_end;
+                    const float w = fmaxf((float)((const _Float16 *)(weights + ((wave & ~1u) + r / 32u) * 128u + r % 32 / 16 * 64 + r / 4 % 2 * 32 + col))[r / 8 % 2 * 4 + r % 4], FLT_MIN);
+#pragma unroll
+                    for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const half4 x = *(const half4 *)(lds + kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
+                        }
                 }
             }
-        } else {
-            // one token after the other
-            for (int r = 0; r < KT; r++) {
-                const int at = t0 + r;
-                if (at < first || at >= last || !(there >> (r / 16) & 1u)) continue;
-                const bool seen = at >= my_begin && at < my_end;
-                const float w = (float)((const _Float16 *)(weights + ((wave & ~1u) + r / 32u) * 128u + r % 32 / 16 * 64 + r / 4 % 2 * 32 + col))[r / 8 % 2 * 4 + r % 4];
-#pragma unroll
-                for (int i = 0; i < (int)kHalf / 32; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const half4 x = *(const half4 *)(lds + kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
-                    }
+            arrived();
+            if constexpr (!E4M3) {
+                if (more) bring(t0 + KT, next.mine, true);
             }
+            t0 += KT;
+            there = next.there;
+            next = find_pages(t0 + KT);
         }
-        arrived();
-        if constexpr (!E4M3) {
-            if (more) bring(t0 + KT, next.mine, true);
-        }
-        t0 += KT;
-        there = next.there;
-        next = find_pages(t0 + KT);
+        if (E4M3 || max(t_begin, high_begin) + KT > whole_end) break;
+        // (as above: an infinite value times a weight that f16 holds as 0)
+        float one = 0.f;
+#pragma unroll
+        for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) one += o[i][j];
+        const bool odd = __any(one != one);
+        if (lane == 0) flags[wave] = odd;
+        __syncthreads();
+        if ((flags[0] | flags[1] | flags[2] | flags[3]) == 0) break;
+        whole_end = t_begin;
     }
 
     sum = sum_of_halves(sum);
@@ -799,8 +848,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     float top = -INFINITY, sum = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
     auto add = [&](const float2 &s, const float4v &part) {
-        const float raised = fmaxf(top, s.x), keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((top - raised) * c),
-                    by = s.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((s.x - raised) * c);
+        const float raised = fmaxf(top, s.x), keep = shrink(top, raised, c), by = shrink(s.x, raised, c);
         sum = sum * keep + s.y * by;
         o = o * keep + part * by;
         top = raised;
