@@ -376,6 +376,7 @@ __global__ __launch_bounds__(64 * WAVES, (WHOLE ? WAVES / 4 : kDecodePerUnit<D, 
             for (uint32_t w = 0; w < WAVES; w++) l += sums[w][h] * shrink(tops[w][h], m, c);
             if (all) {
                 const float to = l == 0.f ? 0.f : v_scale / l;
+                if (l == 0.f) r = float4v{0.f, 0.f, 0.f, 0.f};   // (all scores are -infinity, whatever the values)
                 *(half4_any *)(a.out + (size_t)seq * a.out_stride + (head0 + h) * D + x) =
                     half4{(_Float16)(r[0] * to), (_Float16)(r[1] * to), (_Float16)(r[2] * to), (_Float16)(r[3] * to)};
             } else {
@@ -461,6 +462,7 @@ template <int D, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void k_
     }
     if (group != 0) return;
     const float to = sum == 0.f ? 0.f : v_scale / sum;
+    if (sum == 0.f) o = float4v{0.f, 0.f, 0.f, 0.f};
     *(half4_any *)(a.out + (size_t)seq * a.out_stride + head * D + 4u * lane) =
         half4{(_Float16)(o[0] * to), (_Float16)(o[1] * to), (_Float16)(o[2] * to), (_Float16)(o[3] * to)};
 }

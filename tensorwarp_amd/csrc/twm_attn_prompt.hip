@@ -514,6 +514,12 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                     to[(8u * i + 2u * j + out_half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
         if (out_row < rows && out_half == 0) job.part_sums[(size_t)blockIdx.x * kRows + out_row - row0] = float2{reference, sum};
     } else if (out_row < rows) {
+        if (sum == 0.f) {   // (nothing was seen, or all scores are -infinity, whatever the values)
+#pragma unroll
+            for (int i = 0; i < D / 32; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+        }
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
         const uint32_t token = job.by_group(out_row), head = kv_head * a.group + (out_row - token * a.group);
         _Float16 *out = a.out + (size_t)(start + (int)token) * a.out_stride + head * D + 4u * out_half;
@@ -804,19 +810,29 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
     if (half == 0) tops[wave * 32u + col] = sum;
     __syncthreads();
     sum += tops[(wave ^ 1u) * 32u + col];
+    uint32_t me = lane;   // (as above)
+    asm volatile("" : "+v"(me));
+    const uint32_t out_row = wave_row + (me & 31u), out_half = me >> 5;
     if (parts > 1) {
         // to scratch, rows beside each other
-        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + wave_row - row0 + col;
+        float4v *to = job.parts + (size_t)blockIdx.x * (D / 4 * kRows) + out_row - row0;
 #pragma unroll
         for (int i = 0; i < (int)kHalf / 32; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (row < rows)
-                    to[(sharer * (kHalf / 4) + 8u * i + 2u * j + half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
-        if (row < rows && sharer == 0 && half == 0) job.part_sums[(size_t)blockIdx.x * kRows + wave_row - row0 + col] = float2{reference, sum};
-    } else if (row < rows) {
+                if (out_row < rows)
+                    to[(sharer * (kHalf / 4) + 8u * i + 2u * j + out_half) * kRows] = float4v{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+        if (out_row < rows && sharer == 0 && out_half == 0) job.part_sums[(size_t)blockIdx.x * kRows + out_row - row0] = float2{reference, sum};
+    } else if (out_row < rows) {
+        if (sum == 0.f) {   // (nothing was seen, or all scores are -infinity, whatever the values)
+#pragma unroll
+            for (int i = 0; i < (int)kHalf / 32; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) o[i][j] = 0.f;
+        }
         const float v_scale = E4M3 && a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
-        _Float16 *out = a.out + (size_t)(start + (int)my_token) * a.out_stride + my_head * D + sharer * kHalf + 4u * half;
+        const uint32_t token = job.by_group(out_row), head = kv_head * a.group + (out_row - token * a.group);
+        _Float16 *out = a.out + (size_t)(start + (int)token) * a.out_stride + head * D + sharer * kHalf + 4u * out_half;
 #pragma unroll
         for (int i = 0; i < (int)kHalf / 32; i++)
 #pragma unroll
@@ -879,6 +895,7 @@ template <int D, int SLICES> __global__ __launch_bounds__(256) void k_attn_promp
     }
     const uint32_t row = mine.row0 + r;
     if (row >= mine.rows) return;
+    if (sum == 0.f) o = float4v{0.f, 0.f, 0.f, 0.f};
     const float v_scale = a.kv.v_scales ? a.kv.v_scales[kv_head] : 1.0f, to = sum == 0.f ? 0.f : v_scale / sum;
     const uint32_t token = job.by_group(row), head = kv_head * a.group + (row - token * a.group);
     *(half4_any *)(a.out + (size_t)(mine.start + (int)token) * a.out_stride + head * D + 4u * quad) =

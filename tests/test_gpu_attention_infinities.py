@@ -118,3 +118,15 @@ def test_beside_scores_of_millions(dev, size, dim, width):
     infinite = {(10, 5): INF, (150, 6): -INF}
     pool, table, v = built(n, dim, width, scores, infinite)
     both(dev, pool, table, v, scores, infinite, n, n)
+
+
+@pytest.mark.parametrize("width", [None, 2000])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n,new", [(50, 50), (300, 300), (3100, 5)])
+def test_rows_of_nothing_but_infinitely_low_scores_are_zeros_beside_any_value(dev, n, new, dim, width):
+    pool, table, _ = built(n, dim, width, np.full(n, -np.inf), {(3, 5): INF, (n - 1, 6): float("nan"), (n // 2, 7): -INF})
+    q = np.zeros((new, 4, dim), np.float16)
+    q[:, :, 6] = 1.0
+    kc = pool.upload(dev)
+    assert (run(dev, kc, sequences(dev, table, [n], [new]), q, 4, scale=1.0) == 0).all()
+    assert (run(dev, kc, sequences(dev, table, [n]), q[:1], 4, scale=1.0) == 0).all()
