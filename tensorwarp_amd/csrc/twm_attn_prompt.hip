@@ -396,6 +396,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
         while (t0 < last) {
             // tiles that every row of the workgroup sees whole
             float raise_to = -INFINITY;
+            bool far = false;
             while (t0 >= high_begin && t0 + KT <= whole_end && there_now == (1u << kGroups) - 1u) {
                 const char *const tile = lds + buf * kTile;
                 advance();
@@ -405,6 +406,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                 const float most = largest(s);
                 if (__any((most - reference) * c > 7.0f || fabsf(reference) * c > 1024.0f)) {
                     raise_to = most;   // (rare; outside of this loop, so that the sums never move within it)
+                    far = true;
                     break;
                 }
                 weigh(std::true_type{}, s, p);
@@ -416,7 +418,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                 continue;
             }
             if (t0 >= last) break;
-            // one that some do not, or that lacks pages, or one of large scores
+            // one that some do not, or that lacks pages: for all waves alike, which meet in its midst; or (far) a whole one of too large scores for the short
+            // form of weights, which is this wave's affair: the others may take it as above, and it meets nobody
             const char *const tile = lds + buf * kTile;
             const uint32_t present = there_now;
             advance();
@@ -445,22 +448,25 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                 if (__any((most - reference) * c > 7.0f)) raise(most);
                 weigh(std::false_type{}, s, p);
             }
-            // values: rows that nobody sees become zeros, the others are looked through
-            constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
-            const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
-            const int token = t0 + (int)looked;
-            const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
-            half2v found = {(_Float16)0.f, (_Float16)0.f};
+            bool single = false;
+            if (!far) {
+                // values: rows that nobody sees become zeros, the others are looked through
+                constexpr uint32_t kEach = KT * kUnits / 256, kPerRow = kUnits / kEach;
+                const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
+                const int token = t0 + (int)looked;
+                const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
+                half2v found = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
-            for (uint32_t i = 0; i < kEach; i++) {
-                uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
-                if (dead)
-                    *at = uint4v{0u, 0u, 0u, 0u};
-                else
-                    found = times_0(*at, found);
+                for (uint32_t i = 0; i < kEach; i++) {
+                    uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
+                    if (dead)
+                        *at = uint4v{0u, 0u, 0u, 0u};
+                    else
+                        found = times_0(*at, found);
+                }
+                single = any_wave((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
+                if (single) __syncthreads();   // (flags are read)
             }
-            const bool single = any_wave((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
-            if (single) __syncthreads();   // (flags are read)
             if (!idle && !single) {
                 add_values(tile, p);
             } else if (!idle) {

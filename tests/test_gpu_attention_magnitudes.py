@@ -212,3 +212,69 @@ def test_tokens_without_weight_add_nothing(dev, infinite, value, dim, width):
         assert np.abs(got[behind, :, 12]).max() <= n * 2.0 ** -38 * value + 2.0 ** -25
         if rows > 1:
             assert np.array_equal(got[:599], np.broadcast_to(want, got[:599].shape))
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [1.0, 30.0, 1000.0])
+def test_random_scores_of_thousands_and_more(dev, scale, dim, cache, width):
+    # Results are means of values that are seen, whatever the weights; and where one score leads by more than all roundings of both (dim steps of 2^-23 of
+    # sum |q k|, each) and 30 besides, the others together weigh less than n e^-30 and the result is its value
+    n, heads, kv = 300, 4, 2
+    pool = Pool(np.random.default_rng(dim), 24, kv, 16, dim, cache)
+    table = pool.fill([n], width, spread=4.0)
+    q = (1.5 * np.random.default_rng(int(scale)).standard_normal((n, heads, dim))).astype(np.float16)
+    k, v = (np.repeat(pool.tokens(name, table[0], n), heads // kv, axis=0) for name in "kv")
+    for first, seqs in ((0, sequences(dev, table, [n], [n])), (n - 1, sequences(dev, table, [n]))):
+        got = run(dev, pool.upload(dev), seqs, q[first:], heads, scale=scale)
+        leading = 0
+        for i, row in enumerate(range(first, n)):
+            seen = v[:, :row + 1]
+            low, high = seen.min(1), seen.max(1)
+            room = TINY * np.abs(seen).max(1)
+            assert (got[i] >= low - room - half_step_f16(low)).all() and (got[i] <= high + room + half_step_f16(high)).all(), row
+            products = k[:, :row + 1] * q[row][:, None].astype(np.float64)
+            s, off = scale * products.sum(2), scale * dim * 2.0 ** -23 * np.abs(products).sum(2).max(1)
+            for h in range(heads):
+                order = np.argsort(s[h])
+                if row == 0 or s[h, order[-1]] - s[h, order[-2]] > 2 * off[h] + 30.0:
+                    leading += 1
+                    near(got[i, h], seen[h, order[-1]], room[h] + (row + 1) * np.exp(-30.0) * 2 * np.abs(seen[h]).max(0))
+        assert leading > 0.75 * len(got) * heads or first or scale < 30.0   # (counted on the host: 982 to 1200 of 1200)
+
+
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("dim,heads", [(64, 1), (128, 1), (128, 8), (256, 2)])
+@pytest.mark.parametrize("every", [1, 32, 40, 100])
+def test_rows_of_large_and_of_small_scores_in_turn(dev, every, dim, heads, cache):
+    # rows whose scores have 2^20 added, and rows without, in turn by `every` rows times heads: some waves of a workgroup have such rows and others do not.
+    # What a row comes to is the same; longer than a tile's buffers live, and each token has a value of its own
+    n = 900
+    rng = np.random.default_rng(every + dim)
+    gaps = 4.0 * rng.integers(0, 16, n)
+    pool, table = filled(dim, dim, cache, n, 80, np.zeros((n, dim)))
+    large = 8192.0 if cache == "f16" else 448.0
+    for t in range(n):
+        at = table[0, t // 16], 0, t % 16
+        pool.bits["k"][at] = 0
+        if cache == "f16":
+            pool.bits["k"][at][[0, dim - 3]] = np.array([large, gaps[t]], np.float16).view(np.uint16)
+        else:   # e4m3: 448 and 0, 8, ... 56 (of three bits), so that sums are exact as well
+            gaps[t] = 8.0 * (gaps[t] // 8)
+            codes = {0: 0x00, 8: 0x50, 16: 0x58, 24: 0x5C, 32: 0x60, 40: 0x62, 48: 0x64, 56: 0x66}
+            pool.bits["k"][at][[0, dim - 3]] = 0x7E, codes[int(gaps[t])]
+    q = np.zeros((n, heads, dim), np.float16)
+    q[:, :, dim - 3] = 1.0
+    added = (np.arange(n * heads).reshape(n, heads) // every) % 2 == 1
+    q[added, 0] = 128.0 if cache == "f16" else 2048.0
+    v = pool.tokens("v", table[0], n)[0]
+    p = np.exp(0.125 * (gaps - gaps.max()))
+    total = p.cumsum()[:, None]
+    want, magnitude = (p[:, None] * v).cumsum(0) / total, (p[:, None] * np.abs(v)).cumsum(0) / total
+    # (as above, and rows without the addition have exponents rounded at up to 2^10: 2^-15, where the maximum was raised too, for the weight and the sum)
+    tol = (PROMPT_STEP + 2.0 ** -12 + (n + 16) * 2.0 ** -23) * magnitude + 2.0 ** -33 * np.abs(v).sum(0)
+    kc = pool.upload(dev)
+    for _ in range(3):
+        got = run(dev, kc, sequences(dev, table, [n], [n]), q, heads, scale=0.125)
+        near(got, np.repeat(want[:, None], heads, 1), np.repeat(tol[:, None], heads, 1))
