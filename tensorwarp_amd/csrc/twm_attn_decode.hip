@@ -418,7 +418,8 @@ template <int D, uint32_t THREADS> __global__ __launch_bounds__(THREADS) void k_
     const uint64_t end = begin + steps;
     // the shares that hold its first and its last step
     auto share_of = [&](uint64_t at) {
-        uint32_t w = (uint32_t)min((uint64_t)(d.shares - 1), (uint64_t)((float)at / (float)total * d.shares));
+        // (where steps are fewer than shares, step and share are one)
+        uint32_t w = total <= d.shares ? (uint32_t)at : (uint32_t)min((uint64_t)(d.shares - 1), (uint64_t)((float)at / (float)total * d.shares));
         while (share_begin(d, total, w) > at) w--;
         while (share_begin(d, total, w + 1) <= at) w++;
         return w;
