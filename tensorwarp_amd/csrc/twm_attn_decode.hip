@@ -20,10 +20,10 @@
 // holds of a sequence that others hold too goes to scratch, and a second kernel joins it.  (Joining by the last workgroup to arrive cost the same
 // 5 us.)  Where no sequence is long, each sequence and unit has a workgroup of more waves to itself and nothing is joined.
 //
-// Bound by the reading of the cache where it is long: 32 sequences of up to 8192 tokens, 28 heads on 4 of 128 f16 values, 60.5 us (4.5 TB/s; a copy
-// reaches 5.1); 48 of up to 4096, 32 heads on 32, e4m3, 155 us (4.9 TB/s); one sequence of 131072 58 us, of 32768 20.8 (3.2 TB/s: two launches and
-// eight steps a share are what is left), and of 777 tokens, 14 heads of 64 values, 9.2 us, which are the chain from the length by the table and the
-// keys to the sums.
+// Bound by the reading of the cache where it is long: 32 sequences of up to 8192 tokens, 28 heads on 4 of 128 f16 values, 60 us (4.6 TB/s; a copy
+// reaches 5.1); 48 of up to 4096, 32 heads on 32, e4m3, 152 us (5.5 TB/s); 32 of up to 4096, 16 heads on 8 of 256, 106 us (5.2 TB/s), e4m3 64 (4.3); one
+// sequence of 131072 58 us, of 32768 20.7 - 22.9 (two launches and eight steps a share are what is left), and of 777 tokens, 14 heads of 64
+// values, 9.2 us, which are the chain from the length by the table and the keys to the sums.
 #include "twm_kv.h"
 #include "twm_slices.h"
 
@@ -482,11 +482,12 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
         constexpr int D = decltype(dim)::value;
         constexpr bool E4M3 = decltype(e4m3)::value;
         constexpr uint32_t WHOLE_WAVES = kDecodeWholeWaves<D, E4M3>;
-        // No shares, and nothing to join, where no sequence is long, by as much more as there are many.  28 heads on 4 of 128 values, up to 512 tokens:
-        // one sequence 9.8 us, 10.8 in shares; 32 sequences 11.1 and 17.4; 200 sequences 34 and 38.  Up to 2048, 200 sequences 91 and 97; but up to
-        // 4096 166 either way, 48 of 32 heads in e4m3 160 and 155, and one of 1024 tokens, four steps of its eight waves, 14.4 and 10.6.  And none among
-        // so many sequences that each share's way through their lengths costs more than a long one's wait: 1024 up to 512 tokens 154 us, 188 in
-        // shares, up to 8192 1433 and 1495, 16384 up to 64 (7 heads on one) 342 and 2384.
+        // No shares, and nothing to join, where no sequence can be long by the table's width, by as much more as there are many.  28 heads on 4 of 128 values:
+        // one sequence of 100 tokens 6.6 us, 10.7 in shares; 32 sequences up to 512 11.0 and 13.1, 200 35 and 40; up to 2048, 200 sequences 90 and 98;
+        // but one of 512 10.0 and 9.9, up to 4096 200 sequences 166 either way, 48 of 32 heads in e4m3 160 and 155, and one of 1024 tokens, four steps of eight
+        // waves, 14.4 and 9.9.  And none among so many sequences that each share's way through their lengths costs more than most waits: 1023
+        // up to 512 tokens 179 in shares, 1024 154 without, up to 8192 1485 and 1454, 16384 up to 64 (7 heads on one) 2384 and 352.  The price
+        // is one that is much longer than the others: one of 16384 tokens among 1024 of 100 189 (among 1023, in shares, 121), of 131072 1390 (177).
         if (seen <= std::min<uint64_t>(8, 2 + (uint64_t)a.seqs.seqs * d.units / 64) * (32 * WHOLE_WAVES) || a.seqs.seqs >= 1024) {
             d.shares = d.units;
             d.by_shares = Divisor(d.units);
@@ -502,7 +503,7 @@ hipError_t launch_attn_decode(hipStream_t s, const AttnArgs &a, void *scratch, s
         const size_t slots = 2 * (size_t)d.shares * d.units * d.heads;
         d.part_sums = (float2 *)scratch;
         d.parts = (float *)((char *)scratch + (slots * sizeof(float2) + 255) / 256 * 256);
-        if ((size_t)((char *)(d.parts + slots * D) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 34 MB of 256)
+        if ((size_t)((char *)(d.parts + slots * D) - (char *)scratch) > scratch_bytes) return hipErrorOutOfMemory;   // (at most 17 MB of 256)
         hipLaunchKernelGGL((k_attn_decode<D, E4M3, kDecodeWaves, false>), dim3(d.shares * d.units), dim3(64 * kDecodeWaves), 0, s, d, 0u);
         if (const hipError_t error = hipGetLastError(); error != hipSuccess) return error;
         // sixteen parts of 128 values at once for few sequences, which have many, four otherwise (32 sequences up to 1024 tokens 20.7 us with

@@ -18,13 +18,14 @@
 // products are made one token at a time, for those who see it.  So they are once more in all tiles where sums came to NaN: an infinite value times a weight
 // that f16 rounds to 0 is NaN in a matrix product, where the formula has that infinity.
 //
-// Bound by no single unit where prompts are long: a wave's 32 queries read as many bytes of keys and values from LDS (128 a cycle and compute unit) as
-// keep its matrix instructions busy, and the exponentials come on top; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of
-// 128 f16 values, 500 - 525 us (920 - 960 TFLOP/s of the halves that are seen; a large matrix product reaches 1310).  Workgroups of eight waves
+// Bound by no single unit where prompts are long: matrix units are busy half of the time, vector instructions (the exponentials above all) nearly as long, LDS
+// a fourth; two workgroups a compute unit cover one another in part.  8192 rows, 28 heads on 4 of 128 f16 values, 505 - 534 us (900 - 950 TFLOP/s of the
+// halves that are seen; a large matrix product reaches 1310).  Heads of 64 have half the products for as many exponentials: vector instructions two
+// thirds of the time, 300 us (800 TFLOP/s).  Workgroups of eight waves
 // that take turns with products and exponentials cost their barriers (580 - 596), blocks of products between blocks of exponentials in one wave the
 // registers (579), and 64 queries a wave with the next tile's scores beside this one's exponentials leave one wave a SIMD (heads of 64: 376, with 32 queries
 // 309; of 128 they spill).  Short prompts are the way from the sequence by its pages to the keys, and tiles on the diagonal, which cost two whole ones: 37 rows, 14
-// heads of 64, 5.3 us; 2048 rows in seven prompts 22 - 24 us, of which the longest's eleven tiles are half.
+// heads of 64, 5.3 us; 2048 rows in seven prompts 22.7 us, of which the longest's eleven tiles are half.
 #include "twm_kv.h"
 #include "twm_slices.h"
 
@@ -932,10 +933,10 @@ hipError_t launch_attn_prompt(hipStream_t s, const AttnArgs &a, void *scratch, s
     auto launch = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         const uint64_t capacity = (uint64_t)a.seqs.table_stride << a.kv.page_shift;
-        // Waves in pairs for heads of 256 values, and where no sequence is longer than eight tiles and the chip is not full of them: tiles of 64 rows and
-        // half of a tile's tokens a wave take less time each, if more together.  28 heads on 4 of 128: 128 rows 8.2 us, 9.8 in the other form, 512
-        // 16.9 and 17.4, 1000 in twenty prompts 11.7 and 12.6; 200 rows of 32 heads on 32 in e4m3 10.0 and 12.8; but 1000 rows in five prompts 17.8 and
-        // 16.1, 4000 in twenty 40 and 34, 8192 in one 670 and 500.
+        // Waves in pairs for heads of 256 values, and where no sequence can be longer than eight tiles by the table's width and the chip is not full of
+        // them: tiles of 64 rows and half of a tile's tokens a wave take less time each, if more together.  28 heads on 4 of 128: 128 rows 8.2 us, 9.8 in
+        // the other form, 512 19.1 and 21.3, 1000 in twenty prompts 11.8 and 12.4; 200 rows of 32 heads on 32 in e4m3 10.1 and 14.7; 37 rows of 14 heads
+        // of 64 5.3 and 8.1; but 1000 rows in five prompts 17.8 and 16.1, 4000 in twenty 40 and 34, 8192 in one 670 and 500.
         const uint64_t pairs_tiles = (uint64_t)a.rows * a.group / 64 + a.seqs.seqs;
         const bool pairs = D == 256 || (capacity <= 512 && pairs_tiles * a.kv.kv_heads * capacity <= 2048 * kPromptTile);
         const uint32_t each = pairs ? 64 : 128;

@@ -62,7 +62,7 @@ __device__ __forceinline__ uint2v codes_8(const float (&v)[8], float scale)
 // A workgroup per row.  A thread holds sixteen values of one head: the two runs of eight that a rotation of halves turns into each other,
 // or sixteen neighbours.  The row's sequence is the last one that starts up to it, found among as many at once as there are threads.
 // One row is a launch and the way from the starts by the length and the table to the store (4.0 - 4.8 us); 2048 rows of 36 heads of 128 f16 values
-// into e4m3, 37 MB, take 11.8 us (3.1 TB/s): one round of workgroups, whose loads wait for their sequence.
+// into e4m3, 37 MB, take 11.8 us (3.1 TB/s), into f16 10.3 (3.8), of f32 values 15.6 and 15.1: one round of workgroups, whose loads wait for their sequence.
 template <bool F16> __global__ void k_kv_append(const Append a)
 {
     const uint32_t row = blockIdx.x, dim = a.kv.dim, each = dim >> 4, units = (a.q_heads + 2u * a.kv.kv_heads) * each;
@@ -170,7 +170,7 @@ static_assert(sizeof(Copy) <= 4000, "arguments of a kernel end at 4 KB");
 }  // namespace
 
 // A workgroup per 16 KB piece, four loads of 16 bytes a lane on their way.  Bound by memory where pages are many (500 of 16 KB, keys and values of 28
-// layers, 918 MB read and written: 187 us, 4.9 TB/s, a large copy's 5.1), by the host where they are few (one page 5.5 us, of which the kernel takes 3.0).
+// layers, 918 MB read and written: 187 us, 4.9 TB/s, a large copy's 5.1), by the host where they are few (one page 4.6 - 5.7 us, of which the kernel takes 2.9).
 __global__ __launch_bounds__(256) void k_kv_copy_pages(const Copy c)
 {
     char *base = (char *)c.array[blockIdx.z];
