@@ -35,11 +35,7 @@ namespace twm {
 
 namespace {
 
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef half4 half4_any __attribute__((aligned(2)));
-typedef short short4v __attribute__((ext_vector_type(4)));
 typedef int int2v __attribute__((ext_vector_type(2)));
-#define TWM_LDS(T) __attribute__((address_space(3))) T
 
 constexpr uint32_t kDecodeHeads = 16;   // query heads of one unit: columns of a matrix instruction
 constexpr uint32_t kDecodeWaves = 4, kDecodeStep = 32 * kDecodeWaves;   // of shares
@@ -109,17 +105,6 @@ __device__ __forceinline__ float sum_over_quarters(float v)
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
-
-// eight codes as f16 (exact)
-__device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
-{
-    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
-    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
-    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// 2^(c (m - m')); never 0, so that an infinite sum stays one (and 2^-126 of nothing is nothing where m is -infinity)
-__device__ __forceinline__ float shrink(float m, float to, float c) { return __builtin_amdgcn_exp2f(fmaxf((m - to) * c, -126.0f)); }
 
 // Workgroups of four waves that share a compute unit, by their registers; waves of a workgroup that has a sequence to itself
 template <int D, bool E4M3> constexpr uint32_t kDecodePerUnit = D == 256 ? (E4M3 ? 2 : 1) : D == 128 ? (E4M3 ? 3 : 2) : 3;

@@ -38,11 +38,7 @@ namespace twm {
 
 namespace {
 
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef half4 half4_any __attribute__((aligned(2)));
-typedef short short4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
-#define TWM_LDS(T) __attribute__((address_space(3))) T
 
 constexpr uint32_t kPromptWaves = 4;
 template <int D> constexpr uint32_t kPromptRows = D == 256 ? 64 : 128;   // of a workgroup
@@ -57,18 +53,6 @@ __device__ __forceinline__ float sum_of_halves(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// What sums are multiplied by where the reference moves: 2^(c (from - to)), never 0, so that an infinite sum stays one (of nothing, from = -infinity,
-// nothing is left)
-__device__ __forceinline__ float shrink(float from, float to, float c) { return __builtin_amdgcn_exp2f(fmaxf((from - to) * c, -126.0f)); }
-
-// eight codes as f16 (exact)
-__device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
-{
-    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
-    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
-    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // What is not finite times 0 is NaN, and stays in the sum

@@ -9,6 +9,10 @@ namespace twm {
 // Rows of queries and of fused projections begin at any element; the memory takes vectors there too
 typedef half8 half8_any __attribute__((aligned(2)));
 typedef float4v float4v_any __attribute__((aligned(4)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef half4 half4_any __attribute__((aligned(2)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+#define TWM_LDS(T) __attribute__((address_space(3))) T
 
 // The first element of (page, head) in a cache's array
 __device__ __forceinline__ size_t kv_chunk(const KvView &kv, uint32_t page, uint32_t head)
@@ -24,6 +28,18 @@ __device__ __forceinline__ float exponent_factor(const KvView &kv, float scale, 
     const float c = (float)((double)scale * 1.4426950408889634 * (kv.k_scales ? (double)kv.k_scales[head] : 1.0));
     return c > FLT_MAX ? FLT_MAX : c < FLT_MIN ? FLT_MIN : c;   // (a NaN stays)
 }
+
+// eight codes as f16 (exact)
+__device__ __forceinline__ half8 to_f16(unsigned lo, unsigned hi)
+{
+    const half2v a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.0f, true);
+    const half2v c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.0f, true);
+    return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// What sums are multiplied by where the score that they refer to becomes another: 2^(c (from - to)).  Never 0, so that an infinite sum stays one; 2^-126
+// of what is finite counts for nothing, nor does that of nothing, where from is -infinity.
+__device__ __forceinline__ float shrink(float from, float to, float c) { return __builtin_amdgcn_exp2f(fmaxf((from - to) * c, -126.0f)); }
 
 // v of this lane and of those before it, added up (by moves within rows of sixteen lanes, then across them)
 __device__ __forceinline__ uint32_t wave_sum_up_to(uint32_t v)
