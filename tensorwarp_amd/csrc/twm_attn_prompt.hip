@@ -133,6 +133,76 @@ __device__ __forceinline__ uint32_t parts_of(const Rows &r, const Prompt &job, i
     return max(1u, min(min(job.splits, *tiles / kLeastPart), (uint32_t)sqrtf((float)*tiles * job.balance)));
 }
 
+// The place of a unit in its row of keys (of which 16 rows are read at once) and of values (four rows, four units of each)
+template <int D> __device__ __forceinline__ uint32_t key_place(uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); }
+template <int D> __device__ __forceinline__ uint32_t value_place(uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); }
+
+// A tile's pages: a wave's sixteen rows (or eight) are neighbours, which lie in one; bit g: the page of tokens 16 g .. is in the pool
+struct Pages {
+    int mine;
+    uint32_t there;
+};
+// A lane looks the pages of sixteen tokens up, the wave those of 1024 at once
+struct PagesOf {
+    const int *table;
+    uint32_t pages, page_shift;
+    int last, looked_up, page_of;
+    uint64_t there;
+    __device__ __forceinline__ void look_up(int t0)
+    {
+        looked_up = t0;
+        const int token = t0 + 16 * (int)(threadIdx.x & 63u);
+        page_of = token < last ? table[(uint32_t)token >> page_shift] : -1;
+        there = __ballot((uint32_t)page_of < pages);
+    }
+    // of the tile at t0, and of the run of 16 in it that this wave brings in
+    __device__ __forceinline__ Pages find(int t0, uint32_t run)
+    {
+        if (t0 - looked_up >= 1024) look_up(t0);
+        const uint32_t group = (uint32_t)(t0 - looked_up) >> 4;
+        return Pages{__builtin_amdgcn_readlane(page_of, group + run), (uint32_t)(there >> group) & ((1u << kPromptTile / 16) - 1u)};
+    }
+};
+
+// N units of row r of a tile's values: zeros where nobody sees the row, looked through otherwise; whether any is not finite
+template <int D, uint32_t N> __device__ __forceinline__ bool look_through(char *values, uint32_t r, uint32_t unit, bool dead)
+{
+    half2v found = {(_Float16)0.f, (_Float16)0.f};
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+        uint4v *at = (uint4v *)(values + r * D * 2 + (value_place<D>(r, unit + i) << 4));
+        if (dead)
+            *at = uint4v{0u, 0u, 0u, 0u};
+        else
+            found = times_0(*at, found);
+    }
+    return (__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0;   // (a zero of either sign otherwise)
+}
+// Row r of a tile's values, from a unit on, to the sums of a lane's query, if that sees it
+template <int D, int N> __device__ __forceinline__ void add_one(float16v (&o)[N], const char *values, uint32_t r, uint32_t unit, _Float16 weight, bool seen)
+{
+    const uint32_t half = threadIdx.x >> 5 & 1u;
+    const float w = fmaxf((float)weight, FLT_MIN);   // (an infinite value times 0 would be NaN)
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const half4 x = *(const half4 *)(values + r * D * 2 + (value_place<D>(r, unit + 4u * i + j) << 4) + 8u * half);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
+        }
+}
+// whether any sum is NaN, or one is infinity and another -infinity (one question for all of a lane's)
+template <int N> __device__ __forceinline__ bool any_nan(const float16v (&o)[N])
+{
+    float one = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) one += o[i][j];
+    return one != one;
+}
+
 // LDS of a workgroup
 template <int D> constexpr uint32_t kPromptLds = 4 * kPromptTile * D * 2 + (D == 64 ? kPromptWaves * 64 * 32 * 2 + 16 : 16);
 template <int D> constexpr uint32_t kPairsLds = 2 * kPromptTile * D * 2 + kPromptWaves * 2048 + kPromptWaves * 32 * 4 + 16;
@@ -187,30 +257,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
     float reference, sum;
     float16v o[D / 32];
 
-    // The place of a unit in its row of keys (of which 16 rows are read at once) and of values (four rows, four units of each)
-    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
-    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); };
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
-    // A tile's pages: this wave's rows are kWaveRows (16, or 8) neighbours, which lie in one; bit g: the page of tokens 16 g .. is in the pool.
-    // A lane looks the pages of sixteen tokens up, the wave those of 1024 at once.
-    struct Pages {
-        int mine;
-        uint32_t there;
-    };
     const int t_begin = first & ~(KT - 1);
-    int looked_up = t_begin, page_of = -1;
-    uint64_t page_there = 0;
-    auto look_up = [&](int t0) {
-        looked_up = t0;
-        const int token = t0 + 16 * (int)lane;
-        page_of = token < last ? a.seqs.tables[(size_t)seq * a.seqs.table_stride + ((uint32_t)token >> a.kv.page_shift)] : -1;
-        page_there = __ballot((uint32_t)page_of < a.kv.pages);
-    };
-    auto find_pages = [&](int t0) {
-        if (t0 - looked_up >= 1024) look_up(t0);
-        const uint32_t group = (uint32_t)(t0 - looked_up) >> 4;
-        return Pages{__builtin_amdgcn_readlane(page_of, group + wave * kWaveRows / 16u), (uint32_t)(page_there >> group) & ((1u << kGroups) - 1u)};
-    };
+    PagesOf pages_of{a.seqs.tables + (size_t)seq * a.seqs.table_stride, a.kv.pages, a.kv.page_shift, last, t_begin, -1, 0};
     constexpr int kLoads = (int)(kWaveRows * D * (E4M3 ? 1 : 2) / 1024);   // 1 KB each
     constexpr uint32_t kLoadUnits = D * (E4M3 ? 1 : 2) / 16, kRowsPerLoad = 64 / kLoadUnits;
     uint4v k_held[kLoads], v_held[kLoads];   // e4m3 only
@@ -227,8 +276,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                 v_held[i] = *(const uint4v *)(v_from + i * 1024 + lane * 16u);
             } else {
                 const uint32_t r = r0 + i * kRowsPerLoad + lane / kUnits;   // the row in the tile, and the unit that this lane's place holds
-                const uint32_t row_off = i * 1024u + lane / kUnits * kRow, k_off = row_off + (key_place(r, lane % kUnits) << 4),
-                               v_off = row_off + (value_place(r, lane % kUnits) << 4);
+                const uint32_t row_off = i * 1024u + lane / kUnits * kRow, k_off = row_off + (key_place<D>(r, lane % kUnits) << 4),
+                               v_off = row_off + (value_place<D>(r, lane % kUnits) << 4);
                 char *to = lds + buf * kTile + (r0 + i * kRowsPerLoad) * kRow;
                 __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(k_from + k_off), (TWM_LDS(void) *)to, 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(v_from + v_off), (TWM_LDS(void) *)(to + 2 * kTile), 16, 0, 0);
@@ -242,10 +291,10 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
             for (int i = 0; i < kLoads; i++) {
                 const uint32_t r = wave * kWaveRows + i * kRowsPerLoad + lane / kLoadUnits, unit = lane % kLoadUnits * 2;
                 char *to = lds + buf * kTile + r * kRow;
-                *(half8 *)(to + (key_place(r, unit) << 4)) = to_f16(k_held[i][0], k_held[i][1]);
-                *(half8 *)(to + (key_place(r, unit + 1) << 4)) = to_f16(k_held[i][2], k_held[i][3]);
-                *(half8 *)(to + 2 * kTile + (value_place(r, unit) << 4)) = to_f16(v_held[i][0], v_held[i][1]);
-                *(half8 *)(to + 2 * kTile + (value_place(r, unit + 1) << 4)) = to_f16(v_held[i][2], v_held[i][3]);
+                *(half8 *)(to + (key_place<D>(r, unit) << 4)) = to_f16(k_held[i][0], k_held[i][1]);
+                *(half8 *)(to + (key_place<D>(r, unit + 1) << 4)) = to_f16(k_held[i][2], k_held[i][3]);
+                *(half8 *)(to + 2 * kTile + (value_place<D>(r, unit) << 4)) = to_f16(v_held[i][0], v_held[i][1]);
+                *(half8 *)(to + 2 * kTile + (value_place<D>(r, unit + 1) << 4)) = to_f16(v_held[i][2], v_held[i][3]);
             }
         }
     };
@@ -267,8 +316,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
     uint32_t there, buf;
     Pages next;
     // Where a lane reads keys and values in the first buffers: the number of a unit enters by XOR, rows of whole blocks by addition
-    const uint32_t k_at = col * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
-    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
+    const uint32_t k_at = col * kRow + (key_place<D>(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = 2 * kTile + v_row * kRow + (value_place<D>(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u;
     // S^T of the tile in buffer `tile`; element j of block b: token 32 b + 8 (j / 4) + 4 half + j % 4
     auto scores = [&](const char *tile, float16v (&s)[KT / 32]) {
 #pragma unroll
@@ -346,7 +395,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
         if (advanced) return;
         if (t0 + KT < last) bring(t0 + KT, next, buf ^ 1u);
         there = next.there;
-        next = find_pages(t0 + 2 * KT);
+        next = pages_of.find(t0 + 2 * KT, wave * kWaveRows / 16u);
         advanced = true;
     };
     auto turn = [&]() {
@@ -367,12 +416,12 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
         there = buf = 0;
         next = Pages{-1, 0};
         if (t_begin < last) {
-            look_up(t_begin);
-            const Pages pages = find_pages(t_begin);
+            pages_of.look_up(t_begin);
+            const Pages pages = pages_of.find(t_begin, wave * kWaveRows / 16u);
             there = pages.there;
             bring(t_begin, pages, 0);
             keep(0);
-            next = find_pages(t_begin + KT);
+            next = pages_of.find(t_begin + KT, wave * kWaveRows / 16u);
         }
         arrived();
         t0 = t_begin;
@@ -440,16 +489,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                 const uint32_t looked = threadIdx.x / kPerRow, unit = threadIdx.x % kPerRow * kEach;
                 const int token = t0 + (int)looked;
                 const bool dead = token < first || token >= last || !(present >> (looked / 16) & 1u);
-                half2v found = {(_Float16)0.f, (_Float16)0.f};
-#pragma unroll
-                for (uint32_t i = 0; i < kEach; i++) {
-                    uint4v *at = (uint4v *)(lds + buf * kTile + 2 * kTile + looked * kRow + (value_place(looked, unit + i) << 4));
-                    if (dead)
-                        *at = uint4v{0u, 0u, 0u, 0u};
-                    else
-                        found = times_0(*at, found);
-                }
-                single = any_wave((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);   // (a zero of either sign otherwise)
+                single = any_wave(look_through<D, kEach>(lds + buf * kTile + 2 * kTile, looked, unit, dead));
                 if (single) __syncthreads();   // (flags are read)
             }
             if (!idle && !single) {
@@ -465,27 +505,14 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 64 && !E4M3 
                     const int at = t0 + r;
                     if (at < first || at >= last || !(present >> (r / 16) & 1u)) continue;
                     const bool seen = at >= my_begin && at < my_end;
-                    const float w = fmaxf((float)weights[r * 32 + (int)col], FLT_MIN);   // (an infinite value times 0 would be NaN)
-#pragma unroll
-                    for (int i = 0; i < D / 32; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const half4 x = *(const half4 *)(tile + 2 * kTile + r * kRow + (value_place((uint32_t)r, 4u * i + j) << 4) + 8u * half);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
-                        }
+                    add_one<D>(o, tile + 2 * kTile, (uint32_t)r, 0, weights[r * 32 + (int)col], seen);
                 }
             }
             turn();
         }
         if (E4M3 || max(t_begin, high_begin) + KT > whole_end) break;   // (no tile was taken as whole; e4m3 has no infinity)
         // Sums that are NaN may be an infinite value times a weight that f16 holds as 0, which is that infinity: once more, with no tile taken as whole
-        float one = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; i++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) one += o[i][j];
-        if (!any_wave(one != one)) break;
+        if (!any_wave(any_nan(o))) break;
         whole_end = t_begin;
     }
 
@@ -569,27 +596,9 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
     float reference, sum;
     float16v o[kHalf / 32];
 
-    auto key_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r >> 1) & 7u : r & 15u); };
-    auto value_place = [](uint32_t r, uint32_t unit) { return unit ^ (D == 64 ? (r & 2u) << 1 : (r & 3u) << 2); };
     const uint32_t page_mask = (1u << a.kv.page_shift) - 1u;
-    struct Pages {
-        int mine;
-        uint32_t there;
-    };
     const int t_begin = first & ~(KT - 1);
-    int looked_up = t_begin, page_of = -1;
-    uint64_t page_there = 0;
-    auto look_up = [&](int t0) {
-        looked_up = t0;
-        const int token = t0 + 16 * (int)lane;
-        page_of = token < last ? a.seqs.tables[(size_t)seq * a.seqs.table_stride + ((uint32_t)token >> a.kv.page_shift)] : -1;
-        page_there = __ballot((uint32_t)page_of < a.kv.pages);
-    };
-    auto find_pages = [&](int t0) {
-        if (t0 - looked_up >= 1024) look_up(t0);
-        const uint32_t group = (uint32_t)(t0 - looked_up) >> 4;
-        return Pages{__builtin_amdgcn_readlane(page_of, group + wave), (uint32_t)(page_there >> group) & ((1u << kGroups) - 1u)};
-    };
+    PagesOf pages_of{a.seqs.tables + (size_t)seq * a.seqs.table_stride, a.kv.pages, a.kv.page_shift, last, t_begin, -1, 0};
     constexpr int kLoads = (int)(kWaveRows * D * (E4M3 ? 1 : 2) / 1024);   // 1 KB each
     constexpr uint32_t kLoadUnits = D * (E4M3 ? 1 : 2) / 16, kRowsPerLoad = 64 / kLoadUnits;
     uint4v held[kLoads];   // e4m3 only: keys or values on their way
@@ -607,7 +616,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
                 held[i] = *(const uint4v *)(from + i * 1024 + me * 16u);
             } else {
                 const uint32_t r = r0 + i * kRowsPerLoad + me / kUnits;
-                const uint32_t off = i * 1024u + me / kUnits * kRow + ((value ? value_place(r, me % kUnits) : key_place(r, me % kUnits)) << 4);
+                const uint32_t off = i * 1024u + me / kUnits * kRow + ((value ? value_place<D>(r, me % kUnits) : key_place<D>(r, me % kUnits)) << 4);
                 char *to = lds + (value ? kTile : 0u) + (r0 + i * kRowsPerLoad) * kRow;
                 __builtin_amdgcn_global_load_lds((const TWM_GLOBAL void *)(from + off), (TWM_LDS(void) *)to, 16, 0, 0);
             }
@@ -621,8 +630,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
             for (int i = 0; i < kLoads; i++) {
                 const uint32_t r = r0 + i * kRowsPerLoad + me / kLoadUnits, unit = me % kLoadUnits * 2;
                 char *to = lds + (value ? kTile : 0u) + r * kRow;
-                *(half8 *)(to + ((value ? value_place(r, unit) : key_place(r, unit)) << 4)) = to_f16(held[i][0], held[i][1]);
-                *(half8 *)(to + ((value ? value_place(r, unit + 1) : key_place(r, unit + 1)) << 4)) = to_f16(held[i][2], held[i][3]);
+                *(half8 *)(to + ((value ? value_place<D>(r, unit) : key_place<D>(r, unit)) << 4)) = to_f16(held[i][0], held[i][1]);
+                *(half8 *)(to + ((value ? value_place<D>(r, unit + 1) : key_place<D>(r, unit + 1)) << 4)) = to_f16(held[i][2], held[i][3]);
             }
         }
     };
@@ -633,8 +642,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
 
     const int high_begin = prompt_begin(a, high);
     int whole_end = min(low + 1, last);
-    const uint32_t k_at = (32u * sharer + col) * kRow + (key_place(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
-    const uint32_t v_at = (kTile + v_row * kRow + (value_place(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u) ^ sharer * kHalf * 2u;
+    const uint32_t k_at = (32u * sharer + col) * kRow + (key_place<D>(col, half) << 4), v_row = 4u * half + (lane >> 2 & 3u);
+    const uint32_t v_at = (kTile + v_row * kRow + (value_place<D>(v_row, (lane >> 4 & 1u) * 2u + (lane >> 1 & 1u)) << 4) + (lane & 1u) * 8u) ^ sharer * kHalf * 2u;
     const half8 *const pair_weights = weights + (wave & ~1u) * 128u + lane;
     float16v s;
     float added;
@@ -664,13 +673,13 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
         uint32_t there = 0;
         Pages next{-1, 0};
         if (t0 < last) {
-            look_up(t0);
-            const Pages now = find_pages(t0);
+            pages_of.look_up(t0);
+            const Pages now = pages_of.find(t0, wave);
             there = now.there;
             bring(t0, now.mine, false);
             keep(false);
             bring(t0, now.mine, true);
-            next = find_pages(t0 + KT);
+            next = pages_of.find(t0 + KT, wave);
             arrived();
         }
         while (t0 < last) {
@@ -708,16 +717,7 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
                 const uint32_t looked = r0 + me / 4, unit = me % 4 * (kUnits / 4);
                 const int token = t0 + (int)looked;
                 const bool dead = token < first || token >= last || !(there >> (looked / 16) & 1u);
-                half2v found = {(_Float16)0.f, (_Float16)0.f};
-#pragma unroll
-                for (uint32_t i = 0; i < kUnits / 4; i++) {
-                    uint4v *at = (uint4v *)(lds + kTile + looked * kRow + (value_place(looked, unit + i) << 4));
-                    if (dead)
-                        *at = uint4v{0u, 0u, 0u, 0u};
-                    else
-                        found = times_0(*at, found);
-                }
-                bad = __any((__builtin_bit_cast(uint32_t, found) & 0x7FFF7FFFu) != 0);
+                bad = __any(look_through<D, kUnits / 4>(lds + kTile, looked, unit, dead));
             }
             float most = s[0];
 #pragma unroll
@@ -764,15 +764,8 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
                     const int at = t0 + r;
                     if (at < first || at >= last || !(there >> (r / 16) & 1u)) continue;
                     const bool seen = at >= my_begin && at < my_end;
-                    const float w = fmaxf((float)((const _Float16 *)(weights + ((wave & ~1u) + r / 32u) * 128u + r % 32 / 16 * 64 + r / 4 % 2 * 32 + col))[r / 8 % 2 * 4 + r % 4], FLT_MIN);
-#pragma unroll
-                    for (int i = 0; i < (int)kHalf / 32; i++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const half4 x = *(const half4 *)(lds + kTile + r * kRow + (value_place((uint32_t)r, sharer * kHalf / 8u + 4u * i + j) << 4) + 8u * half);
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[i][4 * j + e] = seen ? fmaf(w, (float)x[e], o[i][4 * j + e]) : o[i][4 * j + e];
-                        }
+                    const _Float16 *of = (const _Float16 *)(weights + ((wave & ~1u) + r / 32u) * 128u + r % 32 / 16 * 64 + r / 4 % 2 * 32 + col);
+                    add_one<D>(o, lds + kTile, (uint32_t)r, sharer * kHalf / 8u, of[r / 8 % 2 * 4 + r % 4], seen);
                 }
             }
             arrived();
@@ -781,16 +774,11 @@ template <int D, bool E4M3> __global__ __launch_bounds__(256, (D == 256 ? 2 : 3)
             }
             t0 += KT;
             there = next.there;
-            next = find_pages(t0 + KT);
+            next = pages_of.find(t0 + KT, wave);
         }
         if (E4M3 || max(t_begin, high_begin) + KT > whole_end) break;
         // (as above: an infinite value times a weight that f16 holds as 0)
-        float one = 0.f;
-#pragma unroll
-        for (int i = 0; i < (int)kHalf / 32; i++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) one += o[i][j];
-        const bool odd = __any(one != one);
+        const bool odd = __any(any_nan(o));
         if (lane == 0) flags[wave] = odd;
         __syncthreads();
         if ((flags[0] | flags[1] | flags[2] | flags[3]) == 0) break;
