@@ -5,6 +5,8 @@
 // over the tokens t that the row sees, r a reference for the row's scores: the largest one when it was set, moved (and the sums with
 // it) only where a weight would pass 2^15, so that sums are rarely touched again and f16 holds the weights with all of its digits down to 2^-22
 // of the largest.
+// A weight enters its product, and the sum that divides it, as the one f16 that it is rounded to: errors of 2.2 - 2.8e-4 of a result's norm, 2.0e-4 being the
+// f16 result's own rounding.  A second term, as twm_attn_decode has it, would be half of the products again, and these are half of a long prompt's time.
 //
 // A workgroup takes 128 queries (of 256 values 64) of one key-value head -- tokens times the query heads that share it, so that short prompts fill
 // tiles too -- and its four waves 32 each.  Keys and values come through LDS, tile by tile, the next tile on its way while this one is worked on;
